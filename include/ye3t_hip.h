@@ -23,11 +23,17 @@
 extern "C" {
 #endif
 
-#define YE3T_HIP_ABI_VERSION 62 /* reference native ABI floor is 42 (execution_plan.py:35) */
+#define YE3T_HIP_ABI_VERSION 63 /* reference native ABI floor is 42 (execution_plan.py:35) */
 
 typedef struct ihipStream_t* ye3t_stream_t; /* == hipStream_t */
 
-enum ye3t_dtype { YE3T_F32 = 0, YE3T_F64 = 1, YE3T_C64 = 2, YE3T_C128 = 3 /* complex: (re, im) pairs */ };
+enum ye3t_dtype {
+  YE3T_F32 = 0,
+  YE3T_F64 = 1,
+  YE3T_C64 = 2, /* complex: (re, im) pairs */
+  YE3T_C128 = 3,
+  YE3T_BF16 = 4 /* embedding, norm and attention only */
+};
 
 enum ye3t_status {
   YE3T_OK = 0,
@@ -815,6 +821,117 @@ int ye3t_hip_product_plan_uses_stream(const ye3t_hip_product_plan* plan);
 /* Kernel name/launch geometry of the last product_forward (for profiling). */
 int ye3t_hip_product_launch_info(const ye3t_hip_product_plan* plan, int64_t samples, int64_t* grid,
                                  int64_t* block, int64_t* lds_bytes);
+
+/* ---- operators around the features: embedding, norm, attention ---------------
+ * No reference counterparts.  They serve a model's own layers before and after
+ * the ACE features; `dtype` may be YE3T_BF16 here.  None of them synchronises,
+ * allocates or uses atomics on data: equal calls give equal bits. */
+
+/* out[i, :] = scale * table[tokens[i], :], [token_count, width]; tokens int32
+ * (token_bytes 4) or int64 (8); a token outside [0, vocabulary) gives zeros.
+ * `row_stride` is the table's, in values.  dtype F32, F64 or BF16; the product
+ * is taken in fp32 (fp64 for F64) and rounded once. */
+int ye3t_hip_embedding(int dtype, const void* tokens, int token_bytes, int64_t token_count, const void* table,
+                       int64_t row_stride, int64_t vocabulary, int64_t width, double scale, void* out,
+                       ye3t_stream_t stream);
+
+/* Device workspace bytes of ye3t_hip_embedding_adjoint (-1 on invalid input). */
+int64_t ye3t_hip_embedding_adjoint_workspace_bytes(int dtype, int64_t token_count, int64_t vocabulary, int64_t width);
+
+/* table_adjoint[v, :] = scale * sum of adjoint[i, :] over the i with
+ * tokens[i] == v, [vocabulary, width], every row written.  The positions are
+ * sorted by token and summed in equal shares in a fixed order, in fp32 (fp64
+ * for F64), whatever the tokens' frequencies; tokens outside the table count
+ * nowhere. */
+int ye3t_hip_embedding_adjoint(int dtype, const void* adjoint, const void* tokens, int token_bytes, int64_t token_count,
+                               int64_t vocabulary, int64_t width, double scale, void* table_adjoint, void* workspace,
+                               int64_t workspace_bytes, ye3t_stream_t stream);
+
+/* total = x + residual; y = total * weight / sqrt(mean(total^2) + epsilon) over
+ * each of `rows` rows of `width` values.  The mean and y come from the unrounded
+ * sum in fp32.  `residual` may be NULL (then `total` may be too).  dtype F32 or
+ * BF16 for all arrays. */
+int ye3t_hip_rms_norm(int dtype, const void* x, const void* residual, const void* weight, int64_t rows, int64_t width,
+                      double epsilon, void* total, void* y, ye3t_stream_t stream);
+
+/* The same with y in 8 bits: codes [rows, width] in the format with four
+ * exponent and three mantissa bits (largest value 448, no infinities) and one
+ * fp32 scale for each 128 columns, scales [rows, ceil(width / 128)]: scale =
+ * max|y| / 448, code = y / scale rounded to nearest even.  Columns of zeros
+ * have scale 0. */
+int ye3t_hip_rms_norm_8bit(int dtype, const void* x, const void* residual, const void* weight, int64_t rows,
+                           int64_t width, double epsilon, void* total, void* codes, void* scales,
+                           ye3t_stream_t stream);
+
+/* Device workspace bytes of ye3t_hip_rms_norm_adjoint (-1 on invalid input). */
+int64_t ye3t_hip_rms_norm_adjoint_workspace_bytes(int dtype, int64_t rows, int64_t width);
+
+/* Gradient of ye3t_hip_rms_norm at `total` (the forward's sum, or its x where
+ * there was no residual) for the output's adjoint and, if not NULL, the sum's
+ * own adjoint: x_adjoint [rows, width] (the residual's is the same) and
+ * weight_adjoint [width], whose sum over rows is fp32 in a fixed order. */
+int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_adjoint, const void* total,
+                              const void* weight, int64_t rows, int64_t width, double epsilon, void* x_adjoint,
+                              void* weight_adjoint, void* workspace, int64_t workspace_bytes, ye3t_stream_t stream);
+
+/* Attention among the atoms of each structure.  Atoms are packed: structure s
+ * has the query atoms offsets[s] .. offsets[s + 1] - 1 and the key atoms of
+ * key_offsets (NULL: the same).  Query head h reads key head
+ * h / (heads / key_heads).  Scores are scale * q . k, then, for cap > 0,
+ * cap * tanh(score / cap), then, with slopes, less slopes[head] times the
+ * distance of the two atoms.  key_mask (NULL: all) is 0 for keys that no row
+ * sees; what they hold is not used.  A row that sees no key gives zeros.
+ * Strides are in values, those of the last axis 1. */
+typedef struct {
+  int dtype;           /* YE3T_F32 or YE3T_BF16: query, key, value, outputs and their adjoints */
+  int64_t queries;     /* query atoms */
+  int64_t keys;        /* key atoms */
+  int64_t structures;
+  int64_t heads;
+  int64_t key_heads;   /* divides heads */
+  int64_t head_width;  /* at most 128 */
+  const void* query;   /* [queries, heads, head_width] */
+  const void* key;     /* [keys, key_heads, head_width] */
+  const void* value;   /* [keys, key_heads, head_width] */
+  int64_t query_row_stride, query_head_stride;
+  int64_t key_row_stride, key_head_stride;
+  int64_t value_row_stride, value_head_stride;
+  const int64_t* offsets;      /* [structures + 1], 0 .. queries, not falling */
+  const int64_t* key_offsets;  /* [structures + 1], 0 .. keys, or NULL */
+  double scale;
+  double cap;                  /* 0: scores are not capped */
+  const float* slopes;         /* [heads], or NULL: no distances */
+  const float* positions;      /* [queries, 3], with slopes */
+  const float* key_positions;  /* [keys, 3], or NULL: positions */
+  const uint8_t* key_mask;     /* [keys], or NULL */
+} ye3t_attention_args;
+
+/* Device workspace bytes of ye3t_hip_atom_attention (0 where it needs none; -1
+ * on invalid input). */
+int64_t ye3t_hip_atom_attention_workspace_bytes(const ye3t_attention_args* args);
+
+/* out [queries, heads, head_width] and, if not NULL, log_sums [queries, heads]
+ * fp32: the natural logarithm of each row's sum of exponentials (-infinity for a row
+ * that sees no key), which the gradient takes.  Few rows against many keys are
+ * split over the keys and joined. */
+int ye3t_hip_atom_attention(const ye3t_attention_args* args, void* out, void* log_sums, void* workspace,
+                            int64_t workspace_bytes, ye3t_stream_t stream);
+
+/* Device workspace bytes of ye3t_hip_atom_attention_adjoint (-1 on invalid input). */
+int64_t ye3t_hip_atom_attention_adjoint_workspace_bytes(const ye3t_attention_args* args, int bias_gradients);
+
+/* Gradients of ye3t_hip_atom_attention for the output's adjoint [queries,
+ * heads, head_width]: query_adjoint, key_adjoint and value_adjoint, contiguous,
+ * in `dtype`.  With slopes_adjoint [heads] also the fp32 gradients to the slopes
+ * and to positions [queries, 3] and key_positions [keys, 3]; without
+ * key_positions the atoms are the same and positions_adjoint holds both parts.
+ * Two atoms at one place have no direction and add nothing to either.  The
+ * rows' sums of D come from the output, or with slopes_adjoint from the scores. */
+int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void* out, const void* log_sums,
+                                    const void* out_adjoint, void* query_adjoint, void* key_adjoint,
+                                    void* value_adjoint, void* slopes_adjoint, void* positions_adjoint,
+                                    void* key_positions_adjoint, void* workspace, int64_t workspace_bytes,
+                                    ye3t_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,441 @@
+// Attention of the atoms of each structure over the structure's atoms.
+//
+//   s_ij = scale q_i . k_j;  s <- cap tanh(s / cap);  s <- s - slope_h |r_i - r_j|
+//   p_ij = softmax over the visible keys j of i's structure,  o_i = sum_j p_ij v_j
+//
+// Gradient, with D_i = sum_j p_ij (go_i . v_j):
+//
+//   dz_ij = p_ij (go_i . v_j - D_i)                     of the biased score
+//   ds_ij = dz_ij (1 - tanh^2)                          of the scaled product
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij go_i
+//   dslope_h = -sum_ij dz_ij |r_i - r_j|,  dr_i = -slope sum_j dz_ij (r_i - r_j) / |r_i - r_j|  (and its negative to r_j)
+//
+// Query heads that share a key head are rows of one problem: row r of a key
+// head is token r / G of query head r % G of its group.  A wave owns 32 rows
+// (32 keys in the key-side gradient) and takes the other axis in tiles that the
+// workgroup stages in LDS.  All products run on the 32 x 32 matrix
+// instructions, bf16 x bf16 -> fp32 or fp32 x fp32 -> fp32, transposed so that
+// a lane holds one row's (key's) values: lane l has column l % 32 and, in
+// register 4 b + j, line 8 b + 4 (l / 32) + j.  Softmax statistics are then a
+// lane's own but for one exchange between the two half waves, and the same
+// registers are the operand of the next product, whose contraction order is
+// chosen to fit them.
+//
+// Scores, the running maximum and sum, and every sum over keys or rows are
+// fp32.  bf16 calls round p and ds to bf16 for the matrix instruction (relative
+// 2^-9 each, as the inputs have) and each output once.
+#pragma once
+
+#include "rows.h"
+
+namespace ye3t {
+namespace attention {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Problem {
+  int64_t queries, keys, structures;
+  int heads, key_heads, group, D;
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int64_t *offsets, *key_offsets;
+  float scale, cap;
+  const float *slopes, *positions, *key_positions;
+  const uint8_t* key_mask;
+};
+
+// 16 bytes of a lane as matrix operand: 8 bf16 or 4 fp32 values
+template <typename T>
+struct Operand;
+template <>
+struct Operand<__bf16> {
+  typedef bf16x8 type;
+};
+template <>
+struct Operand<float> {
+  typedef f32x4 type;
+};
+template <typename T>
+using Op = typename Operand<T>::type;
+
+// c += a b over the 2 kChunk contraction slots of one operand: slot
+// (half wave, element)
+__device__ inline void mma(bf16x8 a, bf16x8 b, f32x16& c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline void mma(f32x4 a, f32x4 b, f32x16& c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+}
+
+__device__ inline f32x16 zeros() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+// A tile of rows in LDS: DP values and 32 bytes of padding, so that 16 byte
+// reads of eight consecutive rows fall into different banks.
+template <typename T, int DP>
+constexpr int kPitch = DP + 32 / int(sizeof(T));
+
+// Contraction over the width: chunk u of line `line` holds values
+// 2 kChunk u + kChunk half ...
+template <typename T, int DP>
+__device__ inline Op<T> line_chunk(const T* tile, int line, int u, int half) {
+  return *reinterpret_cast<const Op<T>*>(tile + line * kPitch<T, DP> + (2 * u + half) * kChunk<T>);
+}
+
+// Contraction over 32 lines of a tile, the transposed operand: column `column`
+// + lane % 32 of the lines that registers 2 kChunk s / 2 ... of an accumulator
+// hold (bf16: lines 16 s + 4 half + 0..3 and + 8; fp32: lines 8 s + 4 half + 0..3).
+template <int DP>
+__device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, int half) {
+  const int lane = threadIdx.x & 31;
+  bf16x8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    r[j] = tile[(16 * s + 8 * (j / 4) + 4 * half + j % 4) * kPitch<__bf16, DP> + column + lane];
+  return r;
+}
+template <int DP>
+__device__ inline f32x4 column_chunk(const float* tile, int s, int column, int half) {
+  const int lane = threadIdx.x & 31;
+  f32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = tile[(8 * s + 4 * half + j) * kPitch<float, DP> + column + lane];
+  return r;
+}
+// and the accumulator's registers as the other operand
+__device__ inline void register_chunk(const f32x16& p, int s, bf16x8& r) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = __bf16(p[8 * s + j]);
+}
+__device__ inline void register_chunk(const f32x16& p, int s, f32x4& r) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = p[4 * s + j];
+}
+template <typename T>
+constexpr int kLineChunks = 32 / (2 * kChunk<T>);
+
+// tanh with a relative error of a few ulp: the odd series where the quotient
+// would cancel.
+__device__ inline float bent(float x) {
+  const float a = fabsf(x), y = x * x;
+  const float series =
+      x + x * y * (-0.333333333f + y * (0.133333333f + y * (-0.0539682540f + y * (0.0218694885f + y * -0.00886323552f))));
+  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * a);
+  const float q = copysignf(1.0f - 2.0f / (e + 1.0f), x);
+  return a < 0.3f ? series : q;
+}
+
+// The largest d with bound(d) <= slot, bound rising, bound(0) <= slot: 64 probes a round.
+template <typename F>
+__device__ inline int64_t find_owner(int64_t count, int64_t slot, F bound) {
+  int64_t lo = 0, hi = count;
+  const int lane = threadIdx.x & 63;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 63) / 64;
+    const int64_t at = lo + lane * step;
+    const uint64_t yes = __ballot(at < hi && bound(at) <= slot);
+    const int k = 63 - __clzll(static_cast<long long>(yes | 1));
+    lo += k * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  return lo;
+}
+
+// The rows or keys of a structure; offsets out of range are clamped, so that no
+// access leaves the arrays whatever they hold.
+struct Span {
+  int64_t begin;
+  int length;
+};
+__device__ inline int64_t clamped(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
+__device__ inline Span span_of(const int64_t* offsets, int64_t d, int64_t most) {
+  const int64_t a = clamped(offsets[d], most), b = clamped(offsets[d + 1], most);
+  return {a, b > a ? int(b - a) : 0};
+}
+
+// Work items of `tile` rows over structures of any lengths without a table of
+// them: structure d's items start at floor(offset_d G / tile) + d, which leaves
+// room for each; an item past its structure's rows has nothing to do.
+struct Item {
+  int64_t structure;
+  int64_t first;  // row in the structure
+};
+__device__ inline Item item_of(const int64_t* offsets, int64_t structures, int64_t most, int group, int tile,
+                               int64_t slot) {
+  auto bound = [&](int64_t d) { return clamped(offsets[d], most) * group / tile + d; };
+  const int64_t d = find_owner(structures, slot, bound);
+  return {d, (slot - bound(d)) * tile};
+}
+inline int64_t item_count(int64_t rows, int64_t structures, int tile) { return rows / tile + structures; }
+
+// ---- loads of a tile ---------------------------------------------------------
+// LINES x DP values of `T`, NT threads, in registers between the load and the
+// LDS write so that the next tile's loads run under this tile's products.
+template <typename T, int DP, int LINES, int NT>
+struct Staged {
+  static constexpr int ROW = DP / kChunk<T>;  // 16 byte chunks of a line
+  static constexpr int N = (LINES * ROW + NT - 1) / NT;
+  static constexpr bool WHOLE = LINES * ROW % NT == 0;
+  // two tiles in flight take 64 registers of a lane at most; a single wave with
+  // wide fp32 rows reads its tile between the barriers
+  static constexpr bool AHEAD = 2 * N * 4 <= 64;
+  Chunk<T, kChunk<T>> v[N];
+
+  // address(line): the line's first value, or null for a line of zeros
+  template <typename F>
+  __device__ inline void load(int D, F address) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int x = n * NT + int(threadIdx.x), line = x / ROW, c = x % ROW * kChunk<T>;
+      const T* p = WHOLE || x < LINES * ROW ? address(line) : nullptr;
+      v[n] = p && c < D ? Chunk<T, kChunk<T>>::load(p + c, D - c) : Chunk<T, kChunk<T>>::zero();
+    }
+  }
+  __device__ inline void write(T* tile) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int x = n * NT + int(threadIdx.x), line = x / ROW, c = x % ROW * kChunk<T>;
+      Op<T> a;
+#pragma unroll
+      for (int q = 0; q < kChunk<T>; ++q) a[q] = v[n].v[q];
+      if (WHOLE || x < LINES * ROW) *reinterpret_cast<Op<T>*>(tile + line * kPitch<T, DP> + c) = a;
+    }
+  }
+};
+
+// A row or key as matrix operand, straight from memory: chunks of this lane's half
+template <typename T, int DP>
+__device__ inline void line_operand(const T* p, int D, int half, Op<T>* r) {
+#pragma unroll
+  for (int u = 0; u < DP / (2 * kChunk<T>); ++u) {
+    const int c = (2 * u + half) * kChunk<T>;
+    const Chunk<T, kChunk<T>> a = p && c < D ? Chunk<T, kChunk<T>>::load(p + c, D - c) : Chunk<T, kChunk<T>>::zero();
+#pragma unroll
+    for (int q = 0; q < kChunk<T>; ++q) r[u][q] = a.v[q];
+  }
+}
+
+// Values of lines 8 b + 4 half + j, column lane % 32, to memory: line = value of
+// the width, the lane's row at `p` (null: none).
+template <typename T, int DP>
+__device__ inline void store_columns(T* p, int D, int half, const f32x16* acc, float factor) {
+  if (!p) return;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int c = 32 * t + 8 * b + 4 * half;
+      Chunk<T, 4> a;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a.v[j] = T(acc[t][4 * b + j] * factor);
+      if (c < D) a.store(p + c, D - c);
+    }
+  }
+}
+
+__device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
+
+// key: x, y, z and whether it is seen
+template <bool BIAS>
+__device__ inline f32x4 key_place(const Problem& p, int64_t key, bool exists) {
+  f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (exists && (!p.key_mask || p.key_mask[key])) {
+    r[3] = 1.0f;
+    if (BIAS) {
+      const float* at = (p.key_positions ? p.key_positions : p.positions) + 3 * key;
+      r[0] = at[0];
+      r[1] = at[1];
+      r[2] = at[2];
+    }
+  }
+  return r;
+}
+
+struct Row {
+  int64_t token;
+  int head;
+  bool exists;
+};
+__device__ inline Row row_of(const Problem& p, int64_t begin, int64_t row, int64_t rows, int key_head) {
+  Row r;
+  r.exists = row < rows;
+  const uint32_t x = r.exists ? uint32_t(row) : 0u;
+  const uint32_t token = p.group == 1 ? x : x / uint32_t(p.group);
+  r.token = begin + token;
+  r.head = key_head * p.group + int(x - token * uint32_t(p.group));
+  return r;
+}
+
+struct Gradient {
+  const void *out, *adjoint;  // [queries, heads, D]
+  const float* log_sums;      // [queries, heads]
+  float* along;               // D_i, [queries, heads]
+  void *dq, *dk, *dv;         // [queries, heads, D], [keys, key_heads, D]
+  float* row_part;            // [queries, heads, 4]: to the position and the slope
+  float* key_part;            // [keys, key_heads, 4]
+};
+
+// p, and the derivative of the bend, of scores as the forward takes them
+struct Weight {
+  float p, slant;
+};
+template <bool BIAS>
+__device__ inline Weight weight_of(const Problem& p, float product, float log_sum2, float slope2, float distance,
+                                   bool seen) {
+  float s, slant = 1.0f;
+  if (p.cap > 0.0f) {
+    const float t = bent(product * (p.scale / p.cap));
+    s = p.cap * kLog2e * t;
+    slant = 1.0f - t * t;
+  } else {
+    s = product * (p.scale * kLog2e);
+  }
+  if (BIAS) s -= slope2 * distance;
+  return {seen ? __builtin_amdgcn_exp2f(s - log_sum2) : 0.0f, slant};
+}
+
+// ---- launches ----------------------------------------------------------------
+inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// Waves of a workgroup: rows enough for the mean structure, four at most.
+inline int waves_for(int64_t rows, int64_t structures) {
+  const int64_t mean = structures > 0 ? (rows + structures - 1) / structures : 0;
+  return mean <= 32 ? 1 : 4;
+}
+
+// Parts of the key axis: where the rows alone give less than four workgroups
+// a compute unit, as many as fill that, each with two tiles of keys or more on
+// average.
+inline int parts_for(int64_t items, int key_heads, int64_t keys, int64_t structures) {
+  const int64_t groups = items * key_heads;
+  if (groups >= 1024 || structures == 0) return 1;
+  int64_t parts = 1024 / groups;
+  const int64_t tiles = keys / structures / 64;
+  if (parts > tiles) parts = tiles;
+  return int(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+}
+
+struct ForwardPlan {
+  int waves, parts;
+  int64_t items, part_bytes, bytes;
+};
+inline ForwardPlan forward_plan(const ye3t_attention_args& a) {
+  ForwardPlan f{};
+  const int64_t group = a.heads / a.key_heads;
+  f.waves = waves_for(a.queries * group, a.structures);
+  f.items = item_count(a.queries * group, a.structures, 32 * f.waves);
+  f.parts = parts_for(f.items, int(a.key_heads), a.keys, a.structures);
+  if (f.parts > 1) {
+    f.part_bytes = up(f.parts * a.queries * a.heads * a.head_width * 4);
+    f.bytes = f.part_bytes + up(f.parts * a.queries * a.heads * 8);
+  }
+  return f;
+}
+
+// workgroups that share the sum over atoms of the slopes' gradient
+constexpr int kSlopeGroups = 256;
+
+struct AdjointPlan {
+  int row_waves, key_waves;
+  int64_t row_items, key_items, along_bytes, row_bytes, key_bytes, bytes;
+};
+inline AdjointPlan adjoint_plan(const ye3t_attention_args& a, bool forces) {
+  AdjointPlan f{};
+  const int64_t group = a.heads / a.key_heads;
+  f.row_waves = waves_for(a.queries * group, a.structures);
+  f.key_waves = waves_for(a.keys, a.structures);
+  f.row_items = item_count(a.queries * group, a.structures, 32 * f.row_waves);
+  f.key_items = item_count(a.keys, a.structures, 32 * f.key_waves);
+  f.along_bytes = up(a.queries * a.heads * 4);
+  if (forces) {
+    f.row_bytes = up(a.queries * a.heads * 16);
+    f.key_bytes = up(a.keys * a.key_heads * 16);
+    f.bytes = up(kSlopeGroups * a.heads * 4);
+  }
+  f.bytes += f.along_bytes + f.row_bytes + f.key_bytes + 256;
+  return f;
+}
+
+inline Problem problem_of(const ye3t_attention_args& a) {
+  Problem p{};
+  p.queries = a.queries;
+  p.keys = a.keys;
+  p.structures = a.structures;
+  p.heads = int(a.heads);
+  p.key_heads = int(a.key_heads);
+  p.group = int(a.heads / a.key_heads);
+  p.D = int(a.head_width);
+  p.q = a.query;
+  p.k = a.key;
+  p.v = a.value;
+  p.q_row = a.query_row_stride;
+  p.q_head = a.query_head_stride;
+  p.k_row = a.key_row_stride;
+  p.k_head = a.key_head_stride;
+  p.v_row = a.value_row_stride;
+  p.v_head = a.value_head_stride;
+  p.offsets = a.offsets;
+  p.key_offsets = a.key_offsets ? a.key_offsets : a.offsets;
+  p.scale = float(a.scale);
+  p.cap = float(a.cap);
+  p.slopes = a.slopes;
+  p.positions = a.positions;
+  p.key_positions = a.key_positions;
+  p.key_mask = a.key_mask;
+  return p;
+}
+
+inline int check_attention(const ye3t_attention_args& a) {
+  YE3T_REQUIRE(a.queries >= 0 && a.keys >= 0 && a.structures >= 0, "atom and structure counts must not be negative");
+  YE3T_REQUIRE(a.heads >= 1 && a.key_heads >= 1 && a.heads % a.key_heads == 0,
+               "heads must be a positive multiple of key_heads");
+  YE3T_REQUIRE(a.head_width >= 1, "head_width must be positive");
+  if (a.head_width > 128) return set_error(YE3T_EUNSUPPORTED, "head_width %lld is above 128", (long long)a.head_width);
+  if (a.dtype != YE3T_F32 && a.dtype != YE3T_BF16)
+    return set_error(YE3T_EDTYPE, "unsupported dtype %d; expected float32 or bfloat16", a.dtype);
+  YE3T_REQUIRE(a.heads <= 65535 && a.queries < (int64_t(1) << 31) / a.heads && a.keys < (int64_t(1) << 31) / a.heads &&
+                   a.structures < (int64_t(1) << 24),
+               "at most 2^31 - 1 rows (atoms times heads), 65535 heads and 2^24 - 1 structures");
+  YE3T_REQUIRE(a.cap >= 0.0, "cap must not be negative");
+  YE3T_REQUIRE((a.slopes == nullptr) == (a.positions == nullptr), "slopes and positions come together");
+  YE3T_REQUIRE(!a.slopes || a.key_positions || (!a.key_offsets && a.queries == a.keys),
+               "keys of their own need key_positions");
+  YE3T_REQUIRE(a.key_offsets || a.queries == a.keys, "keys of their own need key_offsets");
+  return YE3T_OK;
+}
+
+inline int check_pointers(const ye3t_attention_args& a) {
+  YE3T_REQUIRE(a.structures == 0 || a.offsets, "attention needs the structures' offsets");
+  YE3T_REQUIRE((a.queries == 0 || a.query) && (a.keys == 0 || (a.key && a.value)), "attention needs query, key and value");
+  return YE3T_OK;
+}
+
+// Calls f.template operator()<T, DP>() for the call's type and width.
+template <typename F>
+int with_width(int dtype, int64_t D, F f) {
+  if (dtype == YE3T_F32)
+    return D <= 32 ? f.template operator()<float, 32>()
+                   : D <= 64 ? f.template operator()<float, 64>() : f.template operator()<float, 128>();
+  return D <= 32 ? f.template operator()<__bf16, 32>()
+                 : D <= 64 ? f.template operator()<__bf16, 64>() : f.template operator()<__bf16, 128>();
+}
+
+// The gradient's two sides (attention_rows.hip, attention_keys.hip)
+int launch_row_gradient(int dtype, const AdjointPlan& f, const Problem& p, const Gradient& g, bool forces,
+                        hipStream_t s);
+int launch_key_gradient(int dtype, const AdjointPlan& f, const Problem& p, const Gradient& g, bool forces,
+                        hipStream_t s);
+
+}  // namespace attention
+}  // namespace ye3t

@@ -1,0 +1,365 @@
+// Atom attention: forward kernels, the sums of the gradients to slopes and
+// positions, and the entry points.
+#include "attention.h"
+
+namespace ye3t {
+namespace attention {
+namespace {
+
+// ---- forward -----------------------------------------------------------------
+// NW waves of 32 rows, KT keys a tile.  SPLIT: grid axis z takes equal parts of
+// each structure's key tiles and leaves its sums to attention_join_kernel.
+template <typename T, int DP, int NW, int KT, bool BIAS, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
+                                                            float* __restrict__ part, float* __restrict__ part_stats) {
+  constexpr int TILE = 32 * NW, NU = DP / (2 * kChunk<T>), ND = DP / 32;
+  __shared__ __align__(16) T ktile[KT * kPitch<T, DP>];
+  __shared__ __align__(16) T vtile[KT * kPitch<T, DP>];
+  __shared__ f32x4 place[KT];
+  const Item item = item_of(p.offsets, p.structures, p.queries, p.group, TILE, blockIdx.x);
+  const Span own = span_of(p.offsets, item.structure, p.queries);
+  const int64_t rows = int64_t(own.length) * p.group;
+  if (item.first < 0 || item.first >= rows) return;
+  const Span key = span_of(p.key_offsets, item.structure, p.keys);
+  const int key_head = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const Row row = row_of(p, own.begin, item.first + 32 * wave + (lane & 31), rows, key_head);
+  const bool busy = item.first + 32 * wave < rows;  // of the whole wave
+
+  Op<T> q[NU];
+  line_operand<T, DP>(row.exists ? static_cast<const T*>(p.q) + row.token * p.q_row + row.head * p.q_head : nullptr,
+                      p.D, half, q);
+  float x = 0.0f, y = 0.0f, z = 0.0f, slope = 0.0f;
+  if (BIAS && row.exists) {
+    x = p.positions[3 * row.token];
+    y = p.positions[3 * row.token + 1];
+    z = p.positions[3 * row.token + 2];
+    slope = p.slopes[row.head] * kLog2e;
+  }
+  int tiles = (key.length + KT - 1) / KT, tile = 0;
+  if (SPLIT) {
+    const int each = (tiles + gridDim.z - 1) / gridDim.z;
+    tile = int(blockIdx.z) * each;
+    tiles = tile + each < tiles ? tile + each : tiles;
+  }
+  f32x16 acc[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) acc[t] = zeros();
+  float top = -INFINITY, sum = 0.0f;
+  const T* kbase = static_cast<const T*>(p.k) + key_head * p.k_head;
+  const T* vbase = static_cast<const T*>(p.v) + key_head * p.v_head;
+  Staged<T, DP, KT, 64 * NW> ks, vs;
+  f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto fetch = [&](int t) {
+    auto seen = [&](int line) {
+      const int j = t * KT + line;
+      return j < key.length && (!p.key_mask || p.key_mask[key.begin + j]);
+    };
+    // masked keys are read as zeros, whatever they hold
+    ks.load(p.D, [&](int line) { return seen(line) ? kbase + (key.begin + t * KT + line) * p.k_row : nullptr; });
+    vs.load(p.D, [&](int line) { return seen(line) ? vbase + (key.begin + t * KT + line) * p.v_row : nullptr; });
+    if (int(threadIdx.x) < KT) {
+      const int j = t * KT + int(threadIdx.x);
+      next_place = key_place<BIAS>(p, key.begin + j, j < key.length);
+    }
+  };
+  if (ks.AHEAD && tile < tiles) fetch(tile);
+  const float to_log2 = p.scale * kLog2e;
+  const float to_cap = p.cap > 0.0f ? p.scale / p.cap : 0.0f, from_cap = p.cap * kLog2e;
+  for (; tile < tiles; ++tile) {
+    __syncthreads();  // the last tile has been used
+    if (!ks.AHEAD) fetch(tile);
+    ks.write(ktile);
+    vs.write(vtile);
+    if (int(threadIdx.x) < KT) place[threadIdx.x] = next_place;
+    __syncthreads();
+    if (ks.AHEAD && tile + 1 < tiles) fetch(tile + 1);
+    if (!busy) continue;
+    const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
+    f32x16 s[KT / 32];
+    float high = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < KT / 32; ++n) {
+      s[n] = zeros();
+#pragma unroll
+      for (int u = 0; u < NU; ++u) mma(line_chunk<T, DP>(ktile, 32 * n + (lane & 31), u, half), q[u], s[n]);
+      if (p.cap > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = from_cap * bent(s[n][i] * to_cap);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] *= to_log2;
+      }
+      if (BIAS) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const f32x4 at = place[32 * n + 8 * (i / 4) + 4 * half + i % 4];
+          const float dx = x - at[0], dy = y - at[1], dz = z - at[2];
+          s[n][i] -= slope * __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (place[32 * n + 8 * (i / 4) + 4 * half + i % 4][3] == 0.0f) s[n][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) high = fmaxf(high, s[n][i]);
+    }
+    high = fmaxf(high, other_half(high));
+    if (__any(high > top)) {
+      const float now = fmaxf(top, high);
+      const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= shrink;
+#pragma unroll
+      for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] *= shrink;
+    }
+    // a row that has seen no key yet: every exponent is -infinity
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int n = 0; n < KT / 32; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - base);
+        sum += s[n][i];
+      }
+#pragma unroll
+      for (int c = 0; c < kLineChunks<T>; ++c) {
+        Op<T> w;
+        register_chunk(s[n], c, w);
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+          mma(column_chunk<DP>(vtile + 32 * n * kPitch<T, DP>, c, 32 * t, half), w, acc[t]);
+      }
+    }
+  }
+  if (!row.exists) return;
+  sum += other_half(sum);
+  const int64_t at = row.token * p.heads + row.head;
+  if (SPLIT) {
+    const int64_t to = (int64_t(blockIdx.z) * p.queries * p.heads + at);
+    store_columns<float, DP>(part + to * p.D, p.D, half, acc, 1.0f);
+    if (half == 0) {
+      part_stats[2 * to] = top;
+      part_stats[2 * to + 1] = sum;
+    }
+    return;
+  }
+  // a row that sees no key gives zeros
+  store_columns<T, DP>(out + at * p.D, p.D, half, acc, sum == 0.0f ? 0.0f : 1.0f / sum);
+  if (log_sums && half == 0) log_sums[at] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// Joins the parts of a row: a wave a row, a lane a column.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(const float* __restrict__ part,
+                                                             const float* __restrict__ part_stats, int parts,
+                                                             int64_t rows, int D, T* __restrict__ out,
+                                                             float* __restrict__ log_sums) {
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int k = 0; k < parts; ++k) top = fmaxf(top, part_stats[2 * (k * rows + row)]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  for (int k = 0; k < parts; ++k)
+    sum += __builtin_amdgcn_exp2f(part_stats[2 * (k * rows + row)] - base) * part_stats[2 * (k * rows + row) + 1];
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int c = lane; c < D; c += 64) {
+    float v = 0.0f;
+    for (int k = 0; k < parts; ++k)
+      v += __builtin_amdgcn_exp2f(part_stats[2 * (k * rows + row)] - base) * part[(k * rows + row) * D + c];
+    out[row * D + c] = T(v * inverse);
+  }
+  if (log_sums && lane == 0) log_sums[row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// The gradients to positions (a sum over heads) and, per workgroup, to slopes.
+__global__ __launch_bounds__(256) void attention_force_kernel(const float* __restrict__ row_part,
+                                                              const float* __restrict__ key_part, int64_t queries,
+                                                              int64_t keys, int heads, int key_heads, bool shared,
+                                                              float* __restrict__ positions,
+                                                              float* __restrict__ key_positions) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < queries + (shared ? 0 : keys);
+       i += int64_t(gridDim.x) * 256) {
+    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool row = i < queries;
+    const int64_t k = row ? i : i - queries;
+    if (row)
+      for (int h = 0; h < heads; ++h) r += *reinterpret_cast<const f32x4*>(row_part + 4 * (k * heads + h));
+    if (!row || shared)
+      for (int h = 0; h < key_heads; ++h) r += *reinterpret_cast<const f32x4*>(key_part + 4 * (k * key_heads + h));
+    float* to = (row ? positions : key_positions) + 3 * k;
+    to[0] = r[0];
+    to[1] = r[1];
+    to[2] = r[2];
+  }
+}
+
+// dslope_h: a workgroup sums its share of the tokens for every head, a lane a
+// head and a token in turn; attention_slope_kernel adds the shares in order.
+__global__ __launch_bounds__(256) void attention_slope_part_kernel(const float* __restrict__ row_part, int64_t queries,
+                                                                   int heads, float* __restrict__ part) {
+  __shared__ float sums[256];
+  const int64_t each = (queries + gridDim.x - 1) / gridDim.x;
+  const int64_t begin = int64_t(blockIdx.x) * each, end = begin + each < queries ? begin + each : queries;
+  for (int h = 0; h < heads; ++h) {
+    float s = 0.0f;
+    for (int64_t i = begin + threadIdx.x; i < end; i += 256) s += row_part[4 * (i * heads + h) + 3];
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    for (int m = 128; m > 0; m /= 2) {
+      if (int(threadIdx.x) < m) sums[threadIdx.x] += sums[threadIdx.x + m];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) part[blockIdx.x * int64_t(heads) + h] = sums[0];
+    __syncthreads();
+  }
+}
+__global__ __launch_bounds__(64) void attention_slope_kernel(const float* __restrict__ part, int groups, int heads,
+                                                             float* __restrict__ slopes) {
+  const int h = blockIdx.x;
+  float s = 0.0f;
+  for (int g = threadIdx.x; g < groups; g += 64) s += part[g * int64_t(heads) + h];
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) s += __shfl_xor(s, m);
+  if (threadIdx.x == 0) slopes[h] = s;
+}
+
+template <typename T, int DP, int NW, bool BIAS>
+int launch_forward(const ForwardPlan& f, const Problem& p, void* out, float* log_sums, void* workspace, hipStream_t s) {
+  constexpr int KT = NW > 1 && sizeof(T) == 2 ? 64 : 32;
+  float* part = static_cast<float*>(workspace);
+  float* stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + f.part_bytes);
+  const dim3 grid(unsigned(f.items), unsigned(p.key_heads), unsigned(f.parts));
+  if (!fits_grid(f.items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many rows for one launch");
+  if (f.parts == 1) {
+    hipLaunchKernelGGL((attention_kernel<T, DP, NW, KT, BIAS, false>), grid, dim3(64 * NW), 0, s, p,
+                       static_cast<T*>(out), log_sums, part, stats);
+    return check_launch("attention_kernel");
+  }
+  hipLaunchKernelGGL((attention_kernel<T, DP, NW, KT, BIAS, true>), grid, dim3(64 * NW), 0, s, p, static_cast<T*>(out),
+                     log_sums, part, stats);
+  if (int rc = check_launch("attention_kernel")) return rc;
+  const int64_t rows = p.queries * p.heads;
+  hipLaunchKernelGGL((attention_join_kernel<T>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, s, part, stats, f.parts,
+                     rows, p.D, static_cast<T*>(out), log_sums);
+  return check_launch("attention_join_kernel");
+}
+
+struct Forward {
+  const ForwardPlan& f;
+  const Problem& p;
+  void* out;
+  float* log_sums;
+  void* workspace;
+  hipStream_t s;
+  template <typename T, int DP, int NW>
+  int waves() const {
+    return p.slopes ? launch_forward<T, DP, NW, true>(f, p, out, log_sums, workspace, s)
+                    : launch_forward<T, DP, NW, false>(f, p, out, log_sums, workspace, s);
+  }
+  template <typename T, int DP>
+  int operator()() const {
+    return f.waves == 1 ? waves<T, DP, 1>() : waves<T, DP, 4>();
+  }
+};
+
+}  // namespace
+}  // namespace attention
+}  // namespace ye3t
+
+using namespace ye3t;
+using namespace ye3t::attention;
+
+extern "C" {
+
+int64_t ye3t_hip_atom_attention_workspace_bytes(const ye3t_attention_args* args) {
+  clear_error();
+  if (!args || check_attention(*args)) return -1;
+  return forward_plan(*args).bytes;
+}
+
+int ye3t_hip_atom_attention(const ye3t_attention_args* args, void* out, void* log_sums, void* workspace,
+                            int64_t workspace_bytes, ye3t_stream_t stream) {
+  clear_error();
+  YE3T_REQUIRE(args != nullptr, "attention needs arguments");
+  if (int rc = check_attention(*args)) return rc;
+  if (args->queries == 0) return YE3T_OK;
+  if (int rc = check_pointers(*args)) return rc;
+  YE3T_REQUIRE(out && args->structures > 0, "attention needs structures and an output");
+  const ForwardPlan f = forward_plan(*args);
+  YE3T_REQUIRE(f.bytes == 0 || (workspace && workspace_bytes >= f.bytes),
+               "the workspace is smaller than ye3t_hip_atom_attention_workspace_bytes");
+  const Problem p = problem_of(*args);
+  return with_width(args->dtype, p.D, Forward{f, p, out, static_cast<float*>(log_sums), workspace, as_stream(stream)});
+}
+
+int64_t ye3t_hip_atom_attention_adjoint_workspace_bytes(const ye3t_attention_args* args, int bias_gradients) {
+  clear_error();
+  if (!args || check_attention(*args)) return -1;
+  return adjoint_plan(*args, bias_gradients != 0).bytes;
+}
+
+int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void* out, const void* log_sums,
+                                    const void* out_adjoint, void* query_adjoint, void* key_adjoint,
+                                    void* value_adjoint, void* slopes_adjoint, void* positions_adjoint,
+                                    void* key_positions_adjoint, void* workspace, int64_t workspace_bytes,
+                                    ye3t_stream_t stream) {
+  clear_error();
+  YE3T_REQUIRE(args != nullptr, "attention needs arguments");
+  if (int rc = check_attention(*args)) return rc;
+  if (int rc = check_pointers(*args)) return rc;
+  const bool forces = slopes_adjoint != nullptr;
+  YE3T_REQUIRE(args->queries == 0 || (out && log_sums && out_adjoint && query_adjoint),
+               "the gradient needs the output, its sums, its adjoint and an output for the query's");
+  YE3T_REQUIRE(args->keys == 0 || (key_adjoint && value_adjoint), "the gradient needs outputs for key and value");
+  YE3T_REQUIRE(!forces || args->slopes, "gradients to slopes and positions need slopes and positions");
+  YE3T_REQUIRE(!forces || args->queries == 0 || positions_adjoint, "gradients to slopes and positions come together");
+  YE3T_REQUIRE(!forces || !args->key_positions || args->keys == 0 || key_positions_adjoint,
+               "key_positions need an output for their gradient");
+  const AdjointPlan f = adjoint_plan(*args, forces);
+  YE3T_REQUIRE(workspace && workspace_bytes >= f.bytes,
+               "the workspace is smaller than ye3t_hip_atom_attention_adjoint_workspace_bytes");
+  YE3T_REQUIRE(args->structures > 0 || (args->queries == 0 && args->keys == 0), "attention needs structures");
+  const Problem p = problem_of(*args);
+  char* work = static_cast<char*>(workspace);
+  Gradient g{};
+  g.out = out;
+  g.adjoint = out_adjoint;
+  g.log_sums = static_cast<const float*>(log_sums);
+  g.along = reinterpret_cast<float*>(work);
+  g.dq = query_adjoint;
+  g.dk = key_adjoint;
+  g.dv = value_adjoint;
+  g.row_part = reinterpret_cast<float*>(work + f.along_bytes);
+  g.key_part = reinterpret_cast<float*>(work + f.along_bytes + f.row_bytes);
+  float* slope_part = reinterpret_cast<float*>(work + f.along_bytes + f.row_bytes + f.key_bytes);
+  const hipStream_t s = as_stream(stream);
+  if (p.queries > 0)
+    if (int rc = launch_row_gradient(args->dtype, f, p, g, forces, s)) return rc;
+  if (p.keys > 0)
+    if (int rc = launch_key_gradient(args->dtype, f, p, g, forces, s)) return rc;
+  if (!forces) return YE3T_OK;
+  const bool shared = p.key_positions == nullptr;
+  const int64_t atoms = p.queries + (shared ? 0 : p.keys);
+  if (atoms > 0) {
+    const int64_t groups = (atoms + 255) / 256;
+    hipLaunchKernelGGL(attention_force_kernel, dim3(unsigned(groups)), dim3(256), 0, s, g.row_part, g.key_part,
+                       p.queries, p.keys, p.heads, p.key_heads, shared, static_cast<float*>(positions_adjoint),
+                       static_cast<float*>(key_positions_adjoint));
+    if (int rc = check_launch("attention_force_kernel")) return rc;
+  }
+  hipLaunchKernelGGL(attention_slope_part_kernel, dim3(kSlopeGroups), dim3(256), 0, s, g.row_part, p.queries, p.heads,
+                     slope_part);
+  if (int rc = check_launch("attention_slope_part_kernel")) return rc;
+  hipLaunchKernelGGL(attention_slope_kernel, dim3(unsigned(p.heads)), dim3(64), 0, s, slope_part, kSlopeGroups, p.heads,
+                     static_cast<float*>(slopes_adjoint));
+  return check_launch("attention_slope_kernel");
+}
+
+}  // extern "C"

@@ -1,0 +1,161 @@
+// Gradient of atom attention, key side.
+#include "attention.h"
+
+namespace ye3t {
+namespace attention {
+namespace {
+
+// Key side: dk, dv and the key's part of the gradient to its position.  A wave
+// owns 32 keys and walks over the rows of its key head in tiles of 32.
+template <typename T, int DP, int NW, bool BIAS, bool FORCES>
+__global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem p, Gradient g) {
+  constexpr int TILE = 32 * NW, RT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
+  __shared__ __align__(16) T qtile[RT * kPitch<T, DP>];
+  __shared__ __align__(16) T gtile[RT * kPitch<T, DP>];
+  __shared__ f32x4 place[RT];  // x, y, z, slope
+  __shared__ f32x4 stats[RT];  // log sum, D_i, whether the row counts
+  const Item item = item_of(p.key_offsets, p.structures, p.keys, 1, TILE, blockIdx.x);
+  const Span key = span_of(p.key_offsets, item.structure, p.keys);
+  if (item.first < 0 || item.first >= key.length) return;
+  const Span own = span_of(p.offsets, item.structure, p.queries);
+  const int64_t rows = int64_t(own.length) * p.group;
+  const int key_head = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int mine = int(item.first) + 32 * wave + (lane & 31);
+  const bool exists = mine < key.length;
+  const bool busy = int(item.first) + 32 * wave < key.length;
+  const int64_t token = key.begin + mine;
+  const f32x4 here = key_place<BIAS>(p, token, exists);
+  const bool seen = here[3] != 0.0f;
+  Op<T> k[NU], v[NU];
+  line_operand<T, DP>(seen ? static_cast<const T*>(p.k) + token * p.k_row + key_head * p.k_head : nullptr, p.D, half, k);
+  line_operand<T, DP>(seen ? static_cast<const T*>(p.v) + token * p.v_row + key_head * p.v_head : nullptr, p.D, half, v);
+
+  Staged<T, DP, RT, 64 * NW> qs, gs;
+  f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f}, next_stats = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto fetch = [&](int64_t r0) {
+    qs.load(p.D, [&](int line) {
+      const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
+      return r.exists ? static_cast<const T*>(p.q) + r.token * p.q_row + r.head * p.q_head : nullptr;
+    });
+    gs.load(p.D, [&](int line) {
+      const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
+      return r.exists ? static_cast<const T*>(g.adjoint) + (r.token * p.heads + r.head) * p.D : nullptr;
+    });
+    if (int(threadIdx.x) < RT) {
+      const Row r = row_of(p, own.begin, r0 + int(threadIdx.x), rows, key_head);
+      next_place = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      next_stats = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (r.exists) {
+        const int64_t at = r.token * p.heads + r.head;
+        const float log_sum = g.log_sums[at];
+        if (log_sum != -INFINITY) next_stats = f32x4{log_sum * kLog2e, g.along[at], 1.0f, 0.0f};
+        if (BIAS)
+          next_place = f32x4{p.positions[3 * r.token], p.positions[3 * r.token + 1], p.positions[3 * r.token + 2],
+                             p.slopes[r.head] * kLog2e};
+      }
+    }
+  };
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
+  float gx = 0.0f, gy = 0.0f, gz = 0.0f;
+  if (qs.AHEAD && rows > 0) fetch(0);
+  for (int64_t r0 = 0; r0 < rows; r0 += RT) {
+    __syncthreads();
+    if (!qs.AHEAD) fetch(r0);
+    qs.write(qtile);
+    gs.write(gtile);
+    if (int(threadIdx.x) < RT) {
+      place[threadIdx.x] = next_place;
+      stats[threadIdx.x] = next_stats;
+    }
+    __syncthreads();
+    if (qs.AHEAD && r0 + RT < rows) fetch(r0 + RT);
+    if (!busy) continue;
+    f32x16 s = zeros(), dp = zeros();
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      mma(line_chunk<T, DP>(qtile, lane & 31, u, half), k[u], s);
+      mma(line_chunk<T, DP>(gtile, lane & 31, u, half), v[u], dp);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int line = 8 * (i / 4) + 4 * half + i % 4;
+      const f32x4 st = stats[line];
+      float dx = 0.0f, dy = 0.0f, dz = 0.0f, distance = 0.0f, slope = 0.0f;
+      if (BIAS) {
+        const f32x4 r = place[line];
+        dx = here[0] - r[0], dy = here[1] - r[1], dz = here[2] - r[2], slope = r[3];
+        distance = __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+      }
+      const Weight w = weight_of<BIAS>(p, s[i], st[0], slope, distance, seen && st[2] != 0.0f);
+      const float tilt = w.p * (dp[i] - st[1]);
+      s[i] = tilt * w.slant;
+      dp[i] = w.p;
+      if (FORCES) {
+        const float pull = distance > 0.0f ? -tilt * slope / distance : 0.0f;
+        gx += pull * dx;
+        gy += pull * dy;
+        gz += pull * dz;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kLineChunks<T>; ++c) {
+      Op<T> ds, w;
+      register_chunk(s, c, ds);
+      register_chunk(dp, c, w);
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        mma(column_chunk<DP>(qtile, c, 32 * t, half), ds, dk[t]);
+        mma(column_chunk<DP>(gtile, c, 32 * t, half), w, dv[t]);
+      }
+    }
+  }
+  if (!exists) return;
+  const int64_t at = token * p.key_heads + key_head;
+  store_columns<T, DP>(static_cast<T*>(g.dk) + at * p.D, p.D, half, dk, p.scale);
+  store_columns<T, DP>(static_cast<T*>(g.dv) + at * p.D, p.D, half, dv, 1.0f);
+  if (FORCES) {
+    f32x4 r = {gx, gy, gz, 0.0f};
+#pragma unroll
+    for (int a = 0; a < 3; ++a) r[a] = (r[a] + other_half(r[a])) * kLn2;  // the slope was in units of log2
+    if (half == 0) *reinterpret_cast<f32x4*>(g.key_part + 4 * at) = r;
+  }
+}
+
+template <typename T, int DP, int NW, bool BIAS, bool FORCES>
+int launch_keys(const AdjointPlan& f, const Problem& p, const Gradient& g, hipStream_t s) {
+  if (!fits_grid(f.key_items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many keys for one launch");
+  hipLaunchKernelGGL((attention_key_gradient_kernel<T, DP, NW, BIAS, FORCES>),
+                     dim3(unsigned(f.key_items), unsigned(p.key_heads)), dim3(64 * NW), 0, s, p, g);
+  return check_launch("attention_key_gradient_kernel");
+}
+
+struct Side {
+  const AdjointPlan& f;
+  const Problem& p;
+  const Gradient& g;
+  bool forces;
+  hipStream_t s;
+  template <typename T, int DP, int NW>
+  int waves() const {
+    return forces ? launch_keys<T, DP, NW, true, true>(f, p, g, s)
+                  : p.slopes ? launch_keys<T, DP, NW, true, false>(f, p, g, s)
+                             : launch_keys<T, DP, NW, false, false>(f, p, g, s);
+  }
+  template <typename T, int DP>
+  int operator()() const {
+    return f.key_waves == 1 ? waves<T, DP, 1>() : waves<T, DP, 4>();
+  }
+};
+
+}  // namespace
+
+int launch_key_gradient(int dtype, const AdjointPlan& f, const Problem& p, const Gradient& g, bool forces,
+                        hipStream_t s) {
+  return with_width(dtype, p.D, Side{f, p, g, forces, s});
+}
+
+}  // namespace attention
+}  // namespace ye3t

@@ -1,0 +1,442 @@
+// Root-mean-square norm of feature rows with the residual's addition, its
+// gradient, and its rows in 8 bits.
+//
+//   h = x + r,   rho = (mean(h^2) + epsilon)^(-1/2),   y = h rho w
+//   u = g w,     dh = rho (u - h rho^2 mean(u h)) + gh,   dw = sum over rows of g h rho
+//
+// Bound by memory: a value is read and written once and takes a dozen
+// operations.  A row is held in the registers of a group of L lanes (4, 16 or
+// 64 lanes of a wave, or four waves), K chunks of 16 bytes a lane, so that the
+// mean and the output come from one read; rows wider than four waves hold are
+// read again for the output.  h, the means and the weight's sums are fp32; h
+// and y are each rounded once, from the unrounded sum.
+#include "rows.h"
+
+namespace ye3t {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kScaleGroup = 128;  // columns that share a scale of the 8-bit rows
+constexpr float kLargest8 = 448.0f;
+
+// Sum over the L lanes that share a row; every lane gets the same bits.
+template <int L>
+__device__ inline float row_sum(float v, float* part) {
+#pragma unroll
+  for (int m = 1; m < (L < 64 ? L : 64); m *= 2) v += __shfl_xor(v, m);
+  if constexpr (L > 64) {
+    __syncthreads();  // the last sum's parts have been read
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < L / 64; ++w) v += part[w];
+  }
+  return v;
+}
+
+enum { kPlain = 0, kEightBit = 1 };
+
+// K: chunks a lane holds; 0: any number, the row is read twice.
+template <typename T, int L, int K, int MODE>
+__global__ __launch_bounds__(kThreads) void rms_norm_kernel(const T* __restrict__ x, const T* __restrict__ residual,
+                                                            const T* __restrict__ weight, int64_t rows, int W,
+                                                            float epsilon, T* __restrict__ total, T* __restrict__ y,
+                                                            uint8_t* __restrict__ codes, float* __restrict__ scales) {
+  constexpr int V = kChunk<T>;
+  constexpr int H = K > 0 ? K : 1;
+  __shared__ float part[kThreads / 64];
+  const int lane = int(threadIdx.x) % L, per = kThreads / L;
+  const int groups = (W + kScaleGroup - 1) / kScaleGroup;
+  for (int64_t row = int64_t(blockIdx.x) * per + int(threadIdx.x) / L; row < rows; row += int64_t(gridDim.x) * per) {
+    const T* xr = x + row * W;
+    const T* rr = residual ? residual + row * W : nullptr;
+    T* tr = total ? total + row * W : nullptr;
+    float h[H][V];
+    auto sum_of = [&](int c, float* out) {
+      const Chunk<T, V> a = Chunk<T, V>::load(xr + c, W - c);
+#pragma unroll
+      for (int q = 0; q < V; ++q) out[q] = float(a.v[q]);
+      if (rr) {
+        const Chunk<T, V> b = Chunk<T, V>::load(rr + c, W - c);
+#pragma unroll
+        for (int q = 0; q < V; ++q) out[q] += float(b.v[q]);
+      }
+    };
+    auto keep_total = [&](int c, const float* v) {
+      if (!tr) return;
+      Chunk<T, V> a;
+#pragma unroll
+      for (int q = 0; q < V; ++q) a.v[q] = T(v[q]);
+      a.store(tr + c, W - c);
+    };
+    float square = 0.0f;
+#pragma unroll
+    for (int k = 0, c = lane * V; K > 0 ? k < K : c < W; ++k, c += L * V) {
+      float* v = h[K > 0 ? k : 0];
+      if (c < W) {
+        sum_of(c, v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < V; ++q) square += v[q] * v[q];
+    }
+    square = row_sum<L>(square, part);
+    const float rho = 1.0f / sqrtf(square / float(W) + epsilon);
+#pragma unroll
+    for (int k = 0, c = lane * V; K > 0 ? k < K : c < (W + L * V - 1) / (L * V) * (L * V); ++k, c += L * V) {
+      float* v = h[K > 0 ? k : 0];
+      if (K == 0) {
+        if (c < W) {
+          sum_of(c, v);
+        } else {
+#pragma unroll
+          for (int q = 0; q < V; ++q) v[q] = 0.0f;
+        }
+      }
+      float out[V];
+      if (c < W) {
+        keep_total(c, v);
+        const Chunk<T, V> w = Chunk<T, V>::load(weight + c, W - c);
+#pragma unroll
+        for (int q = 0; q < V; ++q) out[q] = v[q] * rho * float(w.v[q]);
+        if constexpr (MODE == kPlain) {
+          Chunk<T, V> a;
+#pragma unroll
+          for (int q = 0; q < V; ++q) a.v[q] = T(out[q]);
+          a.store(y + row * W + c, W - c);
+        }
+      }
+      if constexpr (MODE == kEightBit) {
+        // The 128 columns of a scale are 128 / V neighbouring lanes of a step.
+        float top = 0.0f;
+        if (c < W) {
+#pragma unroll
+          for (int q = 0; q < V; ++q) top = fmaxf(top, fabsf(out[q]));
+        }
+#pragma unroll
+        for (int m = 1; m < kScaleGroup / V; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
+        if (c < W) {
+          const float scale = top / kLargest8;
+          if (c % kScaleGroup == 0) scales[row * groups + c / kScaleGroup] = scale;
+          uint32_t packed[V / 4];
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            // a group of zeros has scale 0 and codes 0; what is not a number stays so
+            out[q] = scale > 0.0f ? out[q] / scale : out[q];
+            out[q] = out[q] > kLargest8 ? kLargest8 : (out[q] < -kLargest8 ? -kLargest8 : out[q]);
+          }
+#pragma unroll
+          for (int q = 0; q < V / 4; ++q) {
+            int word = 0;
+            word = __builtin_amdgcn_cvt_pk_fp8_f32(out[4 * q], out[4 * q + 1], word, false);
+            word = __builtin_amdgcn_cvt_pk_fp8_f32(out[4 * q + 2], out[4 * q + 3], word, true);
+            packed[q] = uint32_t(word);
+          }
+          Chunk<uint8_t, V> a;
+#pragma unroll
+          for (int q = 0; q < V; ++q) a.v[q] = uint8_t(packed[q / 4] >> (8 * (q % 4)));
+          a.store(codes + row * W + c, W - c);
+        }
+      }
+    }
+  }
+}
+
+// The gradient: a workgroup walks over rows and keeps its sums of the weight's
+// gradient, a lane those of its own columns; they are added over the
+// workgroup's groups and written as one of `gridDim.x` partial rows, which
+// rms_norm_weight_kernel adds in order.  K = 0: the row is read twice and the
+// sums stand in the workgroup's own partial row in memory, where each column
+// belongs to one lane.
+template <typename T, int L, int K>
+__global__ __launch_bounds__(kThreads) void rms_norm_adjoint_kernel(const T* __restrict__ adjoint,
+                                                                    const T* __restrict__ total_adjoint,
+                                                                    const T* __restrict__ total,
+                                                                    const T* __restrict__ weight, int64_t rows, int W,
+                                                                    float epsilon, T* __restrict__ dx,
+                                                                    float* __restrict__ partial) {
+  constexpr int V = kChunk<T>;
+  constexpr int H = K > 0 ? K : 1;
+  constexpr int per = kThreads / L;
+  __shared__ float part[kThreads / 64];
+  __shared__ float shared_dw[K > 0 && per > 1 ? L * K * V : 1];
+  const int lane = int(threadIdx.x) % L;
+  const int group = int(threadIdx.x) / L;
+  float* mine = partial + int64_t(blockIdx.x) * W;
+  float dw[H][V];
+#pragma unroll
+  for (int k = 0; k < H; ++k)
+#pragma unroll
+    for (int q = 0; q < V; ++q) dw[k][q] = 0.0f;
+  if (K == 0) {
+    for (int c = threadIdx.x; c < W; c += kThreads) mine[c] = 0.0f;
+    __syncthreads();
+  }
+  for (int64_t row = int64_t(blockIdx.x) * per + group; row < rows; row += int64_t(gridDim.x) * per) {
+    const T* hr = total + row * W;
+    const T* gr = adjoint + row * W;
+    const T* tr = total_adjoint ? total_adjoint + row * W : nullptr;
+    float h[H][V], g[H][V];
+    float square = 0.0f, along = 0.0f;
+    auto read = [&](int c, float* hv, float* gv) {
+      const Chunk<T, V> a = Chunk<T, V>::load(hr + c, W - c), b = Chunk<T, V>::load(gr + c, W - c);
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        hv[q] = float(a.v[q]);
+        gv[q] = float(b.v[q]);
+      }
+    };
+#pragma unroll
+    for (int k = 0, c = lane * V; K > 0 ? k < K : c < W; ++k, c += L * V) {
+      float *hv = h[K > 0 ? k : 0], *gv = g[K > 0 ? k : 0];
+      if (c < W) {
+        read(c, hv, gv);
+        const Chunk<T, V> w = Chunk<T, V>::load(weight + c, W - c);
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          square += hv[q] * hv[q];
+          along += hv[q] * (gv[q] * float(w.v[q]));
+        }
+      }
+    }
+    square = row_sum<L>(square, part);
+    along = row_sum<L>(along, part);
+    const float rho = 1.0f / sqrtf(square / float(W) + epsilon);
+    const float pull = along / float(W) * rho * rho;
+#pragma unroll
+    for (int k = 0, c = lane * V; K > 0 ? k < K : c < W; ++k, c += L * V) {
+      float *hv = h[K > 0 ? k : 0], *gv = g[K > 0 ? k : 0];
+      if (c >= W) continue;
+      if (K == 0) read(c, hv, gv);
+      const Chunk<T, V> w = Chunk<T, V>::load(weight + c, W - c);
+      Chunk<T, V> t = Chunk<T, V>::zero();
+      if (tr) t = Chunk<T, V>::load(tr + c, W - c);
+      Chunk<T, V> a;
+#pragma unroll
+      for (int q = 0; q < V; ++q) a.v[q] = T(rho * (gv[q] * float(w.v[q]) - hv[q] * pull) + float(t.v[q]));
+      a.store(dx + row * W + c, W - c);
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const float part_dw = gv[q] * hv[q] * rho;
+        if (K > 0) dw[k][q] += part_dw;
+        else if (c + q < W) mine[c + q] += part_dw;
+      }
+    }
+  }
+  if constexpr (K > 0) {
+    // groups in turn, so that the order of the sums is fixed
+    for (int turn = 0; turn < per; ++turn) {
+      if (group == turn) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int c = (k * L + lane) * V;
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            if (per > 1) {
+              float& s = shared_dw[c + q];
+              s = turn == 0 ? dw[k][q] : s + dw[k][q];
+              if (turn == per - 1 && c + q < W) mine[c + q] = s;
+            } else if (c + q < W) {
+              mine[c + q] = dw[k][q];
+            }
+          }
+        }
+      }
+      if (per > 1) __syncthreads();
+    }
+  }
+}
+
+// dw[c] = sum of the partial rows' column c: a lane a column, sixteen waves
+// over the rows, their sums added in order.
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float* __restrict__ partial, int count, int W,
+                                                               T* __restrict__ dw) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = int(blockIdx.x) * 64 + lane;
+  float s = 0.0f;
+  if (c < W)
+    for (int p = wave; p < count; p += 16) s += partial[int64_t(p) * W + c];
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < W) {
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t += sums[w][lane];
+    dw[c] = T(t);
+  }
+}
+
+// Workgroups that fill the card: eight of four waves in a compute unit.
+inline int resident_groups(int64_t wanted) { return int(wanted < 2048 ? (wanted < 1 ? 1 : wanted) : 2048); }
+
+// Partial rows of the weight's gradient: fewer for wide rows, so that they stay
+// a small part of the traffic.
+inline int partial_rows(int64_t rows, int per) {
+  int64_t n = (rows + per - 1) / per;
+  return int(n < 1024 ? (n < 1 ? 1 : n) : 1024);
+}
+
+struct Shape {
+  int L, K;
+};
+
+// The group and the chunks of a row of `width` values: the smallest group that
+// holds it in at most eight chunks of 16 bytes a lane (four for the gradient,
+// which keeps three values for each); 0 chunks where 256 lanes do not.
+inline Shape shape_of(int width, int V, int most, int least) {
+  const int lanes[4] = {4, 16, 64, 256};
+  for (int i = 0; i < 4; ++i) {
+    if (lanes[i] < least) continue;
+    const int limit = lanes[i] < 64 ? 2 : most;
+    const int k = (width + lanes[i] * V - 1) / (lanes[i] * V);
+    if (k <= limit) return {lanes[i], k <= 1 ? 1 : k <= 2 ? 2 : k <= 4 ? 4 : 8};
+  }
+  return {256, 0};
+}
+
+template <typename T, int L, int K, int MODE>
+int forward_as(const void* x, const void* r, const void* w, int64_t rows, int W, float eps, void* total, void* y,
+               void* codes, void* scales, hipStream_t s) {
+  constexpr int per = kThreads / L;
+  const dim3 grid(resident_groups((rows + per - 1) / per));
+  hipLaunchKernelGGL((rms_norm_kernel<T, L, K, MODE>), grid, dim3(kThreads), 0, s, static_cast<const T*>(x),
+                     static_cast<const T*>(r), static_cast<const T*>(w), rows, W, eps, static_cast<T*>(total),
+                     static_cast<T*>(y), static_cast<uint8_t*>(codes), static_cast<float*>(scales));
+  return check_launch(MODE == kEightBit ? "rms_norm_8bit_kernel" : "rms_norm_kernel");
+}
+
+template <typename T, int MODE, typename... A>
+int forward_shaped(Shape sh, A... a) {
+  if constexpr (MODE == kPlain) {
+    if (sh.L == 4) return sh.K == 1 ? forward_as<T, 4, 1, MODE>(a...) : forward_as<T, 4, 2, MODE>(a...);
+    if (sh.L == 16) return sh.K == 1 ? forward_as<T, 16, 1, MODE>(a...) : forward_as<T, 16, 2, MODE>(a...);
+  }
+  if (sh.L == 64) {
+    if (sh.K == 1) return forward_as<T, 64, 1, MODE>(a...);
+    if (sh.K == 2) return forward_as<T, 64, 2, MODE>(a...);
+    if (sh.K == 4) return forward_as<T, 64, 4, MODE>(a...);
+    return forward_as<T, 64, 8, MODE>(a...);
+  }
+  if (sh.K == 1) return forward_as<T, 256, 1, MODE>(a...);
+  if (sh.K == 2) return forward_as<T, 256, 2, MODE>(a...);
+  if (sh.K == 4) return forward_as<T, 256, 4, MODE>(a...);
+  if (sh.K == 8) return forward_as<T, 256, 8, MODE>(a...);
+  return forward_as<T, 256, 0, MODE>(a...);
+}
+
+template <typename T, int L, int K>
+int adjoint_as(const void* g, const void* tg, const void* h, const void* w, int64_t rows, int W, float eps, void* dx,
+               void* dw, void* workspace, hipStream_t s) {
+  const int count = partial_rows(rows, kThreads / L);
+  float* partial = static_cast<float*>(workspace);
+  hipLaunchKernelGGL((rms_norm_adjoint_kernel<T, L, K>), dim3(count), dim3(kThreads), 0, s, static_cast<const T*>(g),
+                     static_cast<const T*>(tg), static_cast<const T*>(h), static_cast<const T*>(w), rows, W, eps,
+                     static_cast<T*>(dx), partial);
+  if (int rc = check_launch("rms_norm_adjoint_kernel")) return rc;
+  hipLaunchKernelGGL((rms_norm_weight_kernel<T>), dim3((W + 63) / 64), dim3(1024), 0, s, partial, count, W,
+                     static_cast<T*>(dw));
+  return check_launch("rms_norm_weight_kernel");
+}
+
+template <typename T, typename... A>
+int adjoint_shaped(Shape sh, A... a) {
+  if (sh.L == 4) return sh.K == 1 ? adjoint_as<T, 4, 1>(a...) : adjoint_as<T, 4, 2>(a...);
+  if (sh.L == 16) return sh.K == 1 ? adjoint_as<T, 16, 1>(a...) : adjoint_as<T, 16, 2>(a...);
+  if (sh.L == 64) {
+    if (sh.K == 1) return adjoint_as<T, 64, 1>(a...);
+    if (sh.K == 2) return adjoint_as<T, 64, 2>(a...);
+    return adjoint_as<T, 64, 4>(a...);
+  }
+  if (sh.K == 1) return adjoint_as<T, 256, 1>(a...);
+  if (sh.K == 2) return adjoint_as<T, 256, 2>(a...);
+  if (sh.K == 4) return adjoint_as<T, 256, 4>(a...);
+  return adjoint_as<T, 256, 0>(a...);
+}
+
+int check_norm(int dtype, int64_t rows, int64_t width, double epsilon) {
+  YE3T_REQUIRE(rows >= 0 && width >= 1, "rows and width must be positive");
+  YE3T_REQUIRE(width <= (1 << 24), "rows of more than 2^24 values are not supported");
+  YE3T_REQUIRE(epsilon > 0.0, "epsilon must be positive");
+  if (dtype != YE3T_F32 && dtype != YE3T_BF16)
+    return set_error(YE3T_EDTYPE, "unsupported dtype %d; expected float32 or bfloat16", dtype);
+  return YE3T_OK;
+}
+
+inline Shape adjoint_shape(int dtype, int64_t width) {
+  return shape_of(int(width), dtype == YE3T_F32 ? kChunk<float> : kChunk<__bf16>, 4, 1);
+}
+
+}  // namespace
+}  // namespace ye3t
+
+using namespace ye3t;
+
+extern "C" {
+
+int ye3t_hip_rms_norm(int dtype, const void* x, const void* residual, const void* weight, int64_t rows, int64_t width,
+                      double epsilon, void* total, void* y, ye3t_stream_t stream) {
+  clear_error();
+  if (int rc = check_norm(dtype, rows, width, epsilon)) return rc;
+  if (rows == 0) return YE3T_OK;
+  YE3T_REQUIRE(x && weight && y, "the norm needs rows, a weight and an output");
+  YE3T_REQUIRE(!residual || total, "a residual needs an output for the sum");
+  const int W = int(width);
+  const float eps = float(epsilon);
+  void* none = nullptr;
+  if (dtype == YE3T_F32)
+    return forward_shaped<float, kPlain>(shape_of(W, kChunk<float>, 8, 1), x, residual, weight, rows, W, eps, total, y,
+                                         none, none, as_stream(stream));
+  return forward_shaped<__bf16, kPlain>(shape_of(W, kChunk<__bf16>, 8, 1), x, residual, weight, rows, W, eps, total, y,
+                                        none, none, as_stream(stream));
+}
+
+int ye3t_hip_rms_norm_8bit(int dtype, const void* x, const void* residual, const void* weight, int64_t rows,
+                           int64_t width, double epsilon, void* total, void* codes, void* scales,
+                           ye3t_stream_t stream) {
+  clear_error();
+  if (int rc = check_norm(dtype, rows, width, epsilon)) return rc;
+  if (rows == 0) return YE3T_OK;
+  YE3T_REQUIRE(x && weight && codes && scales, "the norm needs rows, a weight, codes and scales");
+  YE3T_REQUIRE(!residual || total, "a residual needs an output for the sum");
+  const int W = int(width);
+  const float eps = float(epsilon);
+  void* none = nullptr;
+  // a scale's 128 columns lie in one wave: 32 lanes in fp32
+  if (dtype == YE3T_F32)
+    return forward_shaped<float, kEightBit>(shape_of(W, kChunk<float>, 8, 64), x, residual, weight, rows, W, eps, total,
+                                            none, codes, scales, as_stream(stream));
+  return forward_shaped<__bf16, kEightBit>(shape_of(W, kChunk<__bf16>, 8, 64), x, residual, weight, rows, W, eps, total,
+                                           none, codes, scales, as_stream(stream));
+}
+
+int64_t ye3t_hip_rms_norm_adjoint_workspace_bytes(int dtype, int64_t rows, int64_t width) {
+  clear_error();
+  if (check_norm(dtype, rows, width, 1.0)) return -1;
+  return int64_t(partial_rows(rows, kThreads / adjoint_shape(dtype, width).L)) * width * int64_t(sizeof(float));
+}
+
+int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_adjoint, const void* total,
+                              const void* weight, int64_t rows, int64_t width, double epsilon, void* x_adjoint,
+                              void* weight_adjoint, void* workspace, int64_t workspace_bytes, ye3t_stream_t stream) {
+  clear_error();
+  if (int rc = check_norm(dtype, rows, width, epsilon)) return rc;
+  YE3T_REQUIRE(weight && weight_adjoint, "the gradient needs the weight and an output for its gradient");
+  YE3T_REQUIRE(rows == 0 || (adjoint && total && x_adjoint), "the gradient needs the adjoint, the sum and an output");
+  YE3T_REQUIRE(workspace && workspace_bytes >= ye3t_hip_rms_norm_adjoint_workspace_bytes(dtype, rows, width),
+               "the workspace is smaller than ye3t_hip_rms_norm_adjoint_workspace_bytes");
+  const Shape sh = adjoint_shape(dtype, width);
+  const int W = int(width);
+  const float eps = float(epsilon);
+  if (dtype == YE3T_F32)
+    return adjoint_shaped<float>(sh, adjoint, total_adjoint, total, weight, rows, W, eps, x_adjoint, weight_adjoint,
+                                 workspace, as_stream(stream));
+  return adjoint_shaped<__bf16>(sh, adjoint, total_adjoint, total, weight, rows, W, eps, x_adjoint, weight_adjoint,
+                                workspace, as_stream(stream));
+}
+
+}  // extern "C"

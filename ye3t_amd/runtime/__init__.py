@@ -50,6 +50,13 @@ FUSED_OPERATIONS = (
     "ace_product_linear",
     "evaluate_factorized_schedule",
     "neighbor_list",
+    "embedding",
+    "embedding_adjoint",
+    "rms_norm",
+    "rms_norm_adjoint",
+    "rms_norm_8bit",
+    "atom_attention",
+    "atom_attention_adjoint",
 )
 HIP_OPERATIONS = REFERENCE_OPERATIONS + FUSED_OPERATIONS
 
@@ -686,6 +693,11 @@ def __getattr__(name):
         import importlib
 
         return getattr(importlib.import_module("ye3t_amd.runtime.dag"), name)
+    if name in ("embedding", "embedding_adjoint", "rms_norm", "rms_norm_8bit", "rms_norm_adjoint", "atom_attention",
+                "atom_attention_adjoint"):
+        import importlib
+
+        return getattr(importlib.import_module("ye3t_amd.runtime.atoms"), name)
     if name in ("ExecutionPlan", "YE3TExecutionPlan"):
         from ye3t_amd.runtime.execution_plan import ExecutionPlan
 

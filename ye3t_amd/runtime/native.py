@@ -12,10 +12,10 @@ import numpy as np
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "libye3t_hip.so")
-ABI_VERSION = 62
+ABI_VERSION = 63
 _LIB = None
 
-F32, F64 = 0, 1
+F32, F64, BF16 = 0, 1, 4
 EUNSUPPORTED = -5
 
 _vp = ctypes.c_void_p
@@ -76,6 +76,16 @@ class CellGrid(ctypes.Structure):
 class IndexCheck(ctypes.Structure):
     _fields_ = [("data", _vp), ("count", _i64), ("first", _i64), ("limit", _i64), ("width", ctypes.c_int),
                 ("ordered", ctypes.c_int)]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int)] + \
+        [(n, _i64) for n in ("queries", "keys", "structures", "heads", "key_heads", "head_width")] + \
+        [(n, _vp) for n in ("query", "key", "value")] + \
+        [(n, _i64) for n in ("query_row_stride", "query_head_stride", "key_row_stride", "key_head_stride",
+                             "value_row_stride", "value_head_stride")] + \
+        [("offsets", _vp), ("key_offsets", _vp), ("scale", ctypes.c_double), ("cap", ctypes.c_double)] + \
+        [(n, _vp) for n in ("slopes", "positions", "key_positions", "key_mask")]
 
 
 class Caps(ctypes.Structure):
@@ -199,6 +209,24 @@ def lib():
                                           _i64, _vp, _vp]
     L.ye3t_hip_neighbor_fill.argtypes = [ctypes.c_int, _i64, ctypes.POINTER(CellGrid), ctypes.c_double, _vp, _i64,
                                          _vp, _i64, _vp, _vp, _vp, _vp]
+    L.ye3t_hip_embedding.argtypes = [ctypes.c_int, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _i64, ctypes.c_double,
+                                     _vp, _vp]
+    L.ye3t_hip_embedding_adjoint_workspace_bytes.argtypes = [ctypes.c_int, _i64, _i64, _i64]
+    L.ye3t_hip_embedding_adjoint_workspace_bytes.restype = _i64
+    L.ye3t_hip_embedding_adjoint.argtypes = [ctypes.c_int, _vp, _vp, ctypes.c_int, _i64, _i64, _i64, ctypes.c_double,
+                                             _vp, _vp, _i64, _vp]
+    L.ye3t_hip_rms_norm.argtypes = [ctypes.c_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp, _vp, _vp]
+    L.ye3t_hip_rms_norm_8bit.argtypes = [ctypes.c_int, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp, _vp, _vp, _vp]
+    L.ye3t_hip_rms_norm_adjoint_workspace_bytes.argtypes = [ctypes.c_int, _i64, _i64]
+    L.ye3t_hip_rms_norm_adjoint_workspace_bytes.restype = _i64
+    L.ye3t_hip_rms_norm_adjoint.argtypes = [ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp, _vp,
+                                            _vp, _i64, _vp]
+    L.ye3t_hip_atom_attention_workspace_bytes.argtypes = [ctypes.POINTER(AttentionArgs)]
+    L.ye3t_hip_atom_attention_workspace_bytes.restype = _i64
+    L.ye3t_hip_atom_attention.argtypes = [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp, _i64, _vp]
+    L.ye3t_hip_atom_attention_adjoint_workspace_bytes.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_int]
+    L.ye3t_hip_atom_attention_adjoint_workspace_bytes.restype = _i64
+    L.ye3t_hip_atom_attention_adjoint.argtypes = [ctypes.POINTER(AttentionArgs)] + [_vp] * 10 + [_i64, _vp]
     version = L.ye3t_hip_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"ye3t_hip ABI {version} does not match the bindings ({ABI_VERSION})")
@@ -235,6 +263,10 @@ EXPORTED_SYMBOLS = (
     "ye3t_hip_symmetric_power_shared_sparse_monomial_double_backward", "ye3t_hip_code_object_kernel_info",
     "ye3t_hip_part_private_limit", "ye3t_hip_check_indices",
     "ye3t_hip_csr_offsets", "ye3t_hip_position_bounds", "ye3t_hip_last_kernel",
+    "ye3t_hip_embedding", "ye3t_hip_embedding_adjoint_workspace_bytes", "ye3t_hip_embedding_adjoint",
+    "ye3t_hip_rms_norm", "ye3t_hip_rms_norm_8bit", "ye3t_hip_rms_norm_adjoint_workspace_bytes",
+    "ye3t_hip_rms_norm_adjoint", "ye3t_hip_atom_attention_workspace_bytes", "ye3t_hip_atom_attention",
+    "ye3t_hip_atom_attention_adjoint_workspace_bytes", "ye3t_hip_atom_attention_adjoint",
 )
 
 
@@ -1864,3 +1896,182 @@ class FactorizedAngularSegmentedPlanHandle:
                                                                    _dev(out, "adjoint"), _stream()),
                "ye3t_hip_factorized_angular_segmented_adjoint")
         return out
+
+
+# ---- embedding, norm and attention (ye3t_amd.runtime.atoms checks the arguments) ----
+
+def _storage_code(dtype, double=False):
+    """ABI code of a storage type of these operators."""
+    import torch
+
+    if dtype == torch.float32:
+        return F32
+    if dtype == torch.bfloat16:
+        return BF16
+    if double and dtype == torch.float64:
+        return F64
+    raise TypeError(f"unsupported dtype {dtype}; expected float32{', float64' if double else ''} or bfloat16")
+
+
+def _workspace(size, what, device):
+    """``size`` bytes of device memory, of the caching allocator on the current stream."""
+    import torch
+
+    if size < 0:
+        _check(-1, what)
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def embedding(tokens, table, scale):
+    """``ye3t_hip_embedding`` of contiguous ``tokens``; the table's rows may be strided."""
+    import torch
+
+    code = _storage_code(table.dtype, True)
+    V, W = (int(x) for x in table.shape)
+    out = torch.empty((*tokens.shape, W), dtype=table.dtype, device=table.device)
+    if out.numel() == 0:
+        return out
+    if (table.stride(1) != 1 and W > 1) or table.stride(0) < 0:
+        table = table.contiguous()
+    with torch.cuda.device(table.device):
+        _check(lib().ye3t_hip_embedding(code, _dev(tokens, "tokens"), tokens.element_size(), tokens.numel(),
+                                        table.data_ptr(), table.stride(0), V, W, scale, out.data_ptr(), _stream()),
+               "ye3t_hip_embedding")
+    return out
+
+
+def embedding_adjoint(adjoint, tokens, rows, scale):
+    """``ye3t_hip_embedding_adjoint``: ``[rows, width]`` in the adjoint's dtype."""
+    import torch
+
+    code = _storage_code(adjoint.dtype, True)
+    W, N = int(adjoint.shape[-1]), tokens.numel()
+    out = torch.empty((rows, W), dtype=adjoint.dtype, device=adjoint.device)
+    if out.numel() == 0:
+        return out
+    with torch.cuda.device(adjoint.device):
+        size = lib().ye3t_hip_embedding_adjoint_workspace_bytes(code, N, rows, W)
+        work = _workspace(size, "ye3t_hip_embedding_adjoint_workspace_bytes", adjoint.device)
+        _check(lib().ye3t_hip_embedding_adjoint(code, _dev(adjoint, "adjoint"), _dev(tokens, "tokens"),
+                                                tokens.element_size(), N, rows, W, scale, out.data_ptr(),
+                                                work.data_ptr(), size, _stream()), "ye3t_hip_embedding_adjoint")
+    return out
+
+
+def rms_norm(input, weight, residual, epsilon):
+    """``ye3t_hip_rms_norm`` of contiguous rows: ``(y, sum or None)``."""
+    import torch
+
+    code = _storage_code(input.dtype)
+    W = int(input.shape[-1])
+    y = torch.empty_like(input)
+    total = None if residual is None else torch.empty_like(input)
+    if W:
+        with torch.cuda.device(input.device):
+            _check(lib().ye3t_hip_rms_norm(code, _dev(input, "input"), _opt(residual, "residual"),
+                                           _dev(weight, "weight"), input.numel() // W, W, epsilon,
+                                           _opt(total, "total"), y.data_ptr(), _stream()), "ye3t_hip_rms_norm")
+    return y, total
+
+
+def rms_norm_8bit(input, weight, residual, epsilon):
+    """``ye3t_hip_rms_norm_8bit`` of contiguous rows: ``(codes, scales, sum or None)``."""
+    import torch
+
+    code = _storage_code(input.dtype)
+    W = int(input.shape[-1])
+    codes = torch.empty(input.shape, dtype=torch.float8_e4m3fn, device=input.device)
+    scales = torch.empty((*input.shape[:-1], -(-W // 128)), dtype=torch.float32, device=input.device)
+    total = None if residual is None else torch.empty_like(input)
+    if W:
+        with torch.cuda.device(input.device):
+            _check(lib().ye3t_hip_rms_norm_8bit(code, _dev(input, "input"), _opt(residual, "residual"),
+                                                _dev(weight, "weight"), input.numel() // W, W, epsilon,
+                                                _opt(total, "total"), codes.data_ptr(), scales.data_ptr(), _stream()),
+                   "ye3t_hip_rms_norm_8bit")
+    return codes, scales, total
+
+
+def rms_norm_adjoint(adjoint, total, weight, total_adjoint, epsilon):
+    """``ye3t_hip_rms_norm_adjoint``: ``(input_adjoint, weight_adjoint)``."""
+    import torch
+
+    code = _storage_code(total.dtype)
+    W = int(total.shape[-1])
+    dx, dw = torch.empty_like(total), torch.empty_like(weight)
+    if W:
+        rows = total.numel() // W
+        with torch.cuda.device(total.device):
+            size = lib().ye3t_hip_rms_norm_adjoint_workspace_bytes(code, rows, W)
+            work = _workspace(size, "ye3t_hip_rms_norm_adjoint_workspace_bytes", total.device)
+            _check(lib().ye3t_hip_rms_norm_adjoint(code, _dev(adjoint, "adjoint"), _opt(total_adjoint, "total_adjoint"),
+                                                   _dev(total, "total"), _dev(weight, "weight"), rows, W, epsilon,
+                                                   dx.data_ptr(), dw.data_ptr(), work.data_ptr(), size, _stream()),
+                   "ye3t_hip_rms_norm_adjoint")
+    return dx, dw
+
+
+class Attention:
+    """One attention problem: ``ye3t_attention_args`` and the tensors behind it."""
+
+    _TENSORS = ("query", "key", "value", "offsets", "key_offsets", "slopes", "positions", "key_positions", "key_mask")
+
+    def __init__(self, query, key, value, offsets, key_offsets, scale, cap, slopes, positions, key_positions, key_mask):
+        self.query, self.key, self.value = query, key, value
+        self.offsets, self.key_offsets = offsets, key_offsets
+        self.slopes, self.positions, self.key_positions, self.key_mask = slopes, positions, key_positions, key_mask
+        self.scale, self.cap = scale, cap
+        q, k, v = query, key, value
+        pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self.args = AttentionArgs(
+            dtype=_storage_code(q.dtype), queries=q.shape[0], keys=k.shape[0], structures=offsets.numel() - 1,
+            heads=q.shape[1], key_heads=k.shape[1], head_width=q.shape[2], query=q.data_ptr(), key=k.data_ptr(),
+            value=v.data_ptr(), query_row_stride=q.stride(0), query_head_stride=q.stride(1),
+            key_row_stride=k.stride(0), key_head_stride=k.stride(1), value_row_stride=v.stride(0),
+            value_head_stride=v.stride(1), offsets=offsets.data_ptr(), key_offsets=pointer(key_offsets), scale=scale,
+            cap=cap, slopes=pointer(slopes), positions=pointer(positions), key_positions=pointer(key_positions),
+            key_mask=pointer(key_mask))
+
+    def tensors(self):
+        return tuple(getattr(self, n) for n in self._TENSORS)
+
+    def rest(self):
+        return self.scale, self.cap
+
+    @classmethod
+    def of(cls, tensors, rest):
+        q, k, v, offsets, key_offsets, *bias = tensors
+        return cls(q, k, v, offsets, key_offsets, *rest, *bias)
+
+    def forward(self, with_sums):
+        """``(out, log_sums or None)``"""
+        import torch
+
+        q = self.query
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        sums = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if with_sums else None
+        with torch.cuda.device(q.device):
+            size = lib().ye3t_hip_atom_attention_workspace_bytes(ctypes.byref(self.args))
+            work = _workspace(size, "ye3t_hip_atom_attention_workspace_bytes", q.device) if size else None
+            _check(lib().ye3t_hip_atom_attention(ctypes.byref(self.args), out.data_ptr(), _opt(sums, "log_sums"),
+                                                 _opt(work, "workspace"), size, _stream()), "ye3t_hip_atom_attention")
+        return out, sums
+
+    def adjoint(self, adjoint, out, sums, bias):
+        """Gradients to query, key, value, slopes, positions and key_positions."""
+        import torch
+
+        q, k, v = self.query, self.key, self.value
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        ds = torch.empty_like(self.slopes) if bias else None
+        dp = torch.empty_like(self.positions) if bias else None
+        dkp = torch.empty_like(self.key_positions) if bias and self.key_positions is not None else None
+        with torch.cuda.device(q.device):
+            size = lib().ye3t_hip_atom_attention_adjoint_workspace_bytes(ctypes.byref(self.args), int(bias))
+            work = _workspace(size, "ye3t_hip_atom_attention_adjoint_workspace_bytes", q.device)
+            _check(lib().ye3t_hip_atom_attention_adjoint(
+                ctypes.byref(self.args), _dev(out, "out"), _dev(sums, "log_sums"), _dev(adjoint, "adjoint"),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _opt(ds, "slopes_adjoint"), _opt(dp, "positions_adjoint"),
+                _opt(dkp, "key_positions_adjoint"), work.data_ptr(), size, _stream()),
+                "ye3t_hip_atom_attention_adjoint")
+        return dq, dk, dv, ds, dp, dkp
