@@ -35,6 +35,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -96,14 +97,20 @@ __device__ inline Op<T> line_chunk(const T* tile, int line, int u, int half) {
 // Contraction over 32 lines of a tile, the transposed operand: column `column`
 // + lane % 32 of the lines that registers 2 kChunk s / 2 ... of an accumulator
 // hold (bf16: lines 16 s + 4 half + 0..3 and + 8; fp32: lines 8 s + 4 half + 0..3).
+// bf16: the transposing LDS read, where lane l of a block of 16 gives the address
+// of four values of line l / 4, columns 4 (l % 4) .. + 3, and gets four lines of
+// column l.  Every lane of the wave takes part.
 template <int DP>
 __device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, int half) {
-  const int lane = threadIdx.x & 31;
-  bf16x8 r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    r[j] = tile[(16 * s + 8 * (j / 4) + 4 * half + j % 4) * kPitch<__bf16, DP> + column + lane];
-  return r;
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const int lane = threadIdx.x & 63;
+  const __bf16* at = tile + (16 * s + 4 * half + (lane & 15) / 4) * kPitch<__bf16, DP> + column + (lane & 16) + 4 * (lane & 3);
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kPitch<__bf16, DP>));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  const s16x8 both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(bf16x8, both);
 }
 template <int DP>
 __device__ inline f32x4 column_chunk(const float* tile, int s, int column, int half) {
@@ -246,12 +253,13 @@ __device__ inline void store_columns(T* p, int D, int half, const f32x16* acc, f
 
 __device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
 
-// key: x, y, z and whether it is seen
+// key: x, y, z, and what its scores are raised by: 0, or -infinity where it is
+// not seen
 template <bool BIAS>
 __device__ inline f32x4 key_place(const Problem& p, int64_t key, bool exists) {
-  f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 r = {0.0f, 0.0f, 0.0f, -INFINITY};
   if (exists && (!p.key_mask || p.key_mask[key])) {
-    r[3] = 1.0f;
+    r[3] = 0.0f;
     if (BIAS) {
       const float* at = (p.key_positions ? p.key_positions : p.positions) + 3 * key;
       r[0] = at[0];
@@ -286,24 +294,29 @@ struct Gradient {
   float* key_part;            // [keys, key_heads, 4]
 };
 
-// p, and the derivative of the bend, of scores as the forward takes them
-struct Weight {
-  float p, slant;
+// Scores in units of log2 as the forward takes them, and the derivative of the
+// bend; the distance is subtracted by the caller.
+struct Score {
+  float s, slant;
 };
-template <bool BIAS>
-__device__ inline Weight weight_of(const Problem& p, float product, float log_sum2, float slope2, float distance,
-                                   bool seen) {
-  float s, slant = 1.0f;
-  if (p.cap > 0.0f) {
+template <bool CAP>
+__device__ inline Score score_of(const Problem& p, float product) {
+  if (CAP) {
     const float t = bent(product * (p.scale / p.cap));
-    s = p.cap * kLog2e * t;
-    slant = 1.0f - t * t;
-  } else {
-    s = product * (p.scale * kLog2e);
+    return {p.cap * kLog2e * t, 1.0f - t * t};
   }
-  if (BIAS) s -= slope2 * distance;
-  return {seen ? __builtin_amdgcn_exp2f(s - log_sum2) : 0.0f, slant};
+  return {product * (p.scale * kLog2e), 1.0f};
 }
+
+// Keeps what follows from being started before what precedes: reading the places of all 32
+// lines of a tile at once takes more registers than the products leave.
+__device__ inline void in_turn() { __builtin_amdgcn_sched_barrier(0); }
+
+// Waves a SIMD that the register budget is set for.
+template <int DP>
+constexpr int kForwardWaves = DP == 32 ? 4 : DP == 64 ? 3 : 2;
+template <int DP>
+constexpr int kGradientWaves = DP == 32 ? 3 : DP == 64 ? 2 : 1;
 
 // ---- launches ----------------------------------------------------------------
 inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }

@@ -9,8 +9,8 @@ namespace {
 // ---- forward -----------------------------------------------------------------
 // NW waves of 32 rows, KT keys a tile.  SPLIT: grid axis z takes equal parts of
 // each structure's key tiles and leaves its sums to attention_join_kernel.
-template <typename T, int DP, int NW, int KT, bool BIAS, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
+template <typename T, int DP, int NW, int KT, bool BIAS, bool CAP, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, kForwardWaves<DP>) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
                                                             float* __restrict__ part, float* __restrict__ part_stats) {
   constexpr int TILE = 32 * NW, NU = DP / (2 * kChunk<T>), ND = DP / 32;
   __shared__ __align__(16) T ktile[KT * kPitch<T, DP>];
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Problem p, T* __rest
   };
   if (ks.AHEAD && tile < tiles) fetch(tile);
   const float to_log2 = p.scale * kLog2e;
-  const float to_cap = p.cap > 0.0f ? p.scale / p.cap : 0.0f, from_cap = p.cap * kLog2e;
+  const float to_cap = CAP ? p.scale / p.cap : 0.0f, from_cap = p.cap * kLog2e;
   for (; tile < tiles; ++tile) {
     __syncthreads();  // the last tile has been used
     if (!ks.AHEAD) fetch(tile);
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Problem p, T* __rest
       s[n] = zeros();
 #pragma unroll
       for (int u = 0; u < NU; ++u) mma(line_chunk<T, DP>(ktile, 32 * n + (lane & 31), u, half), q[u], s[n]);
-      if (p.cap > 0.0f) {
+      if (CAP) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] = from_cap * bent(s[n][i] * to_cap);
       } else {
@@ -95,13 +95,12 @@ __global__ __launch_bounds__(64 * NW) void attention_kernel(Problem p, T* __rest
         for (int i = 0; i < 16; ++i) {
           const f32x4 at = place[32 * n + 8 * (i / 4) + 4 * half + i % 4];
           const float dx = x - at[0], dy = y - at[1], dz = z - at[2];
-          s[n][i] -= slope * __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+          s[n][i] += at[3] - slope * __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+          if (i % 4 == 3) in_turn();
         }
-      }
-      if (masked) {
+      } else if (masked) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (place[32 * n + 8 * (i / 4) + 4 * half + i % 4][3] == 0.0f) s[n][i] = -INFINITY;
+        for (int i = 0; i < 16; ++i) s[n][i] += place[32 * n + 8 * (i / 4) + 4 * half + i % 4][3];
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) high = fmaxf(high, s[n][i]);
@@ -230,7 +229,7 @@ __global__ __launch_bounds__(64) void attention_slope_kernel(const float* __rest
   if (threadIdx.x == 0) slopes[h] = s;
 }
 
-template <typename T, int DP, int NW, bool BIAS>
+template <typename T, int DP, int NW, bool BIAS, bool CAP>
 int launch_forward(const ForwardPlan& f, const Problem& p, void* out, float* log_sums, void* workspace, hipStream_t s) {
   constexpr int KT = NW > 1 && sizeof(T) == 2 ? 64 : 32;
   float* part = static_cast<float*>(workspace);
@@ -238,11 +237,11 @@ int launch_forward(const ForwardPlan& f, const Problem& p, void* out, float* log
   const dim3 grid(unsigned(f.items), unsigned(p.key_heads), unsigned(f.parts));
   if (!fits_grid(f.items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many rows for one launch");
   if (f.parts == 1) {
-    hipLaunchKernelGGL((attention_kernel<T, DP, NW, KT, BIAS, false>), grid, dim3(64 * NW), 0, s, p,
+    hipLaunchKernelGGL((attention_kernel<T, DP, NW, KT, BIAS, CAP, false>), grid, dim3(64 * NW), 0, s, p,
                        static_cast<T*>(out), log_sums, part, stats);
     return check_launch("attention_kernel");
   }
-  hipLaunchKernelGGL((attention_kernel<T, DP, NW, KT, BIAS, true>), grid, dim3(64 * NW), 0, s, p, static_cast<T*>(out),
+  hipLaunchKernelGGL((attention_kernel<T, DP, NW, KT, BIAS, CAP, true>), grid, dim3(64 * NW), 0, s, p, static_cast<T*>(out),
                      log_sums, part, stats);
   if (int rc = check_launch("attention_kernel")) return rc;
   const int64_t rows = p.queries * p.heads;
@@ -260,8 +259,11 @@ struct Forward {
   hipStream_t s;
   template <typename T, int DP, int NW>
   int waves() const {
-    return p.slopes ? launch_forward<T, DP, NW, true>(f, p, out, log_sums, workspace, s)
-                    : launch_forward<T, DP, NW, false>(f, p, out, log_sums, workspace, s);
+    if (p.cap > 0.0f)
+      return p.slopes ? launch_forward<T, DP, NW, true, true>(f, p, out, log_sums, workspace, s)
+                      : launch_forward<T, DP, NW, false, true>(f, p, out, log_sums, workspace, s);
+    return p.slopes ? launch_forward<T, DP, NW, true, false>(f, p, out, log_sums, workspace, s)
+                    : launch_forward<T, DP, NW, false, false>(f, p, out, log_sums, workspace, s);
   }
   template <typename T, int DP>
   int operator()() const {

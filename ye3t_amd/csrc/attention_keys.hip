@@ -7,13 +7,13 @@ namespace {
 
 // Key side: dk, dv and the key's part of the gradient to its position.  A wave
 // owns 32 keys and walks over the rows of its key head in tiles of 32.
-template <typename T, int DP, int NW, bool BIAS, bool FORCES>
-__global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem p, Gradient g) {
+template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
+__global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_key_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, RT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
   __shared__ __align__(16) T qtile[RT * kPitch<T, DP>];
   __shared__ __align__(16) T gtile[RT * kPitch<T, DP>];
   __shared__ f32x4 place[RT];  // x, y, z, slope
-  __shared__ f32x4 stats[RT];  // log sum, D_i, whether the row counts
+  __shared__ f32x2 stats[RT];  // log sum, or infinity for a row that sees no key or does not exist; D_i
   const Item item = item_of(p.key_offsets, p.structures, p.keys, 1, TILE, blockIdx.x);
   const Span key = span_of(p.key_offsets, item.structure, p.keys);
   if (item.first < 0 || item.first >= key.length) return;
@@ -26,13 +26,14 @@ __global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem
   const bool busy = int(item.first) + 32 * wave < key.length;
   const int64_t token = key.begin + mine;
   const f32x4 here = key_place<BIAS>(p, token, exists);
-  const bool seen = here[3] != 0.0f;
+  const bool seen = here[3] == 0.0f;
   Op<T> k[NU], v[NU];
   line_operand<T, DP>(seen ? static_cast<const T*>(p.k) + token * p.k_row + key_head * p.k_head : nullptr, p.D, half, k);
   line_operand<T, DP>(seen ? static_cast<const T*>(p.v) + token * p.v_row + key_head * p.v_head : nullptr, p.D, half, v);
 
   Staged<T, DP, RT, 64 * NW> qs, gs;
-  f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f}, next_stats = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x2 next_stats = {INFINITY, 0.0f};
   auto fetch = [&](int64_t r0) {
     qs.load(p.D, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
@@ -45,11 +46,11 @@ __global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem
     if (int(threadIdx.x) < RT) {
       const Row r = row_of(p, own.begin, r0 + int(threadIdx.x), rows, key_head);
       next_place = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      next_stats = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      next_stats = f32x2{INFINITY, 0.0f};
       if (r.exists) {
         const int64_t at = r.token * p.heads + r.head;
         const float log_sum = g.log_sums[at];
-        if (log_sum != -INFINITY) next_stats = f32x4{log_sum * kLog2e, g.along[at], 1.0f, 0.0f};
+        if (log_sum != -INFINITY) next_stats = f32x2{log_sum * kLog2e, g.along[at]};
         if (BIAS)
           next_place = f32x4{p.positions[3 * r.token], p.positions[3 * r.token + 1], p.positions[3 * r.token + 2],
                              p.slopes[r.head] * kLog2e};
@@ -82,23 +83,31 @@ __global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int line = 8 * (i / 4) + 4 * half + i % 4;
-      const f32x4 st = stats[line];
-      float dx = 0.0f, dy = 0.0f, dz = 0.0f, distance = 0.0f, slope = 0.0f;
+      const f32x2 st = stats[line];
+      const Score z = score_of<CAP>(p, s[i]);
+      float exponent = z.s - st[0], dx = 0.0f, dy = 0.0f, dz = 0.0f, slope = 0.0f, per = 0.0f;
       if (BIAS) {
         const f32x4 r = place[line];
         dx = here[0] - r[0], dy = here[1] - r[1], dz = here[2] - r[2], slope = r[3];
-        distance = __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
+        const float square = dx * dx + dy * dy + dz * dz;
+        if (FORCES) {
+          per = square > 0.0f ? __builtin_amdgcn_rsqf(square) : 0.0f;
+          exponent -= slope * (square * per);
+        } else {
+          exponent -= slope * __builtin_amdgcn_sqrtf(square);
+        }
       }
-      const Weight w = weight_of<BIAS>(p, s[i], st[0], slope, distance, seen && st[2] != 0.0f);
-      const float tilt = w.p * (dp[i] - st[1]);
-      s[i] = tilt * w.slant;
-      dp[i] = w.p;
+      const float w = __builtin_amdgcn_exp2f(exponent);
+      const float tilt = w * (dp[i] - st[1]);
+      s[i] = tilt * z.slant;
+      dp[i] = w;
       if (FORCES) {
-        const float pull = distance > 0.0f ? -tilt * slope / distance : 0.0f;
+        const float pull = -tilt * slope * per;
         gx += pull * dx;
         gy += pull * dy;
         gz += pull * dz;
       }
+      if (i % 4 == 3) in_turn();
     }
 #pragma unroll
     for (int c = 0; c < kLineChunks<T>; ++c) {
@@ -113,6 +122,11 @@ __global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem
     }
   }
   if (!exists) return;
+  if (!seen) {  // what its scores would have been
+    gx = gy = gz = 0.0f;
+#pragma unroll
+    for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
+  }
   const int64_t at = token * p.key_heads + key_head;
   store_columns<T, DP>(static_cast<T*>(g.dk) + at * p.D, p.D, half, dk, p.scale);
   store_columns<T, DP>(static_cast<T*>(g.dv) + at * p.D, p.D, half, dv, 1.0f);
@@ -124,10 +138,10 @@ __global__ __launch_bounds__(64 * NW) void attention_key_gradient_kernel(Problem
   }
 }
 
-template <typename T, int DP, int NW, bool BIAS, bool FORCES>
+template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
 int launch_keys(const AdjointPlan& f, const Problem& p, const Gradient& g, hipStream_t s) {
   if (!fits_grid(f.key_items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many keys for one launch");
-  hipLaunchKernelGGL((attention_key_gradient_kernel<T, DP, NW, BIAS, FORCES>),
+  hipLaunchKernelGGL((attention_key_gradient_kernel<T, DP, NW, CAP, BIAS, FORCES>),
                      dim3(unsigned(f.key_items), unsigned(p.key_heads)), dim3(64 * NW), 0, s, p, g);
   return check_launch("attention_key_gradient_kernel");
 }
@@ -138,11 +152,15 @@ struct Side {
   const Gradient& g;
   bool forces;
   hipStream_t s;
+  template <typename T, int DP, int NW, bool CAP>
+  int capped() const {
+    return forces ? launch_keys<T, DP, NW, CAP, true, true>(f, p, g, s)
+                  : p.slopes ? launch_keys<T, DP, NW, CAP, true, false>(f, p, g, s)
+                             : launch_keys<T, DP, NW, CAP, false, false>(f, p, g, s);
+  }
   template <typename T, int DP, int NW>
   int waves() const {
-    return forces ? launch_keys<T, DP, NW, true, true>(f, p, g, s)
-                  : p.slopes ? launch_keys<T, DP, NW, true, false>(f, p, g, s)
-                             : launch_keys<T, DP, NW, false, false>(f, p, g, s);
+    return p.cap > 0.0f ? capped<T, DP, NW, true>() : capped<T, DP, NW, false>();
   }
   template <typename T, int DP>
   int operator()() const {

@@ -6,15 +6,18 @@ namespace attention {
 namespace {
 
 // Row side: dq, D_i, and the row's part of the gradients to position and slope
-// (FORCES).  D_i is the dot product of the output with its adjoint.  With FORCES
-// a first walk over the keys sums p, p (go . v) and p |r_i - r_j| instead: D_i
-// from the sums does not have a bf16 output's rounding, which would stand out
-// in gradients kept in fp32, and with D_i = sum p (go . v) / sum p the dz of a row add
-// up to zero as they should, whatever the last bits of the row's log sum are.
-// The slope's gradient takes distances from their mean, -sum dz (d - mean d),
-// for the same reason.
-template <typename T, int DP, int NW, bool BIAS, bool FORCES>
-__global__ __launch_bounds__(64 * NW) void attention_row_gradient_kernel(Problem p, Gradient g) {
+// (FORCES).
+//
+// D_i starts as the dot product of the output with its adjoint.  A bf16 output's
+// rounding would stand out: it shifts all dz_ij of a row by p_ij times the same
+// amount, up to 2^-9 of the largest terms where few keys carry the row.  The dz
+// of a row add up to zero, so what they add up to instead, over the sum of p, is that
+// amount c; everything here is linear in it and is set right after the walk over the
+// keys, dq by the product of the p (and the slants) with the keys.  The key side
+// starts from the D_i that is right.  fp32 calls have no such rounding in dq, and
+// correct only what FORCES sums, where terms of many keys cancel.
+template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
+__global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_row_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, KT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
   __shared__ __align__(16) T ktile[KT * kPitch<T, DP>];
   __shared__ __align__(16) T vtile[KT * kPitch<T, DP>];
@@ -35,7 +38,7 @@ __global__ __launch_bounds__(64 * NW) void attention_row_gradient_kernel(Problem
                       p.D, half, q);
   line_operand<T, DP>(row.exists ? static_cast<const T*>(g.adjoint) + at * p.D : nullptr, p.D, half, go);
   float along = 0.0f;
-  if (!FORCES) {
+  {
     Op<T> o[NU];
     line_operand<T, DP>(row.exists ? static_cast<const T*>(g.out) + at * p.D : nullptr, p.D, half, o);
 #pragma unroll
@@ -44,17 +47,16 @@ __global__ __launch_bounds__(64 * NW) void attention_row_gradient_kernel(Problem
       for (int e = 0; e < kChunk<T>; ++e) along += float(o[u][e]) * float(go[u][e]);
     along += other_half(along);
   }
-  float x = 0.0f, y = 0.0f, z = 0.0f, slope = 0.0f;
+  float x = 0.0f, y = 0.0f, z0 = 0.0f, slope = 0.0f;
   if (BIAS && row.exists) {
     x = p.positions[3 * row.token];
     y = p.positions[3 * row.token + 1];
-    z = p.positions[3 * row.token + 2];
+    z0 = p.positions[3 * row.token + 2];
     slope = p.slopes[row.head] * kLog2e;
   }
-  // a row that sees no key has the sum 0 and no gradient: p = 0 by `seen`
-  const float log_sum = row.exists ? g.log_sums[at] : 0.0f;
-  const bool empty = log_sum == -INFINITY;
-  const float log_sum2 = empty ? 0.0f : log_sum * kLog2e;
+  // a row that sees no key has no gradient: p = 0
+  const float log_sum = row.exists ? g.log_sums[at] : -INFINITY;
+  const float log_sum2 = log_sum == -INFINITY ? INFINITY : log_sum * kLog2e;
 
   const int tiles = (key.length + KT - 1) / KT;
   const T* kbase = static_cast<const T*>(p.k) + key_head * p.k_head;
@@ -73,84 +75,121 @@ __global__ __launch_bounds__(64 * NW) void attention_row_gradient_kernel(Problem
       next_place = key_place<BIAS>(p, key.begin + j, j < key.length);
     }
   };
-  f32x16 acc[ND];
+  constexpr bool RIGHT = sizeof(T) == 2;  // dq is set right
+  f32x16 acc[ND], own_keys[RIGHT ? ND : 1];
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = zeros();
-  float gx = 0.0f, gy = 0.0f, gz = 0.0f, gs = 0.0f, mass = 0.0f, mean = 0.0f;
-  for (int walk = FORCES ? 0 : 1; walk < 2; ++walk) {
-    if (ks.AHEAD && tiles > 0) fetch(0);
-    for (int tile = 0; tile < tiles; ++tile) {
-      __syncthreads();
-      if (!ks.AHEAD) fetch(tile);
-      ks.write(ktile);
-      vs.write(vtile);
-      if (int(threadIdx.x) < KT) place[threadIdx.x] = next_place;
-      __syncthreads();
-      if (ks.AHEAD && tile + 1 < tiles) fetch(tile + 1);
-      if (!busy) continue;
-      f32x16 s = zeros(), dp = zeros();
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        mma(line_chunk<T, DP>(ktile, lane & 31, u, half), q[u], s);
-        mma(line_chunk<T, DP>(vtile, lane & 31, u, half), go[u], dp);
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const f32x4 k = place[8 * (i / 4) + 4 * half + i % 4];
-        float dx = 0.0f, dy = 0.0f, dz = 0.0f, distance = 0.0f;
-        if (BIAS) {
-          dx = x - k[0], dy = y - k[1], dz = z - k[2];
-          distance = __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
-        }
-        const Weight w = weight_of<BIAS>(p, s[i], log_sum2, slope, distance, k[3] != 0.0f && !empty);
-        if (FORCES && walk == 0) {
-          along += w.p * dp[i];
-          mass += w.p;
-          mean += w.p * distance;
-          continue;
-        }
-        const float tilt = w.p * (dp[i] - along);
-        s[i] = tilt * w.slant;
-        if (FORCES) {
-          gs -= tilt * (distance - mean);
-          const float pull = distance > 0.0f ? -tilt / distance : 0.0f;
-          gx += pull * dx;
-          gy += pull * dy;
-          gz += pull * dz;
-        }
-      }
-      if (FORCES && walk == 0) continue;
-#pragma unroll
-      for (int c = 0; c < kLineChunks<T>; ++c) {
-        Op<T> w;
-        register_chunk(s, c, w);
-#pragma unroll
-        for (int t = 0; t < ND; ++t) mma(column_chunk<DP>(ktile, c, 32 * t, half), w, acc[t]);
-      }
+  for (int t = 0; t < (RIGHT ? ND : 1); ++t) own_keys[t] = zeros();
+  // Sums over the keys of dz, p, and with FORCES of their products with the
+  // distance and the direction.  Each tile's are summed by themselves first:
+  // long sums whose terms cancel keep a few more bits.
+  struct Sums {
+    float dz, p, far_dz, far_p;
+    f32x4 to_dz, to_p;
+    __device__ inline void add(const Sums& o) {
+      dz += o.dz, p += o.p, far_dz += o.far_dz, far_p += o.far_p, to_dz += o.to_dz, to_p += o.to_p;
     }
-    if (FORCES && walk == 0) {
-      mass += other_half(mass);
-      const float per = mass > 0.0f ? 1.0f / mass : 0.0f;
-      along = (along + other_half(along)) * per;
-      mean = (mean + other_half(mean)) * per;
+  };
+  const Sums none = {0.0f, 0.0f, 0.0f, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+  Sums all = none;
+  if (ks.AHEAD && tiles > 0) fetch(0);
+  for (int tile = 0; tile < tiles; ++tile) {
+    __syncthreads();
+    if (!ks.AHEAD) fetch(tile);
+    ks.write(ktile);
+    vs.write(vtile);
+    if (int(threadIdx.x) < KT) place[threadIdx.x] = next_place;
+    __syncthreads();
+    if (ks.AHEAD && tile + 1 < tiles) fetch(tile + 1);
+    if (!busy) continue;
+    f32x16 s = zeros(), dp = zeros();
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      mma(line_chunk<T, DP>(ktile, lane & 31, u, half), q[u], s);
+      mma(line_chunk<T, DP>(vtile, lane & 31, u, half), go[u], dp);
+    }
+    Sums now = none;
+    const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const Score z = score_of<CAP>(p, s[i]);
+      float exponent = z.s - log_sum2, dx = 0.0f, dy = 0.0f, dz = 0.0f, distance = 0.0f, per = 0.0f;
+      if (BIAS) {
+        const f32x4 k = place[8 * (i / 4) + 4 * half + i % 4];
+        dx = x - k[0], dy = y - k[1], dz = z0 - k[2];
+        const float square = dx * dx + dy * dy + dz * dz;
+        if (FORCES) {
+          per = square > 0.0f ? __builtin_amdgcn_rsqf(square) : 0.0f;
+          distance = square * per;
+        } else {
+          distance = __builtin_amdgcn_sqrtf(square);
+        }
+        exponent += k[3] - slope * distance;
+      } else if (masked) {
+        exponent += place[8 * (i / 4) + 4 * half + i % 4][3];
+      }
+      const float w = __builtin_amdgcn_exp2f(exponent);
+      const float tilt = w * (dp[i] - along);
+      s[i] = tilt * z.slant;
+      if (RIGHT) dp[i] = w * z.slant;
+      if (RIGHT || FORCES) {
+        now.dz += tilt;
+        now.p += w;
+      }
+      if (FORCES) {
+        now.far_dz += tilt * distance;
+        now.far_p += w * distance;
+        const float a = tilt * per, b = w * per;
+        now.to_dz[0] += a * dx, now.to_dz[1] += a * dy, now.to_dz[2] += a * dz;
+        now.to_p[0] += b * dx, now.to_p[1] += b * dy, now.to_p[2] += b * dz;
+      }
+      if (i % 4 == 3) in_turn();
+    }
+    all.add(now);
+#pragma unroll
+    for (int c = 0; c < kLineChunks<T>; ++c) {
+      Op<T> w, m;
+      register_chunk(s, c, w);
+      if (RIGHT) register_chunk(dp, c, m);
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        const Op<T> k = column_chunk<DP>(ktile, c, 32 * t, half);
+        mma(k, w, acc[t]);
+        if (RIGHT) mma(k, m, own_keys[t]);
+      }
     }
   }
+  float off = 0.0f;
+  if (RIGHT || FORCES) {
+    const float mass = all.p + other_half(all.p);
+    off = all.dz + other_half(all.dz);
+    off = mass > 0.0f ? off / mass : 0.0f;
+    along += off;
+  }
   if (!row.exists) return;
+  if (RIGHT) {
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][i] -= off * own_keys[t][i];
+  }
   store_columns<T, DP>(static_cast<T*>(g.dq) + at * p.D, p.D, half, acc, p.scale);
   if (half == 0) g.along[at] = along;
   if (FORCES) {
     const float m = p.slopes[row.head];
-    f32x4 r = {gx, gy, gz, gs};
+    f32x4 r;
 #pragma unroll
-    for (int a = 0; a < 4; ++a) r[a] = (r[a] + other_half(r[a])) * (a < 3 ? m : 1.0f);
+    for (int a = 0; a < 3; ++a) r[a] = -m * ((all.to_dz[a] + other_half(all.to_dz[a])) - off * (all.to_p[a] + other_half(all.to_p[a])));
+    r[3] = -((all.far_dz + other_half(all.far_dz)) - off * (all.far_p + other_half(all.far_p)));
     if (half == 0) *reinterpret_cast<f32x4*>(g.row_part + 4 * at) = r;
   }
 }
 
-template <typename T, int DP, int NW, bool BIAS, bool FORCES>
+template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
 int launch_rows(const AdjointPlan& f, const Problem& p, const Gradient& g, hipStream_t s) {
   if (!fits_grid(f.row_items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many rows for one launch");
-  hipLaunchKernelGGL((attention_row_gradient_kernel<T, DP, NW, BIAS, FORCES>),
+  hipLaunchKernelGGL((attention_row_gradient_kernel<T, DP, NW, CAP, BIAS, FORCES>),
                      dim3(unsigned(f.row_items), unsigned(p.key_heads)), dim3(64 * NW), 0, s, p, g);
   return check_launch("attention_row_gradient_kernel");
 }
@@ -161,11 +200,15 @@ struct Side {
   const Gradient& g;
   bool forces;
   hipStream_t s;
+  template <typename T, int DP, int NW, bool CAP>
+  int capped() const {
+    return forces ? launch_rows<T, DP, NW, CAP, true, true>(f, p, g, s)
+                  : p.slopes ? launch_rows<T, DP, NW, CAP, true, false>(f, p, g, s)
+                             : launch_rows<T, DP, NW, CAP, false, false>(f, p, g, s);
+  }
   template <typename T, int DP, int NW>
   int waves() const {
-    return forces ? launch_rows<T, DP, NW, true, true>(f, p, g, s)
-                  : p.slopes ? launch_rows<T, DP, NW, true, false>(f, p, g, s)
-                             : launch_rows<T, DP, NW, false, false>(f, p, g, s);
+    return p.cap > 0.0f ? capped<T, DP, NW, true>() : capped<T, DP, NW, false>();
   }
   template <typename T, int DP>
   int operator()() const {
