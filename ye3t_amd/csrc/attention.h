@@ -42,7 +42,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 struct Problem {
   int64_t queries, keys, structures;
-  int heads, key_heads, group, D;
+  int heads, key_heads, group, group_shift, D;  // group_shift: -1 where group is no power of two
+  bool direct;  // rows, heads and width are whole aligned chunks of 16 bytes
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   const int64_t *offsets, *key_offsets;
@@ -82,16 +83,21 @@ __device__ inline f32x16 zeros() {
   return z;
 }
 
-// A tile of rows in LDS: DP values and 32 bytes of padding, so that 16 byte
-// reads of eight consecutive rows fall into different banks.
+// A tile of lines in LDS: DP values each without padding, because the loads that
+// go straight to LDS write a wave's 64 chunks of 16 bytes one after the other.  Chunk c
+// of line l lies at place c ^ turn(l) of its line: eight lines that follow each other
+// then have their chunk c, and four lines their chunks c and c + 1, in different banks.
 template <typename T, int DP>
-constexpr int kPitch = DP + 32 / int(sizeof(T));
+__device__ inline int turn(int line) {
+  constexpr int BYTES = DP * int(sizeof(T)), PER = BYTES >= 256 ? 1 : 256 / BYTES;  // lines in 256 bytes
+  return 2 * (line / PER & (8 / PER - 1));
+}
 
 // Contraction over the width: chunk u of line `line` holds values
 // 2 kChunk u + kChunk half ...
 template <typename T, int DP>
 __device__ inline Op<T> line_chunk(const T* tile, int line, int u, int half) {
-  return *reinterpret_cast<const Op<T>*>(tile + line * kPitch<T, DP> + (2 * u + half) * kChunk<T>);
+  return *reinterpret_cast<const Op<T>*>(tile + line * DP + ((2 * u + half) ^ turn<T, DP>(line)) * kChunk<T>);
 }
 
 // Contraction over 32 lines of a tile, the transposed operand: column `column`
@@ -104,10 +110,11 @@ template <int DP>
 __device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, int half) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const int lane = threadIdx.x & 63;
-  const __bf16* at = tile + (16 * s + 4 * half + (lane & 15) / 4) * kPitch<__bf16, DP> + column + (lane & 16) + 4 * (lane & 3);
+  const int lane = threadIdx.x & 63, line = 4 * half + (lane & 15) / 4;  // turn() has the same value 8 lines on
+  const int chunk = column / 8 + (lane & 16) / 8 + (lane & 3) / 2;
+  const __bf16* at = tile + (16 * s + line) * DP + (chunk ^ turn<__bf16, DP>(line)) * 8 + 4 * (lane & 1);
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kPitch<__bf16, DP>));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * DP));
   typedef short s16x8 __attribute__((ext_vector_type(8)));
   const s16x8 both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_bit_cast(bf16x8, both);
@@ -117,7 +124,10 @@ __device__ inline f32x4 column_chunk(const float* tile, int s, int column, int h
   const int lane = threadIdx.x & 31;
   f32x4 r;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = tile[(8 * s + 4 * half + j) * kPitch<float, DP> + column + lane];
+  for (int j = 0; j < 4; ++j) {
+    const int line = 8 * s + 4 * half + j;
+    r[j] = tile[line * DP + ((column / 4 + lane / 4) ^ turn<float, DP>(line)) * 4 + (lane & 3)];
+  }
   return r;
 }
 // and the accumulator's registers as the other operand
@@ -132,15 +142,41 @@ __device__ inline void register_chunk(const f32x16& p, int s, f32x4& r) {
 template <typename T>
 constexpr int kLineChunks = 32 / (2 * kChunk<T>);
 
-// tanh with a relative error of a few ulp: the odd series where the quotient
-// would cancel.
+// Keeps what follows from being started before what precedes.  Left alone, the
+// compiler reads all operands of a tile from LDS first, which takes more
+// registers than the products leave.
+__device__ inline void in_turn() { __builtin_amdgcn_sched_barrier(0); }
+
+// use(i, load(i)) for i < N with the loads kept DEPTH steps ahead.
+template <int N, int DEPTH = 2, typename Load, typename Use>
+__device__ inline void in_flight(Load load, Use use) {
+  decltype(load(0)) held[DEPTH + 1];
+#pragma unroll
+  for (int i = 0; i < DEPTH && i < N; ++i) held[i] = load(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + DEPTH < N) held[(i + DEPTH) % (DEPTH + 1)] = load(i + DEPTH);
+    use(i, held[i % (DEPTH + 1)]);
+    in_turn();
+  }
+}
+template <typename T>
+struct Two {
+  Op<T> a, b;
+};
+
+// tanh by 1 - 2 / (exp(2 x) + 1), to 2e-7 of 1: for scores whose weights are
+// rounded to bf16.  fp32 calls take the odd series where the quotient cancels, for a
+// relative error of a few ulp (the first term left out is 4e-3 x^13).  No branches:
+// a lane's choice between two short formulas costs less than leaving one out.
+template <typename T>
 __device__ inline float bent(float x) {
-  const float a = fabsf(x), y = x * x;
+  const float q = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * kLog2e * x) + 1.0f);
+  if (sizeof(T) == 2) return q;
+  const float y = x * x;
   const float series =
       x + x * y * (-0.333333333f + y * (0.133333333f + y * (-0.0539682540f + y * (0.0218694885f + y * -0.00886323552f))));
-  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * a);
-  const float q = copysignf(1.0f - 2.0f / (e + 1.0f), x);
-  return a < 0.3f ? series : q;
+  return y < 0.09f ? series : q;
 }
 
 // The largest d with bound(d) <= slot, bound rising, bound(0) <= slot: 64 probes a round.
@@ -187,39 +223,37 @@ __device__ inline Item item_of(const int64_t* offsets, int64_t structures, int64
 inline int64_t item_count(int64_t rows, int64_t structures, int tile) { return rows / tile + structures; }
 
 // ---- loads of a tile ---------------------------------------------------------
-// LINES x DP values of `T`, NT threads, in registers between the load and the
-// LDS write so that the next tile's loads run under this tile's products.
-template <typename T, int DP, int LINES, int NT>
-struct Staged {
-  static constexpr int ROW = DP / kChunk<T>;  // 16 byte chunks of a line
-  static constexpr int N = (LINES * ROW + NT - 1) / NT;
-  static constexpr bool WHOLE = LINES * ROW % NT == 0;
-  // two tiles in flight take 64 registers of a lane at most; a single wave with
-  // wide fp32 rows reads its tile between the barriers
-  static constexpr bool AHEAD = 2 * N * 4 <= 64;
-  Chunk<T, kChunk<T>> v[N];
+__device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-  // address(line): the line's first value, or null for a line of zeros
-  template <typename F>
-  __device__ inline void load(int D, F address) {
+// LINES x DP values of `T` by NT threads.  Where every chunk is 16 whole aligned
+// bytes (`direct`) memory is loaded straight to LDS without passing registers, so that the
+// next tile's loads run under this tile's products and cost none of them; otherwise
+// chunk by chunk through registers.  address(line): the line's first value, or null for
+// a line of zeros.  arrived() waits for the loads of this wave.
+template <typename T, int DP, int LINES, int NT, typename F>
+__device__ inline void load_tile(T* tile, int D, bool direct, F address) {
+  constexpr int ROW = DP / kChunk<T>, SLOTS = LINES * ROW;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int x = n * NT + int(threadIdx.x), line = x / ROW, c = x % ROW * kChunk<T>;
-      const T* p = WHOLE || x < LINES * ROW ? address(line) : nullptr;
-      v[n] = p && c < D ? Chunk<T, kChunk<T>>::load(p + c, D - c) : Chunk<T, kChunk<T>>::zero();
-    }
-  }
-  __device__ inline void write(T* tile) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int x = n * NT + int(threadIdx.x), line = x / ROW, c = x % ROW * kChunk<T>;
+  for (int n = 0; n < (SLOTS + NT - 1) / NT; ++n) {
+    if (SLOTS % NT != 0 && n * NT + 64 * wave >= SLOTS) continue;  // 64 divides SLOTS
+    const int x = n * NT + int(threadIdx.x), line = x / ROW, c = (x % ROW ^ turn<T, DP>(line)) * kChunk<T>;
+    const T* p = address(line);
+    if (direct) {
+      const void* from = p && c < D ? static_cast<const void*>(p + c) : static_cast<const void*>(kZeros);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),
+                                       (__attribute__((address_space(3))) void*)(tile + (n * NT + 64 * wave) * kChunk<T>),
+                                       16, 0, 0);
+    } else {
+      const Chunk<T, kChunk<T>> v = p && c < D ? Chunk<T, kChunk<T>>::load(p + c, D - c) : Chunk<T, kChunk<T>>::zero();
       Op<T> a;
 #pragma unroll
-      for (int q = 0; q < kChunk<T>; ++q) a[q] = v[n].v[q];
-      if (WHOLE || x < LINES * ROW) *reinterpret_cast<Op<T>*>(tile + line * kPitch<T, DP> + c) = a;
+      for (int q = 0; q < kChunk<T>; ++q) a[q] = v.v[q];
+      *reinterpret_cast<Op<T>*>(tile + x * kChunk<T>) = a;
     }
   }
-};
+}
+__device__ inline void arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 // A row or key as matrix operand, straight from memory: chunks of this lane's half
 template <typename T, int DP>
@@ -256,19 +290,56 @@ __device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
 // key: x, y, z, and what its scores are raised by: 0, or -infinity where it is
 // not seen
 template <bool BIAS>
-__device__ inline f32x4 key_place(const Problem& p, int64_t key, bool exists) {
-  f32x4 r = {0.0f, 0.0f, 0.0f, -INFINITY};
-  if (exists && (!p.key_mask || p.key_mask[key])) {
-    r[3] = 0.0f;
-    if (BIAS) {
-      const float* at = (p.key_positions ? p.key_positions : p.positions) + 3 * key;
-      r[0] = at[0];
-      r[1] = at[1];
-      r[2] = at[2];
-    }
+__device__ inline f32x4 key_place(const Problem& p, int64_t key, bool seen) {
+  f32x4 r = {0.0f, 0.0f, 0.0f, seen ? 0.0f : -INFINITY};
+  if (BIAS && seen) {
+    const float* at = (p.key_positions ? p.key_positions : p.positions) + 3 * key;
+    r[0] = at[0];
+    r[1] = at[1];
+    r[2] = at[2];
   }
   return r;
 }
+
+// The keys of a structure in tiles of KT <= 64, two of them in LDS: begin() starts the
+// loads of one, finish() of the tile begun last makes it ready for the workgroup.
+// Whether a key is seen is read a tile ahead of its rows, which masked keys
+// have as zeros, whatever they hold.
+template <typename T, int DP, int KT, int NT, bool BIAS>
+struct KeyTiles {
+  const Problem& p;
+  const Span key;
+  const T *kbase, *vbase;
+  T *ktiles, *vtiles;
+  f32x4* places;
+  f32x4 place;
+  bool ahead;
+
+  __device__ inline bool seen(int tile) const {
+    const int j = tile * KT + (int(threadIdx.x) & 63);
+    return (int(threadIdx.x) & 63) < KT && j < key.length && (!p.key_mask || p.key_mask[key.begin + j]);
+  }
+  __device__ inline void start(int tile) {
+    ahead = seen(tile);
+    begin(tile);
+  }
+  __device__ inline void begin(int tile) {
+    const uint64_t all = __ballot(ahead);
+    const int buffer = tile & 1;
+    const int64_t first = key.begin + int64_t(tile) * KT;
+    load_tile<T, DP, KT, NT>(ktiles + buffer * KT * DP, p.D, p.direct,
+                             [&](int line) { return all >> line & 1 ? kbase + (first + line) * p.k_row : nullptr; });
+    load_tile<T, DP, KT, NT>(vtiles + buffer * KT * DP, p.D, p.direct,
+                             [&](int line) { return all >> line & 1 ? vbase + (first + line) * p.v_row : nullptr; });
+    if (int(threadIdx.x) < KT) place = key_place<BIAS>(p, first + threadIdx.x, ahead);
+    ahead = seen(tile + 1);
+  }
+  __device__ inline void finish(int tile) {
+    if (int(threadIdx.x) < KT) places[(tile & 1) * KT + threadIdx.x] = place;
+    arrived();
+    __syncthreads();
+  }
+};
 
 struct Row {
   int64_t token;
@@ -279,7 +350,7 @@ __device__ inline Row row_of(const Problem& p, int64_t begin, int64_t row, int64
   Row r;
   r.exists = row < rows;
   const uint32_t x = r.exists ? uint32_t(row) : 0u;
-  const uint32_t token = p.group == 1 ? x : x / uint32_t(p.group);
+  const uint32_t token = p.group_shift >= 0 ? x >> p.group_shift : x / uint32_t(p.group);
   r.token = begin + token;
   r.head = key_head * p.group + int(x - token * uint32_t(p.group));
   return r;
@@ -287,6 +358,7 @@ __device__ inline Row row_of(const Problem& p, int64_t begin, int64_t row, int64
 
 struct Gradient {
   const void *out, *adjoint;  // [queries, heads, D]
+  bool direct;                // the adjoint's rows are whole aligned chunks of 16 bytes
   const float* log_sums;      // [queries, heads]
   float* along;               // D_i, [queries, heads]
   void *dq, *dk, *dv;         // [queries, heads, D], [keys, key_heads, D]
@@ -299,26 +371,21 @@ struct Gradient {
 struct Score {
   float s, slant;
 };
-template <bool CAP>
+template <typename T, bool CAP>
 __device__ inline Score score_of(const Problem& p, float product) {
   if (CAP) {
-    const float t = bent(product * (p.scale / p.cap));
+    const float t = bent<T>(product * (p.scale / p.cap));
     return {p.cap * kLog2e * t, 1.0f - t * t};
   }
   return {product * (p.scale * kLog2e), 1.0f};
 }
 
-// Keeps what follows from being started before what precedes: reading the places of all 32
-// lines of a tile at once takes more registers than the products leave.
-__device__ inline void in_turn() { __builtin_amdgcn_sched_barrier(0); }
-
 // Waves a SIMD that the register budget is set for.
-template <int DP>
-constexpr int kForwardWaves = DP == 32 ? 4 : DP == 64 ? 3 : 2;
-template <int DP>
-constexpr int kGradientWaves = DP == 32 ? 3 : DP == 64 ? 2 : 1;
+template <typename T, int DP>
+constexpr int kForwardWaves = DP == 32 ? 3 : 2;
+template <typename T, int DP>
+constexpr int kGradientWaves = DP == 32 ? 2 : DP == 64 ? 2 : 1;
 
-// ---- launches ----------------------------------------------------------------
 inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Waves of a workgroup: rows enough for the mean structure, four at most.
@@ -388,7 +455,16 @@ inline Problem problem_of(const ye3t_attention_args& a) {
   p.heads = int(a.heads);
   p.key_heads = int(a.key_heads);
   p.group = int(a.heads / a.key_heads);
+  p.group_shift = -1;
+  for (int k = 0; k < 16; ++k)
+    if (p.group == 1 << k) p.group_shift = k;
   p.D = int(a.head_width);
+  const int64_t chunk = a.dtype == YE3T_F32 ? kChunk<float> : kChunk<__bf16>;
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.key) |
+                          reinterpret_cast<uintptr_t>(a.value);
+  p.direct = a.head_width % chunk == 0 && bases % 16 == 0 && a.query_row_stride % chunk == 0 &&
+             a.query_head_stride % chunk == 0 && a.key_row_stride % chunk == 0 && a.key_head_stride % chunk == 0 &&
+             a.value_row_stride % chunk == 0 && a.value_head_stride % chunk == 0;
   p.q = a.query;
   p.k = a.key;
   p.v = a.value;

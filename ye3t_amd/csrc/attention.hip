@@ -10,12 +10,12 @@ namespace {
 // NW waves of 32 rows, KT keys a tile.  SPLIT: grid axis z takes equal parts of
 // each structure's key tiles and leaves its sums to attention_join_kernel.
 template <typename T, int DP, int NW, int KT, bool BIAS, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, kForwardWaves<DP>) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
+__global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP>)) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
                                                             float* __restrict__ part, float* __restrict__ part_stats) {
   constexpr int TILE = 32 * NW, NU = DP / (2 * kChunk<T>), ND = DP / 32;
-  __shared__ __align__(16) T ktile[KT * kPitch<T, DP>];
-  __shared__ __align__(16) T vtile[KT * kPitch<T, DP>];
-  __shared__ f32x4 place[KT];
+  __shared__ __align__(16) T ktiles[2 * KT * DP];
+  __shared__ __align__(16) T vtiles[2 * KT * DP];
+  __shared__ f32x4 places[2 * KT];
   const Item item = item_of(p.offsets, p.structures, p.queries, p.group, TILE, blockIdx.x);
   const Span own = span_of(p.offsets, item.structure, p.queries);
   const int64_t rows = int64_t(own.length) * p.group;
@@ -46,34 +46,21 @@ __global__ __launch_bounds__(64 * NW, kForwardWaves<DP>) void attention_kernel(P
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = zeros();
   float top = -INFINITY, sum = 0.0f;
-  const T* kbase = static_cast<const T*>(p.k) + key_head * p.k_head;
-  const T* vbase = static_cast<const T*>(p.v) + key_head * p.v_head;
-  Staged<T, DP, KT, 64 * NW> ks, vs;
-  f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto fetch = [&](int t) {
-    auto seen = [&](int line) {
-      const int j = t * KT + line;
-      return j < key.length && (!p.key_mask || p.key_mask[key.begin + j]);
-    };
-    // masked keys are read as zeros, whatever they hold
-    ks.load(p.D, [&](int line) { return seen(line) ? kbase + (key.begin + t * KT + line) * p.k_row : nullptr; });
-    vs.load(p.D, [&](int line) { return seen(line) ? vbase + (key.begin + t * KT + line) * p.v_row : nullptr; });
-    if (int(threadIdx.x) < KT) {
-      const int j = t * KT + int(threadIdx.x);
-      next_place = key_place<BIAS>(p, key.begin + j, j < key.length);
-    }
-  };
-  if (ks.AHEAD && tile < tiles) fetch(tile);
+  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{p,
+                                              key,
+                                              static_cast<const T*>(p.k) + key_head * p.k_head,
+                                              static_cast<const T*>(p.v) + key_head * p.v_head,
+                                              ktiles,
+                                              vtiles,
+                                              places};
+  if (tile < tiles) tiles_of.start(tile);
   const float to_log2 = p.scale * kLog2e;
   const float to_cap = CAP ? p.scale / p.cap : 0.0f, from_cap = p.cap * kLog2e;
   for (; tile < tiles; ++tile) {
-    __syncthreads();  // the last tile has been used
-    if (!ks.AHEAD) fetch(tile);
-    ks.write(ktile);
-    vs.write(vtile);
-    if (int(threadIdx.x) < KT) place[threadIdx.x] = next_place;
-    __syncthreads();
-    if (ks.AHEAD && tile + 1 < tiles) fetch(tile + 1);
+    tiles_of.finish(tile);
+    if (tile + 1 < tiles) tiles_of.begin(tile + 1);
+    const T *ktile = ktiles + (tile & 1) * KT * DP, *vtile = vtiles + (tile & 1) * KT * DP;
+    const f32x4* place = places + (tile & 1) * KT;
     if (!busy) continue;
     const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
     f32x16 s[KT / 32];
@@ -81,11 +68,11 @@ __global__ __launch_bounds__(64 * NW, kForwardWaves<DP>) void attention_kernel(P
 #pragma unroll
     for (int n = 0; n < KT / 32; ++n) {
       s[n] = zeros();
-#pragma unroll
-      for (int u = 0; u < NU; ++u) mma(line_chunk<T, DP>(ktile, 32 * n + (lane & 31), u, half), q[u], s[n]);
+      in_flight<NU>([&](int u) { return line_chunk<T, DP>(ktile, 32 * n + (lane & 31), u, half); },
+                    [&](int u, const Op<T>& k) { mma(k, q[u], s[n]); });
       if (CAP) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = from_cap * bent(s[n][i] * to_cap);
+        for (int i = 0; i < 16; ++i) s[n][i] = from_cap * bent<T>(s[n][i] * to_cap);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] *= to_log2;
@@ -125,14 +112,12 @@ __global__ __launch_bounds__(64 * NW, kForwardWaves<DP>) void attention_kernel(P
         s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - base);
         sum += s[n][i];
       }
+      Op<T> w[kLineChunks<T>];
 #pragma unroll
-      for (int c = 0; c < kLineChunks<T>; ++c) {
-        Op<T> w;
-        register_chunk(s[n], c, w);
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
-          mma(column_chunk<DP>(vtile + 32 * n * kPitch<T, DP>, c, 32 * t, half), w, acc[t]);
-      }
+      for (int c = 0; c < kLineChunks<T>; ++c) register_chunk(s[n], c, w[c]);
+      in_flight<kLineChunks<T> * ND>(
+          [&](int i) { return column_chunk<DP>(vtile + 32 * n * DP, i / ND, 32 * (i % ND), half); },
+          [&](int i, const Op<T>& v) { mma(v, w[i / ND], acc[i % ND]); });
     }
   }
   if (!row.exists) return;
@@ -333,6 +318,8 @@ int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void*
   Gradient g{};
   g.out = out;
   g.adjoint = out_adjoint;
+  g.direct = reinterpret_cast<uintptr_t>(out_adjoint) % 16 == 0 &&
+             args->head_width % (args->dtype == YE3T_F32 ? kChunk<float> : kChunk<__bf16>) == 0;
   g.log_sums = static_cast<const float*>(log_sums);
   g.along = reinterpret_cast<float*>(work);
   g.dq = query_adjoint;

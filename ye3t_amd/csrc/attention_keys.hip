@@ -8,12 +8,12 @@ namespace {
 // Key side: dk, dv and the key's part of the gradient to its position.  A wave
 // owns 32 keys and walks over the rows of its key head in tiles of 32.
 template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
-__global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_key_gradient_kernel(Problem p, Gradient g) {
+__global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_key_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, RT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
-  __shared__ __align__(16) T qtile[RT * kPitch<T, DP>];
-  __shared__ __align__(16) T gtile[RT * kPitch<T, DP>];
-  __shared__ f32x4 place[RT];  // x, y, z, slope
-  __shared__ f32x2 stats[RT];  // log sum, or infinity for a row that sees no key or does not exist; D_i
+  __shared__ __align__(16) T qtiles[2 * RT * DP];
+  __shared__ __align__(16) T gtiles[2 * RT * DP];
+  __shared__ f32x4 places[2 * RT];  // x, y, z, slope
+  __shared__ f32x2 all_stats[2 * RT];  // log sum, or infinity for a row that sees no key or does not exist; D_i
   const Item item = item_of(p.key_offsets, p.structures, p.keys, 1, TILE, blockIdx.x);
   const Span key = span_of(p.key_offsets, item.structure, p.keys);
   if (item.first < 0 || item.first >= key.length) return;
@@ -25,21 +25,21 @@ __global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_key_gra
   const bool exists = mine < key.length;
   const bool busy = int(item.first) + 32 * wave < key.length;
   const int64_t token = key.begin + mine;
-  const f32x4 here = key_place<BIAS>(p, token, exists);
-  const bool seen = here[3] == 0.0f;
+  const bool seen = exists && (!p.key_mask || p.key_mask[token]);
+  const f32x4 here = key_place<BIAS>(p, token, seen);
   Op<T> k[NU], v[NU];
   line_operand<T, DP>(seen ? static_cast<const T*>(p.k) + token * p.k_row + key_head * p.k_head : nullptr, p.D, half, k);
   line_operand<T, DP>(seen ? static_cast<const T*>(p.v) + token * p.v_row + key_head * p.v_head : nullptr, p.D, half, v);
 
-  Staged<T, DP, RT, 64 * NW> qs, gs;
   f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
   f32x2 next_stats = {INFINITY, 0.0f};
-  auto fetch = [&](int64_t r0) {
-    qs.load(p.D, [&](int line) {
+  auto begin = [&](int64_t r0) {
+    const int buffer = int(r0 / RT) & 1;
+    load_tile<T, DP, RT, 64 * NW>(qtiles + buffer * RT * DP, p.D, p.direct, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(p.q) + r.token * p.q_row + r.head * p.q_head : nullptr;
     });
-    gs.load(p.D, [&](int line) {
+    load_tile<T, DP, RT, 64 * NW>(gtiles + buffer * RT * DP, p.D, g.direct, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(g.adjoint) + (r.token * p.heads + r.head) * p.D : nullptr;
     });
@@ -61,30 +61,34 @@ __global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_key_gra
 #pragma unroll
   for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
   float gx = 0.0f, gy = 0.0f, gz = 0.0f;
-  if (qs.AHEAD && rows > 0) fetch(0);
+  if (rows > 0) begin(0);
   for (int64_t r0 = 0; r0 < rows; r0 += RT) {
-    __syncthreads();
-    if (!qs.AHEAD) fetch(r0);
-    qs.write(qtile);
-    gs.write(gtile);
+    const int buffer = int(r0 / RT) & 1;
     if (int(threadIdx.x) < RT) {
-      place[threadIdx.x] = next_place;
-      stats[threadIdx.x] = next_stats;
+      places[buffer * RT + threadIdx.x] = next_place;
+      all_stats[buffer * RT + threadIdx.x] = next_stats;
     }
+    arrived();
     __syncthreads();
-    if (qs.AHEAD && r0 + RT < rows) fetch(r0 + RT);
+    if (r0 + RT < rows) begin(r0 + RT);
+    const T *qtile = qtiles + buffer * RT * DP, *gtile = gtiles + buffer * RT * DP;
+    const f32x4* place = places + buffer * RT;
+    const f32x2* stats = all_stats + buffer * RT;
     if (!busy) continue;
     f32x16 s = zeros(), dp = zeros();
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      mma(line_chunk<T, DP>(qtile, lane & 31, u, half), k[u], s);
-      mma(line_chunk<T, DP>(gtile, lane & 31, u, half), v[u], dp);
-    }
+    in_flight<NU>(
+        [&](int u) {
+          return Two<T>{line_chunk<T, DP>(qtile, lane & 31, u, half), line_chunk<T, DP>(gtile, lane & 31, u, half)};
+        },
+        [&](int u, const Two<T>& qg) {
+          mma(qg.a, k[u], s);
+          mma(qg.b, v[u], dp);
+        });
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int line = 8 * (i / 4) + 4 * half + i % 4;
       const f32x2 st = stats[line];
-      const Score z = score_of<CAP>(p, s[i]);
+      const Score z = score_of<T, CAP>(p, s[i]);
       float exponent = z.s - st[0], dx = 0.0f, dy = 0.0f, dz = 0.0f, slope = 0.0f, per = 0.0f;
       if (BIAS) {
         const f32x4 r = place[line];
@@ -109,17 +113,21 @@ __global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_key_gra
       }
       if (i % 4 == 3) in_turn();
     }
+    Op<T> ds[kLineChunks<T>], w[kLineChunks<T>];
 #pragma unroll
     for (int c = 0; c < kLineChunks<T>; ++c) {
-      Op<T> ds, w;
-      register_chunk(s, c, ds);
-      register_chunk(dp, c, w);
-#pragma unroll
-      for (int t = 0; t < ND; ++t) {
-        mma(column_chunk<DP>(qtile, c, 32 * t, half), ds, dk[t]);
-        mma(column_chunk<DP>(gtile, c, 32 * t, half), w, dv[t]);
-      }
+      register_chunk(s, c, ds[c]);
+      register_chunk(dp, c, w[c]);
     }
+    in_flight<kLineChunks<T> * ND>(
+        [&](int i) {
+          return Two<T>{column_chunk<DP>(qtile, i / ND, 32 * (i % ND), half),
+                        column_chunk<DP>(gtile, i / ND, 32 * (i % ND), half)};
+        },
+        [&](int i, const Two<T>& qg) {
+          mma(qg.a, ds[i / ND], dk[i % ND]);
+          mma(qg.b, w[i / ND], dv[i % ND]);
+        });
   }
   if (!exists) return;
   if (!seen) {  // what its scores would have been

@@ -17,11 +17,11 @@ namespace {
 // starts from the D_i that is right.  fp32 calls have no such rounding in dq, and
 // correct only what FORCES sums, where terms of many keys cancel.
 template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
-__global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_row_gradient_kernel(Problem p, Gradient g) {
+__global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_row_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, KT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
-  __shared__ __align__(16) T ktile[KT * kPitch<T, DP>];
-  __shared__ __align__(16) T vtile[KT * kPitch<T, DP>];
-  __shared__ f32x4 place[KT];
+  __shared__ __align__(16) T ktiles[2 * KT * DP];
+  __shared__ __align__(16) T vtiles[2 * KT * DP];
+  __shared__ f32x4 places[2 * KT];
   const Item item = item_of(p.offsets, p.structures, p.queries, p.group, TILE, blockIdx.x);
   const Span own = span_of(p.offsets, item.structure, p.queries);
   const int64_t rows = int64_t(own.length) * p.group;
@@ -59,22 +59,13 @@ __global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_row_gra
   const float log_sum2 = log_sum == -INFINITY ? INFINITY : log_sum * kLog2e;
 
   const int tiles = (key.length + KT - 1) / KT;
-  const T* kbase = static_cast<const T*>(p.k) + key_head * p.k_head;
-  const T* vbase = static_cast<const T*>(p.v) + key_head * p.v_head;
-  Staged<T, DP, KT, 64 * NW> ks, vs;
-  f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto fetch = [&](int t) {
-    auto seen = [&](int line) {
-      const int j = t * KT + line;
-      return j < key.length && (!p.key_mask || p.key_mask[key.begin + j]);
-    };
-    ks.load(p.D, [&](int line) { return seen(line) ? kbase + (key.begin + t * KT + line) * p.k_row : nullptr; });
-    vs.load(p.D, [&](int line) { return seen(line) ? vbase + (key.begin + t * KT + line) * p.v_row : nullptr; });
-    if (int(threadIdx.x) < KT) {
-      const int j = t * KT + int(threadIdx.x);
-      next_place = key_place<BIAS>(p, key.begin + j, j < key.length);
-    }
-  };
+  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{p,
+                                              key,
+                                              static_cast<const T*>(p.k) + key_head * p.k_head,
+                                              static_cast<const T*>(p.v) + key_head * p.v_head,
+                                              ktiles,
+                                              vtiles,
+                                              places};
   constexpr bool RIGHT = sizeof(T) == 2;  // dq is set right
   f32x16 acc[ND], own_keys[RIGHT ? ND : 1];
 #pragma unroll
@@ -93,27 +84,27 @@ __global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_row_gra
   };
   const Sums none = {0.0f, 0.0f, 0.0f, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
   Sums all = none;
-  if (ks.AHEAD && tiles > 0) fetch(0);
+  if (tiles > 0) tiles_of.start(0);
   for (int tile = 0; tile < tiles; ++tile) {
-    __syncthreads();
-    if (!ks.AHEAD) fetch(tile);
-    ks.write(ktile);
-    vs.write(vtile);
-    if (int(threadIdx.x) < KT) place[threadIdx.x] = next_place;
-    __syncthreads();
-    if (ks.AHEAD && tile + 1 < tiles) fetch(tile + 1);
+    tiles_of.finish(tile);
+    if (tile + 1 < tiles) tiles_of.begin(tile + 1);
+    const T *ktile = ktiles + (tile & 1) * KT * DP, *vtile = vtiles + (tile & 1) * KT * DP;
+    const f32x4* place = places + (tile & 1) * KT;
     if (!busy) continue;
     f32x16 s = zeros(), dp = zeros();
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      mma(line_chunk<T, DP>(ktile, lane & 31, u, half), q[u], s);
-      mma(line_chunk<T, DP>(vtile, lane & 31, u, half), go[u], dp);
-    }
+    in_flight<NU>(
+        [&](int u) {
+          return Two<T>{line_chunk<T, DP>(ktile, lane & 31, u, half), line_chunk<T, DP>(vtile, lane & 31, u, half)};
+        },
+        [&](int u, const Two<T>& kv) {
+          mma(kv.a, q[u], s);
+          mma(kv.b, go[u], dp);
+        });
     Sums now = none;
     const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const Score z = score_of<CAP>(p, s[i]);
+      const Score z = score_of<T, CAP>(p, s[i]);
       float exponent = z.s - log_sum2, dx = 0.0f, dy = 0.0f, dz = 0.0f, distance = 0.0f, per = 0.0f;
       if (BIAS) {
         const f32x4 k = place[8 * (i / 4) + 4 * half + i % 4];
@@ -147,18 +138,17 @@ __global__ __launch_bounds__(64 * NW, kGradientWaves<DP>) void attention_row_gra
       if (i % 4 == 3) in_turn();
     }
     all.add(now);
+    Op<T> w[kLineChunks<T>], m[RIGHT ? kLineChunks<T> : 1];
 #pragma unroll
     for (int c = 0; c < kLineChunks<T>; ++c) {
-      Op<T> w, m;
-      register_chunk(s, c, w);
-      if (RIGHT) register_chunk(dp, c, m);
-#pragma unroll
-      for (int t = 0; t < ND; ++t) {
-        const Op<T> k = column_chunk<DP>(ktile, c, 32 * t, half);
-        mma(k, w, acc[t]);
-        if (RIGHT) mma(k, m, own_keys[t]);
-      }
+      register_chunk(s, c, w[c]);
+      if constexpr (RIGHT) register_chunk(dp, c, m[c]);
     }
+    in_flight<kLineChunks<T> * ND>([&](int i) { return column_chunk<DP>(ktile, i / ND, 32 * (i % ND), half); },
+                                   [&](int i, const Op<T>& k) {
+                                     mma(k, w[i / ND], acc[i % ND]);
+                                     if constexpr (RIGHT) mma(k, m[i / ND], own_keys[i % ND]);
+                                   });
   }
   float off = 0.0f;
   if (RIGHT || FORCES) {
