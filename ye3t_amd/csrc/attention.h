@@ -85,12 +85,14 @@ __device__ inline f32x16 zeros() {
 
 // A tile of lines in LDS: DP values each without padding, because the loads that
 // go straight to LDS write a wave's 64 chunks of 16 bytes one after the other.  Chunk c
-// of line l lies at place c ^ turn(l) of its line: eight lines that follow each other
-// then have their chunk c, and four lines their chunks c and c + 1, in different banks.
+// of line l lies at place c ^ turn(l) of its line.  LDS serves 256 bytes a cycle from 64
+// banks: 16 lanes of a 16 byte read, which are one chunk of 16 lines, or 32 of a
+// transposing one, four chunks of four lines; turn() puts either into different banks (with
+// turns that repeat after eight lines 44 % of the LDS cycles were conflicts).
 template <typename T, int DP>
 __device__ inline int turn(int line) {
   constexpr int BYTES = DP * int(sizeof(T)), PER = BYTES >= 256 ? 1 : 256 / BYTES;  // lines in 256 bytes
-  return 2 * (line / PER & (8 / PER - 1));
+  return (line & 3) / PER * 4 | (line >> 2 & 3);
 }
 
 // Contraction over the width: chunk u of line `line` holds values
@@ -110,11 +112,11 @@ template <int DP>
 __device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, int half) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const int lane = threadIdx.x & 63, line = 4 * half + (lane & 15) / 4;  // turn() has the same value 8 lines on
+  const int lane = threadIdx.x & 63, line = 4 * half + (lane & 15) / 4;  // turn() repeats 16 lines on
   const int chunk = column / 8 + (lane & 16) / 8 + (lane & 3) / 2;
-  const __bf16* at = tile + (16 * s + line) * DP + (chunk ^ turn<__bf16, DP>(line)) * 8 + 4 * (lane & 1);
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * DP));
+  const __bf16* at = tile + (16 * s + line) * DP + 4 * (lane & 1);
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + (chunk ^ turn<__bf16, DP>(line)) * 8));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * DP + (chunk ^ turn<__bf16, DP>(line + 8)) * 8));
   typedef short s16x8 __attribute__((ext_vector_type(8)));
   const s16x8 both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_bit_cast(bf16x8, both);
@@ -225,32 +227,37 @@ inline int64_t item_count(int64_t rows, int64_t structures, int tile) { return r
 // ---- loads of a tile ---------------------------------------------------------
 __device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-// LINES x DP values of `T` by NT threads.  Where every chunk is 16 whole aligned
-// bytes (`direct`) memory is loaded straight to LDS without passing registers, so that the
-// next tile's loads run under this tile's products and cost none of them; otherwise
-// chunk by chunk through registers.  address(line): the line's first value, or null for
-// a line of zeros.  arrived() waits for the loads of this wave.
+// LINES x DP values of `T` by NT threads into a tile, while another tile is used.  Where
+// every chunk is 16 whole aligned bytes (`direct`) memory is loaded straight to LDS
+// without passing registers; otherwise chunk by chunk through them.  address(line): the
+// line's first value, or null for a line of zeros.  arrived() waits for the loads of this wave.
 template <typename T, int DP, int LINES, int NT, typename F>
 __device__ inline void load_tile(T* tile, int D, bool direct, F address) {
   constexpr int ROW = DP / kChunk<T>, SLOTS = LINES * ROW;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  auto each = [&](auto use) {
 #pragma unroll
-  for (int n = 0; n < (SLOTS + NT - 1) / NT; ++n) {
-    if (SLOTS % NT != 0 && n * NT + 64 * wave >= SLOTS) continue;  // 64 divides SLOTS
-    const int x = n * NT + int(threadIdx.x), line = x / ROW, c = (x % ROW ^ turn<T, DP>(line)) * kChunk<T>;
-    const T* p = address(line);
-    if (direct) {
-      const void* from = p && c < D ? static_cast<const void*>(p + c) : static_cast<const void*>(kZeros);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),
-                                       (__attribute__((address_space(3))) void*)(tile + (n * NT + 64 * wave) * kChunk<T>),
-                                       16, 0, 0);
-    } else {
-      const Chunk<T, kChunk<T>> v = p && c < D ? Chunk<T, kChunk<T>>::load(p + c, D - c) : Chunk<T, kChunk<T>>::zero();
+    for (int n = 0; n < (SLOTS + NT - 1) / NT; ++n) {
+      if (SLOTS % NT != 0 && n * NT + 64 * wave >= SLOTS) continue;  // 64 divides SLOTS
+      const int x = n * NT + int(threadIdx.x), line = x / ROW, c = (x % ROW ^ turn<T, DP>(line)) * kChunk<T>;
+      const T* p = address(line);
+      use(n, x, c, p && c < D ? p + c : nullptr);
+    }
+  };
+  if (direct) {
+    each([&](int n, int, int, const T* p) {
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(p ? p : reinterpret_cast<const T*>(kZeros)),
+          (__attribute__((address_space(3))) void*)(tile + (n * NT + 64 * wave) * kChunk<T>), 16, 0, 0);
+    });
+  } else {
+    each([&](int, int x, int c, const T* p) {
+      const Chunk<T, kChunk<T>> v = p ? Chunk<T, kChunk<T>>::load(p, D - c) : Chunk<T, kChunk<T>>::zero();
       Op<T> a;
 #pragma unroll
       for (int q = 0; q < kChunk<T>; ++q) a[q] = v.v[q];
       *reinterpret_cast<Op<T>*>(tile + x * kChunk<T>) = a;
-    }
+    });
   }
 }
 __device__ inline void arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
@@ -313,26 +320,31 @@ struct KeyTiles {
   T *ktiles, *vtiles;
   f32x4* places;
   f32x4 place;
-  bool ahead;
+  uint8_t mask;  // of this lane's key in the tile after the one begun last, as it was read
 
-  __device__ inline bool seen(int tile) const {
-    const int j = tile * KT + (int(threadIdx.x) & 63);
-    return (int(threadIdx.x) & 63) < KT && j < key.length && (!p.key_mask || p.key_mask[key.begin + j]);
+  __device__ inline bool exists(int tile) const {
+    return (int(threadIdx.x) & 63) < KT && tile * KT + (int(threadIdx.x) & 63) < key.length;
+  }
+  __device__ inline void look(int tile) {
+    mask = 1;
+    if (p.key_mask && exists(tile)) mask = p.key_mask[key.begin + tile * KT + (int(threadIdx.x) & 63)];
   }
   __device__ inline void start(int tile) {
-    ahead = seen(tile);
+    look(tile);
     begin(tile);
   }
+  // Nothing here uses what it loads: a wait would be for the tile's rows too.
   __device__ inline void begin(int tile) {
-    const uint64_t all = __ballot(ahead);
+    const bool seen = exists(tile) && mask;
+    const uint64_t all = __ballot(seen);
     const int buffer = tile & 1;
     const int64_t first = key.begin + int64_t(tile) * KT;
     load_tile<T, DP, KT, NT>(ktiles + buffer * KT * DP, p.D, p.direct,
                              [&](int line) { return all >> line & 1 ? kbase + (first + line) * p.k_row : nullptr; });
     load_tile<T, DP, KT, NT>(vtiles + buffer * KT * DP, p.D, p.direct,
                              [&](int line) { return all >> line & 1 ? vbase + (first + line) * p.v_row : nullptr; });
-    if (int(threadIdx.x) < KT) place = key_place<BIAS>(p, first + threadIdx.x, ahead);
-    ahead = seen(tile + 1);
+    if (int(threadIdx.x) < KT) place = key_place<BIAS>(p, first + threadIdx.x, seen);
+    look(tile + 1);
   }
   __device__ inline void finish(int tile) {
     if (int(threadIdx.x) < KT) places[(tile & 1) * KT + threadIdx.x] = place;

@@ -46,13 +46,9 @@ __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP>)) void attention_ker
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = zeros();
   float top = -INFINITY, sum = 0.0f;
-  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{p,
-                                              key,
-                                              static_cast<const T*>(p.k) + key_head * p.k_head,
-                                              static_cast<const T*>(p.v) + key_head * p.v_head,
-                                              ktiles,
-                                              vtiles,
-                                              places};
+  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{p,      key,    static_cast<const T*>(p.k) + key_head * p.k_head,
+                                                     static_cast<const T*>(p.v) + key_head * p.v_head,
+                                                     ktiles, vtiles, places};
   if (tile < tiles) tiles_of.start(tile);
   const float to_log2 = p.scale * kLog2e;
   const float to_cap = CAP ? p.scale / p.cap : 0.0f, from_cap = p.cap * kLog2e;

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
   line_operand<T, DP>(seen ? static_cast<const T*>(p.v) + token * p.v_row + key_head * p.v_head : nullptr, p.D, half, v);
 
   f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
-  f32x2 next_stats = {INFINITY, 0.0f};
+  f32x2 next_stats = {-INFINITY, 0.0f};
   auto begin = [&](int64_t r0) {
     const int buffer = int(r0 / RT) & 1;
     load_tile<T, DP, RT, 64 * NW>(qtiles + buffer * RT * DP, p.D, p.direct, [&](int line) {
@@ -43,17 +43,16 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(g.adjoint) + (r.token * p.heads + r.head) * p.D : nullptr;
     });
+    // nothing here uses what it loads: a wait would be for the tile's rows too
     if (int(threadIdx.x) < RT) {
       const Row r = row_of(p, own.begin, r0 + int(threadIdx.x), rows, key_head);
-      next_place = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      next_stats = f32x2{INFINITY, 0.0f};
+      next_stats = f32x2{-INFINITY, 0.0f};
       if (r.exists) {
         const int64_t at = r.token * p.heads + r.head;
-        const float log_sum = g.log_sums[at];
-        if (log_sum != -INFINITY) next_stats = f32x2{log_sum * kLog2e, g.along[at]};
+        next_stats = f32x2{g.log_sums[at], g.along[at]};
         if (BIAS)
           next_place = f32x4{p.positions[3 * r.token], p.positions[3 * r.token + 1], p.positions[3 * r.token + 2],
-                             p.slopes[r.head] * kLog2e};
+                             p.slopes[r.head]};
       }
     }
   };
@@ -65,8 +64,10 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
   for (int64_t r0 = 0; r0 < rows; r0 += RT) {
     const int buffer = int(r0 / RT) & 1;
     if (int(threadIdx.x) < RT) {
-      places[buffer * RT + threadIdx.x] = next_place;
-      all_stats[buffer * RT + threadIdx.x] = next_stats;
+      places[buffer * RT + threadIdx.x] = f32x4{next_place[0], next_place[1], next_place[2], next_place[3] * kLog2e};
+      const bool counts = next_stats[0] != -INFINITY;
+      all_stats[buffer * RT + threadIdx.x] =
+          f32x2{counts ? next_stats[0] * kLog2e : INFINITY, counts ? next_stats[1] : 0.0f};
     }
     arrived();
     __syncthreads();

@@ -59,13 +59,9 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ro
   const float log_sum2 = log_sum == -INFINITY ? INFINITY : log_sum * kLog2e;
 
   const int tiles = (key.length + KT - 1) / KT;
-  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{p,
-                                              key,
-                                              static_cast<const T*>(p.k) + key_head * p.k_head,
-                                              static_cast<const T*>(p.v) + key_head * p.v_head,
-                                              ktiles,
-                                              vtiles,
-                                              places};
+  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{
+      p,      key,    static_cast<const T*>(p.k) + key_head * p.k_head, static_cast<const T*>(p.v) + key_head * p.v_head,
+      ktiles, vtiles, places};
   constexpr bool RIGHT = sizeof(T) == 2;  // dq is set right
   f32x16 acc[ND], own_keys[RIGHT ? ND : 1];
 #pragma unroll

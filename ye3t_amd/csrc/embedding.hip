@@ -105,21 +105,37 @@ __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* 
   __shared__ uint32_t of_wave[kWaves][kBins];  // a wave's count of a digit, then its place among the waves
   __shared__ uint32_t wave_sums[kBins / 64];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  uint32_t before = 0, all = 0;
-  if (t < kBins) {
-    for (int r = 0; r < int(gridDim.x); ++r) {
-      const uint32_t n = counts[r * kBins + t];
-      if (r < int(blockIdx.x)) before += n;
-      all += n;
-    }
-    uint32_t sum = all;  // inclusive over the lanes' digits
+  // The runs' counts of a digit are added by four threads, eight loads of each in flight.
+  {
+    constexpr int PARTS = kSortThreads / kBins;
+    const int digit = t % kBins, part = t / kBins;
+    uint32_t before = 0, all = 0;
+    for (int r0 = part; r0 < int(gridDim.x); r0 += 8 * PARTS) {
+      uint32_t n[8];
 #pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const uint32_t up = __shfl_up(sum, m);
-      if (lane >= m) sum += up;
+      for (int k = 0; k < 8; ++k) n[k] = r0 + k * PARTS < int(gridDim.x) ? counts[(r0 + k * PARTS) * kBins + digit] : 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        all += n[k];
+        if (r0 + k * PARTS < int(blockIdx.x)) before += n[k];
+      }
     }
-    if (lane == 63) wave_sums[wave] = sum;
-    next[t] = sum - all + before;
+    of_wave[part][digit] = before;
+    of_wave[PARTS + part][digit] = all;
+    __syncthreads();
+    if (part == 0) {
+      before = all = 0;
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) before += of_wave[k][digit], all += of_wave[PARTS + k][digit];
+      uint32_t sum = all;  // inclusive over the lanes' digits
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const uint32_t up = __shfl_up(sum, m);
+        if (lane >= m) sum += up;
+      }
+      if (lane == 63) wave_sums[wave] = sum;
+      next[t] = sum - all + before;
+    }
   }
   __syncthreads();
   if (t < kBins)
@@ -158,20 +174,48 @@ __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* 
 }
 
 // ---- sums over the sorted positions -------------------------------------------
+// Rows of tokens that do not occur: a workgroup looks 64 of them up in the
+// sorted positions and clears those that are missing.
+template <typename T>
+__device__ inline void clear_missing(const Pair* __restrict__ sorted, int64_t N, int64_t vocabulary, int W,
+                                     int64_t group, T* __restrict__ table) {
+  constexpr int V = kChunk<T>;
+  const int64_t v0 = group * 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t v = v0 + lane;
+  int64_t lo = 0, hi = v < vocabulary ? N : 0;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (int64_t(sorted[mid].token) < v) lo = mid + 1;
+    else hi = mid;
+  }
+  const bool missing = v < vocabulary && !(lo < N && int64_t(sorted[lo].token) == v);
+  uint64_t rows = __ballot(missing);  // the same in every wave
+  const Chunk<T, V> zero = Chunk<T, V>::zero();
+  while (rows) {
+    const int r = __ffsll(static_cast<unsigned long long>(rows)) - 1;
+    rows &= rows - 1;
+    for (int c = int(threadIdx.x) * V; c < W; c += kThreads * V) zero.store(table + (v0 + r) * W + c, W - c);
+  }
+}
+
 // A worker is L lanes with a share of `share` sorted positions and a column
 // chunk of 16 bytes a lane (grid axis y over the columns that L lanes do not
-// hold).  The first token of a share may have begun before it and the last may
-// go on after it: their sums go to `heads` and `tails`, all others to the
-// table.  A share of one token has it as its head.  `ends` keeps the shares' first and last
-// token for the kernel that joins them.
+// hold).  Tokens that lie in the share go to the table.  The sum of a token that began
+// before the share, or fills it and goes on, goes to `heads`, that of one that begins in it and goes on to
+// `tails`; `ends` keeps the shares' first and last token for the kernel that joins them.
 template <typename T, int L>
 __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(
     const Pair* __restrict__ sorted, int64_t N, int64_t share, int64_t workers, const T* __restrict__ adjoint,
-    int64_t vocabulary, int W, typename Wide<T>::type scale, T* __restrict__ table,
+    int64_t vocabulary, int W, typename Wide<T>::type scale, int64_t clearing, T* __restrict__ table,
     typename Wide<T>::type* __restrict__ heads, typename Wide<T>::type* __restrict__ tails,
     uint32_t* __restrict__ ends) {
   typedef typename Wide<T>::type Real;
   constexpr int V = kChunk<T>, AHEAD = 8;
+  if (int64_t(gridDim.x) - blockIdx.x <= clearing) {  // the last workgroups
+    if (blockIdx.y == 0) clear_missing(sorted, N, vocabulary, W, int64_t(gridDim.x) - 1 - blockIdx.x, table);
+    return;
+  }
   const int lane = int(threadIdx.x) % L;
   const int64_t worker = int64_t(blockIdx.x) * (kThreads / L) + int(threadIdx.x) / L;
   const int c = (int(blockIdx.y) * L + lane) * V;
@@ -182,10 +226,10 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(
   for (int q = 0; q < V; ++q) sum[q] = Real(0);
   const uint32_t first = sorted[begin].token;
   uint32_t now = first;
-  bool head = true;
-  auto flush = [&](bool tail) {
-    if (head || tail) {
-      Real* to = (head ? heads : tails) + worker * W + c;
+  bool head = begin > 0 && sorted[begin - 1].token == first;  // began before
+  auto flush = [&](bool goes_on) {
+    if (head || goes_on) {
+      Real* to = (head || now == first ? heads : tails) + worker * W + c;
 #pragma unroll
       for (int q = 0; q < V; ++q)
         if (c + q < W) to[q] = sum[q];
@@ -219,90 +263,62 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(
       for (int q = 0; q < V; ++q) sum[q] += Real(g[k].v[q]);
     }
   }
-  flush(true);
+  flush(end < N && sorted[end].token == now);
   if (lane == 0 && blockIdx.y == 0) {
     ends[2 * worker] = first;
     ends[2 * worker + 1] = now;
   }
 }
 
-// Joins the shares' ends, a workgroup a share: one whose token begins in it (the tail, or the
-// head where the share before ends with another token) adds the heads of the
-// shares after it that go on with that token.  Eight rows of lanes take the
-// shares in turn and are added in order.
+// Joins a token that crosses the ends of shares: the workgroups of the share where it
+// begins add the sums of the shares that it goes on in, found by bisection (the shares'
+// first tokens do not fall).  Eight rows of lanes take the shares in turn, eight loads
+// of each in flight, and are added in order.  Grid axis y takes columns in steps of 32: 2 600
+// shares of one token, 128 columns, took 330 us by one load a lane and all columns in
+// one workgroup.
+constexpr int kJoinColumns = 32, kJoinGroups = 8;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void embedding_join_kernel(
     const uint32_t* __restrict__ ends, int64_t workers, const typename Wide<T>::type* __restrict__ heads,
     const typename Wide<T>::type* __restrict__ tails, int64_t vocabulary, int W, typename Wide<T>::type scale,
     T* __restrict__ table) {
   typedef typename Wide<T>::type Real;
-  constexpr int ROWS = 8, COLS = kThreads / ROWS;
-  __shared__ Real sums[ROWS][COLS];
-  __shared__ int64_t stop;
+  constexpr int COLS = kJoinColumns, ROWS = kThreads / COLS, AHEAD = 8;
+  __shared__ Real sums[ROWS][COLS + 1];
   const int64_t w = blockIdx.x;
   const int col = int(threadIdx.x) % COLS, row = int(threadIdx.x) / COLS;
-  const uint32_t first = ends[2 * w], last = ends[2 * w + 1];
-  for (int which = 0; which < 2; ++which) {
-    // 0: the head, if its token begins here; 1: the tail, if the share has one
-    const uint32_t token = which == 0 ? first : last;
-    if (which == 0 ? (w > 0 && ends[2 * w - 1] == first) : first == last) continue;
-    if (int64_t(token) >= vocabulary) continue;
-    if (threadIdx.x == 0) {
-      // only a token that is the share's last can go on: the shares that begin
-      // with it are a run, found by bisection (first tokens do not fall)
-      int64_t lo = w + 1, hi = workers;
-      if (token != last) hi = lo;
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (ends[2 * mid] == token) lo = mid + 1;
-        else hi = mid;
-      }
-      stop = lo;
-    }
-    __syncthreads();
-    const int64_t until = stop;
-    for (int c0 = 0; c0 < W; c0 += COLS) {
-      const int c = c0 + col;
-      Real s = Real(0);
-      if (c < W) {
-        if (row == 0) s = (which == 0 ? heads : tails)[w * W + c];
-        for (int64_t k = w + 1 + row; k < until; k += ROWS) s += heads[k * W + c];
-      }
-      sums[row][col] = s;
-      __syncthreads();
-      if (row == 0 && c < W) {
-        Real t = Real(0);
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) t += sums[r][col];
-        table[int64_t(token) * W + c] = T(t * scale);
-      }
-      __syncthreads();
-    }
-  }
-}
-
-// Rows of tokens that do not occur: a workgroup looks 64 of them up in the
-// sorted positions and clears those that are missing.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void embedding_clear_kernel(const Pair* __restrict__ sorted, int64_t N,
-                                                                   int64_t vocabulary, int W, T* __restrict__ table) {
-  constexpr int V = kChunk<T>;
-  const int64_t v0 = int64_t(blockIdx.x) * 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t v = v0 + lane;
-  int64_t lo = 0, hi = v < vocabulary ? N : 0;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (int64_t(sorted[mid].token) < v) lo = mid + 1;
+  const uint32_t first = ends[2 * w], token = ends[2 * w + 1];
+  if (w + 1 == workers || ends[2 * w + 2] != token || int64_t(token) >= vocabulary) return;  // ends here
+  if (first == token && w > 0 && ends[2 * w - 1] == token) return;                           // does not begin here
+  int64_t until = w + 2, hi = workers;
+  while (until < hi) {
+    const int64_t mid = (until + hi) >> 1;
+    if (ends[2 * mid] == token) until = mid + 1;
     else hi = mid;
   }
-  const bool missing = v < vocabulary && !(lo < N && int64_t(sorted[lo].token) == v);
-  uint64_t rows = __ballot(missing);  // the same in every wave
-  const Chunk<T, V> zero = Chunk<T, V>::zero();
-  while (rows) {
-    const int r = __ffsll(static_cast<unsigned long long>(rows)) - 1;
-    rows &= rows - 1;
-    for (int c = int(threadIdx.x) * V; c < W; c += kThreads * V) zero.store(table + (v0 + r) * W + c, W - c);
+  for (int c0 = int(blockIdx.y) * COLS; c0 < W; c0 += int(gridDim.y) * COLS) {
+    const int c = c0 + col;
+    Real s = Real(0);
+    if (c < W) {
+      if (row == 0) s = (first == token ? heads : tails)[w * W + c];
+      for (int64_t k0 = w + 1 + row; k0 < until; k0 += AHEAD * ROWS) {
+        Real v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) v[k] = k0 + k * ROWS < until ? heads[(k0 + k * ROWS) * W + c] : Real(0);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) s += v[k];
+      }
+    }
+    sums[row][col] = s;
+    __syncthreads();
+    if (row == 0 && c < W) {
+      Real t = Real(0);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) t += sums[r][col];
+      table[int64_t(token) * W + c] = T(t * scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -313,8 +329,9 @@ struct GradientPlan {
 };
 
 // Sorting: runs of at least 2 048 positions, 128 of them at most.  Sums: lanes
-// enough for a row (256 at most), and shares that give the card about eight
-// waves a SIMD, of 16 positions or more.
+// enough for a row (256 at most), and shares that give the card about two
+// waves a SIMD, of 16 positions or more: eight rows of a lane are in flight at a time, so
+// that is 8 MB of them, and every further share is one more end to join.
 GradientPlan gradient_plan(int64_t N, int64_t vocabulary, int64_t width, int size) {
   GradientPlan p{};
   for (p.passes = 1; p.passes < 4 && (vocabulary >> (8 * p.passes)) > 0; ++p.passes) {}
@@ -324,9 +341,9 @@ GradientPlan gradient_plan(int64_t N, int64_t vocabulary, int64_t width, int siz
   const int V = 16 / size;
   const int64_t chunks = (width + V - 1) / V;
   p.L = 4;
-  while (p.L < kThreads && p.L < chunks) p.L *= 4;
+  while (p.L < kThreads && p.L < chunks) p.L *= 2;
   p.columns = int((chunks + p.L - 1) / p.L);
-  const int64_t most = int64_t(256) * 4 * 8 * 64 / p.L;
+  const int64_t most = int64_t(256) * 4 * 2 * 64 / p.L;
   p.share = (N + most - 1) / most;
   if (p.share < 16) p.share = 16;
   p.workers = (N + p.share - 1) / p.share;
@@ -367,18 +384,22 @@ int gradient_as(const T* adjoint, const Index* tokens, int64_t N, int64_t vocabu
   }
   const Pair* sorted = pairs[(p.passes - 1) & 1];
   const int W = int(width);
-  hipLaunchKernelGGL((embedding_clear_kernel<T>), dim3(unsigned((vocabulary + 63) / 64)), dim3(kThreads), 0, s, sorted,
-                     N, vocabulary, W, table);
-  if (int rc = check_launch("embedding_clear_kernel")) return rc;
-  if (N == 0) return YE3T_OK;
-  const auto sum = p.L == 4 ? embedding_sum_kernel<T, 4>
-                            : p.L == 16 ? embedding_sum_kernel<T, 16>
-                                        : p.L == 64 ? embedding_sum_kernel<T, 64> : embedding_sum_kernel<T, 256>;
-  const int64_t per = kThreads / p.L;
-  hipLaunchKernelGGL(sum, dim3(unsigned((p.workers + per - 1) / per), unsigned(p.columns)), dim3(kThreads), 0, s,
-                     sorted, N, p.share, p.workers, adjoint, vocabulary, W, Real(scale), table, heads, tails, ends);
+  const auto sum = p.L == 4     ? embedding_sum_kernel<T, 4>
+                   : p.L == 8   ? embedding_sum_kernel<T, 8>
+                   : p.L == 16  ? embedding_sum_kernel<T, 16>
+                   : p.L == 32  ? embedding_sum_kernel<T, 32>
+                   : p.L == 64  ? embedding_sum_kernel<T, 64>
+                   : p.L == 128 ? embedding_sum_kernel<T, 128>
+                                : embedding_sum_kernel<T, 256>;
+  const int64_t per = kThreads / p.L, clearing = (vocabulary + 63) / 64;
+  hipLaunchKernelGGL(sum, dim3(unsigned((p.workers + per - 1) / per + clearing), unsigned(p.columns)), dim3(kThreads),
+                     0, s, sorted, N, p.share, p.workers, adjoint, vocabulary, W, Real(scale), clearing, table, heads,
+                     tails, ends);
   if (int rc = check_launch("embedding_sum_kernel")) return rc;
-  hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(unsigned(p.workers)), dim3(kThreads), 0, s, ends, p.workers,
+  if (p.workers < 2) return YE3T_OK;
+  const int64_t columns = (width + kJoinColumns - 1) / kJoinColumns;
+  hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(unsigned(p.workers), unsigned(columns < kJoinGroups ? columns : kJoinGroups)),
+                     dim3(kThreads), 0, s, ends, p.workers,
                      heads, tails, vocabulary, W, Real(scale), table);
   return check_launch("embedding_join_kernel");
 }

@@ -697,7 +697,8 @@ def __getattr__(name):
                 "atom_attention_adjoint"):
         import importlib
 
-        return getattr(importlib.import_module("ye3t_amd.runtime.atoms"), name)
+        globals()[name] = value = getattr(importlib.import_module("ye3t_amd.runtime.atoms"), name)
+        return value
     if name in ("ExecutionPlan", "YE3TExecutionPlan"):
         from ye3t_amd.runtime.execution_plan import ExecutionPlan
 

@@ -1913,6 +1913,30 @@ def _storage_code(dtype, double=False):
     raise TypeError(f"unsupported dtype {dtype}; expected float32{', float64' if double else ''} or bfloat16")
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """The tensors' device as the current one; nothing where it is already."""
+    import torch
+
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _raw_stream():
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _workspace(size, what, device):
     """``size`` bytes of device memory, of the caching allocator on the current stream."""
     import torch
@@ -1933,9 +1957,9 @@ def embedding(tokens, table, scale):
         return out
     if (table.stride(1) != 1 and W > 1) or table.stride(0) < 0:
         table = table.contiguous()
-    with torch.cuda.device(table.device):
+    with _on(table.device):
         _check(lib().ye3t_hip_embedding(code, _dev(tokens, "tokens"), tokens.element_size(), tokens.numel(),
-                                        table.data_ptr(), table.stride(0), V, W, scale, out.data_ptr(), _stream()),
+                                        table.data_ptr(), table.stride(0), V, W, scale, out.data_ptr(), _raw_stream()),
                "ye3t_hip_embedding")
     return out
 
@@ -1949,12 +1973,12 @@ def embedding_adjoint(adjoint, tokens, rows, scale):
     out = torch.empty((rows, W), dtype=adjoint.dtype, device=adjoint.device)
     if out.numel() == 0:
         return out
-    with torch.cuda.device(adjoint.device):
+    with _on(adjoint.device):
         size = lib().ye3t_hip_embedding_adjoint_workspace_bytes(code, N, rows, W)
         work = _workspace(size, "ye3t_hip_embedding_adjoint_workspace_bytes", adjoint.device)
         _check(lib().ye3t_hip_embedding_adjoint(code, _dev(adjoint, "adjoint"), _dev(tokens, "tokens"),
                                                 tokens.element_size(), N, rows, W, scale, out.data_ptr(),
-                                                work.data_ptr(), size, _stream()), "ye3t_hip_embedding_adjoint")
+                                                work.data_ptr(), size, _raw_stream()), "ye3t_hip_embedding_adjoint")
     return out
 
 
@@ -1967,10 +1991,10 @@ def rms_norm(input, weight, residual, epsilon):
     y = torch.empty_like(input)
     total = None if residual is None else torch.empty_like(input)
     if W:
-        with torch.cuda.device(input.device):
+        with _on(input.device):
             _check(lib().ye3t_hip_rms_norm(code, _dev(input, "input"), _opt(residual, "residual"),
                                            _dev(weight, "weight"), input.numel() // W, W, epsilon,
-                                           _opt(total, "total"), y.data_ptr(), _stream()), "ye3t_hip_rms_norm")
+                                           _opt(total, "total"), y.data_ptr(), _raw_stream()), "ye3t_hip_rms_norm")
     return y, total
 
 
@@ -1984,10 +2008,10 @@ def rms_norm_8bit(input, weight, residual, epsilon):
     scales = torch.empty((*input.shape[:-1], -(-W // 128)), dtype=torch.float32, device=input.device)
     total = None if residual is None else torch.empty_like(input)
     if W:
-        with torch.cuda.device(input.device):
+        with _on(input.device):
             _check(lib().ye3t_hip_rms_norm_8bit(code, _dev(input, "input"), _opt(residual, "residual"),
                                                 _dev(weight, "weight"), input.numel() // W, W, epsilon,
-                                                _opt(total, "total"), codes.data_ptr(), scales.data_ptr(), _stream()),
+                                                _opt(total, "total"), codes.data_ptr(), scales.data_ptr(), _raw_stream()),
                    "ye3t_hip_rms_norm_8bit")
     return codes, scales, total
 
@@ -2001,12 +2025,12 @@ def rms_norm_adjoint(adjoint, total, weight, total_adjoint, epsilon):
     dx, dw = torch.empty_like(total), torch.empty_like(weight)
     if W:
         rows = total.numel() // W
-        with torch.cuda.device(total.device):
+        with _on(total.device):
             size = lib().ye3t_hip_rms_norm_adjoint_workspace_bytes(code, rows, W)
             work = _workspace(size, "ye3t_hip_rms_norm_adjoint_workspace_bytes", total.device)
             _check(lib().ye3t_hip_rms_norm_adjoint(code, _dev(adjoint, "adjoint"), _opt(total_adjoint, "total_adjoint"),
                                                    _dev(total, "total"), _dev(weight, "weight"), rows, W, epsilon,
-                                                   dx.data_ptr(), dw.data_ptr(), work.data_ptr(), size, _stream()),
+                                                   dx.data_ptr(), dw.data_ptr(), work.data_ptr(), size, _raw_stream()),
                    "ye3t_hip_rms_norm_adjoint")
     return dx, dw
 
@@ -2050,11 +2074,11 @@ class Attention:
         q = self.query
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         sums = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if with_sums else None
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             size = lib().ye3t_hip_atom_attention_workspace_bytes(ctypes.byref(self.args))
             work = _workspace(size, "ye3t_hip_atom_attention_workspace_bytes", q.device) if size else None
             _check(lib().ye3t_hip_atom_attention(ctypes.byref(self.args), out.data_ptr(), _opt(sums, "log_sums"),
-                                                 _opt(work, "workspace"), size, _stream()), "ye3t_hip_atom_attention")
+                                                 _opt(work, "workspace"), size, _raw_stream()), "ye3t_hip_atom_attention")
         return out, sums
 
     def adjoint(self, adjoint, out, sums, bias):
@@ -2066,12 +2090,12 @@ class Attention:
         ds = torch.empty_like(self.slopes) if bias else None
         dp = torch.empty_like(self.positions) if bias else None
         dkp = torch.empty_like(self.key_positions) if bias and self.key_positions is not None else None
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             size = lib().ye3t_hip_atom_attention_adjoint_workspace_bytes(ctypes.byref(self.args), int(bias))
             work = _workspace(size, "ye3t_hip_atom_attention_adjoint_workspace_bytes", q.device)
             _check(lib().ye3t_hip_atom_attention_adjoint(
                 ctypes.byref(self.args), _dev(out, "out"), _dev(sums, "log_sums"), _dev(adjoint, "adjoint"),
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _opt(ds, "slopes_adjoint"), _opt(dp, "positions_adjoint"),
-                _opt(dkp, "key_positions_adjoint"), work.data_ptr(), size, _stream()),
+                _opt(dkp, "key_positions_adjoint"), work.data_ptr(), size, _raw_stream()),
                 "ye3t_hip_atom_attention_adjoint")
         return dq, dk, dv, ds, dp, dkp
