@@ -19,20 +19,30 @@ constexpr int kThreads = 256;
 constexpr int kScaleGroup = 128;  // columns that share a scale of the 8-bit rows
 constexpr float kLargest8 = 448.0f;
 
-// Sum over the L lanes that share a row; every lane gets the same bits.
+// Sums of two values over the L lanes that share a row; every lane gets the same
+// bits.  `part` has two places for each wave.
 template <int L>
-__device__ inline float row_sum(float v, float* part) {
+__device__ inline void row_sums(float& a, float& b, float* part) {
 #pragma unroll
-  for (int m = 1; m < (L < 64 ? L : 64); m *= 2) v += __shfl_xor(v, m);
-  if constexpr (L > 64) {
-    __syncthreads();  // the last sum's parts have been read
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < L / 64; ++w) v += part[w];
+  for (int m = 1; m < (L < 64 ? L : 64); m *= 2) {
+    const float x = __shfl_xor(a, m), y = __shfl_xor(b, m);
+    a += x;
+    b += y;
   }
-  return v;
+  if constexpr (L > 64) {
+    __syncthreads();  // the last sums' parts have been read
+    if ((threadIdx.x & 63) == 0) {
+      part[2 * (threadIdx.x >> 6)] = a;
+      part[2 * (threadIdx.x >> 6) + 1] = b;
+    }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < L / 64; ++w) {
+      a += part[2 * w];
+      b += part[2 * w + 1];
+    }
+  }
 }
 
 enum { kPlain = 0, kEightBit = 1 };
@@ -45,7 +55,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(const T* __restrict_
                                                             uint8_t* __restrict__ codes, float* __restrict__ scales) {
   constexpr int V = kChunk<T>;
   constexpr int H = K > 0 ? K : 1;
-  __shared__ float part[kThreads / 64];
+  __shared__ float part[2 * kThreads / 64];
   const int lane = int(threadIdx.x) % L, per = kThreads / L;
   const int groups = (W + kScaleGroup - 1) / kScaleGroup;
   for (int64_t row = int64_t(blockIdx.x) * per + int(threadIdx.x) / L; row < rows; row += int64_t(gridDim.x) * per) {
@@ -83,7 +93,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(const T* __restrict_
 #pragma unroll
       for (int q = 0; q < V; ++q) square += v[q] * v[q];
     }
-    square = row_sum<L>(square, part);
+    float unused = 0.0f;
+    row_sums<L>(square, unused, part);
     const float rho = 1.0f / sqrtf(square / float(W) + epsilon);
 #pragma unroll
     for (int k = 0, c = lane * V; K > 0 ? k < K : c < (W + L * V - 1) / (L * V) * (L * V); ++k, c += L * V) {
@@ -96,43 +107,38 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(const T* __restrict_
           for (int q = 0; q < V; ++q) v[q] = 0.0f;
         }
       }
-      float out[V];
-      if (c < W) {
-        keep_total(c, v);
-        const Chunk<T, V> w = Chunk<T, V>::load(weight + c, W - c);
-#pragma unroll
-        for (int q = 0; q < V; ++q) out[q] = v[q] * rho * float(w.v[q]);
-        if constexpr (MODE == kPlain) {
+      if (c < W) keep_total(c, v);
+      const Chunk<T, V> w = c < W ? Chunk<T, V>::load(weight + c, W - c) : Chunk<T, V>::zero();
+      if constexpr (MODE == kPlain) {
+        if (c < W) {
           Chunk<T, V> a;
 #pragma unroll
-          for (int q = 0; q < V; ++q) a.v[q] = T(out[q]);
+          for (int q = 0; q < V; ++q) a.v[q] = T(v[q] * rho * float(w.v[q]));
           a.store(y + row * W + c, W - c);
         }
-      }
-      if constexpr (MODE == kEightBit) {
-        // The 128 columns of a scale are 128 / V neighbouring lanes of a step.
-        float top = 0.0f;
-        if (c < W) {
+      } else {
+        // The 128 columns of a scale are 128 / V neighbouring lanes of a step.  rho
+        // cancels in y / scale = 448 h w / max|h w|, which is formed in fp64 (h w is
+        // exact there), so that a code is wrong only where h is.
+        double out[V], top = 0.0;
 #pragma unroll
-          for (int q = 0; q < V; ++q) top = fmaxf(top, fabsf(out[q]));
+        for (int q = 0; q < V; ++q) {
+          out[q] = double(v[q]) * double(float(w.v[q]));
+          top = fmax(top, fabs(out[q]));
         }
 #pragma unroll
-        for (int m = 1; m < kScaleGroup / V; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
+        for (int m = 1; m < kScaleGroup / V; m *= 2) top = fmax(top, __shfl_xor(top, m));
         if (c < W) {
-          const float scale = top / kLargest8;
+          const float scale = float(top * double(rho)) / kLargest8;
           if (c % kScaleGroup == 0) scales[row * groups + c / kScaleGroup] = scale;
+          // columns of zeros have scale 0 and codes 0; what is not a number stays so
+          const double per = scale > 0.0f ? double(kLargest8) / top : double(scale);
           uint32_t packed[V / 4];
-#pragma unroll
-          for (int q = 0; q < V; ++q) {
-            // a group of zeros has scale 0 and codes 0; what is not a number stays so
-            out[q] = scale > 0.0f ? out[q] / scale : out[q];
-            out[q] = out[q] > kLargest8 ? kLargest8 : (out[q] < -kLargest8 ? -kLargest8 : out[q]);
-          }
 #pragma unroll
           for (int q = 0; q < V / 4; ++q) {
             int word = 0;
-            word = __builtin_amdgcn_cvt_pk_fp8_f32(out[4 * q], out[4 * q + 1], word, false);
-            word = __builtin_amdgcn_cvt_pk_fp8_f32(out[4 * q + 2], out[4 * q + 3], word, true);
+            word = __builtin_amdgcn_cvt_pk_fp8_f32(float(out[4 * q] * per), float(out[4 * q + 1] * per), word, false);
+            word = __builtin_amdgcn_cvt_pk_fp8_f32(float(out[4 * q + 2] * per), float(out[4 * q + 3] * per), word, true);
             packed[q] = uint32_t(word);
           }
           Chunk<uint8_t, V> a;
@@ -148,9 +154,10 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(const T* __restrict_
 // The gradient: a workgroup walks over rows and keeps its sums of the weight's
 // gradient, a lane those of its own columns; they are added over the
 // workgroup's groups and written as one of `gridDim.x` partial rows, which
-// rms_norm_weight_kernel adds in order.  K = 0: the row is read twice and the
-// sums stand in the workgroup's own partial row in memory, where each column
-// belongs to one lane.
+// rms_norm_weight_kernel adds in order.  The next row is read while the present
+// one is summed: a row is one round trip to memory and two sums over lanes, and by itself
+// that is all a wave does.  K = 0: the row is read twice and the sums stand in the workgroup's
+// own partial row in memory, where each column belongs to one lane.
 template <typename T, int L, int K>
 __global__ __launch_bounds__(kThreads) void rms_norm_adjoint_kernel(const T* __restrict__ adjoint,
                                                                     const T* __restrict__ total_adjoint,
@@ -161,72 +168,68 @@ __global__ __launch_bounds__(kThreads) void rms_norm_adjoint_kernel(const T* __r
   constexpr int V = kChunk<T>;
   constexpr int H = K > 0 ? K : 1;
   constexpr int per = kThreads / L;
-  __shared__ float part[kThreads / 64];
+  typedef Chunk<T, V> C;
+  __shared__ float part[2 * kThreads / 64];
   __shared__ float shared_dw[K > 0 && per > 1 ? L * K * V : 1];
   const int lane = int(threadIdx.x) % L;
   const int group = int(threadIdx.x) / L;
   float* mine = partial + int64_t(blockIdx.x) * W;
-  float dw[H][V];
-#pragma unroll
-  for (int k = 0; k < H; ++k)
-#pragma unroll
-    for (int q = 0; q < V; ++q) dw[k][q] = 0.0f;
-  if (K == 0) {
-    for (int c = threadIdx.x; c < W; c += kThreads) mine[c] = 0.0f;
-    __syncthreads();
-  }
-  for (int64_t row = int64_t(blockIdx.x) * per + group; row < rows; row += int64_t(gridDim.x) * per) {
-    const T* hr = total + row * W;
-    const T* gr = adjoint + row * W;
-    const T* tr = total_adjoint ? total_adjoint + row * W : nullptr;
-    float h[H][V], g[H][V];
-    float square = 0.0f, along = 0.0f;
-    auto read = [&](int c, float* hv, float* gv) {
-      const Chunk<T, V> a = Chunk<T, V>::load(hr + c, W - c), b = Chunk<T, V>::load(gr + c, W - c);
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        hv[q] = float(a.v[q]);
-        gv[q] = float(b.v[q]);
-      }
+  const int64_t step = int64_t(gridDim.x) * per;
+  int64_t row = int64_t(blockIdx.x) * per + group;
+  if constexpr (K > 0) {
+    struct RowOf {
+      C h[H], g[H], t[H];
     };
+    C w[H];
+    float dw[H][V];
 #pragma unroll
-    for (int k = 0, c = lane * V; K > 0 ? k < K : c < W; ++k, c += L * V) {
-      float *hv = h[K > 0 ? k : 0], *gv = g[K > 0 ? k : 0];
-      if (c < W) {
-        read(c, hv, gv);
-        const Chunk<T, V> w = Chunk<T, V>::load(weight + c, W - c);
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * L + lane) * V;
+      w[k] = c < W ? C::load(weight + c, W - c) : C::zero();
+#pragma unroll
+      for (int q = 0; q < V; ++q) dw[k][q] = 0.0f;
+    }
+    auto read = [&](int64_t r) {
+      RowOf x;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + lane) * V;
+        x.h[k] = c < W ? C::load(total + r * W + c, W - c) : C::zero();
+        x.g[k] = c < W ? C::load(adjoint + r * W + c, W - c) : C::zero();
+        x.t[k] = c < W && total_adjoint ? C::load(total_adjoint + r * W + c, W - c) : C::zero();
+      }
+      return x;
+    };
+    RowOf next;
+    if (row < rows) next = read(row);
+    for (; row < rows; row += step) {
+      const RowOf x = next;
+      if (row + step < rows) next = read(row + step);
+      float square = 0.0f, along = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-          square += hv[q] * hv[q];
-          along += hv[q] * (gv[q] * float(w.v[q]));
+          const float h = float(x.h[k].v[q]);
+          square += h * h;
+          along += h * (float(x.g[k].v[q]) * float(w[k].v[q]));
         }
+      row_sums<L>(square, along, part);
+      const float rho = 1.0f / sqrtf(square / float(W) + epsilon);
+      const float pull = along / float(W) * rho * rho;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * L + lane) * V;
+        C a;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          const float h = float(x.h[k].v[q]), g = float(x.g[k].v[q]);
+          a.v[q] = T(rho * (g * float(w[k].v[q]) - h * pull) + float(x.t[k].v[q]));
+          dw[k][q] += g * h * rho;
+        }
+        if (c < W) a.store(dx + row * W + c, W - c);
       }
     }
-    square = row_sum<L>(square, part);
-    along = row_sum<L>(along, part);
-    const float rho = 1.0f / sqrtf(square / float(W) + epsilon);
-    const float pull = along / float(W) * rho * rho;
-#pragma unroll
-    for (int k = 0, c = lane * V; K > 0 ? k < K : c < W; ++k, c += L * V) {
-      float *hv = h[K > 0 ? k : 0], *gv = g[K > 0 ? k : 0];
-      if (c >= W) continue;
-      if (K == 0) read(c, hv, gv);
-      const Chunk<T, V> w = Chunk<T, V>::load(weight + c, W - c);
-      Chunk<T, V> t = Chunk<T, V>::zero();
-      if (tr) t = Chunk<T, V>::load(tr + c, W - c);
-      Chunk<T, V> a;
-#pragma unroll
-      for (int q = 0; q < V; ++q) a.v[q] = T(rho * (gv[q] * float(w.v[q]) - hv[q] * pull) + float(t.v[q]));
-      a.store(dx + row * W + c, W - c);
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const float part_dw = gv[q] * hv[q] * rho;
-        if (K > 0) dw[k][q] += part_dw;
-        else if (c + q < W) mine[c + q] += part_dw;
-      }
-    }
-  }
-  if constexpr (K > 0) {
     // groups in turn, so that the order of the sums is fixed
     for (int turn = 0; turn < per; ++turn) {
       if (group == turn) {
@@ -247,6 +250,37 @@ __global__ __launch_bounds__(kThreads) void rms_norm_adjoint_kernel(const T* __r
       }
       if (per > 1) __syncthreads();
     }
+  } else {
+    for (int c = threadIdx.x; c < W; c += kThreads) mine[c] = 0.0f;
+    __syncthreads();
+    for (; row < rows; row += step) {
+      float square = 0.0f, along = 0.0f;
+      for (int c = lane * V; c < W; c += L * V) {
+        const C h = C::load(total + row * W + c, W - c), g = C::load(adjoint + row * W + c, W - c),
+                w = C::load(weight + c, W - c);
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          square += float(h.v[q]) * float(h.v[q]);
+          along += float(h.v[q]) * (float(g.v[q]) * float(w.v[q]));
+        }
+      }
+      row_sums<L>(square, along, part);
+      const float rho = 1.0f / sqrtf(square / float(W) + epsilon);
+      const float pull = along / float(W) * rho * rho;
+      for (int c = lane * V; c < W; c += L * V) {
+        const C hc = C::load(total + row * W + c, W - c), gc = C::load(adjoint + row * W + c, W - c),
+                w = C::load(weight + c, W - c);
+        const C t = total_adjoint ? C::load(total_adjoint + row * W + c, W - c) : C::zero();
+        C a;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          const float h = float(hc.v[q]), g = float(gc.v[q]);
+          a.v[q] = T(rho * (g * float(w.v[q]) - h * pull) + float(t.v[q]));
+          if (c + q < W) mine[c + q] += g * h * rho;
+        }
+        a.store(dx + row * W + c, W - c);
+      }
+    }
   }
 }
 
@@ -259,8 +293,15 @@ __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float* __re
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = int(blockIdx.x) * 64 + lane;
   float s = 0.0f;
-  if (c < W)
-    for (int p = wave; p < count; p += 16) s += partial[int64_t(p) * W + c];
+  if (c < W) {
+    for (int p0 = wave; p0 < count; p0 += 16 * 8) {  // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = p0 + 16 * k < count ? partial[int64_t(p0 + 16 * k) * W + c] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+  }
   sums[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < W) {
@@ -274,11 +315,12 @@ __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float* __re
 // Workgroups that fill the card: eight of four waves in a compute unit.
 inline int resident_groups(int64_t wanted) { return int(wanted < 2048 ? (wanted < 1 ? 1 : wanted) : 2048); }
 
-// Partial rows of the weight's gradient: fewer for wide rows, so that they stay
-// a small part of the traffic.
-inline int partial_rows(int64_t rows, int per) {
-  int64_t n = (rows + per - 1) / per;
-  return int(n < 1024 ? (n < 1 ? 1 : n) : 1024);
+// Partial rows of the weight's gradient, a workgroup each: eight workgroups a
+// compute unit, four for wide rows, whose partial rows would be a larger part of the traffic and
+// whose lanes have more in flight.
+inline int partial_rows(int64_t rows, int per, int64_t width) {
+  const int64_t n = (rows + per - 1) / per, most = width <= 512 ? 2048 : 1024;
+  return int(n < most ? (n < 1 ? 1 : n) : most);
 }
 
 struct Shape {
@@ -287,12 +329,16 @@ struct Shape {
 
 // The group and the chunks of a row of `width` values: the smallest group that
 // holds it in at most eight chunks of 16 bytes a lane (four for the gradient,
-// which keeps three values for each); 0 chunks where 256 lanes do not.
-inline Shape shape_of(int width, int V, int most, int least) {
+// which keeps three values for each); 0 chunks where 256 lanes do not.  Rows too few
+// for a wave on every SIMD are latency, and take four waves if one would hold more than a
+// chunk a lane: 37 rows of 4 096 in bf16, 8 bits, 11.6 us by one wave, 5.1 by four.
+constexpr int64_t kFewRows = 1024;
+
+inline Shape shape_of(int64_t rows, int width, int V, int most, int least) {
   const int lanes[4] = {4, 16, 64, 256};
   for (int i = 0; i < 4; ++i) {
     if (lanes[i] < least) continue;
-    const int limit = lanes[i] < 64 ? 2 : most;
+    const int limit = lanes[i] < 64 ? 2 : lanes[i] == 64 && rows <= kFewRows ? 1 : most;
     const int k = (width + lanes[i] * V - 1) / (lanes[i] * V);
     if (k <= limit) return {lanes[i], k <= 1 ? 1 : k <= 2 ? 2 : k <= 4 ? 4 : 8};
   }
@@ -332,7 +378,7 @@ int forward_shaped(Shape sh, A... a) {
 template <typename T, int L, int K>
 int adjoint_as(const void* g, const void* tg, const void* h, const void* w, int64_t rows, int W, float eps, void* dx,
                void* dw, void* workspace, hipStream_t s) {
-  const int count = partial_rows(rows, kThreads / L);
+  const int count = partial_rows(rows, kThreads / L, W);
   float* partial = static_cast<float*>(workspace);
   hipLaunchKernelGGL((rms_norm_adjoint_kernel<T, L, K>), dim3(count), dim3(kThreads), 0, s, static_cast<const T*>(g),
                      static_cast<const T*>(tg), static_cast<const T*>(h), static_cast<const T*>(w), rows, W, eps,
@@ -367,8 +413,8 @@ int check_norm(int dtype, int64_t rows, int64_t width, double epsilon) {
   return YE3T_OK;
 }
 
-inline Shape adjoint_shape(int dtype, int64_t width) {
-  return shape_of(int(width), dtype == YE3T_F32 ? kChunk<float> : kChunk<__bf16>, 4, 1);
+inline Shape adjoint_shape(int dtype, int64_t rows, int64_t width) {
+  return shape_of(rows, int(width), dtype == YE3T_F32 ? kChunk<float> : kChunk<__bf16>, 4, 1);
 }
 
 }  // namespace
@@ -389,9 +435,9 @@ int ye3t_hip_rms_norm(int dtype, const void* x, const void* residual, const void
   const float eps = float(epsilon);
   void* none = nullptr;
   if (dtype == YE3T_F32)
-    return forward_shaped<float, kPlain>(shape_of(W, kChunk<float>, 8, 1), x, residual, weight, rows, W, eps, total, y,
+    return forward_shaped<float, kPlain>(shape_of(rows, W, kChunk<float>, 8, 1), x, residual, weight, rows, W, eps, total, y,
                                          none, none, as_stream(stream));
-  return forward_shaped<__bf16, kPlain>(shape_of(W, kChunk<__bf16>, 8, 1), x, residual, weight, rows, W, eps, total, y,
+  return forward_shaped<__bf16, kPlain>(shape_of(rows, W, kChunk<__bf16>, 8, 1), x, residual, weight, rows, W, eps, total, y,
                                         none, none, as_stream(stream));
 }
 
@@ -408,16 +454,16 @@ int ye3t_hip_rms_norm_8bit(int dtype, const void* x, const void* residual, const
   void* none = nullptr;
   // a scale's 128 columns lie in one wave: 32 lanes in fp32
   if (dtype == YE3T_F32)
-    return forward_shaped<float, kEightBit>(shape_of(W, kChunk<float>, 8, 64), x, residual, weight, rows, W, eps, total,
+    return forward_shaped<float, kEightBit>(shape_of(rows, W, kChunk<float>, 8, 64), x, residual, weight, rows, W, eps, total,
                                             none, codes, scales, as_stream(stream));
-  return forward_shaped<__bf16, kEightBit>(shape_of(W, kChunk<__bf16>, 8, 64), x, residual, weight, rows, W, eps, total,
+  return forward_shaped<__bf16, kEightBit>(shape_of(rows, W, kChunk<__bf16>, 8, 64), x, residual, weight, rows, W, eps, total,
                                            none, codes, scales, as_stream(stream));
 }
 
 int64_t ye3t_hip_rms_norm_adjoint_workspace_bytes(int dtype, int64_t rows, int64_t width) {
   clear_error();
   if (check_norm(dtype, rows, width, 1.0)) return -1;
-  return int64_t(partial_rows(rows, kThreads / adjoint_shape(dtype, width).L)) * width * int64_t(sizeof(float));
+  return int64_t(partial_rows(rows, kThreads / adjoint_shape(dtype, rows, width).L, width)) * width * int64_t(sizeof(float));
 }
 
 int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_adjoint, const void* total,
@@ -429,7 +475,7 @@ int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_
   YE3T_REQUIRE(rows == 0 || (adjoint && total && x_adjoint), "the gradient needs the adjoint, the sum and an output");
   YE3T_REQUIRE(workspace && workspace_bytes >= ye3t_hip_rms_norm_adjoint_workspace_bytes(dtype, rows, width),
                "the workspace is smaller than ye3t_hip_rms_norm_adjoint_workspace_bytes");
-  const Shape sh = adjoint_shape(dtype, width);
+  const Shape sh = adjoint_shape(dtype, rows, width);
   const int W = int(width);
   const float eps = float(epsilon);
   if (dtype == YE3T_F32)
