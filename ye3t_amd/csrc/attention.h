@@ -37,7 +37,8 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2eExact = 1.4426950408889634;
+constexpr float kLog2e = float(kLog2eExact);
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Problem {
@@ -48,6 +49,7 @@ struct Problem {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   const int64_t *offsets, *key_offsets;
   float scale, cap;
+  float to_log2, to_bend, from_bend;  // of scores: scale in units of log2; the same of 2 / cap; cap in units of log2
   const float *slopes, *positions, *key_positions;
   const uint8_t* key_mask;
 };
@@ -83,6 +85,17 @@ __device__ inline f32x16 zeros() {
   return z;
 }
 
+// The same value; with FRESH unknown to the compiler, so that addresses made from it in
+// a loop are formed there, a few operations a tile, instead of being held in
+// registers.  For short structures, a tile or two a wave, where more waves count
+// for more: 2 000 molecules of 21 atoms, fp32, gradients 205 -> 182 us; structures of 480 atoms
+// 658 -> 698.
+template <bool FRESH>
+__device__ inline unsigned anew(unsigned v) {
+  if (FRESH) asm volatile("" : "+v"(v));
+  return v;
+}
+
 // A tile of lines in LDS: DP values each without padding, because the loads that
 // go straight to LDS write a wave's 64 chunks of 16 bytes one after the other.  Chunk c
 // of line l lies at place c ^ turn(l) of its line.  LDS serves 256 bytes a cycle from 64
@@ -109,12 +122,12 @@ __device__ inline Op<T> line_chunk(const T* tile, int line, int u, int half) {
 // of four values of line l / 4, columns 4 (l % 4) .. + 3, and gets four lines of
 // column l.  Every lane of the wave takes part.
 template <int DP>
-__device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, int half) {
+__device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, unsigned lane) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const int lane = threadIdx.x & 63, line = 4 * half + (lane & 15) / 4;  // turn() repeats 16 lines on
-  const int chunk = column / 8 + (lane & 16) / 8 + (lane & 3) / 2;
-  const __bf16* at = tile + (16 * s + line) * DP + 4 * (lane & 1);
+  const int line = int(lane / 32 * 4 + (lane & 15) / 4);  // turn() repeats 16 lines on
+  const int chunk = column / 8 + int((lane & 16) / 8 + (lane & 3) / 2);
+  const __bf16* at = tile + (16 * s + line) * DP + 4 * int(lane & 1);
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + (chunk ^ turn<__bf16, DP>(line)) * 8));
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * DP + (chunk ^ turn<__bf16, DP>(line + 8)) * 8));
   typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -122,13 +135,13 @@ __device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, int
   return __builtin_bit_cast(bf16x8, both);
 }
 template <int DP>
-__device__ inline f32x4 column_chunk(const float* tile, int s, int column, int half) {
-  const int lane = threadIdx.x & 31;
+__device__ inline f32x4 column_chunk(const float* tile, int s, int column, unsigned lane) {
+  const int half = int(lane / 32), at = int(lane & 31);
   f32x4 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int line = 8 * s + 4 * half + j;
-    r[j] = tile[line * DP + ((column / 4 + lane / 4) ^ turn<float, DP>(line)) * 4 + (lane & 3)];
+    r[j] = tile[line * DP + ((column / 4 + at / 4) ^ turn<float, DP>(line)) * 4 + (at & 3)];
   }
   return r;
 }
@@ -167,18 +180,26 @@ struct Two {
   Op<T> a, b;
 };
 
-// tanh by 1 - 2 / (exp(2 x) + 1), to 2e-7 of 1: for scores whose weights are
-// rounded to bf16.  fp32 calls take the odd series where the quotient cancels, for a
-// relative error of a few ulp (the first term left out is 4e-3 x^13).  No branches:
-// a lane's choice between two short formulas costs less than leaving one out.
+// tanh in the form the kernels use it: t = 1 - 2 r with r = 1 / (exp(2 x) + 1), and
+// 1 - t^2 = 4 (r - r^2).  r is good to 2e-7 of 1, which does for scores whose
+// weights are rounded to bf16.  fp32 calls take r from the odd series of t for
+// small x, for a relative error of t of a few ulp (the first term left out is 4e-3 x^13).
+// No branches: a lane's choice between two short formulas costs less than leaving one out.
+// `exponent` is 2 x in units of log2.
+struct Bend {
+  float t, r;
+};
 template <typename T>
-__device__ inline float bent(float x) {
-  const float q = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * kLog2e * x) + 1.0f);
-  if (sizeof(T) == 2) return q;
-  const float y = x * x;
-  const float series =
-      x + x * y * (-0.333333333f + y * (0.133333333f + y * (-0.0539682540f + y * (0.0218694885f + y * -0.00886323552f))));
-  return y < 0.09f ? series : q;
+__device__ inline Bend bend_of(float exponent) {
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(exponent) + 1.0f);
+  Bend b = {1.0f - 2.0f * r, r};
+  if (sizeof(T) == 4) {
+    const float x = exponent * (0.5f * kLn2), y = x * x;
+    const float series =
+        x + x * y * (-0.333333333f + y * (0.133333333f + y * (-0.0539682540f + y * (0.0218694885f + y * -0.00886323552f))));
+    b.t = y < 0.09f ? series : b.t;
+  }
+  return b;
 }
 
 // The largest d with bound(d) <= slot, bound rising, bound(0) <= slot: 64 probes a round.
@@ -231,15 +252,15 @@ __device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 // every chunk is 16 whole aligned bytes (`direct`) memory is loaded straight to LDS
 // without passing registers; otherwise chunk by chunk through them.  address(line): the
 // line's first value, or null for a line of zeros.  arrived() waits for the loads of this wave.
-template <typename T, int DP, int LINES, int NT, typename F>
+template <typename T, int DP, int LINES, int NT, bool FRESH, typename F>
 __device__ inline void load_tile(T* tile, int D, bool direct, F address) {
   constexpr int ROW = DP / kChunk<T>, SLOTS = LINES * ROW;
-  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), thread = int(anew<FRESH>(threadIdx.x) & 255);
   auto each = [&](auto use) {
 #pragma unroll
     for (int n = 0; n < (SLOTS + NT - 1) / NT; ++n) {
       if (SLOTS % NT != 0 && n * NT + 64 * wave >= SLOTS) continue;  // 64 divides SLOTS
-      const int x = n * NT + int(threadIdx.x), line = x / ROW, c = (x % ROW ^ turn<T, DP>(line)) * kChunk<T>;
+      const int x = n * NT + thread, line = x / ROW, c = (x % ROW ^ turn<T, DP>(line)) * kChunk<T>;
       const T* p = address(line);
       use(n, x, c, p && c < D ? p + c : nullptr);
     }
@@ -308,11 +329,12 @@ __device__ inline f32x4 key_place(const Problem& p, int64_t key, bool seen) {
   return r;
 }
 
-// The keys of a structure in tiles of KT <= 64, two of them in LDS: begin() starts the
-// loads of one, finish() of the tile begun last makes it ready for the workgroup.
-// Whether a key is seen is read a tile ahead of its rows, which masked keys
-// have as zeros, whatever they hold.
-template <typename T, int DP, int KT, int NT, bool BIAS>
+// The keys of a structure in tiles of KT <= 64.  take() makes one ready for the
+// workgroup; with two buffers the next one's loads run meanwhile.  One buffer where a
+// workgroup is one wave: more of them fit a compute unit's LDS, and they hide each other's
+// loads (one row against 9 000 atoms in each of 24 structures 150 -> 119 us).  Whether a key is seen is read a tile ahead of its
+// rows; masked keys have rows of zeros, whatever they hold.
+template <typename T, int DP, int KT, int NT, int BUFFERS, bool FRESH, bool BIAS>
 struct KeyTiles {
   const Problem& p;
   const Span key;
@@ -321,6 +343,11 @@ struct KeyTiles {
   f32x4* places;
   f32x4 place;
   uint8_t mask;  // of this lane's key in the tile after the one begun last, as it was read
+
+  __device__ static inline int buffer(int tile) { return BUFFERS == 2 ? tile & 1 : 0; }
+  __device__ inline const T* keys(int tile) const { return ktiles + buffer(tile) * KT * DP; }
+  __device__ inline const T* values(int tile) const { return vtiles + buffer(tile) * KT * DP; }
+  __device__ inline const f32x4* places_of(int tile) const { return places + buffer(tile) * KT; }
 
   __device__ inline bool exists(int tile) const {
     return (int(threadIdx.x) & 63) < KT && tile * KT + (int(threadIdx.x) & 63) < key.length;
@@ -331,25 +358,29 @@ struct KeyTiles {
   }
   __device__ inline void start(int tile) {
     look(tile);
-    begin(tile);
+    if (BUFFERS == 2) begin(tile);
   }
   // Nothing here uses what it loads: a wait would be for the tile's rows too.
   __device__ inline void begin(int tile) {
     const bool seen = exists(tile) && mask;
     const uint64_t all = __ballot(seen);
-    const int buffer = tile & 1;
     const int64_t first = key.begin + int64_t(tile) * KT;
-    load_tile<T, DP, KT, NT>(ktiles + buffer * KT * DP, p.D, p.direct,
+    load_tile<T, DP, KT, NT, FRESH>(ktiles + buffer(tile) * KT * DP, p.D, p.direct,
                              [&](int line) { return all >> line & 1 ? kbase + (first + line) * p.k_row : nullptr; });
-    load_tile<T, DP, KT, NT>(vtiles + buffer * KT * DP, p.D, p.direct,
+    load_tile<T, DP, KT, NT, FRESH>(vtiles + buffer(tile) * KT * DP, p.D, p.direct,
                              [&](int line) { return all >> line & 1 ? vbase + (first + line) * p.v_row : nullptr; });
     if (int(threadIdx.x) < KT) place = key_place<BIAS>(p, first + threadIdx.x, seen);
     look(tile + 1);
   }
-  __device__ inline void finish(int tile) {
-    if (int(threadIdx.x) < KT) places[(tile & 1) * KT + threadIdx.x] = place;
+  __device__ inline void take(int tile, int tiles) {
+    if (BUFFERS == 1) {
+      __syncthreads();  // the last tile has been used
+      begin(tile);
+    }
+    if (int(threadIdx.x) < KT) places[buffer(tile) * KT + threadIdx.x] = place;
     arrived();
     __syncthreads();
+    if (BUFFERS == 2 && tile + 1 < tiles) begin(tile + 1);
   }
 };
 
@@ -379,24 +410,28 @@ struct Gradient {
 };
 
 // Scores in units of log2 as the forward takes them, and the derivative of the
-// bend; the distance is subtracted by the caller.
+// bend, over 4 (slant_scale()); the distance is subtracted by the caller.
 struct Score {
   float s, slant;
 };
 template <typename T, bool CAP>
 __device__ inline Score score_of(const Problem& p, float product) {
   if (CAP) {
-    const float t = bent<T>(product * (p.scale / p.cap));
-    return {p.cap * kLog2e * t, 1.0f - t * t};
+    const Bend b = bend_of<T>(product * p.to_bend);
+    return {p.from_bend * b.t, b.r - b.r * b.r};
   }
-  return {product * (p.scale * kLog2e), 1.0f};
+  return {product * p.to_log2, 1.0f};
+}
+template <bool CAP>
+__device__ inline float slant_scale() {
+  return CAP ? 4.0f : 1.0f;
 }
 
-// Waves a SIMD that the register budget is set for.
-template <typename T, int DP>
-constexpr int kForwardWaves = DP == 32 ? 3 : 2;
-template <typename T, int DP>
-constexpr int kGradientWaves = DP == 32 ? 2 : DP == 64 ? 2 : 1;
+// Waves a SIMD that the register budget is set for: spills cost more than a wave gains.
+template <typename T, int DP, int NW>
+constexpr int kForwardWaves = DP == 32 ? (NW == 1 ? 4 : 3) : DP == 64 || sizeof(T) == 2 ? 2 : 1;
+template <typename T, int DP, int NW>
+constexpr int kGradientWaves = DP == 32 ? (NW == 1 ? 3 : 2) : DP == 64 ? 2 : 1;
 
 inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -407,15 +442,16 @@ inline int waves_for(int64_t rows, int64_t structures) {
 }
 
 // Parts of the key axis: where the rows alone give less than four workgroups
-// a compute unit, as many as fill that, each with two tiles of keys or more on
-// average.
+// a compute unit, as many as make eight, each with two tiles of 32 keys or more on
+// average, 64 at most (a lane each where they are joined).  24 structures of 9 000
+// atoms, one row each, 16 heads of 128 over 4 key heads, bf16: 119 us; 136 by twice as many.
 inline int parts_for(int64_t items, int key_heads, int64_t keys, int64_t structures) {
   const int64_t groups = items * key_heads;
   if (groups >= 1024 || structures == 0) return 1;
-  int64_t parts = 1024 / groups;
+  int64_t parts = 2048 / groups;
   const int64_t tiles = keys / structures / 64;
   if (parts > tiles) parts = tiles;
-  return int(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+  return int(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
 
 struct ForwardPlan {
@@ -490,6 +526,9 @@ inline Problem problem_of(const ye3t_attention_args& a) {
   p.key_offsets = a.key_offsets ? a.key_offsets : a.offsets;
   p.scale = float(a.scale);
   p.cap = float(a.cap);
+  p.to_log2 = float(a.scale * kLog2eExact);
+  p.to_bend = a.cap > 0.0 ? float(2.0 * kLog2eExact * a.scale / a.cap) : 0.0f;
+  p.from_bend = float(a.cap * kLog2eExact);
   p.slopes = a.slopes;
   p.positions = a.positions;
   p.key_positions = a.key_positions;

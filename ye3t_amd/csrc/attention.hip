@@ -10,12 +10,14 @@ namespace {
 // NW waves of 32 rows, KT keys a tile.  SPLIT: grid axis z takes equal parts of
 // each structure's key tiles and leaves its sums to attention_join_kernel.
 template <typename T, int DP, int NW, int KT, bool BIAS, bool CAP, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP>)) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
+__global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP, NW>)) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
                                                             float* __restrict__ part, float* __restrict__ part_stats) {
   constexpr int TILE = 32 * NW, NU = DP / (2 * kChunk<T>), ND = DP / 32;
-  __shared__ __align__(16) T ktiles[2 * KT * DP];
-  __shared__ __align__(16) T vtiles[2 * KT * DP];
-  __shared__ f32x4 places[2 * KT];
+  constexpr int BUFFERS = NW == 1 ? 1 : 2;
+  constexpr bool FRESH = NW == 1 && !SPLIT;
+  __shared__ __align__(16) T ktiles[BUFFERS * KT * DP];
+  __shared__ __align__(16) T vtiles[BUFFERS * KT * DP];
+  __shared__ f32x4 places[BUFFERS * KT];
   const Item item = item_of(p.offsets, p.structures, p.queries, p.group, TILE, blockIdx.x);
   const Span own = span_of(p.offsets, item.structure, p.queries);
   const int64_t rows = int64_t(own.length) * p.group;
@@ -46,32 +48,30 @@ __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP>)) void attention_ker
 #pragma unroll
   for (int t = 0; t < ND; ++t) acc[t] = zeros();
   float top = -INFINITY, sum = 0.0f;
-  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{p,      key,    static_cast<const T*>(p.k) + key_head * p.k_head,
-                                                     static_cast<const T*>(p.v) + key_head * p.v_head,
-                                                     ktiles, vtiles, places};
+  KeyTiles<T, DP, KT, 64 * NW, BUFFERS, FRESH, BIAS> tiles_of{p,      key,    static_cast<const T*>(p.k) + key_head * p.k_head,
+                                                       static_cast<const T*>(p.v) + key_head * p.v_head,
+                                                       ktiles, vtiles, places};
   if (tile < tiles) tiles_of.start(tile);
-  const float to_log2 = p.scale * kLog2e;
-  const float to_cap = CAP ? p.scale / p.cap : 0.0f, from_cap = p.cap * kLog2e;
   for (; tile < tiles; ++tile) {
-    tiles_of.finish(tile);
-    if (tile + 1 < tiles) tiles_of.begin(tile + 1);
-    const T *ktile = ktiles + (tile & 1) * KT * DP, *vtile = vtiles + (tile & 1) * KT * DP;
-    const f32x4* place = places + (tile & 1) * KT;
+    tiles_of.take(tile, tiles);
+    const T *ktile = tiles_of.keys(tile), *vtile = tiles_of.values(tile);
+    const f32x4* place = tiles_of.places_of(tile);
     if (!busy) continue;
+    const unsigned now_lane = anew<FRESH>(lane) & 63;
     const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
     f32x16 s[KT / 32];
     float high = -INFINITY;
 #pragma unroll
     for (int n = 0; n < KT / 32; ++n) {
       s[n] = zeros();
-      in_flight<NU>([&](int u) { return line_chunk<T, DP>(ktile, 32 * n + (lane & 31), u, half); },
+      in_flight<NU>([&](int u) { return line_chunk<T, DP>(ktile, 32 * n + int(now_lane & 31), u, int(now_lane / 32)); },
                     [&](int u, const Op<T>& k) { mma(k, q[u], s[n]); });
       if (CAP) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = from_cap * bent<T>(s[n][i] * to_cap);
+        for (int i = 0; i < 16; ++i) s[n][i] = p.from_bend * bend_of<T>(s[n][i] * p.to_bend).t;
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] *= to_log2;
+        for (int i = 0; i < 16; ++i) s[n][i] *= p.to_log2;
       }
       if (BIAS) {
 #pragma unroll
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP>)) void attention_ker
 #pragma unroll
       for (int c = 0; c < kLineChunks<T>; ++c) register_chunk(s[n], c, w[c]);
       in_flight<kLineChunks<T> * ND>(
-          [&](int i) { return column_chunk<DP>(vtile + 32 * n * DP, i / ND, 32 * (i % ND), half); },
+          [&](int i) { return column_chunk<DP>(vtile + 32 * n * DP, i / ND, 32 * (i % ND), now_lane); },
           [&](int i, const Op<T>& v) { mma(v, w[i / ND], acc[i % ND]); });
     }
   }
@@ -133,29 +133,44 @@ __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP>)) void attention_ker
   if (log_sums && half == 0) log_sums[at] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// Joins the parts of a row: a wave a row, a lane a column.
+// Joins the parts of a row, 64 at most: a wave a row; first a lane a part for the parts'
+// weights, then a lane a column, eight parts in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(const float* __restrict__ part,
                                                              const float* __restrict__ part_stats, int parts,
                                                              int64_t rows, int D, T* __restrict__ out,
                                                              float* __restrict__ log_sums) {
+  constexpr int AHEAD = 8;
   const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (row >= rows) return;
-  float top = -INFINITY;
-  for (int k = 0; k < parts; ++k) top = fmaxf(top, part_stats[2 * (k * rows + row)]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
-  for (int k = 0; k < parts; ++k)
-    sum += __builtin_amdgcn_exp2f(part_stats[2 * (k * rows + row)] - base) * part_stats[2 * (k * rows + row) + 1];
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int c = lane; c < D; c += 64) {
-    float v = 0.0f;
-    for (int k = 0; k < parts; ++k)
-      v += __builtin_amdgcn_exp2f(part_stats[2 * (k * rows + row)] - base) * part[(k * rows + row) * D + c];
-    out[row * D + c] = T(v * inverse);
+  float top = -INFINITY, sum = 0.0f;
+  if (lane < parts) {
+    top = part_stats[2 * (lane * rows + row)];
+    sum = part_stats[2 * (lane * rows + row) + 1];
   }
-  if (log_sums && lane == 0) log_sums[row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  float most = top;
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+  float weight = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
+  sum *= weight;
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
+  weight *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int c0 = 0; c0 < D; c0 += 64) {
+    const int c = c0 + lane;
+    float v = 0.0f;
+    for (int k0 = 0; k0 < parts; k0 += AHEAD) {
+      float x[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        x[k] = k0 + k < parts && c < D ? part[((k0 + k) * rows + row) * D + c] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) v += __shfl(weight, (k0 + k) & 63) * x[k];
+    }
+    if (c < D) out[row * D + c] = T(v);
+  }
+  if (log_sums && lane == 0) log_sums[row] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // The gradients to positions (a sum over heads) and, per workgroup, to slopes.

@@ -8,12 +8,13 @@ namespace {
 // Key side: dk, dv and the key's part of the gradient to its position.  A wave
 // owns 32 keys and walks over the rows of its key head in tiles of 32.
 template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
-__global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_key_gradient_kernel(Problem p, Gradient g) {
+__global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attention_key_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, RT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
-  __shared__ __align__(16) T qtiles[2 * RT * DP];
-  __shared__ __align__(16) T gtiles[2 * RT * DP];
-  __shared__ f32x4 places[2 * RT];  // x, y, z, slope
-  __shared__ f32x2 all_stats[2 * RT];  // log sum, or infinity for a row that sees no key or does not exist; D_i
+  constexpr int BUFFERS = NW == 1 ? 1 : 2;
+  __shared__ __align__(16) T qtiles[BUFFERS * RT * DP];
+  __shared__ __align__(16) T gtiles[BUFFERS * RT * DP];
+  __shared__ f32x4 places[BUFFERS * RT];  // x, y, z, slope
+  __shared__ f32x2 all_stats[BUFFERS * RT];  // log sum, or infinity for a row that sees no key or does not exist; D_i
   const Item item = item_of(p.key_offsets, p.structures, p.keys, 1, TILE, blockIdx.x);
   const Span key = span_of(p.key_offsets, item.structure, p.keys);
   if (item.first < 0 || item.first >= key.length) return;
@@ -34,12 +35,12 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
   f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
   f32x2 next_stats = {-INFINITY, 0.0f};
   auto begin = [&](int64_t r0) {
-    const int buffer = int(r0 / RT) & 1;
-    load_tile<T, DP, RT, 64 * NW>(qtiles + buffer * RT * DP, p.D, p.direct, [&](int line) {
+    const int buffer = BUFFERS == 2 ? int(r0 / RT) & 1 : 0;
+    load_tile<T, DP, RT, 64 * NW, BUFFERS == 1>(qtiles + buffer * RT * DP, p.D, p.direct, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(p.q) + r.token * p.q_row + r.head * p.q_head : nullptr;
     });
-    load_tile<T, DP, RT, 64 * NW>(gtiles + buffer * RT * DP, p.D, g.direct, [&](int line) {
+    load_tile<T, DP, RT, 64 * NW, BUFFERS == 1>(gtiles + buffer * RT * DP, p.D, g.direct, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(g.adjoint) + (r.token * p.heads + r.head) * p.D : nullptr;
     });
@@ -60,9 +61,13 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
 #pragma unroll
   for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
   float gx = 0.0f, gy = 0.0f, gz = 0.0f;
-  if (rows > 0) begin(0);
+  if (BUFFERS == 2 && rows > 0) begin(0);
   for (int64_t r0 = 0; r0 < rows; r0 += RT) {
-    const int buffer = int(r0 / RT) & 1;
+    const int buffer = BUFFERS == 2 ? int(r0 / RT) & 1 : 0;
+    if (BUFFERS == 1) {
+      __syncthreads();  // the last tile has been used
+      begin(r0);
+    }
     if (int(threadIdx.x) < RT) {
       places[buffer * RT + threadIdx.x] = f32x4{next_place[0], next_place[1], next_place[2], next_place[3] * kLog2e};
       const bool counts = next_stats[0] != -INFINITY;
@@ -71,15 +76,16 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
     }
     arrived();
     __syncthreads();
-    if (r0 + RT < rows) begin(r0 + RT);
+    if (BUFFERS == 2 && r0 + RT < rows) begin(r0 + RT);
     const T *qtile = qtiles + buffer * RT * DP, *gtile = gtiles + buffer * RT * DP;
     const f32x4* place = places + buffer * RT;
     const f32x2* stats = all_stats + buffer * RT;
     if (!busy) continue;
+    const unsigned now_lane = anew<BUFFERS == 1>(lane) & 63;
     f32x16 s = zeros(), dp = zeros();
     in_flight<NU>(
         [&](int u) {
-          return Two<T>{line_chunk<T, DP>(qtile, lane & 31, u, half), line_chunk<T, DP>(gtile, lane & 31, u, half)};
+          return Two<T>{line_chunk<T, DP>(qtile, int(now_lane & 31), u, int(now_lane / 32)), line_chunk<T, DP>(gtile, int(now_lane & 31), u, int(now_lane / 32))};
         },
         [&](int u, const Two<T>& qg) {
           mma(qg.a, k[u], s);
@@ -122,8 +128,8 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
     }
     in_flight<kLineChunks<T> * ND>(
         [&](int i) {
-          return Two<T>{column_chunk<DP>(qtile, i / ND, 32 * (i % ND), half),
-                        column_chunk<DP>(gtile, i / ND, 32 * (i % ND), half)};
+          return Two<T>{column_chunk<DP>(qtile, i / ND, 32 * (i % ND), now_lane),
+                        column_chunk<DP>(gtile, i / ND, 32 * (i % ND), now_lane)};
         },
         [&](int i, const Two<T>& qg) {
           mma(qg.a, ds[i / ND], dk[i % ND]);
@@ -137,7 +143,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ke
     for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
   }
   const int64_t at = token * p.key_heads + key_head;
-  store_columns<T, DP>(static_cast<T*>(g.dk) + at * p.D, p.D, half, dk, p.scale);
+  store_columns<T, DP>(static_cast<T*>(g.dk) + at * p.D, p.D, half, dk, p.scale * slant_scale<CAP>());
   store_columns<T, DP>(static_cast<T*>(g.dv) + at * p.D, p.D, half, dv, 1.0f);
   if (FORCES) {
     f32x4 r = {gx, gy, gz, 0.0f};

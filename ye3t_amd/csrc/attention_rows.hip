@@ -11,17 +11,18 @@ namespace {
 // D_i starts as the dot product of the output with its adjoint.  A bf16 output's
 // rounding would stand out: it shifts all dz_ij of a row by p_ij times the same
 // amount, up to 2^-9 of the largest terms where few keys carry the row.  The dz
-// of a row add up to zero, so what they add up to instead, over the sum of p, is that
-// amount c; everything here is linear in it and is set right after the walk over the
+// of a row add up to zero, so what they add up to instead is that amount c (the p of a row
+// add up to 1 to within fp32's rounding); everything here is linear in it and is set right after the walk over the
 // keys, dq by the product of the p (and the slants) with the keys.  The key side
 // starts from the D_i that is right.  fp32 calls have no such rounding in dq, and
 // correct only what FORCES sums, where terms of many keys cancel.
 template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
-__global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_row_gradient_kernel(Problem p, Gradient g) {
+__global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attention_row_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, KT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
-  __shared__ __align__(16) T ktiles[2 * KT * DP];
-  __shared__ __align__(16) T vtiles[2 * KT * DP];
-  __shared__ f32x4 places[2 * KT];
+  constexpr int BUFFERS = NW == 1 ? 1 : 2;
+  __shared__ __align__(16) T ktiles[BUFFERS * KT * DP];
+  __shared__ __align__(16) T vtiles[BUFFERS * KT * DP];
+  __shared__ f32x4 places[BUFFERS * KT];
   const Item item = item_of(p.offsets, p.structures, p.queries, p.group, TILE, blockIdx.x);
   const Span own = span_of(p.offsets, item.structure, p.queries);
   const int64_t rows = int64_t(own.length) * p.group;
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ro
   const float log_sum2 = log_sum == -INFINITY ? INFINITY : log_sum * kLog2e;
 
   const int tiles = (key.length + KT - 1) / KT;
-  KeyTiles<T, DP, KT, 64 * NW, BIAS> tiles_of{
+  KeyTiles<T, DP, KT, 64 * NW, BUFFERS, BUFFERS == 1, BIAS> tiles_of{
       p,      key,    static_cast<const T*>(p.k) + key_head * p.k_head, static_cast<const T*>(p.v) + key_head * p.v_head,
       ktiles, vtiles, places};
   constexpr bool RIGHT = sizeof(T) == 2;  // dq is set right
@@ -68,29 +69,29 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ro
   for (int t = 0; t < ND; ++t) acc[t] = zeros();
 #pragma unroll
   for (int t = 0; t < (RIGHT ? ND : 1); ++t) own_keys[t] = zeros();
-  // Sums over the keys of dz, p, and with FORCES of their products with the
-  // distance and the direction.  Each tile's are summed by themselves first:
+  // Sums over the keys of dz, and with FORCES of dz and p times the distance and
+  // the direction.  Each tile's are summed by themselves first:
   // long sums whose terms cancel keep a few more bits.
   struct Sums {
-    float dz, p, far_dz, far_p;
+    float dz, far_dz, far_p;
     f32x4 to_dz, to_p;
     __device__ inline void add(const Sums& o) {
-      dz += o.dz, p += o.p, far_dz += o.far_dz, far_p += o.far_p, to_dz += o.to_dz, to_p += o.to_p;
+      dz += o.dz, far_dz += o.far_dz, far_p += o.far_p, to_dz += o.to_dz, to_p += o.to_p;
     }
   };
-  const Sums none = {0.0f, 0.0f, 0.0f, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+  const Sums none = {0.0f, 0.0f, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
   Sums all = none;
   if (tiles > 0) tiles_of.start(0);
   for (int tile = 0; tile < tiles; ++tile) {
-    tiles_of.finish(tile);
-    if (tile + 1 < tiles) tiles_of.begin(tile + 1);
-    const T *ktile = ktiles + (tile & 1) * KT * DP, *vtile = vtiles + (tile & 1) * KT * DP;
-    const f32x4* place = places + (tile & 1) * KT;
+    tiles_of.take(tile, tiles);
+    const T *ktile = tiles_of.keys(tile), *vtile = tiles_of.values(tile);
+    const f32x4* place = tiles_of.places_of(tile);
     if (!busy) continue;
+    const unsigned now_lane = anew<BUFFERS == 1>(lane) & 63;
     f32x16 s = zeros(), dp = zeros();
     in_flight<NU>(
         [&](int u) {
-          return Two<T>{line_chunk<T, DP>(ktile, lane & 31, u, half), line_chunk<T, DP>(vtile, lane & 31, u, half)};
+          return Two<T>{line_chunk<T, DP>(ktile, int(now_lane & 31), u, int(now_lane / 32)), line_chunk<T, DP>(vtile, int(now_lane & 31), u, int(now_lane / 32))};
         },
         [&](int u, const Two<T>& kv) {
           mma(kv.a, q[u], s);
@@ -120,10 +121,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ro
       const float tilt = w * (dp[i] - along);
       s[i] = tilt * z.slant;
       if (RIGHT) dp[i] = w * z.slant;
-      if (RIGHT || FORCES) {
-        now.dz += tilt;
-        now.p += w;
-      }
+      if (RIGHT || FORCES) now.dz += tilt;
       if (FORCES) {
         now.far_dz += tilt * distance;
         now.far_p += w * distance;
@@ -140,19 +138,14 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ro
       register_chunk(s, c, w[c]);
       if constexpr (RIGHT) register_chunk(dp, c, m[c]);
     }
-    in_flight<kLineChunks<T> * ND>([&](int i) { return column_chunk<DP>(ktile, i / ND, 32 * (i % ND), half); },
+    in_flight<kLineChunks<T> * ND>([&](int i) { return column_chunk<DP>(ktile, i / ND, 32 * (i % ND), now_lane); },
                                    [&](int i, const Op<T>& k) {
                                      mma(k, w[i / ND], acc[i % ND]);
                                      if constexpr (RIGHT) mma(k, m[i / ND], own_keys[i % ND]);
                                    });
   }
-  float off = 0.0f;
-  if (RIGHT || FORCES) {
-    const float mass = all.p + other_half(all.p);
-    off = all.dz + other_half(all.dz);
-    off = mass > 0.0f ? off / mass : 0.0f;
-    along += off;
-  }
+  const float off = RIGHT || FORCES ? all.dz + other_half(all.dz) : 0.0f;
+  along += off;
   if (!row.exists) return;
   if (RIGHT) {
 #pragma unroll
@@ -160,7 +153,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP>)) void attention_ro
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][i] -= off * own_keys[t][i];
   }
-  store_columns<T, DP>(static_cast<T*>(g.dq) + at * p.D, p.D, half, acc, p.scale);
+  store_columns<T, DP>(static_cast<T*>(g.dq) + at * p.D, p.D, half, acc, p.scale * slant_scale<CAP>());
   if (half == 0) g.along[at] = along;
   if (FORCES) {
     const float m = p.slopes[row.head];
