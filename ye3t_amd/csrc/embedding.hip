@@ -78,6 +78,29 @@ __device__ inline Pair pair_at(const Index* __restrict__ tokens, const Pair* __r
   return {uint32_t(t < 0 ? vocabulary : t), uint32_t(i)};
 }
 
+// The live lanes of the wave that have this lane's digit.
+__device__ inline uint64_t lanes_of_digit(uint32_t digit, bool live) {
+  uint64_t same = __ballot(live);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const uint64_t set = __ballot((digit >> b) & 1u);
+    same &= ((digit >> b) & 1u) ? set : ~set;
+  }
+  return same;
+}
+
+// A digit's counts by wave become the waves' first places; `next` moves past them.
+__device__ inline void places_of_waves(uint32_t (*of_wave)[kBins], int digit, uint32_t& next) {
+  uint32_t at = next;
+#pragma unroll
+  for (int w = 0; w < kSortThreads / 64; ++w) {
+    const uint32_t n = of_wave[w][digit];
+    of_wave[w][digit] = at;
+    at += n;
+  }
+  next = at;
+}
+
 template <bool FIRST, typename Index>
 __global__ __launch_bounds__(kSortThreads) void digit_count_kernel(const Index* __restrict__ tokens,
                                                                    const Pair* __restrict__ pairs, int64_t N,
@@ -148,27 +171,77 @@ __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* 
     const bool live = i0 + t < end;
     const Pair p = live ? pair_at<FIRST>(tokens, pairs, i0 + t, vocabulary) : Pair{0, 0};
     const uint32_t digit = (p.token >> shift) & (kBins - 1);
-    uint64_t same = __ballot(live);  // the live lanes of this digit
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const uint64_t set = __ballot((digit >> b) & 1u);
-      same &= ((digit >> b) & 1u) ? set : ~set;
-    }
+    const uint64_t same = lanes_of_digit(digit, live);
     const uint32_t rank = uint32_t(__popcll(same & ((uint64_t(1) << lane) - 1)));
     if (live && rank == 0) of_wave[wave][digit] = uint32_t(__popcll(same));
     __syncthreads();
-    if (t < kBins) {
-      uint32_t at = next[t];
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const uint32_t n = of_wave[w][t];
-        of_wave[w][t] = at;
-        at += n;
-      }
-      next[t] = at;
-    }
+    if (t < kBins) places_of_waves(of_wave, t, next[t]);
     __syncthreads();
     if (live) out[of_wave[wave][digit] + rank] = p;
+    __syncthreads();
+  }
+}
+
+// All passes over few positions by one workgroup, in LDS: one launch where the
+// kernels above take two a pass.  Each wave owns an equal run of positions, counts its digits
+// and, once all counts are added up, places them by itself.
+constexpr int kSmallSort = 4096;
+
+template <typename Index>
+__global__ __launch_bounds__(kSortThreads) void small_sort_kernel(const Index* __restrict__ tokens, int N,
+                                                                  int64_t vocabulary, int passes,
+                                                                  Pair* __restrict__ out) {
+  constexpr int kWaves = kSortThreads / 64;
+  __shared__ Pair held[2][kSmallSort];
+  __shared__ uint32_t of_wave[kWaves][kBins];
+  __shared__ uint32_t wave_sums[kBins / 64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int run = (N + kSortThreads - 1) / kSortThreads * 64;
+  const int begin = wave * run, end = begin + run < N ? begin + run : N;
+  for (int i = t; i < N; i += kSortThreads)
+    held[0][i] = pair_at<true>(tokens, static_cast<const Pair*>(nullptr), i, vocabulary);
+  for (int pass = 0; pass < passes; ++pass) {
+    const Pair* in = held[pass & 1];
+    Pair* to = held[~pass & 1];
+    const int shift = 8 * pass;
+    for (int k = t; k < kWaves * kBins; k += kSortThreads) (&of_wave[0][0])[k] = 0;
+    __syncthreads();
+    for (int i = begin + lane; i < end; i += 64) atomicAdd(&of_wave[wave][(in[i].token >> shift) & (kBins - 1)], 1u);
+    __syncthreads();
+    uint32_t own = 0, sum = 0;
+    if (t < kBins) {
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) own += of_wave[w][t];
+      sum = own;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const uint32_t up = __shfl_up(sum, m);
+        if (lane >= m) sum += up;
+      }
+      if (lane == 63) wave_sums[wave] = sum;
+    }
+    __syncthreads();
+    if (t < kBins) {
+      sum -= own;
+      for (int w = 0; w < wave; ++w) sum += wave_sums[w];
+      places_of_waves(of_wave, t, sum);
+    }
+    __syncthreads();
+    for (int i0 = begin; i0 < end; i0 += 64) {
+      const bool live = i0 + lane < end;
+      const Pair p = live ? in[i0 + lane] : Pair{0, 0};
+      const uint32_t digit = (p.token >> shift) & (kBins - 1);
+      const uint64_t same = lanes_of_digit(digit, live);
+      const uint32_t rank = uint32_t(__popcll(same & ((uint64_t(1) << lane) - 1)));
+      const uint32_t at = of_wave[wave][digit] + rank;
+      __threadfence_block();  // every lane has read its digit's place before it moves on
+      if (live && rank == 0) of_wave[wave][digit] = at + uint32_t(__popcll(same));
+      __threadfence_block();
+      if (live) {
+        if (pass + 1 == passes) out[at] = p;
+        else to[at] = p;
+      }
+    }
     __syncthreads();
   }
 }
@@ -190,12 +263,14 @@ __device__ inline void clear_missing(const Pair* __restrict__ sorted, int64_t N,
     else hi = mid;
   }
   const bool missing = v < vocabulary && !(lo < N && int64_t(sorted[lo].token) == v);
-  uint64_t rows = __ballot(missing);  // the same in every wave
+  const uint64_t rows = __ballot(missing);  // the same in every wave
+  if (rows == 0) return;
   const Chunk<T, V> zero = Chunk<T, V>::zero();
-  while (rows) {
-    const int r = __ffsll(static_cast<unsigned long long>(rows)) - 1;
-    rows &= rows - 1;
-    for (int c = int(threadIdx.x) * V; c < W; c += kThreads * V) zero.store(table + (v0 + r) * W + c, W - c);
+  const uint32_t chunks = uint32_t(W + V - 1) / V;
+  for (uint32_t i = threadIdx.x; i < 64 * chunks; i += kThreads) {
+    const uint32_t r = i / chunks;
+    const int c = int(i - r * chunks) * V;
+    if (rows >> r & 1) zero.store(table + (v0 + r) * W + c, W - c);
   }
 }
 
@@ -377,7 +452,12 @@ int gradient_as(const T* adjoint, const Index* tokens, int64_t N, int64_t vocabu
   Real* heads = reinterpret_cast<Real*>(at += p.counts_bytes);
   Real* tails = reinterpret_cast<Real*>(at += p.partial_bytes);
   uint32_t* ends = reinterpret_cast<uint32_t*>(at += p.partial_bytes);
-  for (int k = 0; k < p.passes && N > 0; ++k) {
+  if (N > 0 && N <= kSmallSort) {
+    hipLaunchKernelGGL((small_sort_kernel<Index>), dim3(1), dim3(kSortThreads), 0, s, tokens, int(N), vocabulary,
+                       p.passes, pairs[(p.passes - 1) & 1]);
+    if (int rc = check_launch("small_sort_kernel")) return rc;
+  }
+  for (int k = 0; k < p.passes && N > kSmallSort; ++k) {
     const int rc = k == 0 ? sort_pass<true>(p, tokens, static_cast<const Pair*>(nullptr), N, vocabulary, 0, counts, pairs[0], s)
                           : sort_pass<false>(p, tokens, pairs[(k + 1) & 1], N, vocabulary, 8 * k, counts, pairs[k & 1], s);
     if (rc) return rc;
