@@ -179,6 +179,21 @@ template <typename T>
 struct Two {
   Op<T> a, b;
 };
+template <typename T>
+struct Three {
+  Op<T> a, b, c;
+};
+
+// An operand of a wave's own 32 lines, kept in LDS instead of registers: rows of 128 in
+// bf16 then leave room for two waves a SIMD.  Only the wave itself reads it.
+template <typename T, int DP>
+__device__ inline void keep_lines(T* tile, const Op<T>* r, int lane) {
+#pragma unroll
+  for (int u = 0; u < DP / (2 * kChunk<T>); ++u)
+    *reinterpret_cast<Op<T>*>(tile + (lane & 31) * DP + ((2 * u + lane / 32) ^ turn<T, DP>(lane & 31)) * kChunk<T>) = r[u];
+}
+template <typename T, int DP, int NW>
+constexpr bool kKeepLines = sizeof(T) == 2 && DP == 128 && NW == 4;
 
 // tanh in the form the kernels use it: t = 1 - 2 r with r = 1 / (exp(2 x) + 1), and
 // 1 - t^2 = 4 (r - r^2).  r is good to 2e-7 of 1, which does for scores whose
@@ -407,6 +422,7 @@ struct Gradient {
   void *dq, *dk, *dv;         // [queries, heads, D], [keys, key_heads, D]
   float* row_part;            // [queries, heads, 4]: to the position and the slope
   float* key_part;            // [keys, key_heads, 4]
+  float* sum_part;            // [key_parts, 2, keys, key_heads, D]: dk and dv of the parts of the row axis
 };
 
 // Scores in units of log2 as the forward takes them, and the derivative of the
@@ -423,7 +439,7 @@ __device__ inline Score score_of(const Problem& p, float product) {
   return {product * p.to_log2, 1.0f};
 }
 template <bool CAP>
-__device__ inline float slant_scale() {
+__host__ __device__ constexpr float slant_scale() {
   return CAP ? 4.0f : 1.0f;
 }
 
@@ -431,7 +447,7 @@ __device__ inline float slant_scale() {
 template <typename T, int DP, int NW>
 constexpr int kForwardWaves = DP == 32 ? (NW == 1 ? 4 : 3) : DP == 64 || sizeof(T) == 2 ? 2 : 1;
 template <typename T, int DP, int NW>
-constexpr int kGradientWaves = DP == 32 ? (NW == 1 ? 3 : 2) : DP == 64 ? 2 : 1;
+constexpr int kGradientWaves = DP == 32 ? (NW == 1 ? 3 : 2) : DP == 64 || kKeepLines<T, DP, NW> ? 2 : 1;
 
 inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -475,8 +491,8 @@ inline ForwardPlan forward_plan(const ye3t_attention_args& a) {
 constexpr int kSlopeGroups = 256;
 
 struct AdjointPlan {
-  int row_waves, key_waves;
-  int64_t row_items, key_items, along_bytes, row_bytes, key_bytes, bytes;
+  int row_waves, key_waves, key_parts;
+  int64_t row_items, key_items, along_bytes, row_bytes, key_bytes, slope_bytes, sum_bytes, bytes;
 };
 inline AdjointPlan adjoint_plan(const ye3t_attention_args& a, bool forces) {
   AdjointPlan f{};
@@ -486,12 +502,20 @@ inline AdjointPlan adjoint_plan(const ye3t_attention_args& a, bool forces) {
   f.row_items = item_count(a.queries * group, a.structures, 32 * f.row_waves);
   f.key_items = item_count(a.keys, a.structures, 32 * f.key_waves);
   f.along_bytes = up(a.queries * a.heads * 4);
+  f.key_parts = 1;
   if (forces) {
     f.row_bytes = up(a.queries * a.heads * 16);
     f.key_bytes = up(a.keys * a.key_heads * 16);
-    f.bytes = up(kSlopeGroups * a.heads * 4);
+    f.slope_bytes = up(kSlopeGroups * a.heads * 4);
+  } else if (a.structures > 0) {
+    // Keys that give less than two workgroups a compute unit: the row axis in parts of
+    // eight tiles or more on average, summed by attention_key_join_kernel.
+    const int64_t groups = f.key_items * a.key_heads, tiles = a.queries * group / a.structures / 256;
+    const int64_t parts = groups < 512 ? 1024 / groups : 1;
+    f.key_parts = int(parts < tiles ? (parts < 16 ? parts : 16) : tiles < 1 ? 1 : tiles < 16 ? tiles : 16);
+    if (f.key_parts > 1) f.sum_bytes = up(f.key_parts * 2 * a.keys * a.key_heads * a.head_width * 4);
   }
-  f.bytes += f.along_bytes + f.row_bytes + f.key_bytes + 256;
+  f.bytes = f.along_bytes + f.row_bytes + f.key_bytes + f.slope_bytes + f.sum_bytes + 256;
   return f;
 }
 

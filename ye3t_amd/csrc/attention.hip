@@ -339,6 +339,7 @@ int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void*
   g.row_part = reinterpret_cast<float*>(work + f.along_bytes);
   g.key_part = reinterpret_cast<float*>(work + f.along_bytes + f.row_bytes);
   float* slope_part = reinterpret_cast<float*>(work + f.along_bytes + f.row_bytes + f.key_bytes);
+  g.sum_part = reinterpret_cast<float*>(work + f.along_bytes + f.row_bytes + f.key_bytes + f.slope_bytes);
   const hipStream_t s = as_stream(stream);
   if (p.queries > 0)
     if (int rc = launch_row_gradient(args->dtype, f, p, g, forces, s)) return rc;

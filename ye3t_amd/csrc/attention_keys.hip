@@ -15,6 +15,8 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
   __shared__ __align__(16) T gtiles[BUFFERS * RT * DP];
   __shared__ f32x4 places[BUFFERS * RT];  // x, y, z, slope
   __shared__ f32x2 all_stats[BUFFERS * RT];  // log sum, or infinity for a row that sees no key or does not exist; D_i
+  constexpr bool KEEP = kKeepLines<T, DP, NW>;
+  __shared__ __align__(16) T kept[KEEP ? TILE * DP : 1];
   const Item item = item_of(p.key_offsets, p.structures, p.keys, 1, TILE, blockIdx.x);
   const Span key = span_of(p.key_offsets, item.structure, p.keys);
   if (item.first < 0 || item.first >= key.length) return;
@@ -32,15 +34,18 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
   line_operand<T, DP>(seen ? static_cast<const T*>(p.k) + token * p.k_row + key_head * p.k_head : nullptr, p.D, half, k);
   line_operand<T, DP>(seen ? static_cast<const T*>(p.v) + token * p.v_row + key_head * p.v_head : nullptr, p.D, half, v);
 
+  T* own_lines = kept + (KEEP ? 32 * wave * DP : 0);
+  if constexpr (KEEP) keep_lines<T, DP>(own_lines, v, lane);
+
   f32x4 next_place = {0.0f, 0.0f, 0.0f, 0.0f};
   f32x2 next_stats = {-INFINITY, 0.0f};
   auto begin = [&](int64_t r0) {
     const int buffer = BUFFERS == 2 ? int(r0 / RT) & 1 : 0;
-    load_tile<T, DP, RT, 64 * NW, BUFFERS == 1>(qtiles + buffer * RT * DP, p.D, p.direct, [&](int line) {
+    load_tile<T, DP, RT, 64 * NW, BUFFERS == 1 || KEEP>(qtiles + buffer * RT * DP, p.D, p.direct, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(p.q) + r.token * p.q_row + r.head * p.q_head : nullptr;
     });
-    load_tile<T, DP, RT, 64 * NW, BUFFERS == 1>(gtiles + buffer * RT * DP, p.D, g.direct, [&](int line) {
+    load_tile<T, DP, RT, 64 * NW, BUFFERS == 1 || KEEP>(gtiles + buffer * RT * DP, p.D, g.direct, [&](int line) {
       const Row r = row_of(p, own.begin, r0 + line, rows, key_head);
       return r.exists ? static_cast<const T*>(g.adjoint) + (r.token * p.heads + r.head) * p.D : nullptr;
     });
@@ -61,8 +66,11 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
 #pragma unroll
   for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
   float gx = 0.0f, gy = 0.0f, gz = 0.0f;
-  if (BUFFERS == 2 && rows > 0) begin(0);
-  for (int64_t r0 = 0; r0 < rows; r0 += RT) {
+  // grid axis z: equal parts of the row tiles
+  const int64_t each = ((rows + RT - 1) / RT + gridDim.z - 1) / gridDim.z * RT;
+  const int64_t start = int64_t(blockIdx.z) * each, until = start + each < rows ? start + each : rows;
+  if (BUFFERS == 2 && start < until) begin(start);
+  for (int64_t r0 = start; r0 < until; r0 += RT) {
     const int buffer = BUFFERS == 2 ? int(r0 / RT) & 1 : 0;
     if (BUFFERS == 1) {
       __syncthreads();  // the last tile has been used
@@ -76,21 +84,34 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
     }
     arrived();
     __syncthreads();
-    if (BUFFERS == 2 && r0 + RT < rows) begin(r0 + RT);
+    if (BUFFERS == 2 && r0 + RT < until) begin(r0 + RT);
     const T *qtile = qtiles + buffer * RT * DP, *gtile = gtiles + buffer * RT * DP;
     const f32x4* place = places + buffer * RT;
     const f32x2* stats = all_stats + buffer * RT;
     if (!busy) continue;
-    const unsigned now_lane = anew<BUFFERS == 1>(lane) & 63;
+    const unsigned now_lane = anew<BUFFERS == 1 || KEEP>(lane) & 63;
     f32x16 s = zeros(), dp = zeros();
-    in_flight<NU>(
-        [&](int u) {
-          return Two<T>{line_chunk<T, DP>(qtile, int(now_lane & 31), u, int(now_lane / 32)), line_chunk<T, DP>(gtile, int(now_lane & 31), u, int(now_lane / 32))};
-        },
-        [&](int u, const Two<T>& qg) {
-          mma(qg.a, k[u], s);
-          mma(qg.b, v[u], dp);
-        });
+    const int own_line = int(now_lane & 31), now_half = int(now_lane / 32);
+    if constexpr (KEEP) {
+      in_flight<NU, 1>(
+          [&](int u) {
+            return Three<T>{line_chunk<T, DP>(qtile, own_line, u, now_half), line_chunk<T, DP>(gtile, own_line, u, now_half),
+                            line_chunk<T, DP>(own_lines, own_line, u, now_half)};
+          },
+          [&](int u, const Three<T>& qgv) {
+            mma(qgv.a, k[u], s);
+            mma(qgv.b, qgv.c, dp);
+          });
+    } else {
+      in_flight<NU>(
+          [&](int u) {
+            return Two<T>{line_chunk<T, DP>(qtile, own_line, u, now_half), line_chunk<T, DP>(gtile, own_line, u, now_half)};
+          },
+          [&](int u, const Two<T>& qg) {
+            mma(qg.a, k[u], s);
+            mma(qg.b, v[u], dp);
+          });
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int line = 8 * (i / 4) + 4 * half + i % 4;
@@ -143,6 +164,13 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
     for (int t = 0; t < ND; ++t) dk[t] = dv[t] = zeros();
   }
   const int64_t at = token * p.key_heads + key_head;
+  if (gridDim.z > 1) {
+    const int64_t all = p.keys * p.key_heads;
+    float* to = g.sum_part + (2 * int64_t(blockIdx.z) * all + at) * p.D;
+    store_columns<float, DP>(to, p.D, half, dk, 1.0f);
+    store_columns<float, DP>(to + all * p.D, p.D, half, dv, 1.0f);
+    return;
+  }
   store_columns<T, DP>(static_cast<T*>(g.dk) + at * p.D, p.D, half, dk, p.scale * slant_scale<CAP>());
   store_columns<T, DP>(static_cast<T*>(g.dv) + at * p.D, p.D, half, dv, 1.0f);
   if (FORCES) {
@@ -153,12 +181,30 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
   }
 }
 
+// The parts' sums, a lane a value.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_key_join_kernel(const float* __restrict__ part, int parts, int64_t count,
+                                                                 float scale, T* __restrict__ dk, T* __restrict__ dv) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < 2 * count; i += int64_t(gridDim.x) * 256) {
+    float s = 0.0f;
+    for (int k = 0; k < parts; ++k) s += part[2 * k * count + i];
+    if (i < count) dk[i] = T(s * scale);
+    else dv[i - count] = T(s);
+  }
+}
+
 template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
 int launch_keys(const AdjointPlan& f, const Problem& p, const Gradient& g, hipStream_t s) {
   if (!fits_grid(f.key_items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many keys for one launch");
   hipLaunchKernelGGL((attention_key_gradient_kernel<T, DP, NW, CAP, BIAS, FORCES>),
-                     dim3(unsigned(f.key_items), unsigned(p.key_heads)), dim3(64 * NW), 0, s, p, g);
-  return check_launch("attention_key_gradient_kernel");
+                     dim3(unsigned(f.key_items), unsigned(p.key_heads), unsigned(f.key_parts)), dim3(64 * NW), 0, s, p, g);
+  if (int rc = check_launch("attention_key_gradient_kernel")) return rc;
+  if (f.key_parts == 1) return YE3T_OK;
+  const int64_t count = p.keys * p.key_heads * p.D, groups = (2 * count + 255) / 256;
+  hipLaunchKernelGGL((attention_key_join_kernel<T>), dim3(unsigned(groups < (1 << 20) ? groups : 1 << 20)), dim3(256), 0, s,
+                     g.sum_part, f.key_parts, count, p.scale * slant_scale<CAP>(), static_cast<T*>(g.dk),
+                     static_cast<T*>(g.dv));
+  return check_launch("attention_key_join_kernel");
 }
 
 struct Side {

@@ -23,6 +23,8 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
   __shared__ __align__(16) T ktiles[BUFFERS * KT * DP];
   __shared__ __align__(16) T vtiles[BUFFERS * KT * DP];
   __shared__ f32x4 places[BUFFERS * KT];
+  constexpr bool KEEP = kKeepLines<T, DP, NW>;
+  __shared__ __align__(16) T kept[KEEP ? TILE * DP : 1];
   const Item item = item_of(p.offsets, p.structures, p.queries, p.group, TILE, blockIdx.x);
   const Span own = span_of(p.offsets, item.structure, p.queries);
   const int64_t rows = int64_t(own.length) * p.group;
@@ -48,6 +50,8 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
       for (int e = 0; e < kChunk<T>; ++e) along += float(o[u][e]) * float(go[u][e]);
     along += other_half(along);
   }
+  T* own_lines = kept + (KEEP ? 32 * wave * DP : 0);
+  if constexpr (KEEP) keep_lines<T, DP>(own_lines, go, lane);
   float x = 0.0f, y = 0.0f, z0 = 0.0f, slope = 0.0f;
   if (BIAS && row.exists) {
     x = p.positions[3 * row.token];
@@ -60,7 +64,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
   const float log_sum2 = log_sum == -INFINITY ? INFINITY : log_sum * kLog2e;
 
   const int tiles = (key.length + KT - 1) / KT;
-  KeyTiles<T, DP, KT, 64 * NW, BUFFERS, BUFFERS == 1, BIAS> tiles_of{
+  KeyTiles<T, DP, KT, 64 * NW, BUFFERS, BUFFERS == 1 || KEEP, BIAS> tiles_of{
       p,      key,    static_cast<const T*>(p.k) + key_head * p.k_head, static_cast<const T*>(p.v) + key_head * p.v_head,
       ktiles, vtiles, places};
   constexpr bool RIGHT = sizeof(T) == 2;  // dq is set right
@@ -87,16 +91,29 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
     const T *ktile = tiles_of.keys(tile), *vtile = tiles_of.values(tile);
     const f32x4* place = tiles_of.places_of(tile);
     if (!busy) continue;
-    const unsigned now_lane = anew<BUFFERS == 1>(lane) & 63;
+    const unsigned now_lane = anew<BUFFERS == 1 || KEEP>(lane) & 63;
     f32x16 s = zeros(), dp = zeros();
-    in_flight<NU>(
-        [&](int u) {
-          return Two<T>{line_chunk<T, DP>(ktile, int(now_lane & 31), u, int(now_lane / 32)), line_chunk<T, DP>(vtile, int(now_lane & 31), u, int(now_lane / 32))};
-        },
-        [&](int u, const Two<T>& kv) {
-          mma(kv.a, q[u], s);
-          mma(kv.b, go[u], dp);
-        });
+    const int line = int(now_lane & 31), now_half = int(now_lane / 32);
+    if constexpr (KEEP) {
+      in_flight<NU, 1>(
+          [&](int u) {
+            return Three<T>{line_chunk<T, DP>(ktile, line, u, now_half), line_chunk<T, DP>(vtile, line, u, now_half),
+                            line_chunk<T, DP>(own_lines, line, u, now_half)};
+          },
+          [&](int u, const Three<T>& kvg) {
+            mma(kvg.a, q[u], s);
+            mma(kvg.b, kvg.c, dp);
+          });
+    } else {
+      in_flight<NU>(
+          [&](int u) {
+            return Two<T>{line_chunk<T, DP>(ktile, line, u, now_half), line_chunk<T, DP>(vtile, line, u, now_half)};
+          },
+          [&](int u, const Two<T>& kv) {
+            mma(kv.a, q[u], s);
+            mma(kv.b, go[u], dp);
+          });
+    }
     Sums now = none;
     const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
 #pragma unroll
