@@ -472,6 +472,8 @@ int gradient_as(const T* adjoint, const Index* tokens, int64_t N, int64_t vocabu
                    : p.L == 128 ? embedding_sum_kernel<T, 128>
                                 : embedding_sum_kernel<T, 256>;
   const int64_t per = kThreads / p.L, clearing = (vocabulary + 63) / 64;
+  if (!fits_grid((p.workers + per - 1) / per + clearing, kThreads))
+    return set_error(YE3T_EUNSUPPORTED, "a table of %lld rows is too large for one launch", (long long)vocabulary);
   hipLaunchKernelGGL(sum, dim3(unsigned((p.workers + per - 1) / per + clearing), unsigned(p.columns)), dim3(kThreads),
                      0, s, sorted, N, p.share, p.workers, adjoint, vocabulary, W, Real(scale), clearing, table, heads,
                      tails, ends);
