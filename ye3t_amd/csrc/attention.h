@@ -136,12 +136,15 @@ __device__ inline bf16x8 column_chunk(const __bf16* tile, int s, int column, uns
 }
 template <int DP>
 __device__ inline f32x4 column_chunk(const float* tile, int s, int column, unsigned lane) {
-  const int half = int(lane / 32), at = int(lane & 31);
+  // turn() of line 8 s + 4 half + j, with what the lane adds to it apart from what s and j do: four
+  // addresses serve all of a tile
+  const int half = int(lane / 32), at = int(lane & 31), own = at / 4 ^ half;
   f32x4 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int line = 8 * s + 4 * half + j;
-    r[j] = tile[line * DP + ((column / 4 + at / 4) ^ turn<float, DP>(line)) * 4 + (at & 3)];
+    const int flip = (DP == 32 ? j / 2 : j & 1) * 4 + 2 * (s & 1), across = DP == 32 ? 0 : column / 32 ^ j / 2;
+    const float* from = tile + 4 * half * DP + (own ^ flip) * 4 + (at & 3);
+    r[j] = from[(8 * s + j) * DP + 32 * across];
   }
   return r;
 }
@@ -347,7 +350,7 @@ __device__ inline f32x4 key_place(const Problem& p, int64_t key, bool seen) {
 // The keys of a structure in tiles of KT <= 64.  take() makes one ready for the
 // workgroup; with two buffers the next one's loads run meanwhile.  One buffer where a
 // workgroup is one wave: more of them fit a compute unit's LDS, and they hide each other's
-// loads (one row against 9 000 atoms in each of 24 structures 150 -> 119 us).  Whether a key is seen is read a tile ahead of its
+// loads (one row against 9 000 atoms in each of 24 structures 150 -> 120 us).  Whether a key is seen is read a tile ahead of its
 // rows; masked keys have rows of zeros, whatever they hold.
 template <typename T, int DP, int KT, int NT, int BUFFERS, bool FRESH, bool BIAS>
 struct KeyTiles {
@@ -445,7 +448,8 @@ __host__ __device__ constexpr float slant_scale() {
 
 // Waves a SIMD that the register budget is set for: spills cost more than a wave gains.
 template <typename T, int DP, int NW>
-constexpr int kForwardWaves = DP == 32 ? (NW == 1 ? 4 : 3) : DP == 64 || sizeof(T) == 2 ? 2 : 1;
+constexpr int kForwardWaves =
+    DP == 32 ? (NW == 1 ? 4 : 3) : DP == 64 ? (sizeof(T) == 4 && NW == 1 ? 2 : 3) : sizeof(T) == 2 ? 2 : 1;
 template <typename T, int DP, int NW>
 constexpr int kGradientWaves = DP == 32 ? (NW == 1 ? 3 : 2) : DP == 64 || kKeepLines<T, DP, NW> ? 2 : 1;
 
@@ -460,7 +464,8 @@ inline int waves_for(int64_t rows, int64_t structures) {
 // Parts of the key axis: where the rows alone give less than four workgroups
 // a compute unit, as many as make eight, each with two tiles of 32 keys or more on
 // average, 64 at most (a lane each where they are joined).  24 structures of 9 000
-// atoms, one row each, 16 heads of 128 over 4 key heads, bf16: 119 us; 136 by twice as many.
+// atoms, one row each, 16 heads of 128 over 4 key heads, bf16, before
+// the parts were joined a lane each: 120 us; 136 by twice as many, 150 by half.
 inline int parts_for(int64_t items, int key_heads, int64_t keys, int64_t structures) {
   const int64_t groups = items * key_heads;
   if (groups >= 1024 || structures == 0) return 1;

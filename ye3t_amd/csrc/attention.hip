@@ -7,8 +7,17 @@ namespace attention {
 namespace {
 
 // ---- forward -----------------------------------------------------------------
-// NW waves of 32 rows, KT keys a tile.  SPLIT: grid axis z takes equal parts of
-// each structure's key tiles and leaves its sums to attention_join_kernel.
+// One pass over the keys with the running maximum and sum of the softmax; the scores,
+// their weights and the output rows stay in registers, so memory is read once for each 128 rows
+// and written once.  NW waves of 32 rows, KT keys a tile.  SPLIT: grid axis z takes equal
+// parts of each structure's key tiles and leaves its sums to attention_join_kernel.
+//
+// Bound by what a score costs beside the products: about 17 vector operations with
+// distance and cap, four of them of quarter rate, 5 without.  8 192 atoms, 16
+// heads of 128 over 4, bf16: 0.68 ms, 810 TFLOP/s (1 136 for a large product here); 96
+// structures of 480, 8 heads of 64, distances, cap and mask: 0.20 ms, 240 TFLOP/s.  fp32: 40
+// structures of 1 000, 8 heads of 64, distances: 0.97 ms, 87 of 152 TFLOP/s.  One row against
+// 9 000 atoms in 24 structures: 0.10 ms for 437 MB.
 template <typename T, int DP, int NW, int KT, bool BIAS, bool CAP, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP, NW>)) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
                                                             float* __restrict__ part, float* __restrict__ part_stats) {
