@@ -492,8 +492,8 @@ inline ForwardPlan forward_plan(const ye3t_attention_args& a) {
   return f;
 }
 
-// workgroups that share the sum over atoms of the slopes' gradient
-constexpr int kSlopeGroups = 256;
+// workgroups that share the sum over atoms of a slope's gradient
+constexpr int kSlopeGroups = 64;
 
 struct AdjointPlan {
   int row_waves, key_waves, key_parts;

@@ -204,25 +204,21 @@ __global__ __launch_bounds__(256) void attention_force_kernel(const float* __res
   }
 }
 
-// dslope_h: a workgroup sums its share of the tokens for every head, a lane a
-// head and a token in turn; attention_slope_kernel adds the shares in order.
+// dslope_h: a workgroup sums its share of the tokens for one head, a lane a token in turn;
+// attention_slope_kernel adds the shares in order.
 __global__ __launch_bounds__(256) void attention_slope_part_kernel(const float* __restrict__ row_part, int64_t queries,
                                                                    int heads, float* __restrict__ part) {
-  __shared__ float sums[256];
+  __shared__ float sums[4];
+  const int h = blockIdx.y;
   const int64_t each = (queries + gridDim.x - 1) / gridDim.x;
   const int64_t begin = int64_t(blockIdx.x) * each, end = begin + each < queries ? begin + each : queries;
-  for (int h = 0; h < heads; ++h) {
-    float s = 0.0f;
-    for (int64_t i = begin + threadIdx.x; i < end; i += 256) s += row_part[4 * (i * heads + h) + 3];
-    sums[threadIdx.x] = s;
-    __syncthreads();
-    for (int m = 128; m > 0; m /= 2) {
-      if (int(threadIdx.x) < m) sums[threadIdx.x] += sums[threadIdx.x + m];
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) part[blockIdx.x * int64_t(heads) + h] = sums[0];
-    __syncthreads();
-  }
+  float s = 0.0f;
+  for (int64_t i = begin + threadIdx.x; i < end; i += 256) s += row_part[4 * (i * heads + h) + 3];
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) s += __shfl_xor(s, m);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x * int64_t(heads) + h] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 __global__ __launch_bounds__(64) void attention_slope_kernel(const float* __restrict__ part, int groups, int heads,
                                                              float* __restrict__ slopes) {
@@ -364,7 +360,7 @@ int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void*
                        static_cast<float*>(key_positions_adjoint));
     if (int rc = check_launch("attention_force_kernel")) return rc;
   }
-  hipLaunchKernelGGL(attention_slope_part_kernel, dim3(kSlopeGroups), dim3(256), 0, s, g.row_part, p.queries, p.heads,
+  hipLaunchKernelGGL(attention_slope_part_kernel, dim3(kSlopeGroups, unsigned(p.heads)), dim3(256), 0, s, g.row_part, p.queries, p.heads,
                      slope_part);
   if (int rc = check_launch("attention_slope_part_kernel")) return rc;
   hipLaunchKernelGGL(attention_slope_kernel, dim3(unsigned(p.heads)), dim3(64), 0, s, slope_part, kSlopeGroups, p.heads,

@@ -407,9 +407,10 @@ struct GradientPlan {
 };
 
 // Sorting: runs of at least 2 048 positions, 128 of them at most.  Sums: lanes
-// enough for a row (256 at most), and shares that give the card about two
-// waves a SIMD, of 16 positions or more: eight rows of a lane are in flight at a time, so
-// that is 8 MB of them, and every further share is one more end to join.
+// enough for a row (256 at most), and shares that give the card about two waves a
+// SIMD, of 16 positions or more.  Eight rows of a lane are in flight at a time, and
+// every further share is one more end to join: 200 000 x 128 fp32 by 8 tokens, sums
+// and join 26 + 16 us; 43 + 9 by one wave a SIMD.
 GradientPlan gradient_plan(int64_t N, int64_t vocabulary, int64_t width, int size) {
   GradientPlan p{};
   for (p.passes = 1; p.passes < 4 && (vocabulary >> (8 * p.passes)) > 0; ++p.passes) {}
