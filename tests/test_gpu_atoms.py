@@ -520,3 +520,40 @@ def test_unchecked_offsets_stay_inside(gpu):
         out, sums = runtime.atom_attention(q, k, v, bad, return_log_sums=True, validate=False, **kw)
         runtime.atom_attention_adjoint(q, out, torch.zeros_like(sums), q, k, v, bad, bias_gradients=True, validate=False, **kw)
     torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(gpu):
+    """Tables, rows and keys of more than 2^31 values: the last ones are the last ones."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush("more than 2^31 values: embedding and norm")
+    rows, width = 4_200_003, 512
+    big = torch.zeros((rows, width), dtype=torch.bfloat16, device=gpu)
+    tail = normal((3, width), "bfloat16", 1, gpu)
+    big[-3:] = tail
+    ids = torch.tensor([0, rows - 1, rows - 3], device=gpu)
+    assert torch.equal(runtime.embedding(ids, big), big[ids])
+    weight = normal((width,), "bfloat16", 2, gpu)
+    y = runtime.rms_norm(big, weight)
+    assert torch.equal(y[-3:], runtime.rms_norm(tail, weight)) and not y[:100].any()
+    del y
+    flush("  their gradients")
+    dx, dw = runtime.rms_norm_adjoint(big, big, weight)
+    want = runtime.rms_norm_adjoint(tail, tail, weight)
+    assert torch.equal(dx[-3:], want[0]) and torch.equal(dw, want[1])
+    del dx, big
+    flush("  attention to the last of 17 000 000 keys")
+    keys = 17_000_000
+    k = torch.zeros((keys, 1, 128), dtype=torch.bfloat16, device=gpu)
+    v = torch.zeros_like(k)
+    mask = torch.zeros(keys, dtype=torch.bool, device=gpu)
+    seen = torch.tensor([0, 1, keys - 40, keys - 2, keys - 1], device=gpu)
+    mask[seen] = True
+    k[seen], v[seen] = normal((5, 1, 128), "bfloat16", 3, gpu), normal((5, 1, 128), "bfloat16", 4, gpu)
+    q = normal((1, 2, 128), "bfloat16", 5, gpu)
+    out = runtime.atom_attention(q, k, v, torch.tensor([0, 1], device=gpu), key_offsets=torch.tensor([0, keys], device=gpu),
+                                 key_mask=mask)
+    want, _ = _atoms.attention(q.cpu(), k[seen].cpu(), v[seen].cpu(), torch.tensor([0, 1]), key_offsets=torch.tensor([0, 5]))
+    near(out, want, "bfloat16", what="out")
