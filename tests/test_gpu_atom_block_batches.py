@@ -1,0 +1,30 @@
+"""Features and energies of structures do not depend on the batch that they are in, nor on where they lie."""
+
+import pytest
+
+from tests._util import flush
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("count,centre", [(300, 1000.0), (3000, 0.0)])
+def test_features_of_the_last_structure_of_a_batch(gpu, count, centre):
+    """The batch's neighbour list has the pairs that the structure has by itself: the same edge vectors in the same
+    order, so features equal to within fp32 (the 2e-5 that this package holds fp32 to)."""
+    import torch
+
+    from ye3t_amd.ace.atom_block import AceFeatures, synthetic_structures
+
+    flush(f"features of {count} structures around {centre}, and of the last ones by themselves")
+    features = AceFeatures(3, device=gpu)
+    positions, species, offsets = synthetic_structures(count, 20, 3, seed=6, device=gpu)
+    positions = positions + centre
+    ends = offsets.tolist()
+    held = features(positions, species, offsets)
+    for s in (0, count // 2, count - 2, count - 1):
+        part = slice(ends[s], ends[s + 1])
+        alone = features(positions[part], species[part], torch.tensor([0, ends[s + 1] - ends[s]], device=gpu))
+        size = alone.double().square().mean(0).sqrt().clamp(min=1e-30)
+        worst = float(((held[part] - alone).double().abs() / size).max())
+        flush(f"  structure {s}: {worst:.2e}")
+        assert worst < 2e-5

@@ -62,9 +62,14 @@ class AceFeatures:
         atoms = int(positions.shape[0])
         owner = torch.searchsorted(offsets, torch.arange(atoms, device=offsets.device), right=True) - 1
         with torch.no_grad():
-            # the structures side by side, further apart than the cutoff, make one neighbour list
-            reach = float(positions.abs().max()) * 2.0 + 2.0 * CUTOFF if atoms else 0.0
-            apart = positions.detach().clone()
+            # Structures side by side along x, further apart than the cutoff, make one neighbour list.
+            # Each is laid out from its own corner, in float64: in float32 a large batch, or one far from
+            # the origin, would lose digits of the distances and with them pairs.
+            apart = positions.detach().double()
+            corner = torch.full((offsets.numel() - 1, 3), math.inf, dtype=torch.float64, device=positions.device)
+            corner.scatter_reduce_(0, owner[:, None].expand(-1, 3), apart, "amin")
+            apart = apart - corner[owner]
+            reach = float(apart[:, 0].max()) + 2.0 * CUTOFF if atoms else 0.0
             apart[:, 0] += owner * reach
             pairs = runtime.neighbor_list(apart, CUTOFF)
             rows, centres, neighbours = pairs["target_offsets"], pairs["edge_targets"], pairs["edge_sources"]
