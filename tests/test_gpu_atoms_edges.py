@@ -1,0 +1,75 @@
+"""Embedding, norm and attention where they can go wrong: rows and atoms that are not finite, empty batches, atoms that
+nearly meet or lie far away, large caps, long inputs, and gradients of every variant held to the size of their terms
+element by element."""
+
+import math
+
+import pytest
+
+from tests._util import flush
+from tests.test_gpu_atoms import normal, problem
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["float32", "bfloat16"]
+
+
+def run(q, k, v, offsets, kw, cap=0.0, forces=False, g=None):
+    """{name: tensor} of the forward and its gradients, and the adjoint they were taken for."""
+    from ye3t_amd import runtime
+
+    out, sums = runtime.atom_attention(q, k, v, offsets, cap=cap, return_log_sums=True, **kw)
+    g = normal(tuple(q.shape), str(q.dtype).split(".")[1], 77, q.device) if g is None else g
+    grads = runtime.atom_attention_adjoint(g, out, sums, q, k, v, offsets, cap=cap, bias_gradients=forces, **kw)
+    names = ("q", "k", "v", "slopes", "positions", "key_positions")
+    return {"out": out, "sums": sums, **{n: t for n, t in zip(names, grads) if t is not None}}, g
+
+
+# ---- rows that see nothing -------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [16, 64, 128])
+@pytest.mark.parametrize("lengths", [[5, 9, 4], [40, 210, 30]], ids=str)
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (5.0, False), (0.0, True), (5.0, True)])
+def test_rows_of_a_hidden_structure_that_are_not_finite(gpu, dtype, width, lengths, cap, bias):
+    """Rows that see nothing give zeros and no gradients whatever they hold; the other structures' results keep their
+    bits."""
+    import torch
+
+    flush(f"rows that are not finite and see nothing, {lengths} x {width}, cap {cap}, bias {bias}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, 4, 2, width, dtype, gpu, bias=bias)
+    hidden = slice(lengths[0], lengths[0] + lengths[1])
+    kw["key_mask"] = torch.ones(sum(lengths), dtype=torch.bool, device=gpu)
+    kw["key_mask"][hidden] = False
+    clean, g = run(q, k, v, offsets, kw, cap, bias)
+    assert not clean["out"][hidden].any() and bool((clean["sums"][hidden] == -math.inf).all())
+    for value in (math.nan, math.inf, -math.inf):
+        held = [t.clone() for t in (q, k, v)]
+        for t in held:
+            t[hidden] = value
+        other = dict(kw)
+        if bias:
+            other["positions"] = kw["positions"].clone()
+            other["positions"][hidden] = value
+        for adjoint in (g, g.index_fill(0, torch.arange(hidden.start, hidden.stop, device=gpu), value)):
+            got, _ = run(*held, offsets, other, cap, bias, adjoint)
+            for n, t in got.items():
+                assert torch.equal(t, clean[n]), (value, n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_rows_that_are_not_finite_against_hidden_keys(gpu, dtype):
+    """The same where the keys are split among workgroups and joined."""
+    import torch
+
+    flush(f"few rows that are not finite against hidden keys, {dtype}")
+    q, k, v, offsets, kw = problem([2, 1, 1], 4, 2, 64, dtype, gpu, key_lengths=[3000, 900, 0], bias=True)
+    kw["key_mask"] = torch.ones(3900, dtype=torch.bool, device=gpu)
+    kw["key_mask"][3000:] = False
+    clean, g = run(q, k, v, offsets, kw, 0.0, True)
+    q, kw["positions"] = q.clone(), kw["positions"].clone()
+    q[2:], kw["positions"][2:] = math.nan, math.inf
+    got, _ = run(q, k, v, offsets, kw, 0.0, True, g)
+    assert not got["out"][2:].any() and bool((got["sums"][2:] == -math.inf).all())
+    for n, t in got.items():
+        assert torch.equal(t, clean[n]), n

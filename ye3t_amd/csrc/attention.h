@@ -361,6 +361,7 @@ struct KeyTiles {
   f32x4* places;
   f32x4 place;
   uint8_t mask;  // of this lane's key in the tile after the one begun last, as it was read
+  bool any = false;  // a key of the tiles begun so far is seen: the same in all lanes and waves
 
   __device__ static inline int buffer(int tile) { return BUFFERS == 2 ? tile & 1 : 0; }
   __device__ inline const T* keys(int tile) const { return ktiles + buffer(tile) * KT * DP; }
@@ -382,6 +383,7 @@ struct KeyTiles {
   __device__ inline void begin(int tile) {
     const bool seen = exists(tile) && mask;
     const uint64_t all = __ballot(seen);
+    any |= all != 0;
     const int64_t first = key.begin + int64_t(tile) * KT;
     load_tile<T, DP, KT, NT, FRESH>(ktiles + buffer(tile) * KT * DP, p.D, p.direct,
                              [&](int line) { return all >> line & 1 ? kbase + (first + line) * p.k_row : nullptr; });

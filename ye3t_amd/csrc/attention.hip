@@ -126,6 +126,14 @@ __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP, NW>)) void attention
     }
   }
   if (!row.exists) return;
+  // Keys are hidden from all rows of a structure or from none.  Scores of hidden keys are
+  // -infinity only for rows that are finite themselves: where no key is seen nothing of them counts.
+  if (!tiles_of.any) {
+    top = -INFINITY;
+    sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < ND; ++t) acc[t] = zeros();
+  }
   sum += other_half(sum);
   const int64_t at = row.token * p.heads + row.head;
   if (SPLIT) {

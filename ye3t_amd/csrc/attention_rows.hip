@@ -66,7 +66,6 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
     z0 = p.positions[3 * row.token + 2];
     slope = p.slopes[row.head] * kLog2e;
   }
-  // a row that sees no key has no gradient: p = 0
   const float log_sum = row.exists ? g.log_sums[at] : -INFINITY;
   const float log_sum2 = log_sum == -INFINITY ? INFINITY : log_sum * kLog2e;
 
@@ -168,9 +167,17 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
                                      if constexpr (RIGHT) mma(k, m[i / ND], own_keys[i % ND]);
                                    });
   }
-  const float off = RIGHT || FORCES ? all.dz + other_half(all.dz) : 0.0f;
+  float off = RIGHT || FORCES ? all.dz + other_half(all.dz) : 0.0f;
   along += off;
   if (!row.exists) return;
+  if (log_sum == -INFINITY) {  // a row that sees no key has no gradient, whatever it holds
+    off = along = 0.0f;
+    all = none;
+#pragma unroll
+    for (int t = 0; t < ND; ++t) acc[t] = zeros();
+#pragma unroll
+    for (int t = 0; t < (RIGHT ? ND : 1); ++t) own_keys[t] = zeros();
+  }
   if (RIGHT) {
 #pragma unroll
     for (int t = 0; t < ND; ++t)
