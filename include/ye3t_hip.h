@@ -881,7 +881,8 @@ int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_
  * cap * tanh(score / cap), then, with slopes, less slopes[head] times the
  * distance of the two atoms.  key_mask (NULL: all) is 0 for keys that no row
  * sees; what they hold is not used.  A row that sees no key gives zeros.
- * Strides are in values, those of the last axis 1. */
+ * Strides are in values, those of the last axis 1.  Arrays without values
+ * (positions of no query atoms, say) may be NULL. */
 typedef struct {
   int dtype;           /* YE3T_F32 or YE3T_BF16: query, key, value, outputs and their adjoints */
   int64_t queries;     /* query atoms */

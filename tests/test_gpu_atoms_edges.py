@@ -73,3 +73,40 @@ def test_few_rows_that_are_not_finite_against_hidden_keys(gpu, dtype):
     assert not got["out"][2:].any() and bool((got["sums"][2:] == -math.inf).all())
     for n, t in got.items():
         assert torch.equal(t, clean[n]), n
+
+
+# ---- empty batches ---------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,keys", [([0, 0], [3, 40]), ([5, 2], [0, 0]), ([0], [0]), ([0, 0], None), ([], None), ([], [])],
+                         ids=str)
+@pytest.mark.parametrize("bias", [False, True])
+def test_no_rows_and_no_keys(gpu, dtype, lengths, keys, bias):
+    """Rows without keys give zeros, keys without rows no gradient; autograd too."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"attention of {lengths} to {keys}, bias {bias}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, 4, 2, 32, dtype, gpu, key_lengths=keys, bias=bias)
+    got, _ = run(q, k, v, offsets, kw, 0.0, bias)
+    assert got["out"].shape == q.shape and bool((got["sums"] == -math.inf).all())
+    for n in ("out", "q", "k", "v", "slopes", "positions", "key_positions"):
+        assert n not in got or not got[n].any(), n
+    leaves = [t.requires_grad_() for t in (q, k, v)] + [kw[n].requires_grad_() for n in kw if n != "key_offsets"]
+    out = runtime.atom_attention(q, k, v, offsets, **kw)
+    for t, grad in zip(leaves, torch.autograd.grad(out.sum(), leaves)):
+        assert grad.shape == t.shape and not grad.any()
+
+
+def test_layer_without_atoms(gpu):
+    import torch
+
+    from ye3t_amd.ace.atom_block import AtomBlock
+
+    flush("the layer on structures without atoms")
+    block = AtomBlock(20, 3, width=32, heads=2).to(gpu)
+    for ends in ([0], [0, 0, 0]):
+        energies = block(torch.zeros(0, 20, device=gpu), torch.zeros(0, dtype=torch.int32, device=gpu),
+                         torch.zeros(0, 3, device=gpu), torch.tensor(ends, device=gpu))
+        assert energies.shape == (len(ends) - 1,) and not energies.any()

@@ -582,8 +582,9 @@ inline int check_attention(const ye3t_attention_args& a) {
                    a.structures < (int64_t(1) << 24),
                "at most 2^31 - 1 rows (atoms times heads), 65535 heads and 2^24 - 1 structures");
   YE3T_REQUIRE(a.cap >= 0.0, "cap must not be negative");
-  YE3T_REQUIRE((a.slopes == nullptr) == (a.positions == nullptr), "slopes and positions come together");
-  YE3T_REQUIRE(!a.slopes || a.key_positions || (!a.key_offsets && a.queries == a.keys),
+  // arrays without values may be null
+  YE3T_REQUIRE(a.queries == 0 || (a.slopes == nullptr) == (a.positions == nullptr), "slopes and positions come together");
+  YE3T_REQUIRE(!a.slopes || a.keys == 0 || a.key_positions || (!a.key_offsets && a.queries == a.keys),
                "keys of their own need key_positions");
   YE3T_REQUIRE(a.key_offsets || a.queries == a.keys, "keys of their own need key_offsets");
   return YE3T_OK;

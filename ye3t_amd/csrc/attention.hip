@@ -359,7 +359,7 @@ int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void*
   if (p.keys > 0)
     if (int rc = launch_key_gradient(args->dtype, f, p, g, forces, s)) return rc;
   if (!forces) return YE3T_OK;
-  const bool shared = p.key_positions == nullptr;
+  const bool shared = !args->key_positions && !args->key_offsets;  // keys are the query atoms
   const int64_t atoms = p.queries + (shared ? 0 : p.keys);
   if (atoms > 0) {
     const int64_t groups = (atoms + 255) / 256;
