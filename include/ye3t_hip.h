@@ -926,7 +926,8 @@ int64_t ye3t_hip_atom_attention_adjoint_workspace_bytes(const ye3t_attention_arg
  * in `dtype`.  With slopes_adjoint [heads] also the fp32 gradients to the slopes
  * and to positions [queries, 3] and key_positions [keys, 3]; without
  * key_positions the atoms are the same and positions_adjoint holds both parts.
- * Two atoms at one place have no direction and add nothing to either. */
+ * Two atoms at one place (less than 1.1e-19 apart) have no direction and add
+ * nothing to either. */
 int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void* out, const void* log_sums,
                                     const void* out_adjoint, void* query_adjoint, void* key_adjoint,
                                     void* value_adjoint, void* slopes_adjoint, void* positions_adjoint,

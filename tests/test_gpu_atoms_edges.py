@@ -6,6 +6,7 @@ import math
 
 import pytest
 
+from tests import _atoms_sizes
 from tests._util import flush
 from tests.test_gpu_atoms import normal, problem
 
@@ -110,3 +111,21 @@ def test_layer_without_atoms(gpu):
         energies = block(torch.zeros(0, 20, device=gpu), torch.zeros(0, dtype=torch.int32, device=gpu),
                          torch.zeros(0, 3, device=gpu), torch.tensor(ends, device=gpu))
         assert energies.shape == (len(ends) - 1,) and not energies.any()
+
+
+# ---- atoms that nearly meet, and far away ones -------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [[21], [150]], ids=str)
+def test_forces_of_atoms_that_nearly_meet(gpu, dtype, lengths):
+    """Atoms whose squared distance is below the smallest normal float are at one place."""
+    flush(f"forces of {lengths} atoms, some nearly at one place, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, 2, 2, 24, dtype, gpu, bias=True)
+    kw["positions"][3] = 0.0
+    for atom, x in ((4, 1e-20), (5, 1e-25), (6, -3e-21), (7, 1e-30)):
+        kw["positions"][atom] = 0.0
+        kw["positions"][atom, atom % 3] = x
+    got, g = run(q, k, v, offsets, kw, 0.0, True)
+    exact = _atoms_sizes.attention(q, k, v, offsets, g, **kw)
+    for n, e in exact.items():
+        _atoms_sizes.check(n, got[n], e, dtype)

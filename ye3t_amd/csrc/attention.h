@@ -40,6 +40,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr double kLog2eExact = 1.4426950408889634;
 constexpr float kLog2e = float(kLog2eExact);
 constexpr float kLn2 = 0.6931471805599453f;
+// Atoms whose squared distance is below the smallest normal float are at one place: the
+// reciprocal root takes no subnormal value.
+constexpr float kLeastSquare = 1.17549435e-38f;
 
 struct Problem {
   int64_t queries, keys, structures;

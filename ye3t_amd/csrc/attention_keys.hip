@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
         dx = here[0] - r[0], dy = here[1] - r[1], dz = here[2] - r[2], slope = r[3];
         const float square = dx * dx + dy * dy + dz * dz;
         if (FORCES) {
-          per = square > 0.0f ? __builtin_amdgcn_rsqf(square) : 0.0f;
+          per = square >= kLeastSquare ? __builtin_amdgcn_rsqf(square) : 0.0f;
           exponent -= slope * (square * per);
         } else {
           exponent -= slope * __builtin_amdgcn_sqrtf(square);
