@@ -879,10 +879,11 @@ int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_
  * key_offsets (NULL: the same).  Query head h reads key head
  * h / (heads / key_heads).  Scores are scale * q . k, then, for cap > 0,
  * cap * tanh(score / cap), then, with slopes, less slopes[head] times the
- * distance of the two atoms.  key_mask (NULL: all) is 0 for keys that no row
- * sees; what they hold is not used.  A row that sees no key gives zeros.
- * Strides are in values, those of the last axis 1.  Arrays without values
- * (positions of no query atoms, say) may be NULL. */
+ * distance of the two atoms.  Atoms more than 1.8e19 apart do not see each
+ * other (under a slope of 0 such a distance is not a number).  key_mask (NULL:
+ * all) is 0 for keys that no row sees; what they hold is not used.  A row that
+ * sees no key gives zeros.  Strides are in values, those of the last axis 1.
+ * Arrays without values (positions of no query atoms, say) may be NULL. */
 typedef struct {
   int dtype;           /* YE3T_F32 or YE3T_BF16: query, key, value, outputs and their adjoints */
   int64_t queries;     /* query atoms */

@@ -129,3 +129,47 @@ def test_forces_of_atoms_that_nearly_meet(gpu, dtype, lengths):
     exact = _atoms_sizes.attention(q, k, v, offsets, g, **kw)
     for n, e in exact.items():
         _atoms_sizes.check(n, got[n], e, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [[21, 12], [150, 40]], ids=str)
+@pytest.mark.parametrize("far", [1e20, 1e25, 3e38, math.inf])
+def test_forces_with_hidden_atoms_put_far_away(gpu, dtype, lengths, far):
+    """Hidden atoms whose squared distance overflows reach nothing, see nothing and have no forces."""
+    import torch
+
+    flush(f"forces of {lengths} atoms, hidden ones at {far}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, 2, 2, 24, dtype, gpu, bias=True)
+    kw["key_mask"] = torch.ones(sum(lengths), dtype=torch.bool, device=gpu)
+    kw["key_mask"][2:5] = False
+    kw["positions"][2:4, 0] = far
+    kw["positions"][4] = -far
+    got, g = run(q, k, v, offsets, kw, 0.0, True)
+    visible = kw["key_mask"].nonzero()[:, 0]
+    # what is left when the hidden atoms are taken out
+    ends = offsets.clone()
+    ends[1:] -= 3
+    less = {"slopes": kw["slopes"], "positions": kw["positions"][visible]}
+    exact = _atoms_sizes.attention(q[visible], k[visible], v[visible], ends, g[visible], **less)
+    for n, e in exact.items():
+        _atoms_sizes.check(n, got[n] if n == "slopes" else got[n][visible], e, dtype)
+    for n in ("out", "q", "k", "v", "positions"):
+        assert not got[n][2:5].any(), n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [[21, 12], [150, 40]], ids=str)
+@pytest.mark.parametrize("far", [1e20, 1e25])
+@pytest.mark.parametrize("forces", [False, True])
+def test_gradients_with_atoms_far_away(gpu, dtype, lengths, far, forces):
+    """Atoms that are seen, but so far away that their squared distance overflows: they see themselves alone."""
+    flush(f"gradients of {lengths} atoms, some at {far}, forces {forces}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, 2, 2, 24, dtype, gpu, bias=True)
+    kw["positions"][2, 0] = far
+    kw["positions"][3, 0] = -far
+    kw["positions"][4] = far
+    got, g = run(q, k, v, offsets, kw, 0.0, forces)
+    exact = _atoms_sizes.attention(q, k, v, offsets, g, **kw)
+    for n, e in exact.items():
+        if n in got:
+            _atoms_sizes.check(n, got[n], e, dtype)

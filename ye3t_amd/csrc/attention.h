@@ -43,6 +43,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Atoms whose squared distance is below the smallest normal float are at one place: the
 // reciprocal root takes no subnormal value.
 constexpr float kLeastSquare = 1.17549435e-38f;
+// A squared distance past the largest float is infinite, and so is the distance that scores are lowered
+// by: such atoms do not see each other.  Gradients take the distance as square times
+// reciprocal root, which has to be a number.
+constexpr float kMostSquare = 3.40282347e38f;
 
 struct Problem {
   int64_t queries, keys, structures;

@@ -85,8 +85,11 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
       begin(r0);
     }
     if (int(threadIdx.x) < RT) {
-      places[buffer * RT + threadIdx.x] = f32x4{next_place[0], next_place[1], next_place[2], next_place[3] * kLog2e};
       const bool counts = next_stats[0] != -INFINITY;
+      // A row that sees no key or does not exist: one place for all, with a slope, since zero
+      // times the distance of a key too far away is not a number.
+      places[buffer * RT + threadIdx.x] =
+          counts ? f32x4{next_place[0], next_place[1], next_place[2], next_place[3] * kLog2e} : f32x4{0.0f, 0.0f, 0.0f, 1.0f};
       all_stats[buffer * RT + threadIdx.x] =
           f32x2{counts ? next_stats[0] * kLog2e : INFINITY, counts ? next_stats[1] : 0.0f};
     }
@@ -131,8 +134,8 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
         dx = here[0] - r[0], dy = here[1] - r[1], dz = here[2] - r[2], slope = r[3];
         const float square = dx * dx + dy * dy + dz * dz;
         if (FORCES) {
-          per = square >= kLeastSquare ? __builtin_amdgcn_rsqf(square) : 0.0f;
-          exponent -= slope * (square * per);
+          per = square >= kLeastSquare ? __builtin_amdgcn_rsqf(fminf(square, kMostSquare)) : 0.0f;
+          exponent -= slope * (fminf(square, kMostSquare) * per);
         } else {
           exponent -= slope * __builtin_amdgcn_sqrtf(square);
         }

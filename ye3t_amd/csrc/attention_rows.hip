@@ -131,8 +131,8 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
         dx = x - k[0], dy = y - k[1], dz = z0 - k[2];
         const float square = dx * dx + dy * dy + dz * dz;
         if (FORCES) {
-          per = square >= kLeastSquare ? __builtin_amdgcn_rsqf(square) : 0.0f;
-          distance = square * per;
+          per = square >= kLeastSquare ? __builtin_amdgcn_rsqf(fminf(square, kMostSquare)) : 0.0f;
+          distance = fminf(square, kMostSquare) * per;
         } else {
           distance = __builtin_amdgcn_sqrtf(square);
         }
