@@ -173,3 +173,28 @@ def test_gradients_with_atoms_far_away(gpu, dtype, lengths, far, forces):
     for n, e in exact.items():
         if n in got:
             _atoms_sizes.check(n, got[n], e, dtype)
+
+
+# ---- the longest structure -----------------------------------------------------------
+
+def test_as_many_keys_as_there_may_be(gpu):
+    """2^31 - 256 keys of one structure: the last ones are found, and every one gets its gradient."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    keys = 2 ** 31 - 256
+    flush(f"attention of a row to the last of {keys} keys")
+    k = normal((1, 1, 1), "bfloat16", 1, gpu).expand(keys, 1, 1)
+    v = torch.zeros((keys, 1, 1), dtype=torch.bfloat16, device=gpu)
+    v[-3:, 0, 0] = torch.tensor([3.0, 6.0, 9.0], device=gpu)
+    mask = torch.zeros(keys, dtype=torch.bool, device=gpu)
+    mask[-3:] = True
+    q, offsets, ends = normal((1, 1, 1), "bfloat16", 2, gpu), torch.tensor([0, 1], device=gpu), torch.tensor([0, keys], device=gpu)
+    out = runtime.atom_attention(q, k, v, offsets, key_offsets=ends, key_mask=mask)
+    assert abs(float(out) - 6.0) <= 6.0 * 2.0 ** -8
+    flush("  the gradients of keys without rows")
+    none = q[:0]
+    grads = runtime.atom_attention_adjoint(none, none, torch.zeros((0, 1), device=gpu), none, k, v, torch.tensor([0, 0], device=gpu),
+                                           key_offsets=ends, key_mask=mask)
+    assert not grads[1].any() and not grads[2].any()

@@ -585,9 +585,12 @@ inline int check_attention(const ye3t_attention_args& a) {
   if (a.head_width > 128) return set_error(YE3T_EUNSUPPORTED, "head_width %lld is above 128", (long long)a.head_width);
   if (a.dtype != YE3T_F32 && a.dtype != YE3T_BF16)
     return set_error(YE3T_EDTYPE, "unsupported dtype %d; expected float32 or bfloat16", a.dtype);
-  YE3T_REQUIRE(a.heads <= 65535 && a.queries < (int64_t(1) << 31) / a.heads && a.keys < (int64_t(1) << 31) / a.heads &&
+  // Rows, keys and tiles of one structure are counted in 32 bits.  The first row past the last tile,
+  // and the tile looked at ahead of it, are at most 255 on.
+  constexpr int64_t most = (int64_t(1) << 31) - 256;
+  YE3T_REQUIRE(a.heads <= 65535 && a.queries <= most / a.heads && a.keys <= most / a.heads &&
                    a.structures < (int64_t(1) << 24),
-               "at most 2^31 - 1 rows (atoms times heads), 65535 heads and 2^24 - 1 structures");
+               "at most 2^31 - 256 rows (atoms times heads), 65535 heads and 2^24 - 1 structures");
   YE3T_REQUIRE(a.cap >= 0.0, "cap must not be negative");
   // arrays without values may be null
   YE3T_REQUIRE(a.queries == 0 || (a.slopes == nullptr) == (a.positions == nullptr), "slopes and positions come together");
