@@ -198,3 +198,19 @@ def test_as_many_keys_as_there_may_be(gpu):
     grads = runtime.atom_attention_adjoint(none, none, torch.zeros((0, 1), device=gpu), none, k, v, torch.tensor([0, 0], device=gpu),
                                            key_offsets=ends, key_mask=mask)
     assert not grads[1].any() and not grads[2].any()
+
+
+# ---- caps --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [32, 64, 128])
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1e3, 1e5, 1e7, 1e20])
+def test_caps_of_any_size(gpu, dtype, width, cap):
+    """A cap far above the scores changes nothing."""
+    flush(f"attention capped at {cap}, width {width}, {dtype}")
+    for lengths in ([9], [170]):
+        q, k, v, offsets, kw = problem(lengths, 2, 1, width, dtype, gpu, bias=True)
+        got, g = run(q, k, v, offsets, kw, cap, True)
+        exact = _atoms_sizes.attention(q, k, v, offsets, g, cap=cap, **kw)
+        for n, e in exact.items():
+            _atoms_sizes.check(n, got[n], e, dtype)

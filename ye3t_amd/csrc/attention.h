@@ -26,6 +26,8 @@
 // 2^-9 each, as the inputs have) and each output once.
 #pragma once
 
+#include <type_traits>
+
 #include "rows.h"
 
 namespace ye3t {
@@ -206,19 +208,20 @@ template <typename T, int DP, int NW>
 constexpr bool kKeepLines = sizeof(T) == 2 && DP == 128 && NW == 4;
 
 // tanh in the form the kernels use it: t = 1 - 2 r with r = 1 / (exp(2 x) + 1), and
-// 1 - t^2 = 4 (r - r^2).  r is good to 2e-7 of 1, which does for scores whose
-// weights are rounded to bf16.  fp32 calls take r from the odd series of t for
+// 1 - t^2 = 4 (r - r^2).  r is good to 2e-7 of 1, and capped scores to 2e-7 of the cap: for caps up to
+// kLargestRoughCap 2e-4, a twentieth of the rounding of their weights to bf16.  Larger caps
+// and fp32 calls (FINE) take t from its odd series for
 // small x, for a relative error of t of a few ulp (the first term left out is 4e-3 x^13).
 // No branches: a lane's choice between two short formulas costs less than leaving one out.
 // `exponent` is 2 x in units of log2.
 struct Bend {
   float t, r;
 };
-template <typename T>
+template <bool FINE>
 __device__ inline Bend bend_of(float exponent) {
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(exponent) + 1.0f);
   Bend b = {1.0f - 2.0f * r, r};
-  if (sizeof(T) == 4) {
+  if (FINE) {
     const float x = exponent * (0.5f * kLn2), y = x * x;
     const float series =
         x + x * y * (-0.333333333f + y * (0.133333333f + y * (-0.0539682540f + y * (0.0218694885f + y * -0.00886323552f))));
@@ -226,6 +229,11 @@ __device__ inline Bend bend_of(float exponent) {
   }
   return b;
 }
+
+// How scores are capped: not at all, or by which form of tanh.  96 structures of 480 atoms, 8
+// heads of 64, bf16, distances and mask, forward and gradients: 849 us rough, 999 fine.
+enum Cap { kNoCap, kRoughCap, kFineCap };
+constexpr float kLargestRoughCap = 1024.0f;
 
 // The largest d with bound(d) <= slot, bound rising, bound(0) <= slot: 64 probes a round.
 template <typename F>
@@ -442,17 +450,17 @@ struct Gradient {
 struct Score {
   float s, slant;
 };
-template <typename T, bool CAP>
+template <Cap CAP>
 __device__ inline Score score_of(const Problem& p, float product) {
-  if (CAP) {
-    const Bend b = bend_of<T>(product * p.to_bend);
+  if (CAP != kNoCap) {
+    const Bend b = bend_of<CAP == kFineCap>(product * p.to_bend);
     return {p.from_bend * b.t, b.r - b.r * b.r};
   }
   return {product * p.to_log2, 1.0f};
 }
-template <bool CAP>
+template <Cap CAP>
 __host__ __device__ constexpr float slant_scale() {
-  return CAP ? 4.0f : 1.0f;
+  return CAP != kNoCap ? 4.0f : 1.0f;
 }
 
 // Waves a SIMD that the register budget is set for: spills cost more than a wave gains.
@@ -614,6 +622,15 @@ int with_width(int dtype, int64_t D, F f) {
                    : D <= 64 ? f.template operator()<float, 64>() : f.template operator()<float, 128>();
   return D <= 32 ? f.template operator()<__bf16, 32>()
                  : D <= 64 ? f.template operator()<__bf16, 64>() : f.template operator()<__bf16, 128>();
+}
+
+// Calls f with the call's Cap as a type; fp32 calls are fine ones.
+template <typename T, typename F>
+int with_cap(const Problem& p, F f) {
+  if (p.cap <= 0.0f) return f(std::integral_constant<Cap, kNoCap>());
+  if constexpr (sizeof(T) == 2)
+    if (p.cap <= kLargestRoughCap) return f(std::integral_constant<Cap, kRoughCap>());
+  return f(std::integral_constant<Cap, kFineCap>());
 }
 
 // The gradient's two sides (attention_rows.hip, attention_keys.hip)

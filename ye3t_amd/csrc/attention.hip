@@ -18,7 +18,7 @@ namespace {
 // structures of 480, 8 heads of 64, distances, cap and mask: 0.20 ms, 240 TFLOP/s.  fp32: 40
 // structures of 1 000, 8 heads of 64, distances: 0.97 ms, 87 of 152 TFLOP/s.  One row against
 // 9 000 atoms in 24 structures: 0.10 ms for 437 MB.
-template <typename T, int DP, int NW, int KT, bool BIAS, bool CAP, bool SPLIT>
+template <typename T, int DP, int NW, int KT, bool BIAS, Cap CAP, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP, NW>)) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
                                                             float* __restrict__ part, float* __restrict__ part_stats) {
   constexpr int TILE = 32 * NW, NU = DP / (2 * kChunk<T>), ND = DP / 32;
@@ -75,9 +75,9 @@ __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP, NW>)) void attention
       s[n] = zeros();
       in_flight<NU>([&](int u) { return line_chunk<T, DP>(ktile, 32 * n + int(now_lane & 31), u, int(now_lane / 32)); },
                     [&](int u, const Op<T>& k) { mma(k, q[u], s[n]); });
-      if (CAP) {
+      if (CAP != kNoCap) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = p.from_bend * bend_of<T>(s[n][i] * p.to_bend).t;
+        for (int i = 0; i < 16; ++i) s[n][i] = p.from_bend * bend_of<CAP == kFineCap>(s[n][i] * p.to_bend).t;
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] *= p.to_log2;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64) void attention_slope_kernel(const float* __rest
   if (threadIdx.x == 0) slopes[h] = s;
 }
 
-template <typename T, int DP, int NW, bool BIAS, bool CAP>
+template <typename T, int DP, int NW, bool BIAS, Cap CAP>
 int launch_forward(const ForwardPlan& f, const Problem& p, void* out, float* log_sums, void* workspace, hipStream_t s) {
   constexpr int KT = NW > 1 && sizeof(T) == 2 ? 64 : 32;
   float* part = static_cast<float*>(workspace);
@@ -266,13 +266,14 @@ struct Forward {
   float* log_sums;
   void* workspace;
   hipStream_t s;
+  template <typename T, int DP, int NW, Cap CAP>
+  int capped() const {
+    return p.slopes ? launch_forward<T, DP, NW, true, CAP>(f, p, out, log_sums, workspace, s)
+                    : launch_forward<T, DP, NW, false, CAP>(f, p, out, log_sums, workspace, s);
+  }
   template <typename T, int DP, int NW>
   int waves() const {
-    if (p.cap > 0.0f)
-      return p.slopes ? launch_forward<T, DP, NW, true, true>(f, p, out, log_sums, workspace, s)
-                      : launch_forward<T, DP, NW, false, true>(f, p, out, log_sums, workspace, s);
-    return p.slopes ? launch_forward<T, DP, NW, true, false>(f, p, out, log_sums, workspace, s)
-                    : launch_forward<T, DP, NW, false, false>(f, p, out, log_sums, workspace, s);
+    return with_cap<T>(p, [&](auto cap) { return capped<T, DP, NW, decltype(cap)::value>(); });
   }
   template <typename T, int DP>
   int operator()() const {

@@ -15,7 +15,7 @@ namespace {
 // too few workgroups for that the row axis is taken in parts: 8 192 atoms, 16 heads
 // of 128 over 4, 1.93 -> 1.48 ms.  96 structures of 480 atoms with distances and
 // cap, 8 heads of 64: 0.32 ms, bound by about 20 vector operations a score.
-template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
+template <typename T, int DP, int NW, Cap CAP, bool BIAS, bool FORCES>
 __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attention_key_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, RT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
   constexpr int BUFFERS = NW == 1 ? 1 : 2;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
     for (int i = 0; i < 16; ++i) {
       const int line = 8 * (i / 4) + 4 * half + i % 4;
       const f32x2 st = stats[line];
-      const Score z = score_of<T, CAP>(p, s[i]);
+      const Score z = score_of<CAP>(p, s[i]);
       float exponent = z.s - st[0], dx = 0.0f, dy = 0.0f, dz = 0.0f, slope = 0.0f, per = 0.0f;
       if (BIAS) {
         const f32x4 r = place[line];
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void attention_key_join_kernel(const float* __
   }
 }
 
-template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
+template <typename T, int DP, int NW, Cap CAP, bool BIAS, bool FORCES>
 int launch_keys(const AdjointPlan& f, const Problem& p, const Gradient& g, hipStream_t s) {
   if (!fits_grid(f.key_items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many keys for one launch");
   hipLaunchKernelGGL((attention_key_gradient_kernel<T, DP, NW, CAP, BIAS, FORCES>),
@@ -224,7 +224,7 @@ struct Side {
   const Gradient& g;
   bool forces;
   hipStream_t s;
-  template <typename T, int DP, int NW, bool CAP>
+  template <typename T, int DP, int NW, Cap CAP>
   int capped() const {
     return forces ? launch_keys<T, DP, NW, CAP, true, true>(f, p, g, s)
                   : p.slopes ? launch_keys<T, DP, NW, CAP, true, false>(f, p, g, s)
@@ -232,7 +232,7 @@ struct Side {
   }
   template <typename T, int DP, int NW>
   int waves() const {
-    return p.cap > 0.0f ? capped<T, DP, NW, true>() : capped<T, DP, NW, false>();
+    return with_cap<T>(p, [&](auto cap) { return capped<T, DP, NW, decltype(cap)::value>(); });
   }
   template <typename T, int DP>
   int operator()() const {

@@ -23,7 +23,7 @@ namespace {
 // in bf16 the go lie in LDS so that two waves fit a SIMD: 8 192 atoms, 16 heads of
 // 128 over 4, 1.78 -> 1.25 ms.  96 structures of 480 atoms with distances and cap,
 // 8 heads of 64: 0.32 ms, bound by about 25 vector operations a score.
-template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
+template <typename T, int DP, int NW, Cap CAP, bool BIAS, bool FORCES>
 __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attention_row_gradient_kernel(Problem p, Gradient g) {
   constexpr int TILE = 32 * NW, KT = 32, NU = DP / (2 * kChunk<T>), ND = DP / 32;
   constexpr int BUFFERS = NW == 1 ? 1 : 2;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
     const bool masked = p.key_mask != nullptr || (tile + 1) * KT > key.length;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const Score z = score_of<T, CAP>(p, s[i]);
+      const Score z = score_of<CAP>(p, s[i]);
       float exponent = z.s - log_sum2, dx = 0.0f, dy = 0.0f, dz = 0.0f, distance = 0.0f, per = 0.0f;
       if (BIAS) {
         const f32x4 k = place[8 * (i / 4) + 4 * half + i % 4];
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(64 * NW, (kGradientWaves<T, DP, NW>)) void attentio
   }
 }
 
-template <typename T, int DP, int NW, bool CAP, bool BIAS, bool FORCES>
+template <typename T, int DP, int NW, Cap CAP, bool BIAS, bool FORCES>
 int launch_rows(const AdjointPlan& f, const Problem& p, const Gradient& g, hipStream_t s) {
   if (!fits_grid(f.row_items, 64 * NW)) return set_error(YE3T_EUNSUPPORTED, "too many rows for one launch");
   hipLaunchKernelGGL((attention_row_gradient_kernel<T, DP, NW, CAP, BIAS, FORCES>),
@@ -210,7 +210,7 @@ struct Side {
   const Gradient& g;
   bool forces;
   hipStream_t s;
-  template <typename T, int DP, int NW, bool CAP>
+  template <typename T, int DP, int NW, Cap CAP>
   int capped() const {
     return forces ? launch_rows<T, DP, NW, CAP, true, true>(f, p, g, s)
                   : p.slopes ? launch_rows<T, DP, NW, CAP, true, false>(f, p, g, s)
@@ -218,7 +218,7 @@ struct Side {
   }
   template <typename T, int DP, int NW>
   int waves() const {
-    return p.cap > 0.0f ? capped<T, DP, NW, true>() : capped<T, DP, NW, false>();
+    return with_cap<T>(p, [&](auto cap) { return capped<T, DP, NW, decltype(cap)::value>(); });
   }
   template <typename T, int DP>
   int operator()() const {
