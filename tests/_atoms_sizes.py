@@ -66,9 +66,9 @@ def attention(q, k, v, offsets, g, key_offsets=None, scale=None, cap=0.0, slopes
         for n, x, y in (("out", p @ vv, p @ vv.abs()),):
             for slot, t in zip(result[n], (x, y, y)):
                 slot[i] = heads_first(t)
-        for slot, t, m in zip(result["q"], (ds, scale * near, scale * wide), (kk, kk.abs(), kk.abs())):
+        for slot, t, m in zip(result["q"], (ds, abs(scale) * near, abs(scale) * wide), (kk, kk.abs(), kk.abs())):
             slot[i] = heads_first(t @ m)
-        for slot, t, m in zip(result["k"], (ds, scale * near, scale * wide), (a, a.abs(), a.abs())):
+        for slot, t, m in zip(result["k"], (ds, abs(scale) * near, abs(scale) * wide), (a, a.abs(), a.abs())):
             slot[j] = groups(t.mT @ m)
         for slot, m in zip(result["v"], (go, go.abs(), go.abs())):
             slot[j] = groups(p.mT @ m)

@@ -214,3 +214,26 @@ def test_caps_of_any_size(gpu, dtype, width, cap):
         exact = _atoms_sizes.attention(q, k, v, offsets, g, cap=cap, **kw)
         for n, e in exact.items():
             _atoms_sizes.check(n, got[n], e, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [1e-300, 1e-44, 1e-33, 1e35, 1e300])
+@pytest.mark.parametrize("scale", [0.25, -3.0])
+def test_caps_outside_of_fp32(gpu, dtype, cap, scale):
+    """Caps too small for fp32 leave equal scores, caps too large the scores as they are."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"attention capped at {cap}, scale {scale}, {dtype}")
+    q, k, v, offsets, kw = problem([70, 9], 2, 1, 32, dtype, gpu)
+    q[3] = 0.0  # scores of zero
+    out, sums = runtime.atom_attention(q, k, v, offsets, scale=scale, cap=cap, return_log_sums=True)
+    exact = _atoms_sizes.attention(q, k, v, offsets, q, scale=scale, cap=cap)
+    _atoms_sizes.check("out", out, exact["out"], dtype)
+    grads = runtime.atom_attention_adjoint(q, out, sums, q, k, v, offsets, scale=scale, cap=cap)
+    _atoms_sizes.check("v", grads[2], exact["v"], dtype)
+    if cap > 1:
+        _atoms_sizes.check("q", grads[0], exact["q"], dtype)
+        _atoms_sizes.check("k", grads[1], exact["k"], dtype)
+    assert bool(torch.isfinite(grads[0]).all()) and bool(torch.isfinite(grads[1]).all())

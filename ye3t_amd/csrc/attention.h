@@ -574,10 +574,14 @@ inline Problem problem_of(const ye3t_attention_args& a) {
   p.offsets = a.offsets;
   p.key_offsets = a.key_offsets ? a.key_offsets : a.offsets;
   p.scale = float(a.scale);
-  p.cap = float(a.cap);
   p.to_log2 = float(a.scale * kLog2eExact);
-  p.to_bend = a.cap > 0.0 ? float(2.0 * kLog2eExact * a.scale / a.cap) : 0.0f;
-  p.from_bend = float(a.cap * kLog2eExact);
+  if (a.cap > 0.0) {
+    // Held to what fp32 has room for: scores below 1e-30 are equal, and 1e30 caps none below 3e26.
+    const double cap = a.cap < 1e-30 ? 1e-30 : a.cap > 1e30 ? 1e30 : a.cap, to_bend = 2.0 * kLog2eExact * a.scale / cap;
+    p.cap = float(cap);
+    p.to_bend = to_bend > 1e38 ? 1e38f : to_bend < -1e38 ? -1e38f : float(to_bend);
+    p.from_bend = float(cap * kLog2eExact);
+  }
   p.slopes = a.slopes;
   p.positions = a.positions;
   p.key_positions = a.key_positions;
