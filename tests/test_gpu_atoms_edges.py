@@ -237,3 +237,28 @@ def test_caps_outside_of_fp32(gpu, dtype, cap, scale):
         _atoms_sizes.check("q", grads[0], exact["q"], dtype)
         _atoms_sizes.check("k", grads[1], exact["k"], dtype)
     assert bool(torch.isfinite(grads[0]).all()) and bool(torch.isfinite(grads[1]).all())
+
+
+# ---- norm ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [5, 300, 9000])
+@pytest.mark.parametrize("epsilon", [1e-300, 1e-50, 1e-40])
+def test_norm_with_an_epsilon_below_fp32(gpu, dtype, width, epsilon):
+    """Rows of zeros give zeros for any positive epsilon, other rows what they give without it."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"norm of rows of zeros with epsilon {epsilon}, width {width}, {dtype}")
+    x, w = normal((4, width), dtype, 1, gpu), normal((width,), dtype, 2, gpu)
+    x[1] = 0.0
+    y = runtime.rms_norm(x, w, epsilon=epsilon)
+    assert not y[1].any() and bool(y.isfinite().all())
+    near = runtime.rms_norm(x, w, epsilon=1e-20)
+    assert torch.equal(y, near)
+    codes, scales = runtime.rms_norm_8bit(x, w, epsilon=epsilon)
+    assert not codes[1].float().any() and not scales[1].any() and bool(codes.float().isfinite().all())
+    dx, dw = runtime.rms_norm_adjoint(x, x, w, epsilon=epsilon)
+    assert bool(dx.isfinite().all()) and bool(dw.isfinite().all()) and not dx[1].any()
+    assert torch.equal(dw, runtime.rms_norm_adjoint(x, x, w, epsilon=1e-20)[1])

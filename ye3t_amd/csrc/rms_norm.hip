@@ -417,6 +417,9 @@ int check_norm(int dtype, int64_t rows, int64_t width, double epsilon) {
   return YE3T_OK;
 }
 
+// fp32's smallest normal value at least: rows of zeros divide by its root.
+inline float held_epsilon(double epsilon) { return epsilon < 1.17549435e-38 ? 1.17549435e-38f : float(epsilon); }
+
 inline Shape adjoint_shape(int dtype, int64_t rows, int64_t width) {
   return shape_of(rows, int(width), dtype == YE3T_F32 ? kChunk<float> : kChunk<__bf16>, 4, 1);
 }
@@ -436,7 +439,7 @@ int ye3t_hip_rms_norm(int dtype, const void* x, const void* residual, const void
   YE3T_REQUIRE(x && weight && y, "the norm needs rows, a weight and an output");
   YE3T_REQUIRE(!residual || total, "a residual needs an output for the sum");
   const int W = int(width);
-  const float eps = float(epsilon);
+  const float eps = held_epsilon(epsilon);
   void* none = nullptr;
   if (dtype == YE3T_F32)
     return forward_shaped<float, kPlain>(shape_of(rows, W, kChunk<float>, 8, 1), x, residual, weight, rows, W, eps, total, y,
@@ -454,7 +457,7 @@ int ye3t_hip_rms_norm_8bit(int dtype, const void* x, const void* residual, const
   YE3T_REQUIRE(x && weight && codes && scales, "the norm needs rows, a weight, codes and scales");
   YE3T_REQUIRE(!residual || total, "a residual needs an output for the sum");
   const int W = int(width);
-  const float eps = float(epsilon);
+  const float eps = held_epsilon(epsilon);
   void* none = nullptr;
   // a scale's 128 columns lie in one wave: 32 lanes in fp32
   if (dtype == YE3T_F32)
@@ -481,7 +484,7 @@ int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_
                "the workspace is smaller than ye3t_hip_rms_norm_adjoint_workspace_bytes");
   const Shape sh = adjoint_shape(dtype, rows, width);
   const int W = int(width);
-  const float eps = float(epsilon);
+  const float eps = held_epsilon(epsilon);
   if (dtype == YE3T_F32)
     return adjoint_shaped<float>(sh, adjoint, total_adjoint, total, weight, rows, W, eps, x_adjoint, weight_adjoint,
                                  workspace, as_stream(stream));
