@@ -22,6 +22,16 @@ def _tracked(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _require_one_device(name, first, *rest):
+    """A call's kernels run on the device of its first tensor, and read no other one's memory."""
+    _require_device(first, name)
+    for t in rest:
+        if t is not None:
+            _require_device(t, name)
+            if t.device != first.device:
+                raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+
+
 def _unit_rows(t):
     """``t``, or a contiguous copy where the last axis is not laid out value after value."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -72,8 +82,7 @@ def embedding(tokens, table, *, scale=1.0, validate=True):
     range-checks the tokens first (one kernel and one wait); a caller that has
     checked them before may skip it.  A token outside the table that is not
     checked gives a row of zeros and no gradient."""
-    _require_device(table, "embedding")
-    _require_device(tokens, "embedding")
+    _require_one_device("embedding", table, tokens)
     if table.ndim != 2:
         raise ValueError("table must be [rows, width]")
     tokens = _tokens(tokens, int(table.shape[0]), validate, "embedding")
@@ -90,8 +99,7 @@ def embedding_adjoint(adjoint, tokens, rows, *, scale=1.0, validate=True):
     The positions are sorted by token and summed in equal shares in a fixed
     order in float32 (float64 for float64): equal calls give equal bits, and a
     token that most rows share costs no more than any other."""
-    _require_device(adjoint, "embedding_adjoint")
-    _require_device(tokens, "embedding_adjoint")
+    _require_one_device("embedding_adjoint", adjoint, tokens)
     rows = int(rows)
     if rows < 0:
         raise ValueError("rows must be non-negative")
@@ -104,14 +112,12 @@ def embedding_adjoint(adjoint, tokens, rows, *, scale=1.0, validate=True):
 # ---- norm ----------------------------------------------------------------------
 
 def _norm_rows(input, weight, residual, name):
-    _require_device(input, name)
-    _require_device(weight, name)
+    _require_one_device(name, input, weight, residual)
     if input.ndim < 1 or weight.ndim != 1 or int(weight.shape[0]) != int(input.shape[-1]):
         raise ValueError("weight must be [width] with input [..., width]")
     if weight.dtype != input.dtype:
         raise ValueError(f"weight must have dtype {input.dtype}")
     if residual is not None:
-        _require_device(residual, name)
         if residual.shape != input.shape or residual.dtype != input.dtype:
             raise ValueError("residual must have the input's shape and dtype")
 
@@ -206,9 +212,7 @@ def _validate_offsets(pairs):
 def _attention_problem(query, key, value, offsets, key_offsets, scale, cap, slopes, positions, key_positions,
                        key_mask, validate, name):
     """The checked arguments as ``native.Attention``."""
-    for t in (query, key, value, offsets, key_offsets, slopes, positions, key_positions, key_mask):
-        if t is not None:
-            _require_device(t, name)
+    _require_one_device(name, query, key, value, offsets, key_offsets, slopes, positions, key_positions, key_mask)
     if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape or query.shape[2] != key.shape[2]:
         raise ValueError("query must be [atoms, heads, width], key and value [atoms, key_heads, width]")
     if query.dtype not in (torch.float32, torch.bfloat16):
@@ -326,11 +330,10 @@ def atom_attention_adjoint(adjoint, out, log_sums, query, key, value, offsets, *
     positions holds both of an atom's parts and the last is None."""
     problem = _attention_problem(query, key, value, offsets, key_offsets, scale, cap, slopes, positions,
                                  key_positions, key_mask, validate, "atom_attention_adjoint")
+    _require_one_device("atom_attention_adjoint", query, adjoint, out, log_sums)
     for t, n in ((adjoint, "adjoint"), (out, "out")):
-        _require_device(t, "atom_attention_adjoint")
         if t.shape != query.shape or t.dtype != query.dtype:
             raise ValueError(f"{n} must have the query's shape and dtype")
-    _require_device(log_sums, "atom_attention_adjoint")
     if log_sums.dtype != torch.float32 or tuple(log_sums.shape) != tuple(query.shape[:2]):
         raise ValueError("log_sums must be float32 [atoms, heads]")
     if bias_gradients and slopes is None:
