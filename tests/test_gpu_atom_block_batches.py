@@ -28,3 +28,33 @@ def test_features_of_the_last_structure_of_a_batch(gpu, count, centre):
         worst = float(((held[part] - alone).double().abs() / size).max())
         flush(f"  structure {s}: {worst:.2e}")
         assert worst < 2e-5
+
+
+def test_what_hidden_atoms_hold_reaches_nothing(gpu):
+    """Energies, forces and parameter gradients with NaN in the features and positions of hidden atoms."""
+    import math
+
+    import torch
+
+    from ye3t_amd.ace.atom_block import AtomBlock
+
+    flush("the layer with hidden atoms that hold no numbers")
+    torch.manual_seed(3)
+    block = AtomBlock(40, 3, width=64, heads=4, cap=8.0).to(gpu)
+    features, positions = torch.randn(30, 40, device=gpu), torch.randn(30, 3, device=gpu) * 3.0
+    species = torch.randint(3, (30,), device=gpu)
+    offsets = torch.tensor([0, 12, 12, 20, 30], device=gpu)
+    mask = torch.ones(30, dtype=torch.bool, device=gpu)
+    mask[[2, 5, *range(12, 20)]] = False  # two atoms, and a whole structure
+
+    def everything(value):
+        x, r = features.clone(), positions.clone()
+        x[~mask], r[~mask] = value, value
+        x.requires_grad_(), r.requires_grad_()
+        energies = block(x, species, r, offsets, key_mask=mask)
+        return [energies, *torch.autograd.grad(energies.square().sum(), [x, r, *block.parameters()])]
+
+    want = everything(0.5)
+    assert float(want[0][1]) == 0.0 and float(want[0][2]) == 0.0
+    for value in (math.nan, math.inf):
+        assert all(torch.equal(a, b) for a, b in zip(everything(value), want))

@@ -101,8 +101,12 @@ class AtomBlock(torch.nn.Module):
 
     def forward(self, features, species, positions, offsets, key_mask=None):
         """``[structures]`` energies of ``features [N, F]``, ``species [N]``, ``positions [N, 3]``
-        (float32) and row offsets ``[structures + 1]``; ``key_mask [N]`` hides ghost atoms."""
+        (float32) and row offsets ``[structures + 1]``; ``key_mask [N]`` hides ghost atoms: what their
+        features and positions hold reaches nothing."""
         atoms = int(features.shape[0])
+        if key_mask is not None:
+            # their rows are computed with the others', and zero times what is not a number is none either
+            features, positions = (t.masked_fill(~key_mask[:, None], 0.0) for t in (features, positions))
         mixed = runtime.rms_norm(features, self.feature_norm) @ self.mix
         vectors = runtime.embedding(species, self.species, scale=math.sqrt(self.width))
         y, x = runtime.rms_norm(mixed, self.attend_norm, residual=vectors)
@@ -112,7 +116,7 @@ class AtomBlock(torch.nn.Module):
         y, x = runtime.rms_norm(seen.reshape(atoms, self.width) @ self.join, self.out_norm, residual=x)
         each = (y @ self.readout).float()
         if key_mask is not None:
-            each = each * key_mask
+            each = each.masked_fill(~key_mask, 0.0)
         return torch.segment_reduce(each, "sum", offsets=offsets, axis=0, initial=0)
 
     def descriptors(self, features):
