@@ -262,3 +262,14 @@ def test_norm_with_an_epsilon_below_fp32(gpu, dtype, width, epsilon):
     dx, dw = runtime.rms_norm_adjoint(x, x, w, epsilon=epsilon)
     assert bool(dx.isfinite().all()) and bool(dw.isfinite().all()) and not dx[1].any()
     assert torch.equal(dw, runtime.rms_norm_adjoint(x, x, w, epsilon=1e-20)[1])
+
+
+def test_last_kernel_of_the_norm_in_8_bits(gpu):
+    import torch
+
+    from ye3t_amd import runtime
+    from ye3t_amd.runtime import native
+
+    flush("the kernel that the norm in 8 bits reports")
+    runtime.rms_norm_8bit(torch.ones(3, 8, device=gpu), torch.ones(8, device=gpu))
+    assert native.last_kernel() == "rms_norm_kernel"

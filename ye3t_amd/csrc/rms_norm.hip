@@ -357,7 +357,7 @@ int forward_as(const void* x, const void* r, const void* w, int64_t rows, int W,
   hipLaunchKernelGGL((rms_norm_kernel<T, L, K, MODE>), grid, dim3(kThreads), 0, s, static_cast<const T*>(x),
                      static_cast<const T*>(r), static_cast<const T*>(w), rows, W, eps, static_cast<T*>(total),
                      static_cast<T*>(y), static_cast<uint8_t*>(codes), static_cast<float*>(scales));
-  return check_launch(MODE == kEightBit ? "rms_norm_8bit_kernel" : "rms_norm_kernel");
+  return check_launch("rms_norm_kernel");
 }
 
 template <typename T, int MODE, typename... A>
