@@ -273,3 +273,18 @@ def test_last_kernel_of_the_norm_in_8_bits(gpu):
     flush("the kernel that the norm in 8 bits reports")
     runtime.rms_norm_8bit(torch.ones(3, 8, device=gpu), torch.ones(8, device=gpu))
     assert native.last_kernel() == "rms_norm_kernel"
+
+
+def test_refusals_of_the_norms_gradient_name_their_argument(gpu):
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush("what the norm's gradient refuses")
+    x, w = torch.ones(3, 8, device=gpu), torch.ones(8, device=gpu)
+    with pytest.raises(ValueError, match="^adjoint must"):
+        runtime.rms_norm_adjoint(x[:2], x, w)
+    with pytest.raises(ValueError, match="^total_adjoint must"):
+        runtime.rms_norm_adjoint(x, x, w, total_adjoint=x.bfloat16())
+    with pytest.raises(ValueError, match="^residual must"):
+        runtime.rms_norm(x, w, residual=x[:2])

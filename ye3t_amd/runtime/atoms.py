@@ -111,15 +111,16 @@ def embedding_adjoint(adjoint, tokens, rows, *, scale=1.0, validate=True):
 
 # ---- norm ----------------------------------------------------------------------
 
-def _norm_rows(input, weight, residual, name):
-    _require_one_device(name, input, weight, residual)
+def _norm_rows(input, weight, name, **rows):
+    """Checks ``input`` and ``weight``, and that the others (by their arguments' names) are like ``input``."""
+    _require_one_device(name, input, weight, *rows.values())
     if input.ndim < 1 or weight.ndim != 1 or int(weight.shape[0]) != int(input.shape[-1]):
         raise ValueError("weight must be [width] with input [..., width]")
     if weight.dtype != input.dtype:
         raise ValueError(f"weight must have dtype {input.dtype}")
-    if residual is not None:
-        if residual.shape != input.shape or residual.dtype != input.dtype:
-            raise ValueError("residual must have the input's shape and dtype")
+    for n, t in rows.items():
+        if t is not None and (t.shape != input.shape or t.dtype != input.dtype):
+            raise ValueError(f"{n} must have the input's shape and dtype")
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -151,7 +152,7 @@ def rms_norm(input, weight, *, residual=None, epsilon=1e-6):
     float32 or bfloat16; the mean and ``y`` come from the unrounded sum in
     float32, ``y`` and ``h`` are rounded once each.  Differentiable
     (:func:`rms_norm_adjoint`); the gradient is taken at the rounded ``h``."""
-    _norm_rows(input, weight, residual, "rms_norm")
+    _norm_rows(input, weight, "rms_norm", residual=residual)
     epsilon = float(epsilon)
     input = input.contiguous()
     residual = None if residual is None else residual.contiguous()
@@ -166,8 +167,7 @@ def rms_norm_adjoint(adjoint, total, weight, *, total_adjoint=None, epsilon=1e-6
     there was no residual) for the output's ``adjoint`` and the sum's
     ``total_adjoint``: ``(input_adjoint, weight_adjoint)``; the residual's is
     the input's.  The weight's sum over rows is float32 in a fixed order."""
-    _norm_rows(total, weight, adjoint, "rms_norm_adjoint")
-    _norm_rows(total, weight, total_adjoint, "rms_norm_adjoint")
+    _norm_rows(total, weight, "rms_norm_adjoint", adjoint=adjoint, total_adjoint=total_adjoint)
     return native.rms_norm_adjoint(adjoint.contiguous(), total.contiguous(), weight.contiguous(),
                                    None if total_adjoint is None else total_adjoint.contiguous(), float(epsilon))
 
@@ -181,7 +181,7 @@ def rms_norm_8bit(input, weight, *, residual=None, epsilon=1e-6):
     [..., ceil(width / 128)]`` is float32, one for each 128 columns (the
     largest value over 448, 0 for columns of zeros), so that ``y`` is about
     ``codes * scales``.  Not differentiable."""
-    _norm_rows(input, weight, residual, "rms_norm_8bit")
+    _norm_rows(input, weight, "rms_norm_8bit", residual=residual)
     if _tracked(input, weight, residual):
         raise NotImplementedError("rms_norm_8bit: no gradient (use rms_norm)")
     codes, scales, total = native.rms_norm_8bit(input.contiguous(), weight.contiguous(),
