@@ -288,3 +288,119 @@ def test_refusals_of_the_norms_gradient_name_their_argument(gpu):
         runtime.rms_norm_adjoint(x, x, w, total_adjoint=x.bfloat16())
     with pytest.raises(ValueError, match="^residual must"):
         runtime.rms_norm(x, w, residual=x[:2])
+
+
+# ---- every gradient variant, element by element --------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [[1, 12, 20], [70, 33, 150], [600]], ids=str)
+@pytest.mark.parametrize("heads,key_heads,width", [(2, 2, 16), (4, 2, 64), (3, 1, 100), (4, 2, 128)])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("mask", [False, True])
+def test_gradients_with_distances_and_without_forces(gpu, dtype, lengths, heads, key_heads, width, cap, mask):
+    """Distances that no gradient is wanted of; 600 atoms also take the key side's row axis in parts."""
+    import torch
+
+    flush(f"gradients of {lengths} with distances, {heads}/{key_heads} x {width}, cap {cap}, mask {mask}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, heads, key_heads, width, dtype, gpu, bias=True, mask=mask)
+    got, g = run(q, k, v, offsets, kw, cap, False)
+    assert set(got) == {"out", "sums", "q", "k", "v"}
+    exact = _atoms_sizes.attention(q, k, v, offsets, g, cap=cap, **kw)
+    for n in ("out", "q", "k", "v"):
+        _atoms_sizes.check(n, got[n], exact[n], dtype)
+    again, _ = run(q, k, v, offsets, kw, cap, False)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_autograd_with_distances_and_without_forces(gpu, dtype):
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"autograd in query, key and value beside distances, {dtype}")
+    q, k, v, offsets, kw = problem([30, 90], 4, 2, 40, dtype, gpu, bias=True)
+    got, g = run(q, k, v, offsets, kw, 5.0, False)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = runtime.atom_attention(*leaves, offsets, cap=5.0, **kw)
+    for n, t in zip("qkv", torch.autograd.grad(out, leaves, g)):
+        assert torch.equal(t, got[n])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,keys", [([1, 1, 0, 2], [900, 0, 7, 3000]), ([1], [5000]), ([3], [1]), ([150], [40]), ([400], [33])],
+                         ids=str)
+@pytest.mark.parametrize("heads,key_heads,width", [(8, 8, 32), (4, 1, 64), (16, 4, 128)])
+@pytest.mark.parametrize("forces", [False, True])
+def test_gradients_to_other_atoms_by_element(gpu, dtype, lengths, keys, heads, key_heads, width, forces):
+    """Few rows give each of many keys little: the last tile's keys are held to their own size."""
+    flush(f"gradients of {lengths} to {keys}, {heads}/{key_heads} x {width}, forces {forces}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, heads, key_heads, width, dtype, gpu, key_lengths=keys, bias=True)
+    got, g = run(q, k, v, offsets, kw, 0.0, forces)
+    exact = _atoms_sizes.attention(q, k, v, offsets, g, **kw)
+    for n, e in exact.items():
+        if n in got:
+            _atoms_sizes.check(n, got[n], e, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [[1, 12, 20], [70, 33, 150], [700]], ids=str)
+@pytest.mark.parametrize("heads,key_heads,width", [(1, 1, 8), (6, 3, 80), (4, 1, 128)])
+@pytest.mark.parametrize("mask", [False, True])
+def test_gradients_without_distances_by_element(gpu, dtype, lengths, heads, key_heads, width, mask):
+    flush(f"gradients of {lengths}, {heads}/{key_heads} x {width}, mask {mask}, {dtype}")
+    q, k, v, offsets, kw = problem(lengths, heads, key_heads, width, dtype, gpu, mask=mask)
+    got, g = run(q, k, v, offsets, kw)
+    exact = _atoms_sizes.attention(q, k, v, offsets, g, **kw)
+    for n, e in exact.items():
+        _atoms_sizes.check(n, got[n], e, dtype)
+
+
+# ---- embedding gradients of many tokens ------------------------------------------------
+
+@pytest.mark.parametrize("count,rows,width", [(70001, 8, 128), (70001, 40000, 128), (300001, 300, 16), (600007, 8, 4),
+                                              (600007, 100003, 5), (9001, 3, 1030), (5000, 1 << 17, 3), (5000, (1 << 24) + 5, 1),
+                                              (3000, (1 << 24) + 5, 1)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float64"])
+def test_embedding_gradients_of_many_tokens(gpu, dtype, count, rows, width):
+    """Shares of more than 16 positions, sort runs of more than 2 048, all four sort passes: each element within its
+    terms' size (fp32: sums of up to 600 007 terms in shares, below 1e-4 of it; fp64 1e-12; bf16 one rounding more)."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"embedding gradient of {count} tokens by {rows} x {width}, {dtype}")
+    g = torch.Generator().manual_seed(count)
+    tokens = (torch.exp(torch.rand(count, generator=g, dtype=torch.float64) * math.log(rows + 1.0)) - 1.0).long().clamp_(0, rows - 1)
+    tokens[::7] = rows - 1
+    adjoint = normal((count, width), dtype, 2, gpu)
+    exact, size = (torch.zeros((rows, width), dtype=torch.float64).index_add_(0, tokens, t)
+                   for t in (adjoint.double().cpu(), adjoint.double().cpu().abs()))
+    allowed = size * {"float32": 1e-4, "float64": 1e-12, "bfloat16": 1e-4}[dtype] + exact.abs() * (2.0 ** -8 if dtype == "bfloat16" else 0)
+    for index in (torch.int32, torch.int64):
+        got = runtime.embedding_adjoint(adjoint, tokens.to(index).to(gpu), rows)
+        assert bool(((got.double().cpu() - exact).abs() <= allowed).all())
+    assert torch.equal(got, runtime.embedding_adjoint(adjoint, tokens.to(gpu), rows))
+
+
+def test_embedding_gradients_past_32_bits(gpu):
+    """Adjoints and tables of more than 2^31 values: the last rows are the last ones."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush("embedding gradients of more than 2^31 values")
+    rows, width = 4_200_003, 512
+    tail = normal((3, width), "bfloat16", 1, gpu)
+    adjoint = torch.zeros((rows, width), dtype=torch.bfloat16, device=gpu)
+    adjoint[-3:] = tail
+    tokens = torch.zeros(rows, dtype=torch.int32, device=gpu)
+    tokens[-3:] = torch.tensor([5, 6, 5], device=gpu)
+    grad = runtime.embedding_adjoint(adjoint, tokens, 7)
+    assert torch.equal(grad[6], tail[1]) and not grad[:5].any()
+    assert torch.equal(grad[5], (tail[0].float() + tail[2].float()).bfloat16())
+    del adjoint
+    flush("  tables of more than 2^31 values")
+    tokens = torch.tensor([rows - 1, 0, rows - 3], device=gpu)
+    grad = runtime.embedding_adjoint(tail, tokens, rows)
+    assert torch.equal(grad[tokens], tail) and int((grad != 0).any(1).sum()) == 3
