@@ -58,3 +58,25 @@ def test_what_hidden_atoms_hold_reaches_nothing(gpu):
     assert float(want[0][1]) == 0.0 and float(want[0][2]) == 0.0
     for value in (math.nan, math.inf):
         assert all(torch.equal(a, b) for a, b in zip(everything(value), want))
+
+
+def test_batches_without_atoms_and_atoms_without_neighbours(gpu):
+    """Energies and forces of nothing, of lone atoms, and of a batch with empty structures."""
+    import torch
+
+    from ye3t_amd.ace.atom_block import AceFeatures, AtomBlock, energies_and_forces
+
+    flush("energies and forces without atoms, and of lone atoms")
+    torch.manual_seed(3)
+    features = AceFeatures(3, device=gpu)
+    block = AtomBlock(features.width, 3, width=64, heads=4).to(gpu)
+    for ends, positions in (([0], []), ([0, 0, 0], []), ([0, 1], [[1.0, 2.0, 3.0]]),
+                            ([0, 0, 1, 1, 3, 3], [[0.0, 0.0, 0.0], [0.0, 0.0, 0.0], [0.0, 0.0, 30.0]])):
+        positions = torch.tensor(positions, device=gpu).reshape(-1, 3)
+        species = torch.zeros(len(positions), dtype=torch.int32, device=gpu)
+        energies, forces = energies_and_forces(features, block, positions, species, torch.tensor(ends, device=gpu))
+        assert energies.shape == (len(ends) - 1,) and forces.shape == positions.shape
+        assert bool(energies.isfinite().all()) and bool(forces.isfinite().all())
+        for s in range(len(ends) - 1):
+            if ends[s] == ends[s + 1]:
+                assert float(energies[s]) == 0.0

@@ -60,6 +60,8 @@ class AceFeatures:
 
     def __call__(self, positions, species, offsets):
         atoms = int(positions.shape[0])
+        if atoms == 0:
+            return torch.zeros((0, self.width), device=positions.device)
         owner = torch.searchsorted(offsets, torch.arange(atoms, device=offsets.device), right=True) - 1
         with torch.no_grad():
             # Structures side by side along x, further apart than the cutoff, make one neighbour list.
@@ -69,7 +71,7 @@ class AceFeatures:
             corner = torch.full((offsets.numel() - 1, 3), math.inf, dtype=torch.float64, device=positions.device)
             corner.scatter_reduce_(0, owner[:, None].expand(-1, 3), apart, "amin")
             apart = apart - corner[owner]
-            reach = float(apart[:, 0].max()) + 2.0 * CUTOFF if atoms else 0.0
+            reach = float(apart[:, 0].max()) + 2.0 * CUTOFF
             apart[:, 0] += owner * reach
             pairs = runtime.neighbor_list(apart, CUTOFF)
             rows, centres, neighbours = pairs["target_offsets"], pairs["edge_targets"], pairs["edge_sources"]
