@@ -850,7 +850,8 @@ int ye3t_hip_embedding_adjoint(int dtype, const void* adjoint, const void* token
 /* total = x + residual; y = total * weight / sqrt(mean(total^2) + epsilon) over
  * each of `rows` rows of `width` values.  The mean and y come from the unrounded
  * sum in fp32.  `residual` may be NULL (then `total` may be too).  dtype F32 or
- * BF16 for all arrays. */
+ * BF16 for all arrays.  An epsilon below fp32's smallest normal value counts as
+ * that one, here and in the gradient. */
 int ye3t_hip_rms_norm(int dtype, const void* x, const void* residual, const void* weight, int64_t rows, int64_t width,
                       double epsilon, void* total, void* y, ye3t_stream_t stream);
 
@@ -883,7 +884,9 @@ int ye3t_hip_rms_norm_adjoint(int dtype, const void* adjoint, const void* total_
  * other (under a slope of 0 such a distance is not a number).  key_mask (NULL:
  * all) is 0 for keys that no row sees; what they hold is not used.  A row that
  * sees no key gives zeros.  Strides are in values, those of the last axis 1.
- * Arrays without values (positions of no query atoms, say) may be NULL. */
+ * Arrays without values (positions of no query atoms, say) may be NULL.
+ * queries * heads and keys * heads are at most 2^31 - 256; a cap is held to
+ * 1e-30 .. 1e30. */
 typedef struct {
   int dtype;           /* YE3T_F32 or YE3T_BF16: query, key, value, outputs and their adjoints */
   int64_t queries;     /* query atoms */

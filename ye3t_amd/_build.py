@@ -16,8 +16,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libye3t_hip.so")
 SOURCES = ("api.hip", "attention.hip", "attention_keys.hip", "attention_rows.hip", "density.hip", "density_grad.hip",
-           "density_grad_mfma.hip", "density_mfma.hip", "density_mfma64.hip", "density_species.hip", "embedding.hip", "factorized.hip", "monomial.hip", "neighbors.hip", "product.hip",
-           "rms_norm.hip")
+           "density_grad_mfma.hip", "density_mfma.hip", "density_mfma64.hip", "density_species.hip", "embedding.hip",
+           "factorized.hip", "monomial.hip", "neighbors.hip", "product.hip", "rms_norm.hip")
 ARCH = os.environ.get("YE3T_HIP_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

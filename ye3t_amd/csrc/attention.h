@@ -22,8 +22,8 @@
 // chosen to fit them.
 //
 // Scores, the running maximum and sum, and every sum over keys or rows are
-// fp32.  bf16 calls round p and ds to bf16 for the matrix instruction (relative
-// 2^-9 each, as the inputs have) and each output once.
+// fp32.  bf16 calls round p and ds to bf16 for the matrix instruction (at most
+// 2^-8 relative each, as the inputs are) and each output once.
 #pragma once
 
 #include <type_traits>
@@ -209,9 +209,9 @@ constexpr bool kKeepLines = sizeof(T) == 2 && DP == 128 && NW == 4;
 
 // tanh in the form the kernels use it: t = 1 - 2 r with r = 1 / (exp(2 x) + 1), and
 // 1 - t^2 = 4 (r - r^2).  r is good to 2e-7 of 1, and capped scores to 2e-7 of the cap: for caps up to
-// kLargestRoughCap 2e-4, a twentieth of the rounding of their weights to bf16.  Larger caps
-// and fp32 calls (FINE) take t from its odd series for
-// small x, for a relative error of t of a few ulp (the first term left out is 4e-3 x^13).
+// kLargestRoughCap 2e-4, a twentieth of the rounding of their weights to bf16.  Larger
+// caps and fp32 calls (FINE) take t from its odd series for small x, for a relative error
+// of t of a few ulp (the first term left out is 4e-3 x^13).
 // No branches: a lane's choice between two short formulas costs less than leaving one out.
 // `exponent` is 2 x in units of log2.
 struct Bend {

@@ -14,10 +14,11 @@ namespace {
 //
 // Bound by what a score costs beside the products: about 17 vector operations with
 // distance and cap, four of them of quarter rate, 5 without.  8 192 atoms, 16
-// heads of 128 over 4, bf16: 0.68 ms, 810 TFLOP/s (1 136 for a large product here); 96
-// structures of 480, 8 heads of 64, distances, cap and mask: 0.20 ms, 240 TFLOP/s.  fp32: 40
-// structures of 1 000, 8 heads of 64, distances: 0.97 ms, 87 of 152 TFLOP/s.  One row against
-// 9 000 atoms in 24 structures: 0.10 ms for 437 MB.
+// heads of 128 over 4, bf16: 0.68 ms, 810 TFLOP/s (1 136 for a large product here), the
+// matrix units busy for 34 % of the time and the vector units for 58 %; 96 structures of
+// 480, 8 heads of 64, distances, cap and mask: 0.21 ms, 232 TFLOP/s.  fp32: 40 structures
+// of 1 000, 8 heads of 64, distances: 0.98 ms, 87 of 152 TFLOP/s (matrix units 57 %, vector
+// units 25 %).  One row against 9 000 atoms in 24 structures: 0.10 ms for 437 MB.
 template <typename T, int DP, int NW, int KT, bool BIAS, Cap CAP, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (kForwardWaves<T, DP, NW>)) void attention_kernel(Problem p, T* __restrict__ out, float* __restrict__ log_sums,
                                                             float* __restrict__ part, float* __restrict__ part_stats) {

@@ -6,7 +6,8 @@ Atoms are packed one structure after the other, with the row offsets of the
 density's CSR (int64, from 0 to the atom count) for the structures.  Storage is
 float32 or bfloat16 (the embedding also float64, for double-precision
 densities); means, softmax statistics and sums are held in 32 bits or more.
-The forward operators are differentiable once; each has its adjoint as a
+bfloat16 attention rounds the softmax weights, and in the gradient the
+gradients of the scores, to bfloat16 for the matrix instructions.  The forward operators are differentiable once; each has its adjoint as a
 function of its own.  No reference counterparts.
 """
 
@@ -267,7 +268,7 @@ def _attention_problem(query, key, value, offsets, key_offsets, scale, cap, slop
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, slopes, positions, key_positions, problem):
-        # the problem holds detached views of these, with contiguous copies where they were needed
+        # the problem holds these themselves, or contiguous copies where they were needed
         out, sums = problem.forward(True)
         ctx.save_for_backward(out, sums, *problem.tensors())
         ctx.problem = problem.rest()
@@ -297,12 +298,14 @@ def atom_attention(query, key, value, offsets, *, key_offsets=None, scale=None, 
       offsets of their own over the same structures (a few moved atoms against
       whole structures, for instance).
     * ``scale``: of the scores, ``D ** -0.5`` by default.
-    * ``cap``: scores become ``cap * tanh(score / cap)``.
+    * ``cap``: scores become ``cap * tanh(score / cap)``; 0: they stay as they are.
     * ``slopes [H]`` and ``positions [N, 3]`` (float32; ``key_positions [M, 3]``
       with ``key_offsets``): scores are lowered by ``slopes[h]`` times the
-      distance of the two atoms, after the cap.
+      distance of the two atoms, after the cap.  Atoms more than 1.8e19 apart do
+      not see each other; atoms less than 1.1e-19 apart have no direction.
     * ``key_mask`` bool ``[M]``: False for atoms that no row sees (ghosts,
-      padding); what they hold is not used.  A row that sees nothing gives zeros.
+      padding); what they hold is not used for other atoms' rows.  A row that
+      sees nothing gives zeros and has no gradient, whatever it holds.
     * ``return_log_sums``: also ``[N, H]`` float32, the logarithm of each row's
       sum of exponentials (-infinity for a row that sees nothing), which
       :func:`atom_attention_adjoint` takes.
