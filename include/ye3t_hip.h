@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define YE3T_HIP_ABI_VERSION 63 /* reference native ABI floor is 42 (execution_plan.py:35) */
+#define YE3T_HIP_ABI_VERSION 64 /* reference native ABI floor is 42 (execution_plan.py:35) */
 
 typedef struct ihipStream_t* ye3t_stream_t; /* == hipStream_t */
 
@@ -32,7 +32,7 @@ enum ye3t_dtype {
   YE3T_F64 = 1,
   YE3T_C64 = 2, /* complex: (re, im) pairs */
   YE3T_C128 = 3,
-  YE3T_BF16 = 4 /* embedding, norm and attention only */
+  YE3T_BF16 = 4 /* operators around the features only */
 };
 
 enum ye3t_status {
@@ -822,7 +822,7 @@ int ye3t_hip_product_plan_uses_stream(const ye3t_hip_product_plan* plan);
 int ye3t_hip_product_launch_info(const ye3t_hip_product_plan* plan, int64_t samples, int64_t* grid,
                                  int64_t* block, int64_t* lds_bytes);
 
-/* ---- operators around the features: embedding, norm, attention ---------------
+/* ---- operators around the features: embedding, norm, attention, products, dropout
  * No reference counterparts.  They serve a model's own layers before and after
  * the ACE features; `dtype` may be YE3T_BF16 here.  None of them synchronises,
  * allocates or uses atomics on data: equal calls give equal bits. */
@@ -937,6 +937,64 @@ int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void*
                                     void* value_adjoint, void* slopes_adjoint, void* positions_adjoint,
                                     void* key_positions_adjoint, void* workspace, int64_t workspace_bytes,
                                     ye3t_stream_t stream);
+
+/* Atoms by species: `order` [rows] int32, the rows sorted by their species
+ * (int32, species_bytes 4, or int64, 8), rows of one species as they came, and
+ * `offsets` [species + 1] int64, where each species begins in it.  Rows of a
+ * species outside [0, species) come last, behind offsets[species]. */
+int64_t ye3t_hip_species_groups_workspace_bytes(int64_t rows, int64_t species);
+int ye3t_hip_species_groups(const void* species_of_rows, int species_bytes, int64_t rows, int64_t species, void* order,
+                            void* offsets, void* workspace, int64_t workspace_bytes, ye3t_stream_t stream);
+
+/* y = residual + D(act(x W + b)).  One weight and bias for all rows, or
+ * (groups_given) one for each of `groups` species, with the order and offsets of
+ * ye3t_hip_species_groups.  Rows behind the last species have x W + b = 0.
+ * Sums are fp32; fp32 products are good to fp32's rounding (three bf16 parts of
+ * each value), for values above 2^-110.  D drops a value where 16 bits of Philox
+ * 4x32-10 are below drop_below (the probability times 65536) and scales the
+ * others by 65536 / (65536 - drop_below): key the seed, counter (column / 8,
+ * layer, row low, row high), eight values of 16 bits in ascending order. */
+typedef struct {
+  int dtype;         /* YE3T_F32 or YE3T_BF16, of all arrays */
+  int64_t rows, inputs, outputs;
+  int groups_given;  /* 0: one weight for all rows */
+  int64_t groups;
+  const int32_t* order;
+  const int64_t* offsets;
+  const void* input; /* [rows, inputs] */
+  int64_t input_row_stride;
+  const void* weight;  /* [groups, inputs, outputs], or [groups, outputs, inputs] where `turned` */
+  int64_t weight_group_stride, weight_row_stride; /* the last axis has stride 1 */
+  int turned;
+  const void* bias;     /* [groups, outputs], or NULL */
+  const void* residual; /* [rows, outputs], or NULL */
+  int activation;       /* 0 none, 1 relu, 2 silu, 3 gelu (by the normal distribution's integral) */
+  int64_t drop_below;   /* 0 .. 65536 */
+  uint32_t layer;
+  uint64_t seed;
+  const int64_t* device_seed; /* NULL, or one value in device memory that is taken instead of `seed` */
+} ye3t_linear_args;
+
+/* out [rows, outputs] and, if not NULL, preactivation [rows, outputs] = x W + b,
+ * rounded, which the gradient of an activation takes. */
+int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out, ye3t_stream_t stream);
+
+/* Device workspace bytes of ye3t_hip_linear_adjoint (-1 on invalid input). */
+int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args);
+
+/* Gradients of ye3t_hip_linear for the output's adjoint [rows, outputs], at the
+ * rounded preactivation (NULL without an activation): input_adjoint [rows,
+ * inputs], weight_adjoint in the weight's layout without gaps, bias_adjoint
+ * [groups, outputs]; each may be NULL, the weight's only with the bias's.  The
+ * residual's is the adjoint itself.  dz = D(adjoint) act' is rounded to `dtype`. */
+int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, const void* preactivation,
+                            void* input_adjoint, void* weight_adjoint, void* bias_adjoint, void* workspace,
+                            int64_t workspace_bytes, ye3t_stream_t stream);
+
+/* y = residual + D(x) of [rows, width] (residual may be NULL), D as in
+ * ye3t_hip_linear.  Without a residual it is its own gradient. */
+int ye3t_hip_dropout(int dtype, const void* x, const void* residual, int64_t rows, int64_t width, int64_t below,
+                     uint32_t layer, uint64_t seed, const int64_t* device_seed, void* y, ye3t_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,355 @@
+// Products of atoms' rows with learned weights, one weight for all or one for each species.
+//
+//   z = x W + b                   (W, b of the row's species)
+//   y = residual + D(act(z))      D: dropout
+//
+// Gradient for the adjoint g of y:
+//
+//   dz = D(g) act'(z),  dx = dz W^T,  dW = x^T dz,  db = sum of dz over rows
+//
+// Rows of one species are found through an order of the rows (species.hip), so
+// neither x nor y is moved.  A workgroup owns a tile of one species' rows (forward and dx,
+// linear_rows.hip) or of a weight's gradient over a share of the rows
+// (linear_weights.hip), stages both operands in LDS and multiplies with the
+// 32 x 32 x 16 matrix instruction, bf16 x bf16 -> fp32.
+//
+// fp32 operands are held as three bf16 parts, x = h + m + l: h is x rounded to
+// bf16, m the rest rounded, l what is left, 24 bits in all.  A product takes the
+// six terms hh, hm, mh, mm, hl, lh; those left out are below 2^-26 of it, less than
+// fp32's own rounding (Henry, Tang and Heinecke, "Leveraging the bfloat16
+// artificial intelligence datatype for higher-precision computations", 2019).  Six bf16
+// instructions do the work of eight fp32 ones of the same length at sixteen times the
+// rate.  Values of 2^-110 and below lose their last bits, 2^-133 at most.  A value
+// that is not finite, or rounds to infinity in bf16, would leave NaN where fp32
+// leaves an infinity or a number: results that are not finite are computed
+// again, value by value in fp32 (exact_dot).
+#pragma once
+
+#include "random.h"
+#include "tiles.h"
+
+namespace ye3t {
+namespace linear {
+
+using namespace tiles;
+
+constexpr float kLog2e = 1.44269504f;
+
+enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
+
+// Phi(z), the normal distribution's integral, and exp(-z^2 / 2).  The smaller tail is
+// exp(-x^2) f(x) / 2 with x = |z| / sqrt 2; f, the scaled complementary error function,
+// is a polynomial in t = 1 / (1 + 0.44 x) fitted for the least relative error, 1.9e-7 up to
+// x = 14 (beyond, exp(-x^2) is zero).
+struct Normal {
+  float phi, bell;
+};
+__device__ inline Normal normal_of(float z) {
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.311126984f * fabsf(z));
+  const float f =
+      t * (0.248216531f +
+           t * (0.248935427f +
+                t * (0.216934685f +
+                     t * (0.216993537f + t * (-0.0222940624f + t * (0.298866830f + t * (-0.279152495f + t * 0.0714997336f)))))));
+  const float bell = __builtin_amdgcn_exp2f(z * z * (-0.5f * kLog2e)), tail = 0.5f * bell * f;
+  return {z < 0.0f ? tail : 1.0f - tail, bell};
+}
+
+__device__ inline float activated(int act, float z) {
+  if (act == kRelu) return z <= 0.0f ? 0.0f : z;
+  if (act == kSilu) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
+  if (act == kGelu) return z * normal_of(z).phi;
+  return z;
+}
+
+__device__ inline float slope_of(int act, float z) {
+  if (act == kRelu) return z > 0.0f ? 1.0f : 0.0f;
+  if (act == kSilu) {
+    const float e = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
+    return e + z * e * (1.0f - e);
+  }
+  if (act == kGelu) {
+    const Normal n = normal_of(z);
+    return n.phi + z * n.bell * 0.398942280f;
+  }
+  return 1.0f;
+}
+
+// ---- operands ------------------------------------------------------------------
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+
+// A tile of a matrix operand: LINES rows or columns of the result by KT of the
+// contraction, as bf16, kParts of it one after the other.
+//   along   LINES x KT: memory runs along the contraction
+//   across  KT x LINES: memory runs across it, and the transposing read turns it
+template <typename T, int LINES, int KT, bool ACROSS>
+struct Tile {
+  static constexpr int kValues = LINES * KT, kChunks = kValues / 8, kRow = (ACROSS ? LINES : KT) / 8;
+  static constexpr int kBytes = kParts<T> * kValues * 2;
+
+  // chunk x of the tile, in the order of its lines (across: of its contraction)
+  __device__ static inline int line_of(int x) { return x / kRow; }
+  __device__ static inline int column_of(int x) { return x % kRow * 8; }
+  __device__ static inline void put(__bf16* tile, int x, const Chunk<T, 8>& c) {
+    const int line = line_of(x);
+    __bf16* to = tile + (line * kRow + (x % kRow ^ turn<__bf16, kRow * 8>(line))) * 8;
+    bf16x8 part[kParts<T>];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (kParts<T> == 1) {
+        part[0][q] = __bf16(c.v[q]);
+      } else {
+        const float v = float(c.v[q]);
+        const __bf16 h = __bf16(v);
+        const float rest = v - float(h);
+        const __bf16 m = __bf16(rest);
+        part[0][q] = h;
+        part[1 % kParts<T>][q] = m;
+        part[2 % kParts<T>][q] = __bf16(rest - float(m));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kParts<T>; ++n) *reinterpret_cast<bf16x8*>(to + n * kValues) = part[n];
+  }
+
+  // Operand of 32 lines from `line`, contraction k .. k + 15: a lane holds line
+  // lane % 32, contraction k + 8 (lane / 32) + 0 .. 7.
+  __device__ static inline bf16x8 operand(const __bf16* tile, int line, int k, int lane) {
+    const int half = lane / 32;
+    if (!ACROSS) {
+      const int own = line + (lane & 31);
+      return *reinterpret_cast<const bf16x8*>(tile + own * KT + ((k / 8 + half) ^ turn<__bf16, KT>(own)) * 8);
+    }
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    // lane l of a block of 16 gives the address of four values of contraction l / 4, lines
+    // 4 (l % 4) .. + 3, and gets four of line l's
+    const int at = k + 8 * half + (lane & 15) / 4, chunk = line / 8 + (lane & 16) / 8 + (lane & 3) / 2;
+    const __bf16* from = tile + at * LINES + 4 * (lane & 1);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from + (chunk ^ turn<__bf16, LINES>(at)) * 8));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(from + 4 * LINES + (chunk ^ turn<__bf16, LINES>(at + 4)) * 8));
+    const s16x8 both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, both);
+  }
+};
+
+// The chunks of a tile that one of NT threads loads and puts.
+template <typename T, int LINES, int KT, bool ACROSS, int NT>
+struct Loads {
+  typedef Tile<T, LINES, KT, ACROSS> Of;
+  static constexpr int kEach = (Of::kChunks + NT - 1) / NT;
+  Chunk<T, 8> held[kEach];
+
+  // address(line, column, n): chunk n of this thread; null: zeros.  left(column): values that exist from there on.
+  template <typename A, typename L>
+  __device__ inline void load(A address, L left) {
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const int x = n * NT + int(threadIdx.x);
+      if (Of::kChunks % NT != 0 && x >= Of::kChunks) continue;
+      const int c = Of::column_of(x), most = left(c);
+      const T* p = address(Of::line_of(x), c, n);
+      held[n] = p && most > 0 ? Chunk<T, 8>::load(p, most) : Chunk<T, 8>::zero();
+    }
+  }
+  __device__ inline void put(__bf16* tile) const {
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const int x = n * NT + int(threadIdx.x);
+      if (Of::kChunks % NT != 0 && x >= Of::kChunks) continue;
+      Of::put(tile, x, held[n]);
+    }
+  }
+};
+
+// A workgroup's tile: WM x WN waves of FM x FN squares of 32 x 32 each, times WK shares of
+// the contraction, of which a step takes BK each.
+template <int WM_, int WN_, int WK_, int FM_, int FN_, int BK_, int BUFFERS_, int WAVES_>
+struct Shape {
+  static constexpr int WM = WM_, WN = WN_, WK = WK_, FM = FM_, FN = FN_, BK = BK_, BUFFERS = BUFFERS_;
+  static constexpr int TM = WM * FM * 32, TN = WN * FN * 32, KT = WK * BK, NT = 64 * WM * WN * WK;
+  static constexpr int kPerSimd = WAVES_;  // waves a SIMD that the registers are set for
+  // rows of a wave's square rows on their way out: 16 bytes more than the values, so that 16 rows' chunks lie in
+  // different banks
+  static constexpr int kOutRow = FN * 32 + 4;
+  static constexpr int kOutBytes = WM * WN * WK * 32 * kOutRow * 4;
+};
+
+__device__ inline void multiply(const bf16x8& a, const bf16x8& b, f32x16& c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// sum[i][j] += the wave's squares over one step of the contraction.  The columns' operand comes first, so
+// that a lane holds row lane % 32 and, in register 4 b + j, column 8 b + 4 (lane / 32) + j.
+template <typename T, typename S, typename A, typename B>
+__device__ inline void multiply_tiles(const __bf16* a, const __bf16* b, int wm, int wn, int wk, int lane,
+                                      f32x16 (*sum)[S::FN]) {
+  constexpr int P = kParts<T>;
+#pragma unroll
+  for (int k = 0; k < S::BK; k += 16) {
+    bf16x8 x[S::FM][P], y[S::FN][P];
+#pragma unroll
+    for (int n = 0; n < P; ++n) {
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+        x[i][n] = A::operand(a + n * A::kValues, (wm * S::FM + i) * 32, wk * S::BK + k, lane);
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j)
+        y[j][n] = B::operand(b + n * B::kValues, (wn * S::FN + j) * 32, wk * S::BK + k, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) {
+        if constexpr (P == 3) {
+          multiply(y[j][2], x[i][0], sum[i][j]);
+          multiply(y[j][0], x[i][2], sum[i][j]);
+          multiply(y[j][1], x[i][1], sum[i][j]);
+          multiply(y[j][1], x[i][0], sum[i][j]);
+          multiply(y[j][0], x[i][1], sum[i][j]);
+        }
+        multiply(y[j][0], x[i][0], sum[i][j]);
+      }
+  }
+}
+
+// Passes the wave's squares through LDS and gives them out eight columns of a row at a time, so that memory
+// is read and written along rows: use(row, column, values) of the workgroup's tile.  The
+// shares of the contraction are added in order.
+template <typename S, typename F>
+__device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, int wn, int wk, int lane, F use) {
+  constexpr int CHUNKS = S::FN * 4, STRIDE = S::kOutRow, BLOCK = 32 * STRIDE;
+  const int wave = (wk * S::WM + wm) * S::WN + wn;
+  float* own = reinterpret_cast<float*>(lds) + wave * BLOCK;
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i) {
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        f32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = sum[i][j][4 * b + q];
+        *reinterpret_cast<f32x4*>(own + (lane & 31) * STRIDE + 32 * j + 8 * b + 4 * (lane / 32)) = v;
+      }
+    if (S::WK == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int n = 0; n < 32 * CHUNKS / 64; ++n) {
+        const int r = n * (64 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS * 8;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = own[r * STRIDE + c + q];
+        use((wm * S::FM + i) * 32 + r, wn * S::FN * 32 + c, v);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      static_assert(S::WK == 1 || (S::FM == 1 && S::WM == 1 && S::WN == 1), "shares of one wave's rows");
+      __syncthreads();
+      for (int x = int(threadIdx.x); x < 32 * CHUNKS; x += S::NT) {
+        const int r = x / CHUNKS, c = x % CHUNKS * 8;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < S::WK; ++w)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] += reinterpret_cast<const float*>(lds)[w * BLOCK + r * STRIDE + c + q];
+        use(r, c, v);
+      }
+    }
+  }
+}
+
+// sum of a(k) b(k) over k < K in fp32, for results that are not finite
+template <typename A, typename B>
+__device__ float exact_dot(A a, B b, int64_t K) {
+  float s = 0.0f;
+#pragma unroll 4
+  for (int64_t k = 0; k < K; ++k) s = fmaf(a(k), b(k), s);
+  return s;
+}
+__device__ inline bool any_not_finite(const float* v) {
+  float worst = 0.0f;  // 0 v is NaN for infinities and NaN
+#pragma unroll
+  for (int q = 0; q < 8; ++q) worst += 0.0f * v[q];
+  return worst != 0.0f;
+}
+
+// Consecutive tiles run on one XCD, which has an L2 of its own: workgroups go to the eight XCDs in turn.
+__device__ inline int64_t tile_of_group() {
+  const unsigned n = gridDim.x, b = blockIdx.x, x = b & 7;
+  return int64_t(x) * (n / 8) + (x < n % 8 ? x : n % 8) + b / 8;
+}
+
+// A row's number in memory, -1 for one that an order names outside of the rows
+__device__ inline int64_t row_at(const int32_t* order, int64_t i, int64_t rows) {
+  if (!order) return i;
+  const int64_t r = order[i];
+  return r >= 0 && r < rows ? r : -1;
+}
+
+inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// ---- the two kinds of product ----------------------------------------------------
+// out[i, n] = sum over k of a[i, k] b_g[k, n], g the group of row i.  Rows behind the last group have no
+// weight: a sum of zero and no bias.
+template <typename T>
+struct RowProduct {
+  const T* a;
+  int64_t a_row;
+  const T* b;
+  int64_t b_group, b_row;  // b[g][k][n], or b[g][n][k] where `b_across` is false
+  bool b_across;
+  int K, N;
+  int64_t rows, groups;
+  bool grouped;            // false: one weight for all rows
+  const int32_t* order;
+  const int64_t* offsets;
+  // epilogue
+  const T* bias;           // [groups][N] or null
+  const T* residual;       // [rows][N] or null
+  T* kept;                 // a row's sum and bias, or null
+  T* out;
+  int activation;
+  Dropout dropout;
+  unsigned tiles_n;
+};
+
+// out_g[m, n] = sum over the group's rows i of a[i, m] b[i, n], and column sums of one of the two
+template <typename T>
+struct WeightProduct {
+  const T *a, *b;
+  int64_t a_row, b_row;
+  int M, N;
+  int64_t rows, groups;
+  bool grouped;
+  const int32_t* order;
+  const int64_t* offsets;
+  T* out;          // [groups][M][N]
+  T* sums;         // [groups][M] or [groups][N], or null
+  bool sums_of_a;
+  int64_t share;   // rows of one workgroup
+  float* part;     // sums of the shares of groups with several, [2 rows / share + 1][M][N]
+  float* sums_part;
+  unsigned tiles_m, tiles_n;
+};
+
+template <typename T>
+int launch_rows(RowProduct<T> p, hipStream_t s);
+template <typename T>
+int launch_weights(WeightProduct<T> p, hipStream_t s);
+
+// Shares of the rows of a weight's gradient, and the workspace for their sums.
+struct SharePlan {
+  int64_t share, slots, part_bytes, sums_bytes, bytes;
+};
+SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N);
+
+}  // namespace linear
+}  // namespace ye3t

@@ -1,0 +1,247 @@
+// The gradient to weights and biases: products over the rows of each group.
+#include "linear.h"
+
+namespace ye3t {
+namespace linear {
+namespace {
+
+// Where the sums of a group's shares begin; only groups of several shares have any there.
+__device__ inline int64_t part_of(int64_t begin, int64_t share) { return 2 * begin / share; }
+
+template <typename T, typename S>
+__global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(const WeightProduct<T> p) {
+  typedef Tile<T, S::TM, S::KT, true> A;
+  typedef Tile<T, S::TN, S::KT, true> B;
+  static_assert(S::TM == S::TN, "either operand's columns can be summed");
+  constexpr int STEP = A::kBytes + B::kBytes;
+  constexpr int LDS = S::BUFFERS * STEP > S::kOutBytes ? S::BUFFERS * STEP : S::kOutBytes;
+  __shared__ __align__(256) char lds[LDS];
+  const int lane = int(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int wn = wave % S::WN, wm = wave / S::WN % S::WM, wk = wave / (S::WN * S::WM);
+
+  const int64_t tile = tile_of_group(), tiles = int64_t(p.tiles_m) * p.tiles_n, slot = tile / tiles;
+  const int tile_m = int(tile % tiles / p.tiles_n), tile_n = int(tile % p.tiles_n);
+  const int m0 = tile_m * S::TM, n0 = tile_n * S::TN;
+  int64_t group = 0, begin = 0, first = slot * p.share, length = p.rows;
+  if (p.grouped) {
+    auto bound = [&](int64_t d) { return clamped(p.offsets[d], p.rows) / p.share + d; };
+    group = find_owner(p.groups, slot, bound);
+    first = (slot - bound(group)) * p.share;
+    begin = clamped(p.offsets[group], p.rows);
+    length = clamped(p.offsets[group + 1], p.rows) - begin;
+  }
+  if (first && first >= length) return;  // the first share of a group without rows writes its zeros
+  const int64_t row0 = begin + first;
+  const int64_t left = length - first;
+  const int live = int(left < 0 ? 0 : left < p.share ? left : p.share);
+
+  Loads<T, S::TM, S::KT, true, S::NT> a;
+  Loads<T, S::TN, S::KT, true, S::NT> b;
+  constexpr int EACH = decltype(a)::kEach;
+  int64_t row[EACH];  // of the chunks that the next load takes
+  auto look = [&](int k0) {
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const int k = k0 + A::line_of(n * S::NT + int(threadIdx.x));
+      row[n] = k < live ? row_at(p.order, row0 + k, p.rows) : -1;
+    }
+  };
+  auto load = [&](int k0) {
+    a.load([&](int, int c, int n) { return row[n] >= 0 ? p.a + row[n] * p.a_row + m0 + c : nullptr; },
+           [&](int c) { return p.M - m0 - c; });
+    b.load([&](int, int c, int n) { return row[n] >= 0 ? p.b + row[n] * p.b_row + n0 + c : nullptr; },
+           [&](int c) { return p.N - n0 - c; });
+    look(k0 + S::KT);
+  };
+  auto tile_a = [&](int t) { return reinterpret_cast<__bf16*>(lds + (S::BUFFERS == 2 ? t & 1 : 0) * STEP); };
+  auto tile_b = [&](int t) { return reinterpret_cast<__bf16*>(lds + (S::BUFFERS == 2 ? t & 1 : 0) * STEP + A::kBytes); };
+
+  f32x16 sum[S::FM][S::FN];
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) sum[i][j] = zeros();
+  // column sums of one operand, by the workgroups of its first tile of the other
+  const bool summing = p.sums && (p.sums_of_a ? tile_n == 0 : tile_m == 0);
+  constexpr int ACROSS = S::TM / 8, DOWN = S::NT / ACROSS;
+  float column[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) column[q] = 0.0f;
+
+  const int steps = (live + S::KT - 1) / S::KT;
+  look(0);
+  if (steps) load(0);
+  for (int t = 0; t < steps; ++t) {
+    if (S::BUFFERS == 1 && t) __syncthreads();  // the last tile has been used
+    a.put(tile_a(t));
+    b.put(tile_b(t));
+    if (t + 1 < steps) load((t + 1) * S::KT);
+    __syncthreads();
+    multiply_tiles<T, S, A, B>(tile_a(t), tile_b(t), wm, wn, wk, lane, sum);
+    if (summing) {
+      const __bf16* from = p.sums_of_a ? tile_a(t) : tile_b(t);
+      const int c = int(threadIdx.x) % ACROSS;
+      for (int k = int(threadIdx.x) / ACROSS; k < S::KT; k += DOWN) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+#pragma unroll
+        for (int n = kParts<T> - 1; n >= 0; --n) {
+          const bf16x8 part = *reinterpret_cast<const bf16x8*>(from + n * A::kValues + k * S::TM + (c ^ turn<__bf16, S::TM>(k)) * 8);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] += float(part[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) column[q] += v[q];
+      }
+    }
+  }
+  __syncthreads();
+
+  const bool whole = length <= p.share;
+  const int64_t part = part_of(begin, p.share) + first / p.share;
+  if (summing) {
+    float* held = reinterpret_cast<float*>(lds);
+    static_assert(DOWN * S::TM * 4 <= LDS, "column sums fit the tiles' memory");
+#pragma unroll
+    for (int q = 0; q < 8; ++q) held[int(threadIdx.x) / ACROSS * S::TM + int(threadIdx.x) % ACROSS * 8 + q] = column[q];
+    __syncthreads();
+    const int c = int(threadIdx.x), at = (p.sums_of_a ? m0 : n0) + c, most = p.sums_of_a ? p.M : p.N;
+    if (c < S::TM && at < most) {
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DOWN; ++k) s += held[k * S::TM + c];
+      if (kParts<T> == 3 && 0.0f * s != 0.0f) {  // not finite: again from the values themselves
+        const T* v = p.sums_of_a ? p.a : p.b;
+        const int64_t step = p.sums_of_a ? p.a_row : p.b_row;
+        s = exact_dot([&](int64_t k) { const int64_t r = row_at(p.order, row0 + k, p.rows); return r < 0 ? 0.0f : float(v[r * step + at]); },
+                      [](int64_t) { return 1.0f; }, live);
+      }
+      if (whole) p.sums[group * most + at] = T(s);
+      else p.sums_part[part * most + at] = s;
+    }
+    __syncthreads();
+  }
+  give_out<S>(lds, sum, wm, wn, wk, lane, [&](int r, int c, float* v) {
+    const int m = m0 + r, n = n0 + c, most = p.N - n;
+    if (m >= p.M || most <= 0) return;
+    if (kParts<T> == 3 && any_not_finite(v)) {
+      for (int q = 0; q < 8 && q < most; ++q)
+        v[q] = exact_dot([&](int64_t k) { const int64_t i = row_at(p.order, row0 + k, p.rows); return i < 0 ? 0.0f : float(p.a[i * p.a_row + m]); },
+                         [&](int64_t k) { const int64_t i = row_at(p.order, row0 + k, p.rows); return i < 0 ? 0.0f : float(p.b[i * p.b_row + n + q]); },
+                         live);
+    }
+    if (whole) {
+      Chunk<T, 8> out;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) out.v[q] = T(v[q]);
+      out.store(p.out + (group * p.M + m) * p.N + n, most);
+    } else {
+      Chunk<float, 8> out;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) out.v[q] = v[q];
+      out.store(p.part + (part * p.M + m) * p.N + n, most);
+    }
+  });
+}
+
+// Adds the sums of the shares of each group that has several, in order; the workgroups behind those of the
+// products add the column sums.
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void weight_join_kernel(const WeightProduct<T> p, unsigned product_groups) {
+  const bool columns = blockIdx.x >= product_groups;
+  const int64_t size = columns ? (p.sums_of_a ? p.M : p.N) : int64_t(p.M) * p.N;
+  const float* part = columns ? p.sums_part : p.part;
+  T* out = columns ? p.sums : p.out;
+  const int64_t at = (int64_t(columns ? blockIdx.x - product_groups : blockIdx.x) * kJoinThreads + threadIdx.x) * 8;
+  for (int64_t g = blockIdx.y; g < (p.grouped ? p.groups : 1); g += gridDim.y) {
+    const int64_t begin = p.grouped ? clamped(p.offsets[g], p.rows) : 0;
+    const int64_t length = (p.grouped ? clamped(p.offsets[g + 1], p.rows) : p.rows) - begin;
+    if (length <= p.share || at >= size) continue;
+    const float* from = part + part_of(begin, p.share) * size + at;
+    const int shares = int((length + p.share - 1) / p.share);
+    float s[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) s[q] = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < shares; ++k) {
+      const Chunk<float, 8> v = Chunk<float, 8>::load(from + k * size, size - at < 8 ? int(size - at) : 8);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s[q] += v.v[q];
+    }
+    Chunk<T, 8> o;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o.v[q] = T(s[q]);
+    o.store(out + g * size + at, size - at < 8 ? int(size - at) : 8);
+  }
+}
+
+template <typename T>
+struct Shapes;
+template <>
+struct Shapes<__bf16> {
+  typedef Shape<2, 2, 1, 2, 2, 64, 2, 2> Large;
+  typedef Shape<2, 2, 1, 1, 1, 64, 2, 4> Middle;
+};
+template <>
+struct Shapes<float> {
+  typedef Shape<2, 2, 1, 2, 2, 32, 1, 2> Large;
+  typedef Shape<2, 2, 1, 1, 1, 32, 1, 3> Middle;
+};
+
+// Tiles of 128 x 128, or of 64 x 64 for narrow weights
+inline bool narrow(int64_t M, int64_t N) { return M <= 64 || N <= 64; }
+
+template <typename T, typename S>
+int launch_shaped(WeightProduct<T> p, hipStream_t s) {
+  p.tiles_m = p.M ? unsigned((p.M + S::TM - 1) / S::TM) : 1;  // no rows or columns: there may be sums
+  p.tiles_n = p.N ? unsigned((p.N + S::TN - 1) / S::TN) : 1;
+  const int64_t slots = p.grouped ? p.rows / p.share + p.groups : (p.rows + p.share - 1) / p.share;
+  const int64_t groups = (slots ? slots : 1) * p.tiles_m * p.tiles_n;
+  if (!fits_grid(groups, S::NT))
+    return set_error(YE3T_EUNSUPPORTED, "weights of %d x %d for %lld species are too many for one launch", p.M, p.N,
+                     (long long)p.groups);
+  hipLaunchKernelGGL((weight_product_kernel<T, S>), dim3(unsigned(groups)), dim3(S::NT), 0, s, p);
+  return check_launch("weight_product_kernel");
+}
+
+}  // namespace
+
+// Shares that give the card about four workgroups a compute unit, of 512 rows or more
+SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N) {
+  SharePlan f{};
+  const int64_t t = narrow(M, N) ? 64 : 128, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
+  const int64_t parts = tiles == 0 ? 1024 : tiles < 1024 ? 1024 / tiles : 1;
+  f.share = (rows + parts - 1) / parts;
+  if (f.share < 512) f.share = 512;
+  if (f.share > (1 << 30)) f.share = 1 << 30;
+  f.slots = f.share < rows ? 2 * rows / f.share + 1 : 0;
+  f.part_bytes = up(f.slots * M * N * 4);
+  f.sums_bytes = up(f.slots * (M > N ? M : N) * 4);
+  f.bytes = f.part_bytes + f.sums_bytes;
+  return f;
+}
+
+template <typename T>
+int launch_weights(WeightProduct<T> p, hipStream_t s) {
+  const int64_t groups = p.grouped ? p.groups : 1;
+  if (groups == 0 || ((p.M == 0 || p.N == 0) && !p.sums)) return YE3T_OK;
+  if (int rc = narrow(p.M, p.N) ? launch_shaped<T, typename Shapes<T>::Middle>(p, s)
+                                : launch_shaped<T, typename Shapes<T>::Large>(p, s))
+    return rc;
+  if (p.rows <= p.share) return YE3T_OK;
+  const int64_t per = kJoinThreads * 8, product = (int64_t(p.M) * p.N + per - 1) / per;
+  const int64_t column = p.sums ? ((p.sums_of_a ? p.M : p.N) + per - 1) / per : 0;
+  if (!fits_grid(product + column, kJoinThreads))
+    return set_error(YE3T_EUNSUPPORTED, "a weight of %d x %d is too large for one launch", p.M, p.N);
+  hipLaunchKernelGGL((weight_join_kernel<T>), dim3(unsigned(product + column), unsigned(groups < 65535 ? groups : 65535)),
+                     dim3(kJoinThreads), 0, s, p, unsigned(product));
+  return check_launch("weight_join_kernel");
+}
+template int launch_weights<float>(WeightProduct<float>, hipStream_t);
+template int launch_weights<__bf16>(WeightProduct<__bf16>, hipStream_t);
+
+}  // namespace linear
+}  // namespace ye3t

@@ -57,6 +57,13 @@ FUSED_OPERATIONS = (
     "rms_norm_8bit",
     "atom_attention",
     "atom_attention_adjoint",
+    "linear",
+    "linear_adjoint",
+    "species_groups",
+    "species_linear",
+    "species_linear_adjoint",
+    "dropout",
+    "dropout_adjoint",
 )
 HIP_OPERATIONS = REFERENCE_OPERATIONS + FUSED_OPERATIONS
 
@@ -698,6 +705,12 @@ def __getattr__(name):
         import importlib
 
         globals()[name] = value = getattr(importlib.import_module("ye3t_amd.runtime.atoms"), name)
+        return value
+    if name in ("linear", "linear_adjoint", "species_groups", "species_linear", "species_linear_adjoint", "dropout",
+                "dropout_adjoint", "SpeciesGroups"):
+        import importlib
+
+        globals()[name] = value = getattr(importlib.import_module("ye3t_amd.runtime.products"), name)
         return value
     if name in ("ExecutionPlan", "YE3TExecutionPlan"):
         from ye3t_amd.runtime.execution_plan import ExecutionPlan

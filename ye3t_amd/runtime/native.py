@@ -12,7 +12,7 @@ import numpy as np
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "libye3t_hip.so")
-ABI_VERSION = 63
+ABI_VERSION = 64
 _LIB = None
 
 F32, F64, BF16 = 0, 1, 4
@@ -86,6 +86,17 @@ class AttentionArgs(ctypes.Structure):
                              "value_row_stride", "value_head_stride")] + \
         [("offsets", _vp), ("key_offsets", _vp), ("scale", ctypes.c_double), ("cap", ctypes.c_double)] + \
         [(n, _vp) for n in ("slopes", "positions", "key_positions", "key_mask")]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("rows", ctypes.c_int64), ("inputs", ctypes.c_int64),
+                ("outputs", ctypes.c_int64), ("groups_given", ctypes.c_int), ("groups", ctypes.c_int64),
+                ("order", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("input", ctypes.c_void_p),
+                ("input_row_stride", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("weight_group_stride", ctypes.c_int64), ("weight_row_stride", ctypes.c_int64),
+                ("turned", ctypes.c_int), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("activation", ctypes.c_int), ("drop_below", ctypes.c_int64), ("layer", ctypes.c_uint32),
+                ("seed", ctypes.c_uint64), ("device_seed", ctypes.c_void_p)]
 
 
 class Caps(ctypes.Structure):
@@ -227,6 +238,15 @@ def lib():
     L.ye3t_hip_atom_attention_adjoint_workspace_bytes.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_int]
     L.ye3t_hip_atom_attention_adjoint_workspace_bytes.restype = _i64
     L.ye3t_hip_atom_attention_adjoint.argtypes = [ctypes.POINTER(AttentionArgs)] + [_vp] * 10 + [_i64, _vp]
+    L.ye3t_hip_species_groups_workspace_bytes.argtypes = [_i64, _i64]
+    L.ye3t_hip_species_groups_workspace_bytes.restype = _i64
+    L.ye3t_hip_species_groups.argtypes = [_vp, ctypes.c_int, _i64, _i64, _vp, _vp, _vp, _i64, _vp]
+    L.ye3t_hip_linear.argtypes = [ctypes.POINTER(LinearArgs), _vp, _vp, _vp]
+    L.ye3t_hip_linear_adjoint_workspace_bytes.argtypes = [ctypes.POINTER(LinearArgs)]
+    L.ye3t_hip_linear_adjoint_workspace_bytes.restype = _i64
+    L.ye3t_hip_linear_adjoint.argtypes = [ctypes.POINTER(LinearArgs)] + [_vp] * 6 + [_i64, _vp]
+    L.ye3t_hip_dropout.argtypes = [ctypes.c_int, _vp, _vp, _i64, _i64, _i64, ctypes.c_uint32, ctypes.c_uint64, _vp, _vp,
+                                   _vp]
     version = L.ye3t_hip_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"ye3t_hip ABI {version} does not match the bindings ({ABI_VERSION})")
@@ -267,6 +287,8 @@ EXPORTED_SYMBOLS = (
     "ye3t_hip_rms_norm", "ye3t_hip_rms_norm_8bit", "ye3t_hip_rms_norm_adjoint_workspace_bytes",
     "ye3t_hip_rms_norm_adjoint", "ye3t_hip_atom_attention_workspace_bytes", "ye3t_hip_atom_attention",
     "ye3t_hip_atom_attention_adjoint_workspace_bytes", "ye3t_hip_atom_attention_adjoint",
+    "ye3t_hip_species_groups_workspace_bytes", "ye3t_hip_species_groups", "ye3t_hip_linear",
+    "ye3t_hip_linear_adjoint_workspace_bytes", "ye3t_hip_linear_adjoint", "ye3t_hip_dropout",
 )
 
 
@@ -2099,3 +2121,96 @@ class Attention:
                 _opt(dkp, "key_positions_adjoint"), work.data_ptr(), size, _raw_stream()),
                 "ye3t_hip_atom_attention_adjoint")
         return dq, dk, dv, ds, dp, dkp
+
+
+# ---- products with learned weights and dropout (ye3t_amd.runtime.linear checks the arguments) ----
+
+def species_groups(species, count):
+    """``ye3t_hip_species_groups`` of contiguous ``species [rows]``: ``(order, offsets)``."""
+    import torch
+
+    N = species.numel()
+    order = torch.empty(N, dtype=torch.int32, device=species.device)
+    offsets = torch.empty(count + 1, dtype=torch.int64, device=species.device)
+    with _on(species.device):
+        size = lib().ye3t_hip_species_groups_workspace_bytes(N, count)
+        work = _workspace(size, "ye3t_hip_species_groups_workspace_bytes", species.device)
+        _check(lib().ye3t_hip_species_groups(_dev(species, "species"), species.element_size(), N, count,
+                                             order.data_ptr(), offsets.data_ptr(), work.data_ptr(), size, _raw_stream()),
+               "ye3t_hip_species_groups")
+    return order, offsets
+
+
+class Linear:
+    """One product with learned weights: ``ye3t_linear_args`` and the tensors behind it.  ``input [rows, inputs]`` with
+    unit columns, ``weight [(species,) inputs, outputs]`` with unit columns or unit rows, ``bias`` and ``residual``
+    contiguous; ``below``, ``layer`` and ``seed`` (an int or an int64 tensor) of the dropped values."""
+
+    def __init__(self, input, weight, bias, residual, order, offsets, activation, below, layer, seed):
+        import torch
+
+        self.input, self.weight, self.bias, self.residual = input, weight, bias, residual
+        self.order, self.offsets = order, offsets
+        self.activation, self.below, self.layer, self.seed = activation, below, layer, seed
+        self.turned = weight.stride(-1) != 1 and weight.shape[-1] > 1
+        held = isinstance(seed, torch.Tensor)
+        pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self.args = LinearArgs(
+            dtype=_storage_code(input.dtype), rows=input.shape[0], inputs=input.shape[1], outputs=weight.shape[-1],
+            groups_given=order is not None, groups=weight.shape[0] if order is not None else 0, order=pointer(order),
+            offsets=pointer(offsets), input=input.data_ptr(), input_row_stride=input.stride(0), weight=weight.data_ptr(),
+            weight_group_stride=weight.stride(0) if order is not None else 0,
+            weight_row_stride=weight.stride(-1 if self.turned else -2), turned=self.turned, bias=pointer(bias),
+            residual=pointer(residual), activation=activation, drop_below=below, layer=layer,
+            seed=0 if held else seed, device_seed=seed.data_ptr() if held else None)
+
+    def forward(self, keep):
+        """``(out, preactivation or None)``"""
+        import torch
+
+        x = self.input
+        out = torch.empty((x.shape[0], self.weight.shape[-1]), dtype=x.dtype, device=x.device)
+        kept = torch.empty_like(out) if keep else None
+        with _on(x.device):
+            _check(lib().ye3t_hip_linear(ctypes.byref(self.args), _opt(kept, "preactivation"), out.data_ptr(),
+                                         _raw_stream()), "ye3t_hip_linear")
+        return out, kept
+
+    def adjoint(self, adjoint, kept, need_input, need_weight, need_bias):
+        """Gradients to input, weight and bias, None where they are not needed."""
+        import torch
+
+        x, w = self.input, self.weight
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_input else None
+        dw = db = None
+        if need_weight or need_bias:
+            shape = (*w.shape[:-2], w.shape[-1], w.shape[-2]) if self.turned else w.shape
+            dw = torch.empty(shape, dtype=w.dtype, device=w.device)
+        if need_bias:
+            db = torch.empty((*w.shape[:-2], w.shape[-1]), dtype=w.dtype, device=w.device)
+        with _on(x.device):
+            size = lib().ye3t_hip_linear_adjoint_workspace_bytes(ctypes.byref(self.args))
+            work = _workspace(size, "ye3t_hip_linear_adjoint_workspace_bytes", x.device)
+            _check(lib().ye3t_hip_linear_adjoint(ctypes.byref(self.args), _dev(adjoint, "adjoint"),
+                                                 _opt(kept, "preactivation"), _opt(dx, "input_adjoint"),
+                                                 _opt(dw, "weight_adjoint"), _opt(db, "bias_adjoint"), work.data_ptr(),
+                                                 size, _raw_stream()), "ye3t_hip_linear_adjoint")
+        if not need_weight:
+            dw = None
+        return dx, dw.transpose(-1, -2) if dw is not None and self.turned else dw, db
+
+
+def dropout(input, residual, below, layer, seed):
+    """``ye3t_hip_dropout`` of contiguous rows."""
+    import torch
+
+    code = _storage_code(input.dtype)
+    held = isinstance(seed, torch.Tensor)
+    y = torch.empty_like(input)
+    W = int(input.shape[-1])
+    if W:
+        with _on(input.device):
+            _check(lib().ye3t_hip_dropout(code, _dev(input, "input"), _opt(residual, "residual"), input.numel() // W, W,
+                                          below, layer, 0 if held else seed, seed.data_ptr() if held else None,
+                                          y.data_ptr(), _raw_stream()), "ye3t_hip_dropout")
+    return y
