@@ -25,6 +25,8 @@
 // again, value by value in fp32 (exact_dot).
 #pragma once
 
+#include <type_traits>
+
 #include "random.h"
 #include "tiles.h"
 
@@ -73,6 +75,15 @@ __device__ inline float slope_of(int act, float z) {
     return n.phi + z * n.bell * 0.398942280f;
   }
   return 1.0f;
+}
+
+// f(0) .. f(N - 1) with the number as a type
+template <int N, int I = 0, typename F>
+__device__ inline void repeat(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    repeat<N, I + 1>(f);
+  }
 }
 
 // ---- operands ------------------------------------------------------------------
@@ -165,6 +176,37 @@ struct Loads {
   }
 };
 
+// The same straight to LDS, where every chunk is 16 whole aligned bytes.  A wave's 64 chunks lie one after the
+// other, so the thread at place x of a line takes the chunk that belongs there.  The instruction has no
+// result, but the compiler takes every transposing read of LDS to wait for it and would wait for the next tile's
+// loads before it reads this one's (8192^3, both operands along and across: 1 004 and 1 094 us by
+// the builtin, 968 and 970 so); it is written out, and the kernels count the loads themselves.
+template <int LINES, int KT, bool ACROSS, int NT>
+struct DirectLoads {
+  typedef Tile<__bf16, LINES, KT, ACROSS> Of;
+  static constexpr int kEach = Of::kChunks / NT;
+  static_assert(Of::kChunks % NT == 0, "every thread loads as many chunks");
+
+  __device__ static inline int line_of(int n) { return Of::line_of(n * NT + int(threadIdx.x)); }
+  __device__ static inline int column_of(int n) {
+    const int x = n * NT + int(threadIdx.x);
+    return (x % Of::kRow ^ turn<__bf16, Of::kRow * 8>(Of::line_of(x))) * 8;
+  }
+  __device__ static inline const __bf16* none() { return reinterpret_cast<const __bf16*>(kZeros); }
+  // Chunk n of this thread
+  __device__ static inline void load(__bf16* tile, int n, int wave, const __bf16* p) {
+    const unsigned to = unsigned(uintptr_t((__attribute__((address_space(3))) void*)(tile + (n * NT + 64 * wave) * 8)));
+    // m0, the place in LDS, takes one instruction between to be there
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "m0");
+  }
+};
+
+// All but the newest N loads of this wave have arrived, its reads of LDS are done, and so are the other waves'.
+template <int N>
+__device__ inline void arrive_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 // A workgroup's tile: WM x WN waves of FM x FN squares of 32 x 32 each, times WK shares of
 // the contraction, of which a step takes BK each.
 template <int WM_, int WN_, int WK_, int FM_, int FN_, int BK_, int BUFFERS_, int WAVES_>
@@ -184,35 +226,91 @@ __device__ inline void multiply(const bf16x8& a, const bf16x8& b, f32x16& c) {
 
 // sum[i][j] += the wave's squares over one step of the contraction.  The columns' operand comes first, so
 // that a lane holds row lane % 32 and, in register 4 b + j, column 8 b + 4 (lane / 32) + j.
+template <typename T, typename S>
+struct Operands {
+  bf16x8 x[S::FM][kParts<T>], y[S::FN][kParts<T>];
+};
+template <typename T, typename S, typename A, typename B>
+__device__ inline void read_operands(const __bf16* a, const __bf16* b, int wm, int wn, int k, int lane, Operands<T, S>& o) {
+#pragma unroll
+  for (int n = 0; n < kParts<T>; ++n) {
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) o.y[j][n] = B::operand(b + n * B::kValues, (wn * S::FN + j) * 32, k, lane);
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) o.x[i][n] = A::operand(a + n * A::kValues, (wm * S::FM + i) * 32, k, lane);
+  }
+}
+template <typename T, typename S>
+__device__ inline void multiply_operands(const Operands<T, S>& o, f32x16 (*sum)[S::FN]) {
+  constexpr int P = kParts<T>;
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      if constexpr (P == 3) {
+        multiply(o.y[j][2], o.x[i][0], sum[i][j]);
+        multiply(o.y[j][0], o.x[i][2], sum[i][j]);
+        multiply(o.y[j][1], o.x[i][1], sum[i][j]);
+        multiply(o.y[j][1], o.x[i][0], sum[i][j]);
+        multiply(o.y[j][0], o.x[i][1], sum[i][j]);
+      }
+      multiply(o.y[j][0], o.x[i][0], sum[i][j]);
+    }
+}
 template <typename T, typename S, typename A, typename B>
 __device__ inline void multiply_tiles(const __bf16* a, const __bf16* b, int wm, int wn, int wk, int lane,
                                       f32x16 (*sum)[S::FN]) {
-  constexpr int P = kParts<T>;
 #pragma unroll
   for (int k = 0; k < S::BK; k += 16) {
-    bf16x8 x[S::FM][P], y[S::FN][P];
+    Operands<T, S> o;
+    read_operands<T, S, A, B>(a, b, wm, wn, wk * S::BK + k, lane, o);
+    multiply_operands<T, S>(o, sum);
+  }
+}
+
+// sum[i][j] over all `steps` tiles of direct loads.  load(t, part, parts): issues a part of tile t's LOADS loads of
+// a thread; with(t): while tile t is there.  A step of 16 along the contraction reads the
+// operands of the next one between its products, and the last of a tile meets the other waves first, so
+// that no product waits for a barrier.  With two buffers a tile's loads are issued in the first half
+// of the one before: in four parts, the last right before the wait, 8192^3 took 970 us, so 893.
+template <typename S, typename A, typename B, int LOADS, typename TileA, typename TileB, typename Load, typename With>
+__device__ inline void multiply_direct(int steps, TileA tile_a, TileB tile_b, int wm, int wn, int wk, int lane, Load load,
+                                       With with, f32x16 (*sum)[S::FN]) {
+  typedef __bf16 T;
+  constexpr int AHEAD = S::BUFFERS - 1, SUB = S::BK / 16, PARTS = AHEAD == 1 ? SUB / 2 : SUB;
+  typedef std::integral_constant<int, 0> Zero;
+  typedef std::integral_constant<int, 1> One;
 #pragma unroll
-    for (int n = 0; n < P; ++n) {
-#pragma unroll
-      for (int i = 0; i < S::FM; ++i)
-        x[i][n] = A::operand(a + n * A::kValues, (wm * S::FM + i) * 32, wk * S::BK + k, lane);
-#pragma unroll
-      for (int j = 0; j < S::FN; ++j)
-        y[j][n] = B::operand(b + n * B::kValues, (wn * S::FN + j) * 32, wk * S::BK + k, lane);
-    }
-#pragma unroll
-    for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-      for (int j = 0; j < S::FN; ++j) {
-        if constexpr (P == 3) {
-          multiply(y[j][2], x[i][0], sum[i][j]);
-          multiply(y[j][0], x[i][2], sum[i][j]);
-          multiply(y[j][1], x[i][1], sum[i][j]);
-          multiply(y[j][1], x[i][0], sum[i][j]);
-          multiply(y[j][0], x[i][1], sum[i][j]);
-        }
-        multiply(y[j][0], x[i][0], sum[i][j]);
+  for (int t = 0; t < AHEAD; ++t)
+    if (t < steps) load(t, Zero(), One());
+  auto meet = [&](int t) {  // tile t is there, and tile t - 1 has been read
+    if (t + AHEAD <= steps) arrive_and_meet<(AHEAD - 1) * LOADS>();
+    else arrive_and_meet<0>();
+  };
+  Operands<T, S> o[2];
+  if (steps) {
+    meet(0);
+    read_operands<T, S, A, B>(tile_a(0), tile_b(0), wm, wn, wk * S::BK, lane, o[0]);
+  }
+  for (int t = 0; t < steps; ++t) {
+    repeat<SUB>([&](auto sub) {
+      constexpr int k = decltype(sub)::value;
+      if constexpr (k < PARTS) {
+        if (t + AHEAD < steps) load(t + AHEAD, sub, std::integral_constant<int, PARTS>());
       }
+      if constexpr (k == 0) with(t);
+      if constexpr (k + 1 < SUB) {
+        read_operands<T, S, A, B>(tile_a(t), tile_b(t), wm, wn, wk * S::BK + 16 * (k + 1), lane, o[(k + 1) & 1]);
+      } else if (t + 1 < steps) {
+        meet(t + 1);
+        read_operands<T, S, A, B>(tile_a(t + 1), tile_b(t + 1), wm, wn, wk * S::BK, lane, o[(k + 1) & 1]);
+      }
+      multiply_operands<T, S>(o[k & 1], sum);
+      repeat<S::FM * S::FN>([&](auto) {  // one read of LDS, one product
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      });
+    });
   }
 }
 
@@ -224,8 +322,8 @@ __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, i
   constexpr int CHUNKS = S::FN * 4, STRIDE = S::kOutRow, BLOCK = 32 * STRIDE;
   const int wave = (wk * S::WM + wm) * S::WN + wn;
   float* own = reinterpret_cast<float*>(lds) + wave * BLOCK;
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i) {
+  repeat<S::FM>([&](auto number) {
+    constexpr int i = decltype(number)::value;
 #pragma unroll
     for (int j = 0; j < S::FN; ++j)
 #pragma unroll
@@ -263,7 +361,32 @@ __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, i
         use(r, c, v);
       }
     }
-  }
+  });
+}
+
+// The same without LDS: the halves of the wave exchange what makes eight columns of a lane's row whole.
+// use(row, column, values)
+template <typename S, typename F>
+__device__ inline void hand_out(const f32x16 (*sum)[S::FN], int wm, int wn, int lane, F use) {
+  const int half = lane / 32;
+  repeat<S::FM>([&](auto number) {
+    constexpr int i = decltype(number)::value;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+      for (int b = 0; b < 4; b += 2) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, float(sum[i][j][4 * b + q])),
+                                                             __builtin_bit_cast(unsigned, float(sum[i][j][4 * b + 4 + q])),
+                                                             false, false);
+          v[q] = __builtin_bit_cast(float, unsigned(both[0]));
+          v[4 + q] = __builtin_bit_cast(float, unsigned(both[1]));
+        }
+        use((wm * S::FM + i) * 32 + (lane & 31), (wn * S::FN + j) * 32 + 8 * (b + half), v);
+      }
+  });
 }
 
 // sum of a(k) b(k) over k < K in fp32, for results that are not finite
@@ -285,6 +408,19 @@ __device__ inline bool any_not_finite(const float* v) {
 __device__ inline int64_t tile_of_group() {
   const unsigned n = gridDim.x, b = blockIdx.x, x = b & 7;
   return int64_t(x) * (n / 8) + (x < n % 8 ? x : n % 8) + b / 8;
+}
+
+// Rows and columns of tiles: four rows of tiles go together through the columns, so that the 32 or 64 tiles that run on
+// an XCD at a time share few rows and columns.
+struct Place {
+  int64_t row;
+  int column;
+};
+__device__ inline Place place_of(int64_t tile, int64_t rows, unsigned columns) {
+  const int64_t band = tile / (4 * int64_t(columns)), left = rows - 4 * band;
+  const int high = left < 4 ? int(left) : 4;
+  const unsigned in = unsigned(tile - band * 4 * columns);
+  return {4 * band + in % high, int(in / high)};
 }
 
 // A row's number in memory, -1 for one that an order names outside of the rows
@@ -349,7 +485,11 @@ int launch_weights(WeightProduct<T> p, hipStream_t s);
 struct SharePlan {
   int64_t share, slots, part_bytes, sums_bytes, bytes;
 };
-SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N);
+template <typename T>
+SharePlan share_plan(const WeightProduct<T>& p);
+// and the most bytes that a call of these sizes takes, whatever its operands' addresses are
+template <typename T>
+int64_t most_share_bytes(WeightProduct<T> p);
 
 }  // namespace linear
 }  // namespace ye3t

@@ -91,23 +91,39 @@ int forward_as(const ye3t_linear_args& a, void* kept, void* out, hipStream_t s) 
 
 inline bool shaped(const ye3t_linear_args& a) { return a.activation != kNone || a.drop_below > 0; }
 
-struct AdjointPlan {
-  int64_t dz_bytes, bytes;
-  SharePlan shares;
-};
-AdjointPlan adjoint_plan(const ye3t_linear_args& a) {
-  AdjointPlan f{};
-  f.dz_bytes = shaped(a) ? up(a.rows * a.outputs * (a.dtype == YE3T_F32 ? 4 : 2)) : 0;
-  f.shares = share_plan(a.rows, a.groups_given ? a.groups : 1, a.turned ? a.outputs : a.inputs,
-                        a.turned ? a.inputs : a.outputs);
-  f.bytes = f.dz_bytes + f.shares.bytes + 256;
-  return f;
+// dW = x^T dz, or its transpose where the weight is kept turned
+template <typename T>
+WeightProduct<T> weights_of(const ye3t_linear_args& a, const T* dz) {
+  WeightProduct<T> p{};
+  const T* x = static_cast<const T*>(a.input);
+  p.a = a.turned ? dz : x;
+  p.b = a.turned ? x : dz;
+  p.a_row = a.turned ? a.outputs : a.input_row_stride;
+  p.b_row = a.turned ? a.input_row_stride : a.outputs;
+  p.M = int(a.turned ? a.outputs : a.inputs);
+  p.N = int(a.turned ? a.inputs : a.outputs);
+  p.rows = a.rows;
+  p.groups = a.groups;
+  p.grouped = a.groups_given != 0;
+  p.order = p.grouped ? a.order : nullptr;
+  p.offsets = p.grouped ? a.offsets : nullptr;
+  p.sums_of_a = a.turned != 0;
+  return p;
+}
+
+// dz in the workspace and the sums of the shares behind it; the same whatever the adjoint's address is.
+int64_t dz_bytes(const ye3t_linear_args& a) {
+  return shaped(a) ? up(a.rows * a.outputs * (a.dtype == YE3T_F32 ? 4 : 2)) : 0;
+}
+int64_t adjoint_bytes(const ye3t_linear_args& a) {
+  const int64_t shares = a.dtype == YE3T_F32 ? most_share_bytes(weights_of<float>(a, nullptr))
+                                             : most_share_bytes(weights_of<__bf16>(a, nullptr));
+  return dz_bytes(a) + shares + 256;
 }
 
 template <typename T>
 int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept, void* input_adjoint,
                void* weight_adjoint, void* bias_adjoint, char* work, hipStream_t s) {
-  const AdjointPlan f = adjoint_plan(a);
   const T* dz = static_cast<const T*>(adjoint);
   if (shaped(a) && a.rows > 0 && a.outputs > 0) {
     T* to = reinterpret_cast<T*>(work);
@@ -131,26 +147,13 @@ int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept,
     if (int rc = launch_rows(p, s)) return rc;
   }
   if (weight_adjoint) {
-    // dW = x^T dz, or its transpose where the weight is kept turned
-    WeightProduct<T> p{};
-    const T* x = static_cast<const T*>(a.input);
-    p.a = a.turned ? dz : x;
-    p.b = a.turned ? x : dz;
-    p.a_row = a.turned ? a.outputs : a.input_row_stride;
-    p.b_row = a.turned ? a.input_row_stride : a.outputs;
-    p.M = int(a.turned ? a.outputs : a.inputs);
-    p.N = int(a.turned ? a.inputs : a.outputs);
-    p.rows = a.rows;
-    p.groups = a.groups;
-    p.grouped = a.groups_given != 0;
-    p.order = p.grouped ? a.order : nullptr;
-    p.offsets = p.grouped ? a.offsets : nullptr;
+    WeightProduct<T> p = weights_of<T>(a, dz);
+    const SharePlan f = share_plan(p);
     p.out = static_cast<T*>(weight_adjoint);
     p.sums = static_cast<T*>(bias_adjoint);
-    p.sums_of_a = a.turned != 0;
-    p.share = f.shares.share;
-    p.part = reinterpret_cast<float*>(work + f.dz_bytes);
-    p.sums_part = reinterpret_cast<float*>(work + f.dz_bytes + f.shares.part_bytes);
+    p.share = f.share;
+    p.part = reinterpret_cast<float*>(work + dz_bytes(a));
+    p.sums_part = reinterpret_cast<float*>(work + dz_bytes(a) + f.part_bytes);
     if (int rc = launch_weights(p, s)) return rc;
   }
   return YE3T_OK;
@@ -179,7 +182,7 @@ int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args) {
   clear_error();
   if (!args) return set_error(YE3T_EINVAL, "the product needs its arguments");
   if (linear::check_linear(*args)) return -1;
-  return linear::adjoint_plan(*args).bytes;
+  return linear::adjoint_bytes(*args);
 }
 
 int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, const void* preactivation,
@@ -194,7 +197,7 @@ int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, c
   YE3T_REQUIRE(!any || args->activation == linear::kNone || preactivation,
                "the gradient of an activation needs the preactivation");
   YE3T_REQUIRE(!bias_adjoint || weight_adjoint, "the bias's gradient comes with the weight's");
-  YE3T_REQUIRE(workspace && workspace_bytes >= linear::adjoint_plan(*args).bytes,
+  YE3T_REQUIRE(workspace && workspace_bytes >= linear::adjoint_bytes(*args),
                "the workspace is smaller than ye3t_hip_linear_adjoint_workspace_bytes");
   char* work = static_cast<char*>(workspace);
   return args->dtype == YE3T_F32

@@ -8,13 +8,13 @@ namespace {
 // Where the sums of a group's shares begin; only groups of several shares have any there.
 __device__ inline int64_t part_of(int64_t begin, int64_t share) { return 2 * begin / share; }
 
-template <typename T, typename S>
+template <typename T, typename S, bool DIRECT>
 __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(const WeightProduct<T> p) {
   typedef Tile<T, S::TM, S::KT, true> A;
   typedef Tile<T, S::TN, S::KT, true> B;
   static_assert(S::TM == S::TN, "either operand's columns can be summed");
   constexpr int STEP = A::kBytes + B::kBytes;
-  constexpr int LDS = S::BUFFERS * STEP > S::kOutBytes ? S::BUFFERS * STEP : S::kOutBytes;
+  constexpr int LDS = S::BUFFERS * STEP > S::kOutBytes || DIRECT ? S::BUFFERS * STEP : S::kOutBytes;
   __shared__ __align__(256) char lds[LDS];
   const int lane = int(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int wn = wave % S::WN, wm = wave / S::WN % S::WM, wk = wave / (S::WN * S::WM);
@@ -35,27 +35,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
   const int64_t left = length - first;
   const int live = int(left < 0 ? 0 : left < p.share ? left : p.share);
 
-  Loads<T, S::TM, S::KT, true, S::NT> a;
-  Loads<T, S::TN, S::KT, true, S::NT> b;
-  constexpr int EACH = decltype(a)::kEach;
-  int64_t row[EACH];  // of the chunks that the next load takes
-  auto look = [&](int k0) {
-#pragma unroll
-    for (int n = 0; n < EACH; ++n) {
-      const int k = k0 + A::line_of(n * S::NT + int(threadIdx.x));
-      row[n] = k < live ? row_at(p.order, row0 + k, p.rows) : -1;
-    }
-  };
-  auto load = [&](int k0) {
-    a.load([&](int, int c, int n) { return row[n] >= 0 ? p.a + row[n] * p.a_row + m0 + c : nullptr; },
-           [&](int c) { return p.M - m0 - c; });
-    b.load([&](int, int c, int n) { return row[n] >= 0 ? p.b + row[n] * p.b_row + n0 + c : nullptr; },
-           [&](int c) { return p.N - n0 - c; });
-    look(k0 + S::KT);
-  };
-  auto tile_a = [&](int t) { return reinterpret_cast<__bf16*>(lds + (S::BUFFERS == 2 ? t & 1 : 0) * STEP); };
-  auto tile_b = [&](int t) { return reinterpret_cast<__bf16*>(lds + (S::BUFFERS == 2 ? t & 1 : 0) * STEP + A::kBytes); };
-
+  auto tile_a = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP); };
+  auto tile_b = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP + A::kBytes); };
   f32x16 sum[S::FM][S::FN];
 #pragma unroll
   for (int i = 0; i < S::FM; ++i)
@@ -67,33 +48,72 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
   float column[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) column[q] = 0.0f;
+  auto add_columns = [&](int t) {
+    if (!summing) return;
+    const __bf16* from = p.sums_of_a ? tile_a(t) : tile_b(t);
+    const int c = int(threadIdx.x) % ACROSS;
+    for (int k = int(threadIdx.x) / ACROSS; k < S::KT; k += DOWN) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+#pragma unroll
+      for (int n = kParts<T> - 1; n >= 0; --n) {
+        const bf16x8 part = *reinterpret_cast<const bf16x8*>(from + n * A::kValues + k * S::TM + (c ^ turn<__bf16, S::TM>(k)) * 8);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += float(part[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) column[q] += v[q];
+    }
+  };
 
   const int steps = (live + S::KT - 1) / S::KT;
+  // rows of this thread's chunks, the same for both operands, of the tile that is loaded next; -1: none
+  constexpr int EACH = (A::kChunks + S::NT - 1) / S::NT;
+  int64_t row[EACH];
+  auto look = [&](int t) {
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const int k = t * S::KT + A::line_of(n * S::NT + int(threadIdx.x));
+      row[n] = k < live ? row_at(p.order, row0 + k, p.rows) : -1;
+    }
+  };
   look(0);
-  if (steps) load(0);
-  for (int t = 0; t < steps; ++t) {
-    if (S::BUFFERS == 1 && t) __syncthreads();  // the last tile has been used
-    a.put(tile_a(t));
-    b.put(tile_b(t));
-    if (t + 1 < steps) load((t + 1) * S::KT);
-    __syncthreads();
-    multiply_tiles<T, S, A, B>(tile_a(t), tile_b(t), wm, wn, wk, lane, sum);
-    if (summing) {
-      const __bf16* from = p.sums_of_a ? tile_a(t) : tile_b(t);
-      const int c = int(threadIdx.x) % ACROSS;
-      for (int k = int(threadIdx.x) / ACROSS; k < S::KT; k += DOWN) {
-        float v[8];
+  if constexpr (DIRECT) {
+    // Columns past the weight's repeat others: their results go nowhere.
+    DirectLoads<S::TM, S::KT, true, S::NT> a;
+    DirectLoads<S::TN, S::KT, true, S::NT> b;
+    static_assert(decltype(a)::kEach == EACH, "both operands' chunks are of the same rows");
+    auto load = [&](int t, auto part, auto parts) {
+      constexpr int P = decltype(part)::value, OF = decltype(parts)::value;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
-#pragma unroll
-        for (int n = kParts<T> - 1; n >= 0; --n) {
-          const bf16x8 part = *reinterpret_cast<const bf16x8*>(from + n * A::kValues + k * S::TM + (c ^ turn<__bf16, S::TM>(k)) * 8);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] += float(part[q]);
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) column[q] += v[q];
+      for (int n = EACH * P / OF; n < EACH * (P + 1) / OF; ++n) {
+        const int c = a.column_of(n);
+        a.load(tile_a(t), n, wave, row[n] < 0 ? a.none() : p.a + row[n] * p.a_row + (m0 + c < p.M ? m0 + c : 0));
+        b.load(tile_b(t), n, wave, row[n] < 0 ? b.none() : p.b + row[n] * p.b_row + (n0 + c < p.N ? n0 + c : 0));
       }
+      if (P + 1 == OF) look(t + 1);
+    };
+    multiply_direct<S, A, B, 2 * EACH>(steps, tile_a, tile_b, wm, wn, wk, lane, load, add_columns, sum);
+  } else {
+    Loads<T, S::TM, S::KT, true, S::NT> a;
+    Loads<T, S::TN, S::KT, true, S::NT> b;
+    auto load = [&](int t) {
+      a.load([&](int, int c, int n) { return row[n] >= 0 ? p.a + row[n] * p.a_row + m0 + c : nullptr; },
+             [&](int c) { return p.M - m0 - c; });
+      b.load([&](int, int c, int n) { return row[n] >= 0 ? p.b + row[n] * p.b_row + n0 + c : nullptr; },
+             [&](int c) { return p.N - n0 - c; });
+      look(t + 1);
+    };
+    if (steps) load(0);
+    for (int t = 0; t < steps; ++t) {
+      if (S::BUFFERS == 1 && t) __syncthreads();  // the last tile has been used
+      a.put(tile_a(t));
+      b.put(tile_b(t));
+      if (t + 1 < steps) load(t + 1);
+      __syncthreads();
+      multiply_tiles<T, S, A, B>(tile_a(t), tile_b(t), wm, wn, wk, lane, sum);
+      add_columns(t);
     }
   }
   __syncthreads();
@@ -122,7 +142,7 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
     }
     __syncthreads();
   }
-  give_out<S>(lds, sum, wm, wn, wk, lane, [&](int r, int c, float* v) {
+  auto finish = [&](int r, int c, float* v) {
     const int m = m0 + r, n = n0 + c, most = p.N - n;
     if (m >= p.M || most <= 0) return;
     if (kParts<T> == 3 && any_not_finite(v)) {
@@ -142,7 +162,9 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
       for (int q = 0; q < 8; ++q) out.v[q] = v[q];
       out.store(p.part + (part * p.M + m) * p.N + n, most);
     }
-  });
+  };
+  if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);
+  else give_out<S>(lds, sum, wm, wn, wk, lane, finish);
 }
 
 // Adds the sums of the shares of each group that has several, in order; the workgroups behind those of the
@@ -184,6 +206,7 @@ template <>
 struct Shapes<__bf16> {
   typedef Shape<2, 2, 1, 2, 2, 64, 2, 2> Large;
   typedef Shape<2, 2, 1, 1, 1, 64, 2, 4> Middle;
+  typedef Shape<2, 4, 1, 4, 2, 64, 2, 2> Square;
 };
 template <>
 struct Shapes<float> {
@@ -191,10 +214,20 @@ struct Shapes<float> {
   typedef Shape<2, 2, 1, 1, 1, 32, 1, 3> Middle;
 };
 
-// Tiles of 128 x 128, or of 64 x 64 for narrow weights
-inline bool narrow(int64_t M, int64_t N) { return M <= 64 || N <= 64; }
+// Whether every chunk of eight values of both operands is whole and aligned
+template <typename T>
+bool direct(const WeightProduct<T>& p) {
+  return (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0 && p.M % 8 == 0 &&
+         p.N % 8 == 0 && p.a_row % 8 == 0 && p.b_row % 8 == 0;
+}
 
-template <typename T, typename S>
+// Tiles of 256 x 256 for wide weights of direct loads, of 64 x 64 for narrow ones, else of 128 x 128
+enum WeightTile { kMiddleTile = 64, kLargeTile = 128, kSquareTile = 256 };
+inline WeightTile tile_for(int64_t M, int64_t N, bool direct) {
+  return M <= 64 || N <= 64 ? kMiddleTile : direct && M >= 512 && N >= 512 ? kSquareTile : kLargeTile;
+}
+
+template <typename T, typename S, bool DIRECT = false>
 int launch_shaped(WeightProduct<T> p, hipStream_t s) {
   p.tiles_m = p.M ? unsigned((p.M + S::TM - 1) / S::TM) : 1;  // no rows or columns: there may be sums
   p.tiles_n = p.N ? unsigned((p.N + S::TN - 1) / S::TN) : 1;
@@ -203,16 +236,16 @@ int launch_shaped(WeightProduct<T> p, hipStream_t s) {
   if (!fits_grid(groups, S::NT))
     return set_error(YE3T_EUNSUPPORTED, "weights of %d x %d for %lld species are too many for one launch", p.M, p.N,
                      (long long)p.groups);
-  hipLaunchKernelGGL((weight_product_kernel<T, S>), dim3(unsigned(groups)), dim3(S::NT), 0, s, p);
+  hipLaunchKernelGGL((weight_product_kernel<T, S, DIRECT>), dim3(unsigned(groups)), dim3(S::NT), 0, s, p);
   return check_launch("weight_product_kernel");
 }
 
 }  // namespace
 
-// Shares that give the card about four workgroups a compute unit, of 512 rows or more
-SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N) {
+// Shares that give the card about four workgroups a compute unit, one of tiles of 256 x 256, of 512 rows or more
+SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N, bool direct) {
   SharePlan f{};
-  const int64_t t = narrow(M, N) ? 64 : 128, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
+  const int64_t t = tile_for(M, N, direct), tiles = ((M + t - 1) / t) * ((N + t - 1) / t) * (t == kSquareTile ? 4 : 1);
   const int64_t parts = tiles == 0 ? 1024 : tiles < 1024 ? 1024 / tiles : 1;
   f.share = (rows + parts - 1) / parts;
   if (f.share < 512) f.share = 512;
@@ -225,12 +258,36 @@ SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N) {
 }
 
 template <typename T>
+SharePlan share_plan(const WeightProduct<T>& p) {
+  return share_plan(p.rows, p.grouped ? p.groups : 1, p.M, p.N, sizeof(T) == 2 && direct(p));
+}
+template <typename T>
+int64_t most_share_bytes(WeightProduct<T> p) {
+  const int64_t groups = p.grouped ? p.groups : 1;
+  const int64_t some = share_plan(p.rows, groups, p.M, p.N, false).bytes, direct = share_plan(p.rows, groups, p.M, p.N, sizeof(T) == 2).bytes;
+  return some > direct ? some : direct;
+}
+template int64_t most_share_bytes(WeightProduct<float>);
+template int64_t most_share_bytes(WeightProduct<__bf16>);
+template SharePlan share_plan(const WeightProduct<float>&);
+template SharePlan share_plan(const WeightProduct<__bf16>&);
+
+template <typename T>
 int launch_weights(WeightProduct<T> p, hipStream_t s) {
   const int64_t groups = p.grouped ? p.groups : 1;
   if (groups == 0 || ((p.M == 0 || p.N == 0) && !p.sums)) return YE3T_OK;
-  if (int rc = narrow(p.M, p.N) ? launch_shaped<T, typename Shapes<T>::Middle>(p, s)
-                                : launch_shaped<T, typename Shapes<T>::Large>(p, s))
-    return rc;
+  const WeightTile tile = tile_for(p.M, p.N, sizeof(T) == 2 && direct(p));
+  int rc = YE3T_OK;
+  if constexpr (sizeof(T) == 2) {
+    rc = tile == kSquareTile   ? launch_shaped<T, typename Shapes<T>::Square, true>(p, s)
+         : tile == kLargeTile  ? direct(p) ? launch_shaped<T, typename Shapes<T>::Large, true>(p, s)
+                                           : launch_shaped<T, typename Shapes<T>::Large>(p, s)
+                               : launch_shaped<T, typename Shapes<T>::Middle>(p, s);
+  } else {
+    rc = tile == kLargeTile ? launch_shaped<T, typename Shapes<T>::Large>(p, s)
+                            : launch_shaped<T, typename Shapes<T>::Middle>(p, s);
+  }
+  if (rc) return rc;
   if (p.rows <= p.share) return YE3T_OK;
   const int64_t per = kJoinThreads * 8, product = (int64_t(p.M) * p.N + per - 1) / per;
   const int64_t column = p.sums ? ((p.sums_of_a ? p.M : p.N) + per - 1) / per : 0;
