@@ -975,9 +975,15 @@ typedef struct {
   const int64_t* device_seed; /* NULL, or one value in device memory that is taken instead of `seed` */
 } ye3t_linear_args;
 
+/* Device workspace bytes of ye3t_hip_linear (0 where it needs none; -1 on
+ * invalid input). */
+int64_t ye3t_hip_linear_workspace_bytes(const ye3t_linear_args* args);
+
 /* out [rows, outputs] and, if not NULL, preactivation [rows, outputs] = x W + b,
- * rounded, which the gradient of an activation takes. */
-int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out, ye3t_stream_t stream);
+ * rounded, which the gradient of an activation takes.  A long contraction of few
+ * rows is split among workgroups and joined. */
+int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out, void* workspace,
+                    int64_t workspace_bytes, ye3t_stream_t stream);
 
 /* Device workspace bytes of ye3t_hip_linear_adjoint (-1 on invalid input). */
 int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args);

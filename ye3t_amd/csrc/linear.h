@@ -57,11 +57,18 @@ __device__ inline Normal normal_of(float z) {
   return {z < 0.0f ? tail : 1.0f - tail, bell};
 }
 
-__device__ inline float activated(int act, float z) {
-  if (act == kRelu) return z <= 0.0f ? 0.0f : z;
-  if (act == kSilu) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
-  if (act == kGelu) return z * normal_of(z).phi;
-  return z;
+// Eight values; the choice is made once for them.
+__device__ inline void activate(int act, float* v) {
+  if (act == kRelu) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = v[q] <= 0.0f ? 0.0f : v[q];
+  } else if (act == kSilu) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = v[q] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v[q]));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = v[q] * normal_of(v[q]).phi;
+  }
 }
 
 __device__ inline float slope_of(int act, float z) {
@@ -315,11 +322,11 @@ __device__ inline void multiply_direct(int steps, TileA tile_a, TileB tile_b, in
 }
 
 // Passes the wave's squares through LDS and gives them out eight columns of a row at a time, so that memory
-// is read and written along rows: use(row, column, values) of the workgroup's tile.  The
+// is read and written along rows: use(rows, columns, values) of some chunks of the workgroup's tile.  The
 // shares of the contraction are added in order.
 template <typename S, typename F>
 __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, int wn, int wk, int lane, F use) {
-  constexpr int CHUNKS = S::FN * 4, STRIDE = S::kOutRow, BLOCK = 32 * STRIDE;
+  constexpr int CHUNKS = S::FN * 4, STRIDE = S::kOutRow, BLOCK = 32 * STRIDE, EACH = 32 * CHUNKS / 64;
   const int wave = (wk * S::WM + wm) * S::WN + wn;
   float* own = reinterpret_cast<float*>(lds) + wave * BLOCK;
   repeat<S::FM>([&](auto number) {
@@ -333,31 +340,34 @@ __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, i
         for (int q = 0; q < 4; ++q) v[q] = sum[i][j][4 * b + q];
         *reinterpret_cast<f32x4*>(own + (lane & 31) * STRIDE + 32 * j + 8 * b + 4 * (lane / 32)) = v;
       }
-    if (S::WK == 1) {
+    if constexpr (S::WK == 1) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
+      int r[EACH], c[EACH];
+      float v[EACH][8];
 #pragma unroll
-      for (int n = 0; n < 32 * CHUNKS / 64; ++n) {
-        const int r = n * (64 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS * 8;
-        float v[8];
+      for (int n = 0; n < EACH; ++n) {
+        const int x = n * 64 + lane, row = x / CHUNKS, column = x % CHUNKS * 8;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = own[r * STRIDE + c + q];
-        use((wm * S::FM + i) * 32 + r, wn * S::FN * 32 + c, v);
+        for (int q = 0; q < 8; ++q) v[n][q] = own[row * STRIDE + column + q];
+        r[n] = (wm * S::FM + i) * 32 + row;
+        c[n] = wn * S::FN * 32 + column;
       }
+      use(r, c, v);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     } else {
       static_assert(S::WK == 1 || (S::FM == 1 && S::WM == 1 && S::WN == 1), "shares of one wave's rows");
       __syncthreads();
       for (int x = int(threadIdx.x); x < 32 * CHUNKS; x += S::NT) {
-        const int r = x / CHUNKS, c = x % CHUNKS * 8;
-        float v[8];
+        int r[1] = {x / CHUNKS}, c[1] = {x % CHUNKS * 8};
+        float v[1][8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+        for (int q = 0; q < 8; ++q) v[0][q] = 0.0f;
 #pragma unroll
         for (int w = 0; w < S::WK; ++w)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] += reinterpret_cast<const float*>(lds)[w * BLOCK + r * STRIDE + c + q];
+          for (int q = 0; q < 8; ++q) v[0][q] += reinterpret_cast<const float*>(lds)[w * BLOCK + r[0] * STRIDE + c[0] + q];
         use(r, c, v);
       }
     }
@@ -365,27 +375,28 @@ __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, i
 }
 
 // The same without LDS: the halves of the wave exchange what makes eight columns of a lane's row whole.
-// use(row, column, values)
 template <typename S, typename F>
 __device__ inline void hand_out(const f32x16 (*sum)[S::FN], int wm, int wn, int lane, F use) {
   const int half = lane / 32;
   repeat<S::FM>([&](auto number) {
-    constexpr int i = decltype(number)::value;
+    constexpr int i = decltype(number)::value, EACH = 2 * S::FN;
+    int r[EACH], c[EACH];
+    float v[EACH][8];
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j)
+    for (int n = 0; n < EACH; ++n) {
+      const int j = n / 2, b = n % 2 * 2;
 #pragma unroll
-      for (int b = 0; b < 4; b += 2) {
-        float v[8];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, float(sum[i][j][4 * b + q])),
-                                                             __builtin_bit_cast(unsigned, float(sum[i][j][4 * b + 4 + q])),
-                                                             false, false);
-          v[q] = __builtin_bit_cast(float, unsigned(both[0]));
-          v[4 + q] = __builtin_bit_cast(float, unsigned(both[1]));
-        }
-        use((wm * S::FM + i) * 32 + (lane & 31), (wn * S::FN + j) * 32 + 8 * (b + half), v);
+      for (int q = 0; q < 4; ++q) {
+        const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, float(sum[i][j][4 * b + q])),
+                                                           __builtin_bit_cast(unsigned, float(sum[i][j][4 * b + 4 + q])),
+                                                           false, false);
+        v[n][q] = __builtin_bit_cast(float, unsigned(both[0]));
+        v[n][4 + q] = __builtin_bit_cast(float, unsigned(both[1]));
       }
+      r[n] = (wm * S::FM + i) * 32 + (lane & 31);
+      c[n] = (wn * S::FN + j) * 32 + 8 * (b + half);
+    }
+    use(r, c, v);
   });
 }
 
@@ -455,6 +466,8 @@ struct RowProduct {
   int activation;
   Dropout dropout;
   unsigned tiles_n;
+  int parts, part_steps;   // parts of the contraction, and steps of each where there are several
+  float* part;             // their sums, [parts][rows][N], rows in the order
 };
 
 // out_g[m, n] = sum over the group's rows i of a[i, m] b[i, n], and column sums of one of the two
@@ -476,8 +489,11 @@ struct WeightProduct {
   unsigned tiles_m, tiles_n;
 };
 
+// Bytes of device memory that a product takes beside its operands, and the product
 template <typename T>
-int launch_rows(RowProduct<T> p, hipStream_t s);
+int64_t row_bytes(const RowProduct<T>& p);
+template <typename T>
+int launch_rows(RowProduct<T> p, void* work, hipStream_t s);
 template <typename T>
 int launch_weights(WeightProduct<T> p, hipStream_t s);
 

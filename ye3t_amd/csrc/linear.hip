@@ -73,7 +73,7 @@ RowProduct<T> rows_of(const ye3t_linear_args& a) {
 }
 
 template <typename T>
-int forward_as(const ye3t_linear_args& a, void* kept, void* out, hipStream_t s) {
+RowProduct<T> forward_of(const ye3t_linear_args& a) {
   RowProduct<T> p = rows_of<T>(a);
   p.a = static_cast<const T*>(a.input);
   p.a_row = a.input_row_stride;
@@ -82,11 +82,33 @@ int forward_as(const ye3t_linear_args& a, void* kept, void* out, hipStream_t s) 
   p.N = int(a.outputs);
   p.bias = static_cast<const T*>(a.bias);
   p.residual = static_cast<const T*>(a.residual);
-  p.kept = static_cast<T*>(kept);
-  p.out = static_cast<T*>(out);
   p.activation = a.activation;
   p.dropout = dropout_of(a.drop_below, a.layer, a.seed, a.device_seed);
-  return launch_rows(p, s);
+  return p;
+}
+
+// dx = dz W^T
+template <typename T>
+RowProduct<T> backward_of(const ye3t_linear_args& a, const T* dz) {
+  RowProduct<T> p = rows_of<T>(a);
+  p.a = dz;
+  p.a_row = a.outputs;
+  p.b_across = a.turned != 0;
+  p.K = int(a.outputs);
+  p.N = int(a.inputs);
+  return p;
+}
+
+template <typename T>
+int forward_as(const ye3t_linear_args& a, void* kept, void* out, void* work, hipStream_t s) {
+  RowProduct<T> p = forward_of<T>(a);
+  p.kept = static_cast<T*>(kept);
+  p.out = static_cast<T*>(out);
+  return launch_rows(p, work, s);
+}
+
+int64_t forward_bytes(const ye3t_linear_args& a) {
+  return a.dtype == YE3T_F32 ? row_bytes(forward_of<float>(a)) : row_bytes(forward_of<__bf16>(a));
 }
 
 inline bool shaped(const ye3t_linear_args& a) { return a.activation != kNone || a.drop_below > 0; }
@@ -115,10 +137,13 @@ WeightProduct<T> weights_of(const ye3t_linear_args& a, const T* dz) {
 int64_t dz_bytes(const ye3t_linear_args& a) {
   return shaped(a) ? up(a.rows * a.outputs * (a.dtype == YE3T_F32 ? 4 : 2)) : 0;
 }
+// dx and dW are made one after the other: what one takes for its parts the other takes after it.
 int64_t adjoint_bytes(const ye3t_linear_args& a) {
+  const int64_t parts = a.dtype == YE3T_F32 ? row_bytes(backward_of<float>(a, nullptr))
+                                            : row_bytes(backward_of<__bf16>(a, nullptr));
   const int64_t shares = a.dtype == YE3T_F32 ? most_share_bytes(weights_of<float>(a, nullptr))
                                              : most_share_bytes(weights_of<__bf16>(a, nullptr));
-  return dz_bytes(a) + shares + 256;
+  return dz_bytes(a) + (shares > parts ? shares : parts) + 256;
 }
 
 template <typename T>
@@ -137,14 +162,9 @@ int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept,
     dz = to;
   }
   if (input_adjoint) {
-    RowProduct<T> p = rows_of<T>(a);
-    p.a = dz;
-    p.a_row = a.outputs;
-    p.b_across = a.turned != 0;
-    p.K = int(a.outputs);
-    p.N = int(a.inputs);
+    RowProduct<T> p = backward_of(a, dz);
     p.out = static_cast<T*>(input_adjoint);
-    if (int rc = launch_rows(p, s)) return rc;
+    if (int rc = launch_rows(p, work + dz_bytes(a), s)) return rc;
   }
   if (weight_adjoint) {
     WeightProduct<T> p = weights_of<T>(a, dz);
@@ -167,15 +187,27 @@ using namespace ye3t;
 
 extern "C" {
 
-int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out, ye3t_stream_t stream) {
+int64_t ye3t_hip_linear_workspace_bytes(const ye3t_linear_args* args) {
+  clear_error();
+  if (!args) return set_error(YE3T_EINVAL, "the product needs its arguments");
+  if (linear::check_linear(*args)) return -1;
+  return linear::forward_bytes(*args);
+}
+
+int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out, void* workspace,
+                    int64_t workspace_bytes, ye3t_stream_t stream) {
   clear_error();
   YE3T_REQUIRE(args, "the product needs its arguments");
   if (int rc = linear::check_linear(*args)) return rc;
   if (args->rows == 0 || args->outputs == 0) return YE3T_OK;
   if (int rc = linear::check_pointers(*args)) return rc;
   YE3T_REQUIRE(out, "the product needs an output");
-  return args->dtype == YE3T_F32 ? linear::forward_as<float>(*args, preactivation, out, as_stream(stream))
-                                 : linear::forward_as<__bf16>(*args, preactivation, out, as_stream(stream));
+  const int64_t bytes = linear::forward_bytes(*args);
+  YE3T_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes),
+               "the workspace is smaller than ye3t_hip_linear_workspace_bytes");
+  return args->dtype == YE3T_F32
+             ? linear::forward_as<float>(*args, preactivation, out, workspace, as_stream(stream))
+             : linear::forward_as<__bf16>(*args, preactivation, out, workspace, as_stream(stream));
 }
 
 int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args) {

@@ -5,6 +5,54 @@ namespace ye3t {
 namespace linear {
 namespace {
 
+// What follows the sums: some chunks of a lane, row (-1: none) and column of each.  What they need is loaded together.
+template <typename T, int EACH>
+__device__ inline void epilogue(const RowProduct<T>& p, const T* weight, const T* bias, uint64_t seed, int K,
+                                const int64_t (&row)[EACH], const int (&n)[EACH], float (&v)[EACH][8]) {
+  int64_t at[EACH];
+  int left[EACH];
+  Chunk<T, 8> offset[EACH], more[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    left[e] = row[e] < 0 ? 0 : p.N - n[e];
+    at[e] = row[e] * p.N + n[e];
+    if (left[e] <= 0) continue;
+    if (bias) offset[e] = Chunk<T, 8>::load(bias + n[e], left[e]);
+    if (p.residual) more[e] = Chunk<T, 8>::load(p.residual + at[e], left[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (left[e] <= 0) continue;
+    if (kParts<T> == 3 && any_not_finite(v[e])) {
+      const T* x = p.a + row[e] * p.a_row;
+      const int64_t k_step = p.b_across ? p.b_row : 1, n_step = p.b_across ? 1 : p.b_row;
+      for (int q = 0; q < 8 && q < left[e]; ++q) {
+        const T* w = weight + (n[e] + q) * n_step;
+        v[e][q] = exact_dot([&](int64_t k) { return float(x[k]); }, [&](int64_t k) { return float(w[k * k_step]); }, K);
+      }
+    }
+    if (bias) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[e][q] += float(offset[e].v[q]);
+    }
+    Chunk<T, 8> out;
+    if (p.kept) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) out.v[q] = T(v[e][q]);
+      out.store(p.kept + at[e], left[e]);
+    }
+    if (p.activation != kNone) activate(p.activation, v[e]);
+    if (p.dropout.below) drop(p.dropout, seed, row[e], uint32_t(n[e]) / 8, v[e]);
+    if (p.residual) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[e][q] += float(more[e].v[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) out.v[q] = T(v[e][q]);
+    out.store(p.out + at[e], left[e]);
+  }
+}
+
 template <typename T, typename S, bool ACROSS, bool DIRECT>
 __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const RowProduct<T> p) {
   typedef Tile<T, S::TM, S::KT, false> A;
@@ -39,7 +87,13 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
   for (int i = 0; i < S::FM; ++i)
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) sum[i][j] = zeros();
-  const int steps = (K + S::KT - 1) / S::KT;
+  int steps = (K + S::KT - 1) / S::KT, begin_step = 0;
+  if constexpr (S::WK > 1) {
+    if (p.parts > 1) {  // this workgroup's part of the contraction
+      begin_step = int(blockIdx.y) * p.part_steps;
+      steps = steps - begin_step < p.part_steps ? (steps > begin_step ? steps - begin_step : 0) : p.part_steps;
+    }
+  }
   auto tile_a = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP); };
   auto tile_b = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP + A::kBytes); };
   if constexpr (DIRECT) {
@@ -100,59 +154,78 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
         b.load([&](int n, int c, int) { return n0 + n < p.N ? weight + int64_t(n0 + n) * p.b_row + k0 + c : nullptr; },
                [&](int c) { return K - k0 - c; });
     };
-    if (steps) load(0);
+    if (steps) load(begin_step * S::KT);
     for (int t = 0; t < steps; ++t) {
       if (S::BUFFERS == 1 && t) __syncthreads();  // the last tile has been used
       a.put(tile_a(t));
       b.put(tile_b(t));
-      if (t + 1 < steps) load((t + 1) * S::KT);
+      if (t + 1 < steps) load((begin_step + t + 1) * S::KT);
       __syncthreads();
       multiply_tiles<T, S, A, B>(tile_a(t), tile_b(t), wm, wn, wk, lane, sum);
     }
     __syncthreads();
   }
 
+  if constexpr (S::WK > 1) {
+    if (p.parts > 1) {
+      give_out<S>(lds, sum, wm, wn, wk, lane, [&](const auto& r, const auto& c, auto& v) {
+        const int left = p.N - n0 - c[0];
+        if (r[0] >= live || left <= 0) return;
+        Chunk<float, 8> out;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) out.v[q] = v[0][q];
+        out.store(p.part + (blockIdx.y * p.rows + row0 + r[0]) * p.N + n0 + c[0], left);
+      });
+      return;
+    }
+  }
   const uint64_t seed = p.dropout.below ? seed_of(p.dropout) : 0;
-  auto finish = [&](int r, int c, float* v) {
-    const int n = n0 + c, left = p.N - n;
-    if (r >= live || left <= 0) return;
-    const int64_t row = row_at(p.order, row0 + r, p.rows);
-    if (row < 0) return;
-    if (kParts<T> == 3 && any_not_finite(v)) {
-      for (int q = 0; q < 8 && q < left; ++q) {
-        const int64_t k_step = ACROSS ? p.b_row : 1, n_step = ACROSS ? 1 : p.b_row;
-        const T *x = p.a + row * p.a_row, *w = weight + (n + q) * n_step;
-        v[q] = exact_dot([&](int64_t k) { return float(x[k]); }, [&](int64_t k) { return float(w[k * k_step]); }, K);
-      }
-    }
-    if (p.bias && !(p.grouped && group == p.groups)) {
-      const Chunk<T, 8> bias = Chunk<T, 8>::load(p.bias + group * p.N + n, left);
+  const T* bias = p.bias && !(p.grouped && group == p.groups) ? p.bias + group * p.N : nullptr;
+  auto finish = [&](const auto& r, const auto& c, auto& v) {
+    constexpr int EACH = sizeof(v) / sizeof(v[0]);
+    int64_t row[EACH];
+    int n[EACH];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] += float(bias.v[q]);
+    for (int e = 0; e < EACH; ++e) {
+      row[e] = r[e] < live ? row_at(p.order, row0 + r[e], p.rows) : -1;
+      n[e] = n0 + c[e];
     }
-    const int64_t at = row * p.N + n;
-    Chunk<T, 8> out;
-    if (p.kept) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) out.v[q] = T(v[q]);
-      out.store(p.kept + at, left);
-    }
-    if (p.activation != kNone) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = activated(p.activation, v[q]);
-    }
-    if (p.dropout.below) drop(p.dropout, seed, row, uint32_t(n) / 8, v);
-    if (p.residual) {
-      const Chunk<T, 8> more = Chunk<T, 8>::load(p.residual + at, left);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] += float(more.v[q]);
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) out.v[q] = T(v[q]);
-    out.store(p.out + at, left);
+    epilogue(p, weight, bias, seed, K, row, n, v);
   };
   if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);
   else give_out<S>(lds, sum, wm, wn, wk, lane, finish);
+}
+
+// Adds the parts of the contraction in order and goes on as the product's own epilogue.  A lane a chunk of eight columns.
+constexpr int kJoinThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void row_join_kernel(const RowProduct<T> p, int chunks) {
+  const int64_t x = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, i = x / chunks;
+  if (i >= p.rows) return;
+  int64_t row[1] = {row_at(p.order, i, p.rows)}, group = 0;
+  int n[1] = {int(x - i * chunks) * 8};
+  if (p.grouped) {  // the group of row i: the number of offsets behind the first that are not above it
+    int64_t lo = 0, hi = p.groups;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (p.offsets[mid + 1] <= i) lo = mid + 1;
+      else hi = mid;
+    }
+    group = lo;
+  }
+  const bool none = p.grouped && group == p.groups;
+  const int left = p.N - n[0];
+  float v[1][8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[0][q] = 0.0f;
+#pragma unroll 4
+  for (int k = 0; k < p.parts; ++k) {
+    const Chunk<float, 8> a = Chunk<float, 8>::load(p.part + (k * p.rows + i) * p.N + n[0], left);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[0][q] += a.v[q];
+  }
+  epilogue(p, p.b + group * p.b_group, p.bias && !none ? p.bias + group * p.N : nullptr,
+           p.dropout.below ? seed_of(p.dropout) : 0, none ? 0 : p.K, row, n, v);
 }
 
 template <typename T, typename S, bool DIRECT = false>
@@ -162,8 +235,13 @@ int launch_shaped(RowProduct<T> p, hipStream_t s) {
   if (!fits_grid(items * p.tiles_n, S::NT))
     return set_error(YE3T_EUNSUPPORTED, "%lld rows of %d columns are too many for one launch", (long long)p.rows, p.N);
   hipLaunchKernelGGL((p.b_across ? row_product_kernel<T, S, true, DIRECT> : row_product_kernel<T, S, false, DIRECT>),
-                     dim3(unsigned(items * p.tiles_n)), dim3(S::NT), 0, s, p);
-  return check_launch("row_product_kernel");
+                     dim3(unsigned(items * p.tiles_n), unsigned(p.parts)), dim3(S::NT), 0, s, p);
+  if (int rc = check_launch("row_product_kernel")) return rc;
+  if (p.parts == 1) return YE3T_OK;
+  const int64_t chunks = (p.N + 7) / 8;
+  hipLaunchKernelGGL((row_join_kernel<T>), dim3(unsigned((p.rows * chunks + kJoinThreads - 1) / kJoinThreads)),
+                     dim3(kJoinThreads), 0, s, p, int(chunks));
+  return check_launch("row_join_kernel");
 }
 
 template <typename T>
@@ -174,6 +252,7 @@ struct Shapes<__bf16> {
   typedef Shape<2, 2, 1, 1, 1, 64, 2, 4> Middle;
   typedef Shape<1, 1, 8, 1, 1, 64, 1, 2> Few;
   typedef Shape<2, 4, 1, 4, 2, 64, 2, 2> Square;
+  typedef Shape<2, 2, 1, 2, 2, 32, 3, 3> Direct;
 };
 template <>
 struct Shapes<float> {
@@ -189,27 +268,64 @@ bool direct(const RowProduct<T>& p) {
          p.a_row % 8 == 0 && p.b_row % 8 == 0 && p.b_group % 8 == 0 && (!p.b_across || p.N % 8 == 0);
 }
 
+// Which shape a product takes, and in how many parts of the contraction
+enum Kind { kFew, kMiddle, kLarge, kDirect, kSquare };
+struct Choice {
+  Kind kind;
+  int parts, part_steps;
+};
+template <typename T>
+Choice choice_of(const RowProduct<T>& p, bool direct) {
+  auto tiles = [&](int64_t t) { return ((p.rows + t - 1) / t + (p.grouped ? p.groups : 0)) * ((p.N + t - 1) / t); };
+  if (direct && p.rows > 64) {
+    // Direct loads: tiles of 256 x 256 read half of what those of 128 x 128 do, but one workgroup fills a compute unit
+    // and nothing hides how it begins and ends, nor a last round that is not full.  65 536 x 2 048 x 2 048: 609 us, by
+    // tiles of 128 x 128 767; 40 000 x 512 x 1 024 76 and 64; 40 000 x 2 048 x 512 (1.2 rounds) 116 and 104.
+    const int64_t wide = tiles(256);
+    if (p.K >= 1024 && wide * 4 >= (wide + 255) / 256 * 256 * 3) return {kSquare, 1, 0};
+    if (tiles(128) >= 256) return {kDirect, 1, 0};
+  }
+  // Tiles of 128 x 128 where they give every compute unit one, of 64 x 64 where those do, else of 32 x 32 with the
+  // contraction shared by eight waves, and by several workgroups where it is long and they are few.
+  if (p.rows > 64 && tiles(128) >= 256) return {kLarge, 1, 0};
+  if (p.rows > 32 && tiles(64) >= 256) return {kMiddle, 1, 0};
+  const int64_t groups = ((p.rows + 31) / 32 + (p.grouped ? p.groups : 0)) * ((p.N + 31) / 32);
+  const int steps = (p.K + Shapes<T>::Few::KT - 1) / Shapes<T>::Few::KT;
+  if (steps < 4 || groups > 256) return {kFew, 1, 0};
+  int parts = int(512 / groups);
+  if (parts > steps / 2) parts = steps / 2;
+  const int each = (steps + parts - 1) / parts;
+  return {kFew, (steps + each - 1) / each, each};
+}
+
 }  // namespace
 
 template <typename T>
-int launch_rows(RowProduct<T> p, hipStream_t s) {
+int64_t row_bytes(const RowProduct<T>& p) {
+  if (p.rows == 0 || p.N == 0) return 0;
+  const Choice c = choice_of(p, false);  // direct or not, it is the last choice that has parts
+  return c.parts > 1 ? up(c.parts * p.rows * p.N * 4) : 0;
+}
+
+template <typename T>
+int launch_rows(RowProduct<T> p, void* work, hipStream_t s) {
   if (p.rows == 0 || p.N == 0) return YE3T_OK;
-  auto tiles = [&](int64_t t) { return ((p.rows + t - 1) / t + (p.grouped ? p.groups : 0)) * ((p.N + t - 1) / t); };
+  const Choice c = choice_of(p, sizeof(T) == 2 && direct(p));
+  p.parts = c.parts;
+  p.part_steps = c.part_steps;
+  p.part = static_cast<float*>(work);
   if constexpr (sizeof(T) == 2) {
-    // Direct loads: tiles of 256 x 256 halve what is read, but one workgroup fills a compute unit, and nothing hides how
-    // it begins and ends.  40 000 x 512 x 1 024: 74 us, by tiles of 128 x 128 63; 16 384 x 1 024 x 4 096: 150 and 163.
-    if (direct(p) && p.K >= 1024 && p.rows > 64 && tiles(256) >= 256)
-      return launch_shaped<T, typename Shapes<T>::Square, true>(p, s);
-    if (direct(p) && p.rows > 64 && tiles(128) >= 256) return launch_shaped<T, typename Shapes<T>::Large, true>(p, s);
+    if (c.kind == kSquare) return launch_shaped<T, typename Shapes<T>::Square, true>(p, s);
+    if (c.kind == kDirect) return launch_shaped<T, typename Shapes<T>::Direct, true>(p, s);
   }
-  // tiles of 128 x 128 where they give every compute unit one, of 64 x 64 where those do, else of 32 x 32 with the
-  // contraction shared by eight waves
-  if (p.rows > 64 && tiles(128) >= 256) return launch_shaped<T, typename Shapes<T>::Large>(p, s);
-  if (p.rows > 32 && tiles(64) >= 256) return launch_shaped<T, typename Shapes<T>::Middle>(p, s);
+  if (c.kind == kLarge) return launch_shaped<T, typename Shapes<T>::Large>(p, s);
+  if (c.kind == kMiddle) return launch_shaped<T, typename Shapes<T>::Middle>(p, s);
   return launch_shaped<T, typename Shapes<T>::Few>(p, s);
 }
-template int launch_rows<float>(RowProduct<float>, hipStream_t);
-template int launch_rows<__bf16>(RowProduct<__bf16>, hipStream_t);
+template int64_t row_bytes(const RowProduct<float>&);
+template int64_t row_bytes(const RowProduct<__bf16>&);
+template int launch_rows<float>(RowProduct<float>, void*, hipStream_t);
+template int launch_rows<__bf16>(RowProduct<__bf16>, void*, hipStream_t);
 
 }  // namespace linear
 }  // namespace ye3t

@@ -142,25 +142,32 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
     }
     __syncthreads();
   }
-  auto finish = [&](int r, int c, float* v) {
-    const int m = m0 + r, n = n0 + c, most = p.N - n;
-    if (m >= p.M || most <= 0) return;
-    if (kParts<T> == 3 && any_not_finite(v)) {
-      for (int q = 0; q < 8 && q < most; ++q)
-        v[q] = exact_dot([&](int64_t k) { const int64_t i = row_at(p.order, row0 + k, p.rows); return i < 0 ? 0.0f : float(p.a[i * p.a_row + m]); },
-                         [&](int64_t k) { const int64_t i = row_at(p.order, row0 + k, p.rows); return i < 0 ? 0.0f : float(p.b[i * p.b_row + n + q]); },
-                         live);
-    }
-    if (whole) {
-      Chunk<T, 8> out;
+  auto finish = [&](const auto& r, const auto& c, auto& v) {
+    constexpr int EACH = sizeof(v) / sizeof(v[0]);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) out.v[q] = T(v[q]);
-      out.store(p.out + (group * p.M + m) * p.N + n, most);
-    } else {
-      Chunk<float, 8> out;
+    for (int e = 0; e < EACH; ++e) {
+      const int m = m0 + r[e], n = n0 + c[e], most = p.N - n;
+      if (m >= p.M || most <= 0) continue;
+      if (kParts<T> == 3 && any_not_finite(v[e])) {
+        auto value = [&](const T* from, int64_t step, int at, int64_t k) {
+          const int64_t i = row_at(p.order, row0 + k, p.rows);
+          return i < 0 ? 0.0f : float(from[i * step + at]);
+        };
+        for (int q = 0; q < 8 && q < most; ++q)
+          v[e][q] = exact_dot([&](int64_t k) { return value(p.a, p.a_row, m, k); },
+                              [&](int64_t k) { return value(p.b, p.b_row, n + q, k); }, live);
+      }
+      if (whole) {
+        Chunk<T, 8> out;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) out.v[q] = v[q];
-      out.store(p.part + (part * p.M + m) * p.N + n, most);
+        for (int q = 0; q < 8; ++q) out.v[q] = T(v[e][q]);
+        out.store(p.out + (group * p.M + m) * p.N + n, most);
+      } else {
+        Chunk<float, 8> out;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) out.v[q] = v[e][q];
+        out.store(p.part + (part * p.M + m) * p.N + n, most);
+      }
     }
   };
   if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);

@@ -28,6 +28,13 @@ struct Pair {
   uint32_t token, position;
 };
 
+// Where sorted positions go: as pairs, or (species.hip) something else.  begin(): the first place of each digit.
+struct Pairs {
+  Pair* out;
+  __device__ inline void put(uint32_t at, const Pair& p) const { out[at] = p; }
+  __device__ inline void begin(int, uint32_t) const {}
+};
+
 template <bool FIRST, typename Index>
 __device__ inline Pair pair_at(const Index* __restrict__ tokens, const Pair* __restrict__ pairs, int64_t i,
                                int64_t vocabulary) {
@@ -75,12 +82,12 @@ __global__ __launch_bounds__(kSortThreads) void digit_count_kernel(const Index* 
   if (threadIdx.x < kBins) counts[blockIdx.x * kBins + threadIdx.x] = bins[threadIdx.x];
 }
 
-template <bool FIRST, typename Index>
+template <bool FIRST, typename Index, typename Out>
 __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* __restrict__ tokens,
                                                                    const Pair* __restrict__ pairs, int64_t N,
                                                                    int64_t run, int64_t vocabulary, int shift,
                                                                    const uint32_t* __restrict__ counts,
-                                                                   Pair* __restrict__ out) {
+                                                                   const Out out) {
   constexpr int kWaves = kSortThreads / 64;
   __shared__ uint32_t next[kBins];            // where this run's next position of a digit goes
   __shared__ uint32_t of_wave[kWaves][kBins];  // a wave's count of a digit, then its place among the waves
@@ -122,6 +129,7 @@ __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* 
   if (t < kBins)
     for (int w = 0; w < wave; ++w) next[t] += wave_sums[w];
   __syncthreads();
+  if (blockIdx.x == 0 && t < kBins) out.begin(t, next[t]);
   const int64_t begin = int64_t(blockIdx.x) * run, end = begin + run < N ? begin + run : N;
   for (int64_t i0 = begin; i0 < end; i0 += kSortThreads) {
     for (int k = t; k < kWaves * kBins; k += kSortThreads) (&of_wave[0][0])[k] = 0;
@@ -135,7 +143,7 @@ __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* 
     __syncthreads();
     if (t < kBins) places_of_waves(of_wave, t, next[t]);
     __syncthreads();
-    if (live) out[of_wave[wave][digit] + rank] = p;
+    if (live) out.put(of_wave[wave][digit] + rank, p);
     __syncthreads();
   }
 }
@@ -145,10 +153,10 @@ __global__ __launch_bounds__(kSortThreads) void digit_place_kernel(const Index* 
 // and, once all counts are added up, places them by itself.
 constexpr int kSmallSort = 4096;
 
-template <typename Index>
+template <typename Index, typename Out>
 __global__ __launch_bounds__(kSortThreads) void small_sort_kernel(const Index* __restrict__ tokens, int N,
                                                                   int64_t vocabulary, int passes,
-                                                                  Pair* __restrict__ out) {
+                                                                  const Out out) {
   constexpr int kWaves = kSortThreads / 64;
   __shared__ Pair held[2][kSmallSort];
   __shared__ uint32_t of_wave[kWaves][kBins];
@@ -182,6 +190,7 @@ __global__ __launch_bounds__(kSortThreads) void small_sort_kernel(const Index* _
     if (t < kBins) {
       sum -= own;
       for (int w = 0; w < wave; ++w) sum += wave_sums[w];
+      if (pass + 1 == passes) out.begin(t, sum);
       places_of_waves(of_wave, t, sum);
     }
     __syncthreads();
@@ -196,7 +205,7 @@ __global__ __launch_bounds__(kSortThreads) void small_sort_kernel(const Index* _
       if (live && rank == 0) of_wave[wave][digit] = at + uint32_t(__popcll(same));
       __threadfence_block();
       if (live) {
-        if (pass + 1 == passes) out[at] = p;
+        if (pass + 1 == passes) out.put(at, p);
         else to[at] = p;
       }
     }
@@ -223,15 +232,22 @@ inline SortPlan sort_plan(int64_t N, int64_t vocabulary) {
   return p;
 }
 
-template <bool FIRST, typename Index>
+template <bool FIRST, typename Index, typename Out>
 int sort_pass(const SortPlan& p, const Index* tokens, const Pair* in, int64_t N, int64_t vocabulary, int shift,
-              uint32_t* counts, Pair* out, hipStream_t s) {
+              uint32_t* counts, const Out& out, hipStream_t s) {
   hipLaunchKernelGGL((digit_count_kernel<FIRST, Index>), dim3(unsigned(p.runs)), dim3(kSortThreads), 0, s, tokens, in,
                      N, p.run, vocabulary, shift, counts);
   if (int rc = check_launch("digit_count_kernel")) return rc;
-  hipLaunchKernelGGL((digit_place_kernel<FIRST, Index>), dim3(unsigned(p.runs)), dim3(kSortThreads), 0, s, tokens, in,
-                     N, p.run, vocabulary, shift, counts, out);
+  hipLaunchKernelGGL((digit_place_kernel<FIRST, Index, Out>), dim3(unsigned(p.runs)), dim3(kSortThreads), 0, s, tokens,
+                     in, N, p.run, vocabulary, shift, counts, out);
   return check_launch("digit_place_kernel");
+}
+
+template <typename Index, typename Out>
+int small_sort(const SortPlan& p, const Index* tokens, int64_t N, int64_t vocabulary, const Out& out, hipStream_t s) {
+  hipLaunchKernelGGL((small_sort_kernel<Index, Out>), dim3(1), dim3(kSortThreads), 0, s, tokens, int(N), vocabulary,
+                     p.passes, out);
+  return check_launch("small_sort_kernel");
 }
 
 // The positions in the order of their tokens, in `p.bytes` of `work`.
@@ -241,14 +257,11 @@ int sort_tokens(const SortPlan& p, const Index* tokens, int64_t N, int64_t vocab
   Pair* pairs[2] = {reinterpret_cast<Pair*>(work), reinterpret_cast<Pair*>(work + p.pairs_bytes)};
   uint32_t* counts = reinterpret_cast<uint32_t*>(work + 2 * p.pairs_bytes);
   *sorted = pairs[(p.passes - 1) & 1];
-  if (N > 0 && N <= kSmallSort) {
-    hipLaunchKernelGGL((small_sort_kernel<Index>), dim3(1), dim3(kSortThreads), 0, s, tokens, int(N), vocabulary,
-                       p.passes, *sorted);
-    if (int rc = check_launch("small_sort_kernel")) return rc;
-  }
+  if (N > 0 && N <= kSmallSort) return small_sort(p, tokens, N, vocabulary, Pairs{*sorted}, s);
   for (int k = 0; k < p.passes && N > kSmallSort; ++k) {
-    const int rc = k == 0 ? sort_pass<true>(p, tokens, static_cast<const Pair*>(nullptr), N, vocabulary, 0, counts, pairs[0], s)
-                          : sort_pass<false>(p, tokens, pairs[(k + 1) & 1], N, vocabulary, 8 * k, counts, pairs[k & 1], s);
+    const int rc = k == 0 ? sort_pass<true>(p, tokens, static_cast<const Pair*>(nullptr), N, vocabulary, 0, counts, Pairs{pairs[0]}, s)
+                          : sort_pass<false>(p, tokens, pairs[(k + 1) & 1], N, vocabulary, 8 * k, counts,
+                                            Pairs{pairs[k & 1]}, s);
     if (rc) return rc;
   }
   return YE3T_OK;

@@ -6,6 +6,7 @@ or a call fails, a ``RuntimeError`` carrying the library's message is raised.
 """
 
 import ctypes
+import struct
 import os
 
 import numpy as np
@@ -88,15 +89,17 @@ class AttentionArgs(ctypes.Structure):
         [(n, _vp) for n in ("slopes", "positions", "key_positions", "key_mask")]
 
 
-class LinearArgs(ctypes.Structure):
-    _fields_ = [("dtype", ctypes.c_int), ("rows", ctypes.c_int64), ("inputs", ctypes.c_int64),
-                ("outputs", ctypes.c_int64), ("groups_given", ctypes.c_int), ("groups", ctypes.c_int64),
-                ("order", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("input", ctypes.c_void_p),
-                ("input_row_stride", ctypes.c_int64), ("weight", ctypes.c_void_p),
-                ("weight_group_stride", ctypes.c_int64), ("weight_row_stride", ctypes.c_int64),
-                ("turned", ctypes.c_int), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
-                ("activation", ctypes.c_int), ("drop_below", ctypes.c_int64), ("layer", ctypes.c_uint32),
-                ("seed", ctypes.c_uint64), ("device_seed", ctypes.c_void_p)]
+# ye3t_linear_args, packed as bytes: a Structure of as many fields takes three times as long to fill, which shows in the
+# smallest calls
+_LINEAR_ARGS = struct.Struct("@iqqqiqPPPqPqqiPPiqIQP")
+_LINEAR_FIELDS = ("dtype", "rows", "inputs", "outputs", "groups_given", "groups", "order", "offsets", "input",
+                  "input_row_stride", "weight", "weight_group_stride", "weight_row_stride", "turned", "bias", "residual",
+                  "activation", "drop_below", "layer", "seed", "device_seed")
+
+
+def linear_args(**fields):
+    """``ye3t_linear_args`` by the fields' names, those that are not given zero."""
+    return _LINEAR_ARGS.pack(*(fields.get(n, 0) for n in _LINEAR_FIELDS))
 
 
 class Caps(ctypes.Structure):
@@ -241,10 +244,12 @@ def lib():
     L.ye3t_hip_species_groups_workspace_bytes.argtypes = [_i64, _i64]
     L.ye3t_hip_species_groups_workspace_bytes.restype = _i64
     L.ye3t_hip_species_groups.argtypes = [_vp, ctypes.c_int, _i64, _i64, _vp, _vp, _vp, _i64, _vp]
-    L.ye3t_hip_linear.argtypes = [ctypes.POINTER(LinearArgs), _vp, _vp, _vp]
-    L.ye3t_hip_linear_adjoint_workspace_bytes.argtypes = [ctypes.POINTER(LinearArgs)]
+    L.ye3t_hip_linear_workspace_bytes.argtypes = [_vp]
+    L.ye3t_hip_linear_workspace_bytes.restype = _i64
+    L.ye3t_hip_linear.argtypes = [_vp, _vp, _vp, _vp, _i64, _vp]
+    L.ye3t_hip_linear_adjoint_workspace_bytes.argtypes = [_vp]
     L.ye3t_hip_linear_adjoint_workspace_bytes.restype = _i64
-    L.ye3t_hip_linear_adjoint.argtypes = [ctypes.POINTER(LinearArgs)] + [_vp] * 6 + [_i64, _vp]
+    L.ye3t_hip_linear_adjoint.argtypes = [_vp] + [_vp] * 6 + [_i64, _vp]
     L.ye3t_hip_dropout.argtypes = [ctypes.c_int, _vp, _vp, _i64, _i64, _i64, ctypes.c_uint32, ctypes.c_uint64, _vp, _vp,
                                    _vp]
     version = L.ye3t_hip_abi_version()
@@ -287,7 +292,8 @@ EXPORTED_SYMBOLS = (
     "ye3t_hip_rms_norm", "ye3t_hip_rms_norm_8bit", "ye3t_hip_rms_norm_adjoint_workspace_bytes",
     "ye3t_hip_rms_norm_adjoint", "ye3t_hip_atom_attention_workspace_bytes", "ye3t_hip_atom_attention",
     "ye3t_hip_atom_attention_adjoint_workspace_bytes", "ye3t_hip_atom_attention_adjoint",
-    "ye3t_hip_species_groups_workspace_bytes", "ye3t_hip_species_groups", "ye3t_hip_linear",
+    "ye3t_hip_species_groups_workspace_bytes", "ye3t_hip_species_groups",
+    "ye3t_hip_linear_workspace_bytes", "ye3t_hip_linear",
     "ye3t_hip_linear_adjoint_workspace_bytes", "ye3t_hip_linear_adjoint", "ye3t_hip_dropout",
 )
 
@@ -2147,22 +2153,20 @@ class Linear:
     contiguous; ``below``, ``layer`` and ``seed`` (an int or an int64 tensor) of the dropped values."""
 
     def __init__(self, input, weight, bias, residual, order, offsets, activation, below, layer, seed):
-        import torch
-
         self.input, self.weight, self.bias, self.residual = input, weight, bias, residual
-        self.order, self.offsets = order, offsets
-        self.activation, self.below, self.layer, self.seed = activation, below, layer, seed
-        self.turned = weight.stride(-1) != 1 and weight.shape[-1] > 1
-        held = isinstance(seed, torch.Tensor)
-        pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        self.args = LinearArgs(
-            dtype=_storage_code(input.dtype), rows=input.shape[0], inputs=input.shape[1], outputs=weight.shape[-1],
-            groups_given=order is not None, groups=weight.shape[0] if order is not None else 0, order=pointer(order),
-            offsets=pointer(offsets), input=input.data_ptr(), input_row_stride=input.stride(0), weight=weight.data_ptr(),
-            weight_group_stride=weight.stride(0) if order is not None else 0,
-            weight_row_stride=weight.stride(-1 if self.turned else -2), turned=self.turned, bias=pointer(bias),
-            residual=pointer(residual), activation=activation, drop_below=below, layer=layer,
-            seed=0 if held else seed, device_seed=seed.data_ptr() if held else None)
+        self.order, self.offsets, self.seed = order, offsets, seed
+        rows, inputs = input.shape
+        outputs = weight.shape[-1]
+        strides = weight.stride()
+        turned = self.turned = strides[-1] != 1 and outputs > 1
+        number = isinstance(seed, int)
+        grouped = order is not None
+        self.args = _LINEAR_ARGS.pack(
+            _storage_code(input.dtype), rows, inputs, outputs, grouped, weight.shape[0] if grouped else 0,
+            order.data_ptr() if grouped else 0, offsets.data_ptr() if grouped else 0, input.data_ptr(), input.stride(0),
+            weight.data_ptr(), strides[0] if grouped else 0, strides[-1 if turned else -2], turned,
+            0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), activation, below, layer,
+            seed if number else 0, 0 if number else seed.data_ptr())
 
     def forward(self, keep):
         """``(out, preactivation or None)``"""
@@ -2172,8 +2176,10 @@ class Linear:
         out = torch.empty((x.shape[0], self.weight.shape[-1]), dtype=x.dtype, device=x.device)
         kept = torch.empty_like(out) if keep else None
         with _on(x.device):
-            _check(lib().ye3t_hip_linear(ctypes.byref(self.args), _opt(kept, "preactivation"), out.data_ptr(),
-                                         _raw_stream()), "ye3t_hip_linear")
+            size = lib().ye3t_hip_linear_workspace_bytes(self.args)
+            work = _workspace(size, "ye3t_hip_linear_workspace_bytes", x.device) if size else None
+            _check(lib().ye3t_hip_linear(self.args, _opt(kept, "preactivation"), out.data_ptr(), _opt(work, "workspace"),
+                                         size, _raw_stream()), "ye3t_hip_linear")
         return out, kept
 
     def adjoint(self, adjoint, kept, need_input, need_weight, need_bias):
@@ -2189,9 +2195,9 @@ class Linear:
         if need_bias:
             db = torch.empty((*w.shape[:-2], w.shape[-1]), dtype=w.dtype, device=w.device)
         with _on(x.device):
-            size = lib().ye3t_hip_linear_adjoint_workspace_bytes(ctypes.byref(self.args))
+            size = lib().ye3t_hip_linear_adjoint_workspace_bytes(self.args)
             work = _workspace(size, "ye3t_hip_linear_adjoint_workspace_bytes", x.device)
-            _check(lib().ye3t_hip_linear_adjoint(ctypes.byref(self.args), _dev(adjoint, "adjoint"),
+            _check(lib().ye3t_hip_linear_adjoint(self.args, _dev(adjoint, "adjoint"),
                                                  _opt(kept, "preactivation"), _opt(dx, "input_adjoint"),
                                                  _opt(dw, "weight_adjoint"), _opt(db, "bias_adjoint"), work.data_ptr(),
                                                  size, _raw_stream()), "ye3t_hip_linear_adjoint")

@@ -136,45 +136,44 @@ def _laid_out(weight):
     return weight.contiguous()
 
 
-def _checked(name, input, weight, groups, activation, probability, seed, layer, **others):
-    """Checks the arguments of a product; ``others``: tensors of the output's type.  ``(activation, below, layer, seed)``."""
+def _checked(name, input, weight, groups, bias, rows, rows_names, activation, probability, seed, layer):
+    """Checks the arguments of a product; ``rows``: tensors of the output's shape or None, with their names for a refusal.
+    ``(activation, below, layer, seed)``."""
+    device, dtype, shape, matrix = input.device, input.dtype, input.shape, weight.shape
     order, offsets = (None, None) if groups is None else groups
-    _require_one_device(name, input, weight, order, offsets, *others.values())
-    if input.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"unsupported dtype {input.dtype}; expected float32 or bfloat16")
-    if input.ndim < 1 or weight.ndim != (2 if groups is None else 3) or input.shape[-1] != weight.shape[-2]:
+    others = (weight, bias, order, offsets, *rows)
+    if not input.is_cuda or any([t is not None and t.device != device for t in others]):
+        _require_one_device(name, input, *others)  # says what is wrong
+    if dtype != torch.float32 and dtype != torch.bfloat16:
+        raise TypeError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+    if not shape or len(matrix) != (2 if groups is None else 3) or shape[-1] != matrix[-2]:
         lead = "" if groups is None else "species, "
         raise ValueError(f"weight must be [{lead}inputs, outputs] with input [..., inputs]")
-    for n, t in {"weight": weight, **others}.items():
-        if t is not None and t.dtype != input.dtype:
-            raise ValueError(f"{n} must have dtype {input.dtype}")
-    for n in ("residual", "adjoint", "preactivation"):
-        t = others.get(n)
-        if t is not None and tuple(t.shape) != (*input.shape[:-1], weight.shape[-1]):
-            raise ValueError(f"{n} must be [..., outputs] with input [..., inputs]")
-    bias = others.get("bias")
-    if bias is not None and tuple(bias.shape) != (*weight.shape[:-2], weight.shape[-1]):
-        raise ValueError(f"bias must be {[*weight.shape[:-2], weight.shape[-1]]}")
+    if weight.dtype != dtype:
+        raise ValueError(f"weight must have dtype {dtype}")
+    if bias is not None and (bias.dtype != dtype or bias.shape != (*matrix[:-2], matrix[-1])):
+        raise ValueError(f"bias must be {[*matrix[:-2], matrix[-1]]} of dtype {dtype}")
+    for n, t in zip(rows_names, rows):
+        if t is not None and (t.dtype != dtype or t.shape != (*shape[:-1], matrix[-1])):
+            raise ValueError(f"{n} must be [..., outputs] of dtype {dtype} with input [..., inputs]")
     if groups is not None:
         if order.dtype != torch.int32 or offsets.dtype != torch.int64 or order.ndim != 1 or offsets.ndim != 1 or \
                 not order.is_contiguous() or not offsets.is_contiguous():
             raise ValueError("groups must be of species_groups")
-        if order.numel() != math.prod(input.shape[:-1]):
+        if len(order) != math.prod(shape[:-1]):
             raise ValueError("groups must be of the input's rows")
-        if offsets.numel() != weight.shape[0] + 1:
+        if len(offsets) != matrix[0] + 1:
             raise ValueError("weight must have a matrix for each species of the groups")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}")
-    return ACTIVATIONS[activation], *_dropped(probability, seed, layer, input.device, "dropout")
+    if seed is None and probability == 0.0 and layer == 0:
+        return ACTIVATIONS[activation], 0, 0, 0
+    return ACTIVATIONS[activation], *_dropped(probability, seed, layer, device, "dropout")
 
 
-def _rows(t, columns):
+def _rows(t):
     """``[rows, columns]`` of ``t [..., columns]``."""
-    return t if t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), columns)
-
-
-def _whole(t, columns=None):
-    return None if t is None else (t if columns is None else _rows(t, columns)).contiguous()
+    return t if t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
 
 
 class _Linear(torch.autograd.Function):
@@ -209,11 +208,12 @@ class _Linear(torch.autograd.Function):
 
 
 def _product(name, input, weight, groups, bias, activation, residual, probability, seed, layer, return_preactivation):
-    shape = _checked(name, input, weight, groups, activation, probability, seed, layer, bias=bias, residual=residual)
+    shape = _checked(name, input, weight, groups, bias, (residual,), ("residual",), activation, probability, seed, layer)
     order, offsets = (None, None) if groups is None else groups
     columns = weight.shape[-1]
     lead = input.shape[:-1]
-    args = (_unit_rows(_rows(input, input.shape[-1])), _laid_out(weight), _whole(bias), _whole(residual, columns))
+    args = (_unit_rows(_rows(input)), _laid_out(weight), None if bias is None else bias.contiguous(),
+            None if residual is None else _rows(residual).contiguous())
     if _tracked(*args):
         out, kept = _Linear.apply(*args, order, offsets, shape)
         if return_preactivation and kept is None:  # without an activation
@@ -227,14 +227,14 @@ def _product(name, input, weight, groups, bias, activation, residual, probabilit
 
 
 def _product_adjoint(name, adjoint, input, weight, groups, preactivation, bias, activation, probability, seed, layer):
-    shape = _checked(name, input, weight, groups, activation, probability, seed, layer, adjoint=adjoint,
-                     preactivation=preactivation)
+    shape = _checked(name, input, weight, groups, None, (adjoint, preactivation), ("adjoint", "preactivation"), activation,
+                     probability, seed, layer)
     if activation is not None and preactivation is None:
         raise ValueError(f"{name}: the gradient of {activation} needs the preactivation")
     order, offsets = (None, None) if groups is None else groups
-    problem = native.Linear(_unit_rows(_rows(input, input.shape[-1])), _laid_out(weight), None, None, order, offsets, *shape)
-    columns = weight.shape[-1]
-    dx, dw, db = problem.adjoint(_whole(adjoint, columns), _whole(preactivation, columns), True, True, bool(bias))
+    problem = native.Linear(_unit_rows(_rows(input)), _laid_out(weight), None, None, order, offsets, *shape)
+    kept = None if preactivation is None else _rows(preactivation).contiguous()
+    dx, dw, db = problem.adjoint(_rows(adjoint).contiguous(), kept, True, True, bool(bias))
     return dx.reshape(input.shape), dw, db
 
 
