@@ -158,27 +158,30 @@ struct Tile {
 template <typename T, int LINES, int KT, bool ACROSS, int NT>
 struct Loads {
   typedef Tile<T, LINES, KT, ACROSS> Of;
-  static constexpr int kEach = (Of::kChunks + NT - 1) / NT;
+  static constexpr int kEach = Of::kChunks / NT;
   Chunk<T, 8> held[kEach];
 
-  // address(line, column, n): chunk n of this thread; null: zeros.  left(column): values that exist from there on.
-  template <typename A, typename L>
-  __device__ inline void load(A address, L left) {
+  __device__ static inline int line_of(int n) { return Of::line_of(n * NT + int(threadIdx.x)); }
+  __device__ static inline int column_of(int n) { return Of::column_of(n * NT + int(threadIdx.x)); }
+  static_assert(Of::kChunks % NT == 0, "every thread loads as many chunks");
+  // Whole chunks
+  __device__ inline void load(const T* const* from) {
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) held[n] = Chunk<T, 8>::load(from[n]);
+  }
+  // left(n): values that exist from from[n] on
+  template <typename L>
+  __device__ inline void load(const T* const* from, L left) {
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-      const int x = n * NT + int(threadIdx.x);
-      if (Of::kChunks % NT != 0 && x >= Of::kChunks) continue;
-      const int c = Of::column_of(x), most = left(c);
-      const T* p = address(Of::line_of(x), c, n);
-      held[n] = p && most > 0 ? Chunk<T, 8>::load(p, most) : Chunk<T, 8>::zero();
+      const int most = left(n);
+      held[n] = most > 0 ? Chunk<T, 8>::load(from[n], most) : Chunk<T, 8>::zero();
     }
   }
   __device__ inline void put(__bf16* tile) const {
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-      const int x = n * NT + int(threadIdx.x);
-      if (Of::kChunks % NT != 0 && x >= Of::kChunks) continue;
-      Of::put(tile, x, held[n]);
+      Of::put(tile, n * NT + int(threadIdx.x), held[n]);
     }
   }
 };
@@ -322,9 +325,9 @@ __device__ inline void multiply_direct(int steps, TileA tile_a, TileB tile_b, in
 }
 
 // Passes the wave's squares through LDS and gives them out eight columns of a row at a time, so that memory
-// is read and written along rows: use(rows, columns, values) of some chunks of the workgroup's tile.  The
+// is read and written along rows: use(rows, columns, values) of BATCH chunks of the workgroup's tile.  The
 // shares of the contraction are added in order.
-template <typename S, typename F>
+template <typename S, int BATCH, typename F>
 __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, int wn, int wk, int lane, F use) {
   constexpr int CHUNKS = S::FN * 4, STRIDE = S::kOutRow, BLOCK = 32 * STRIDE, EACH = 32 * CHUNKS / 64;
   const int wave = (wk * S::WM + wm) * S::WN + wn;
@@ -343,17 +346,20 @@ __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, i
     if constexpr (S::WK == 1) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      int r[EACH], c[EACH];
-      float v[EACH][8];
 #pragma unroll
-      for (int n = 0; n < EACH; ++n) {
-        const int x = n * 64 + lane, row = x / CHUNKS, column = x % CHUNKS * 8;
+      for (int first = 0; first < EACH; first += BATCH) {
+        int r[BATCH], c[BATCH];
+        float v[BATCH][8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[n][q] = own[row * STRIDE + column + q];
-        r[n] = (wm * S::FM + i) * 32 + row;
-        c[n] = wn * S::FN * 32 + column;
+        for (int n = 0; n < BATCH; ++n) {
+          const int x = (first + n) * 64 + lane, row = x / CHUNKS, column = x % CHUNKS * 8;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[n][q] = own[row * STRIDE + column + q];
+          r[n] = (wm * S::FM + i) * 32 + row;
+          c[n] = wn * S::FN * 32 + column;
+        }
+        use(r, c, v);
       }
-      use(r, c, v);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     } else {
@@ -489,23 +495,15 @@ struct WeightProduct {
   unsigned tiles_m, tiles_n;
 };
 
-// Bytes of device memory that a product takes beside its operands, and the product
+// Bytes of device memory that a product takes beside its operands, whatever their addresses are, and the product
 template <typename T>
 int64_t row_bytes(const RowProduct<T>& p);
 template <typename T>
 int launch_rows(RowProduct<T> p, void* work, hipStream_t s);
 template <typename T>
-int launch_weights(WeightProduct<T> p, hipStream_t s);
-
-// Shares of the rows of a weight's gradient, and the workspace for their sums.
-struct SharePlan {
-  int64_t share, slots, part_bytes, sums_bytes, bytes;
-};
+int64_t weight_bytes(WeightProduct<T> p);
 template <typename T>
-SharePlan share_plan(const WeightProduct<T>& p);
-// and the most bytes that a call of these sizes takes, whatever its operands' addresses are
-template <typename T>
-int64_t most_share_bytes(WeightProduct<T> p);
+int launch_weights(WeightProduct<T> p, void* work, hipStream_t s);
 
 }  // namespace linear
 }  // namespace ye3t

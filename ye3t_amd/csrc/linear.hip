@@ -141,8 +141,8 @@ int64_t dz_bytes(const ye3t_linear_args& a) {
 int64_t adjoint_bytes(const ye3t_linear_args& a) {
   const int64_t parts = a.dtype == YE3T_F32 ? row_bytes(backward_of<float>(a, nullptr))
                                             : row_bytes(backward_of<__bf16>(a, nullptr));
-  const int64_t shares = a.dtype == YE3T_F32 ? most_share_bytes(weights_of<float>(a, nullptr))
-                                             : most_share_bytes(weights_of<__bf16>(a, nullptr));
+  const int64_t shares = a.dtype == YE3T_F32 ? weight_bytes(weights_of<float>(a, nullptr))
+                                             : weight_bytes(weights_of<__bf16>(a, nullptr));
   return dz_bytes(a) + (shares > parts ? shares : parts) + 256;
 }
 
@@ -168,13 +168,9 @@ int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept,
   }
   if (weight_adjoint) {
     WeightProduct<T> p = weights_of<T>(a, dz);
-    const SharePlan f = share_plan(p);
     p.out = static_cast<T*>(weight_adjoint);
     p.sums = static_cast<T*>(bias_adjoint);
-    p.share = f.share;
-    p.part = reinterpret_cast<float*>(work + dz_bytes(a));
-    p.sums_part = reinterpret_cast<float*>(work + dz_bytes(a) + f.part_bytes);
-    if (int rc = launch_weights(p, s)) return rc;
+    if (int rc = launch_weights(p, work + dz_bytes(a), s)) return rc;
   }
   return YE3T_OK;
 }

@@ -96,25 +96,27 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
   }
   auto tile_a = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP); };
   auto tile_b = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP + A::kBytes); };
+  // Lines past the tile's rows or columns repeat others: their results go nowhere.  Past the contraction there are
+  // zeros in both operands.
+  typedef std::conditional_t<DIRECT, DirectLoads<S::TM, S::KT, false, S::NT>, Loads<T, S::TM, S::KT, false, S::NT>> LoadsA;
+  typedef std::conditional_t<DIRECT, DirectLoads<S::TN, S::KT, ACROSS, S::NT>, Loads<T, S::TN, S::KT, ACROSS, S::NT>> LoadsB;
+  LoadsA a;
+  LoadsB b;
+  const T *a_from[LoadsA::kEach], *b_from[LoadsB::kEach];  // of the next tile
+  const int64_t b_step = ACROSS ? S::KT * p.b_row : S::KT;
+#pragma unroll
+  for (int n = 0; n < LoadsA::kEach; ++n) {
+    const int line = a.line_of(n);
+    const int64_t row = row_at(p.order, row0 + (line < live ? line : 0), p.rows);
+    a_from[n] = p.a + (row < 0 ? 0 : row) * p.a_row + a.column_of(n) + begin_step * S::KT;
+  }
+#pragma unroll
+  for (int n = 0; n < LoadsB::kEach; ++n) {
+    const int line = b.line_of(n), c = b.column_of(n);
+    b_from[n] = (ACROSS ? weight + line * p.b_row + (n0 + c < p.N ? n0 + c : 0)
+                        : weight + (n0 + line < p.N ? n0 + line : 0) * p.b_row + c) + begin_step * b_step;
+  }
   if constexpr (DIRECT) {
-    // Lines past the tile's rows or columns repeat others: their results go nowhere.  Past the contraction there
-    // are zeros.
-    DirectLoads<S::TM, S::KT, false, S::NT> a;
-    DirectLoads<S::TN, S::KT, ACROSS, S::NT> b;
-    const T *a_from[decltype(a)::kEach], *b_from[decltype(b)::kEach];  // of the next tile
-#pragma unroll
-    for (int n = 0; n < decltype(a)::kEach; ++n) {
-      const int line = a.line_of(n);
-      const int64_t row = row_at(p.order, row0 + (line < live ? line : 0), p.rows);
-      a_from[n] = p.a + (row < 0 ? 0 : row) * p.a_row + a.column_of(n);
-    }
-#pragma unroll
-    for (int n = 0; n < decltype(b)::kEach; ++n) {
-      const int line = b.line_of(n), c = b.column_of(n);
-      b_from[n] = ACROSS ? weight + line * p.b_row + (n0 + c < p.N ? n0 + c : 0)
-                         : weight + (n0 + line < p.N ? n0 + line : 0) * p.b_row + c;
-    }
-    const int64_t b_step = ACROSS ? S::KT * p.b_row : S::KT;
     auto load = [&](int t, auto part, auto parts) {
       auto each = [&](auto& loads, __bf16* tile, const T** from, int64_t step, auto exists) {
         constexpr int EACH = std::remove_reference_t<decltype(loads)>::kEach, P = decltype(part)::value, OF = decltype(parts)::value;
@@ -133,26 +135,24 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
         each(b, tile_b(t), b_from, b_step, [&](int n) { return k0 + (ACROSS ? b.line_of(n) : b.column_of(n)) < K; });
       }
     };
-    multiply_direct<S, A, B, decltype(a)::kEach + decltype(b)::kEach>(steps, tile_a, tile_b, wm, wn, wk, lane, load,
+    multiply_direct<S, A, B, LoadsA::kEach + LoadsB::kEach>(steps, tile_a, tile_b, wm, wn, wk, lane, load,
                                                                       [](int) {}, sum);
   } else {
-    Loads<T, S::TM, S::KT, false, S::NT> a;
-    Loads<T, S::TN, S::KT, ACROSS, S::NT> b;
-    const T* a_line[decltype(a)::kEach];
-#pragma unroll
-    for (int n = 0; n < decltype(a)::kEach; ++n) {
-      const int line = A::line_of(n * S::NT + int(threadIdx.x));
-      const int64_t row = line < live ? row_at(p.order, row0 + line, p.rows) : -1;
-      a_line[n] = row >= 0 ? p.a + row * p.a_row : nullptr;
-    }
+    const bool whole = !ACROSS || n0 + S::TN <= p.N;  // no chunk of b has columns past the last
     auto load = [&](int k0) {
-      a.load([&](int, int c, int n) { return a_line[n] ? a_line[n] + k0 + c : nullptr; }, [&](int c) { return K - k0 - c; });
-      if (ACROSS)
-        b.load([&](int k, int c, int) { return k0 + k < K ? weight + int64_t(k0 + k) * p.b_row + n0 + c : nullptr; },
-               [&](int c) { return p.N - n0 - c; });
-      else
-        b.load([&](int n, int c, int) { return n0 + n < p.N ? weight + int64_t(n0 + n) * p.b_row + k0 + c : nullptr; },
-               [&](int c) { return K - k0 - c; });
+      if (k0 + S::KT <= K && whole) {
+        a.load(a_from);
+        b.load(b_from);
+      } else {
+        a.load(a_from, [&](int n) { return K - k0 - a.column_of(n); });
+        b.load(b_from, [&](int n) {
+          return !ACROSS ? K - k0 - b.column_of(n) : k0 + b.line_of(n) < K ? p.N - n0 - b.column_of(n) : 0;
+        });
+      }
+#pragma unroll
+      for (int n = 0; n < LoadsA::kEach; ++n) a_from[n] += S::KT;
+#pragma unroll
+      for (int n = 0; n < LoadsB::kEach; ++n) b_from[n] += b_step;
     };
     if (steps) load(begin_step * S::KT);
     for (int t = 0; t < steps; ++t) {
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
 
   if constexpr (S::WK > 1) {
     if (p.parts > 1) {
-      give_out<S>(lds, sum, wm, wn, wk, lane, [&](const auto& r, const auto& c, auto& v) {
+      give_out<S, 1>(lds, sum, wm, wn, wk, lane, [&](const auto& r, const auto& c, auto& v) {
         const int left = p.N - n0 - c[0];
         if (r[0] >= live || left <= 0) return;
         Chunk<float, 8> out;
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
     epilogue(p, weight, bias, seed, K, row, n, v);
   };
   if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);
-  else give_out<S>(lds, sum, wm, wn, wk, lane, finish);
+  else give_out<S, sizeof(T) == 4 ? S::FN : 2 * S::FN>(lds, sum, wm, wn, wk, lane, finish);
 }
 
 // Adds the parts of the contraction in order and goes on as the product's own epilogue.  A lane a chunk of eight columns.
@@ -256,7 +256,8 @@ struct Shapes<__bf16> {
 };
 template <>
 struct Shapes<float> {
-  typedef Shape<2, 2, 1, 2, 2, 32, 1, 2> Large;
+  typedef Shape<2, 2, 1, 2, 2, 32, 1, 3> Large;
+  typedef Shape<2, 2, 1, 2, 1, 32, 1, 3> Tall;
   typedef Shape<2, 2, 1, 1, 1, 32, 1, 3> Middle;
   typedef Shape<1, 1, 8, 1, 1, 32, 1, 2> Few;
 };
@@ -269,7 +270,7 @@ bool direct(const RowProduct<T>& p) {
 }
 
 // Which shape a product takes, and in how many parts of the contraction
-enum Kind { kFew, kMiddle, kLarge, kDirect, kSquare };
+enum Kind { kFew, kMiddle, kTall, kLarge, kDirect, kSquare };
 struct Choice {
   Kind kind;
   int parts, part_steps;
@@ -286,7 +287,18 @@ Choice choice_of(const RowProduct<T>& p, bool direct) {
     if (tiles(128) >= 256) return {kDirect, 1, 0};
   }
   // Tiles of 128 x 128 where they give every compute unit one, of 64 x 64 where those do, else of 32 x 32 with the
-  // contraction shared by eight waves, and by several workgroups where it is long and they are few.
+  // contraction shared by eight waves, and by several workgroups where it is long and they are few.  fp32: tiles of
+  // 128 x 64 where the contraction is short, for more workgroups that hide each other's loads, or where 128
+  // columns leave much of the last tile empty.  200 003 x 161 x 96: 90 us, by 128 x 128 97; 60 000 x 512 x 192: 105
+  // and 126; 16 384 x 1 024 x 1 024: 252 and 227; 30 011 x 128 x 128 by 89 species: 23, by 64 x 64 21.
+  if constexpr (sizeof(T) == 4) {
+    const int64_t tall = ((p.rows + 127) / 128 + (p.grouped ? p.groups : 0)) * ((p.N + 63) / 64);
+    const bool empty = (p.N + 127) / 128 * 128 * 5 > (p.N + 63) / 64 * 64 * 6;
+    if (p.rows > 64 && (p.K < 256 || empty)) {
+      if (tall >= 1024) return {kTall, 1, 0};
+      if (tiles(64) >= 256) return {kMiddle, 1, 0};
+    }
+  }
   if (p.rows > 64 && tiles(128) >= 256) return {kLarge, 1, 0};
   if (p.rows > 32 && tiles(64) >= 256) return {kMiddle, 1, 0};
   const int64_t groups = ((p.rows + 31) / 32 + (p.grouped ? p.groups : 0)) * ((p.N + 31) / 32);
@@ -317,6 +329,9 @@ int launch_rows(RowProduct<T> p, void* work, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (c.kind == kSquare) return launch_shaped<T, typename Shapes<T>::Square, true>(p, s);
     if (c.kind == kDirect) return launch_shaped<T, typename Shapes<T>::Direct, true>(p, s);
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (c.kind == kTall) return launch_shaped<T, typename Shapes<T>::Tall>(p, s);
   }
   if (c.kind == kLarge) return launch_shaped<T, typename Shapes<T>::Large>(p, s);
   if (c.kind == kMiddle) return launch_shaped<T, typename Shapes<T>::Middle>(p, s);

@@ -98,11 +98,22 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
   } else {
     Loads<T, S::TM, S::KT, true, S::NT> a;
     Loads<T, S::TN, S::KT, true, S::NT> b;
+    const bool whole_columns = m0 + S::TM <= p.M && n0 + S::TN <= p.N;
     auto load = [&](int t) {
-      a.load([&](int, int c, int n) { return row[n] >= 0 ? p.a + row[n] * p.a_row + m0 + c : nullptr; },
-             [&](int c) { return p.M - m0 - c; });
-      b.load([&](int, int c, int n) { return row[n] >= 0 ? p.b + row[n] * p.b_row + n0 + c : nullptr; },
-             [&](int c) { return p.N - n0 - c; });
+      const T *a_from[EACH], *b_from[EACH];
+#pragma unroll
+      for (int n = 0; n < EACH; ++n) {
+        const int64_t r = row[n] < 0 ? 0 : row[n];
+        a_from[n] = p.a + r * p.a_row + m0 + a.column_of(n);
+        b_from[n] = p.b + r * p.b_row + n0 + b.column_of(n);
+      }
+      if ((t + 1) * S::KT <= live && whole_columns) {
+        a.load(a_from);
+        b.load(b_from);
+      } else {
+        a.load(a_from, [&](int n) { return row[n] < 0 ? 0 : p.M - m0 - a.column_of(n); });
+        b.load(b_from, [&](int n) { return row[n] < 0 ? 0 : p.N - n0 - b.column_of(n); });
+      }
       look(t + 1);
     };
     if (steps) load(0);
@@ -171,8 +182,13 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
     }
   };
   if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);
-  else give_out<S>(lds, sum, wm, wn, wk, lane, finish);
+  else give_out<S, S::FN>(lds, sum, wm, wn, wk, lane, finish);
 }
+
+struct SharePlan {
+  int tile;
+  int64_t share, slots, part_bytes, sums_bytes, bytes;
+};
 
 // Adds the sums of the shares of each group that has several, in order; the workgroups behind those of the
 // products add the column sums.
@@ -228,12 +244,43 @@ bool direct(const WeightProduct<T>& p) {
          p.N % 8 == 0 && p.a_row % 8 == 0 && p.b_row % 8 == 0;
 }
 
-// Tiles of 256 x 256 for wide weights of direct loads, of 64 x 64 for narrow ones, else of 128 x 128
+// Shares of the rows and the tile of the weight that a workgroup owns: the largest tile that gives the card
+// enough workgroups with shares of kLeastShare rows, 256 of 256 x 256 (direct loads), 512 of 128 x 128.  Tiles of 64 x 64
+// also where those of 128 x 128 would be a quarter empty.  fp32: 2 000 rows, 512 x 512, 21 us by 64 x 64, 26 by 128 x
+// 128; 200 003 rows, 161 x 96, 118 and 127; 16 384 rows, 1 024 x 1 024, 286 and 215; bf16, by 256 x 256 57,
+// by 128 x 128 58, and with 4 096 columns 142 and 183.
+constexpr int64_t kLeastShare = 256;
 enum WeightTile { kMiddleTile = 64, kLargeTile = 128, kSquareTile = 256 };
-inline WeightTile tile_for(int64_t M, int64_t N, bool direct) {
-  return M <= 64 || N <= 64 ? kMiddleTile : direct && M >= 512 && N >= 512 ? kSquareTile : kLargeTile;
+inline WeightTile tile_for(int64_t rows, int64_t groups, int64_t M, int64_t N, bool direct) {
+  auto whole = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+  const int64_t shares = rows / kLeastShare + groups;
+  if (direct && M >= 512 && N >= 512 && whole(256) * shares >= 256) return kSquareTile;
+  return whole(128) * shares < 512 || whole(128) * 16 > whole(64) * 5 ? kMiddleTile : kLargeTile;
 }
 
+// Workgroups that the shares make: 256 of 256 x 256, which each fill a compute unit, else 512 of 128 x 128 and 1 024 of
+// 64 x 64; 2 048 of either where there are groups, whose lengths differ (fp32, eight species, 16 384 rows, 1 024 x
+// 2 048: 652 us, by 512 workgroups 900).
+SharePlan share_plan(int64_t rows, int64_t groups, bool grouped, int64_t M, int64_t N, bool direct) {
+  SharePlan f{};
+  f.tile = tile_for(rows, groups, M, N, direct);
+  const int64_t t = f.tile, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
+  const int64_t most = t == kSquareTile ? 256 : grouped ? 2048 : t == kLargeTile ? 512 : 1024;
+  const int64_t parts = tiles == 0 ? most : tiles < most ? most / tiles : 1;
+  f.share = (rows + parts - 1) / parts;
+  if (f.share < kLeastShare) f.share = kLeastShare;
+  if (f.share > (1 << 30)) f.share = 1 << 30;
+  f.slots = f.share < rows ? 2 * rows / f.share + 1 : 0;
+  f.part_bytes = up(f.slots * M * N * 4);
+  f.sums_bytes = up(f.slots * (M > N ? M : N) * 4);
+  f.bytes = f.part_bytes + f.sums_bytes;
+  return f;
+}
+
+template <typename T>
+SharePlan share_plan(const WeightProduct<T>& p) {
+  return share_plan(p.rows, p.grouped ? p.groups : 1, p.grouped, p.M, p.N, sizeof(T) == 2 && direct(p));
+}
 template <typename T, typename S, bool DIRECT = false>
 int launch_shaped(WeightProduct<T> p, hipStream_t s) {
   p.tiles_m = p.M ? unsigned((p.M + S::TM - 1) / S::TM) : 1;  // no rows or columns: there may be sums
@@ -249,50 +296,32 @@ int launch_shaped(WeightProduct<T> p, hipStream_t s) {
 
 }  // namespace
 
-// Shares that give the card about four workgroups a compute unit, one of tiles of 256 x 256, of 512 rows or more
-SharePlan share_plan(int64_t rows, int64_t groups, int64_t M, int64_t N, bool direct) {
-  SharePlan f{};
-  const int64_t t = tile_for(M, N, direct), tiles = ((M + t - 1) / t) * ((N + t - 1) / t) * (t == kSquareTile ? 4 : 1);
-  const int64_t parts = tiles == 0 ? 1024 : tiles < 1024 ? 1024 / tiles : 1;
-  f.share = (rows + parts - 1) / parts;
-  if (f.share < 512) f.share = 512;
-  if (f.share > (1 << 30)) f.share = 1 << 30;
-  f.slots = f.share < rows ? 2 * rows / f.share + 1 : 0;
-  f.part_bytes = up(f.slots * M * N * 4);
-  f.sums_bytes = up(f.slots * (M > N ? M : N) * 4);
-  f.bytes = f.part_bytes + f.sums_bytes;
-  return f;
-}
-
 template <typename T>
-SharePlan share_plan(const WeightProduct<T>& p) {
-  return share_plan(p.rows, p.grouped ? p.groups : 1, p.M, p.N, sizeof(T) == 2 && direct(p));
-}
-template <typename T>
-int64_t most_share_bytes(WeightProduct<T> p) {
+int64_t weight_bytes(WeightProduct<T> p) {
   const int64_t groups = p.grouped ? p.groups : 1;
-  const int64_t some = share_plan(p.rows, groups, p.M, p.N, false).bytes, direct = share_plan(p.rows, groups, p.M, p.N, sizeof(T) == 2).bytes;
+  const int64_t some = share_plan(p.rows, groups, p.grouped, p.M, p.N, false).bytes, direct = share_plan(p.rows, groups, p.grouped, p.M, p.N, sizeof(T) == 2).bytes;
   return some > direct ? some : direct;
 }
-template int64_t most_share_bytes(WeightProduct<float>);
-template int64_t most_share_bytes(WeightProduct<__bf16>);
-template SharePlan share_plan(const WeightProduct<float>&);
-template SharePlan share_plan(const WeightProduct<__bf16>&);
+template int64_t weight_bytes(WeightProduct<float>);
+template int64_t weight_bytes(WeightProduct<__bf16>);
 
 template <typename T>
-int launch_weights(WeightProduct<T> p, hipStream_t s) {
+int launch_weights(WeightProduct<T> p, void* work, hipStream_t s) {
   const int64_t groups = p.grouped ? p.groups : 1;
   if (groups == 0 || ((p.M == 0 || p.N == 0) && !p.sums)) return YE3T_OK;
-  const WeightTile tile = tile_for(p.M, p.N, sizeof(T) == 2 && direct(p));
+  const SharePlan f = share_plan(p);
+  p.share = f.share;
+  p.part = static_cast<float*>(work);
+  p.sums_part = reinterpret_cast<float*>(static_cast<char*>(work) + f.part_bytes);
   int rc = YE3T_OK;
   if constexpr (sizeof(T) == 2) {
-    rc = tile == kSquareTile   ? launch_shaped<T, typename Shapes<T>::Square, true>(p, s)
-         : tile == kLargeTile  ? direct(p) ? launch_shaped<T, typename Shapes<T>::Large, true>(p, s)
-                                           : launch_shaped<T, typename Shapes<T>::Large>(p, s)
-                               : launch_shaped<T, typename Shapes<T>::Middle>(p, s);
+    if (f.tile == kSquareTile) rc = launch_shaped<T, typename Shapes<T>::Square, true>(p, s);
+    else if (f.tile == kMiddleTile) rc = launch_shaped<T, typename Shapes<T>::Middle>(p, s);
+    else if (direct(p)) rc = launch_shaped<T, typename Shapes<T>::Large, true>(p, s);
+    else rc = launch_shaped<T, typename Shapes<T>::Large>(p, s);
   } else {
-    rc = tile == kLargeTile ? launch_shaped<T, typename Shapes<T>::Large>(p, s)
-                            : launch_shaped<T, typename Shapes<T>::Middle>(p, s);
+    rc = f.tile == kLargeTile ? launch_shaped<T, typename Shapes<T>::Large>(p, s)
+                              : launch_shaped<T, typename Shapes<T>::Middle>(p, s);
   }
   if (rc) return rc;
   if (p.rows <= p.share) return YE3T_OK;
@@ -304,8 +333,8 @@ int launch_weights(WeightProduct<T> p, hipStream_t s) {
                      dim3(kJoinThreads), 0, s, p, unsigned(product));
   return check_launch("weight_join_kernel");
 }
-template int launch_weights<float>(WeightProduct<float>, hipStream_t);
-template int launch_weights<__bf16>(WeightProduct<__bf16>, hipStream_t);
+template int launch_weights<float>(WeightProduct<float>, void*, hipStream_t);
+template int launch_weights<__bf16>(WeightProduct<__bf16>, void*, hipStream_t);
 
 }  // namespace linear
 }  // namespace ye3t
