@@ -31,11 +31,11 @@ def philox(counter, key):
     return c
 
 
-def kept(rows, columns, probability, seed, layer):
-    """[rows, columns]: 0 for dropped values, 1 / (1 - p) for the others, p in steps of 2^-16."""
+def kept(rows, columns, probability, seed, layer, first=0):
+    """[rows, columns]: 0 for dropped values, 1 / (1 - p) for the others, p in steps of 2^-16; rows from ``first`` on."""
     below = int(math.floor(probability * 65536 + 0.5))
     chunks = -(-columns // 8)
-    row, chunk = (a.reshape(-1).astype(np.uint64) for a in np.meshgrid(np.arange(rows), np.arange(chunks), indexing="ij"))
+    row, chunk = (a.reshape(-1).astype(np.uint64) for a in np.meshgrid(np.arange(first, first + rows), np.arange(chunks), indexing="ij"))
     words = philox((chunk, np.full_like(chunk, layer), row & np.uint64(0xFFFFFFFF), row >> np.uint64(32)),
                    (seed % 2 ** 32, seed % 2 ** 64 >> 32))
     halves = np.stack([h for w in words for h in (w & np.uint64(0xFFFF), w >> np.uint64(16))], -1)
@@ -83,7 +83,7 @@ def forward(x, weight, bias, residual, species=None, activation=None, keep=None)
     """out and preactivation."""
     x, w, bias, residual = d(x), d(weight), d(bias), d(residual)
     w = w if species is not None else w[None]
-    bias = None if bias is None else bias.reshape(len(w), -1)
+    bias = None if bias is None else bias.reshape(len(w), w.shape[-1])
     z = torch.zeros(len(x), w.shape[-1], dtype=torch.float64)
     wide = torch.zeros_like(z)
     for k, rows in enumerate(members(species, len(w), len(x))):

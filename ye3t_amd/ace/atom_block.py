@@ -4,12 +4,14 @@ norms and attention among the atoms of each structure, with energies and forces.
     features  = B(density(edge vectors))                      stage 1 and stage 2
     x         = scale * table[species] + norm(features) M     embedding, rms_norm
     x         = x + attention(norm(x)) O                      rms_norm, atom_attention
+    x         = x + D(species' matrix of silu(norm(x) M'))    linear, species_linear, where there is a hidden width
     energy    = sum over a structure's atoms of norm(x) . r   rms_norm
 
+In training values of the features and of what is added to x may be dropped (D; dropout).
 :class:`AceFeatures` makes the features of positions, differentiable through
 the fused density and the product's reverse mode; :class:`AtomBlock` is the layer.
 ``python -m ye3t_amd.ace.atom_block`` fits one to synthetic energies and prints
-energies and forces.  The matrix products with the weights are Torch's.
+energies and forces.  The products with the weights of the first two lines are Torch's.
 """
 
 import dataclasses
@@ -85,9 +87,11 @@ class AceFeatures:
 
 
 class AtomBlock(torch.nn.Module):
-    """Energies of packed structures from their atoms' features and species."""
+    """Energies of packed structures from their atoms' features and species.  ``hidden``: the width of a feed-forward
+    part behind the attention, whose second matrix is the species' own (0: none); ``dropout``: the share of values that
+    are dropped in training, of the features and of the feed-forward part."""
 
-    def __init__(self, feature_width, species_count, width=128, heads=8, cap=0.0):
+    def __init__(self, feature_width, species_count, width=128, heads=8, cap=0.0, hidden=0, dropout=0.0):
         super().__init__()
         if width % heads:
             raise ValueError("width must be a multiple of heads")
@@ -100,22 +104,39 @@ class AtomBlock(torch.nn.Module):
         # distances in Angstrom: from local heads to heads that see the whole structure
         self.slope_logs = torch.nn.Parameter(torch.linspace(0.0, -3.0, heads))
         self.out_norm, self.readout = ones(width), torch.nn.Parameter(torch.randn(width) / width)
+        self.species_count, self.hidden, self.dropout = int(species_count), int(hidden), float(dropout)
+        if hidden:
+            zeros = lambda *n: torch.nn.Parameter(torch.zeros(*n))  # noqa: E731
+            self.hidden_norm, self.widen, self.widen_bias = ones(width), matrix(width, hidden), zeros(hidden)
+            self.narrow = torch.nn.Parameter(torch.randn(species_count, hidden, width) / math.sqrt(hidden))
+            self.narrow_bias = zeros(species_count, width)
 
-    def forward(self, features, species, positions, offsets, key_mask=None):
+    def forward(self, features, species, positions, offsets, key_mask=None, seed=None):
         """``[structures]`` energies of ``features [N, F]``, ``species [N]``, ``positions [N, 3]``
         (float32) and row offsets ``[structures + 1]``; ``key_mask [N]`` hides ghost atoms: what their
-        features and positions hold reaches nothing."""
+        features and positions hold reaches nothing.  With a ``seed`` (another one each step) values are dropped."""
         atoms = int(features.shape[0])
         if key_mask is not None:
             # their rows are computed with the others', and zero times what is not a number is none either
             features, positions = (t.masked_fill(~key_mask[:, None], 0.0) for t in (features, positions))
+        dropped = self.dropout if seed is not None else 0.0
+        if dropped:
+            features = runtime.dropout(features, dropped, seed, layer=0)
         mixed = runtime.rms_norm(features, self.feature_norm) @ self.mix
         vectors = runtime.embedding(species, self.species, scale=math.sqrt(self.width))
         y, x = runtime.rms_norm(mixed, self.attend_norm, residual=vectors)
         q, k, v = (y @ self.project).reshape(atoms, 3, self.heads, self.width // self.heads).unbind(1)
         seen = runtime.atom_attention(q, k, v, offsets, cap=self.cap, slopes=self.slope_logs.float().exp(),
                                       positions=positions, key_mask=key_mask)
-        y, x = runtime.rms_norm(seen.reshape(atoms, self.width) @ self.join, self.out_norm, residual=x)
+        joined = seen.reshape(atoms, self.width) @ self.join
+        if self.hidden:
+            y, x = runtime.rms_norm(joined, self.hidden_norm, residual=x)
+            wide = runtime.linear(y, self.widen, self.widen_bias, activation="silu")
+            groups = runtime.species_groups(species, self.species_count, validate=False)  # the embedding has checked them
+            y = runtime.rms_norm(runtime.species_linear(wide, self.narrow, groups, self.narrow_bias, residual=x,
+                                                        dropout=dropped, seed=seed, layer=1), self.out_norm)
+        else:
+            y, x = runtime.rms_norm(joined, self.out_norm, residual=x)
         each = (y @ self.readout).float()
         if key_mask is not None:
             each = each.masked_fill(~key_mask, 0.0)
@@ -147,11 +168,11 @@ def synthetic_structures(count, atoms, species_count, seed, device="cuda"):
     return positions.to(device), species.to(device), offsets.to(device)
 
 
-def main(steps=20):
+def main(steps=20, hidden=0, dropout=0.0):
     species_count = 4
     features = AceFeatures(species_count)
     torch.manual_seed(0)
-    block = AtomBlock(features.width, species_count).cuda()
+    block = AtomBlock(features.width, species_count, hidden=hidden, dropout=dropout).cuda()
     positions, species, offsets = synthetic_structures(16, 40, species_count, seed=1)
     held = features(positions, species, offsets).detach()
     atoms = (offsets[1:] - offsets[:-1]).float()
@@ -159,7 +180,7 @@ def main(steps=20):
     optimiser = torch.optim.Adam(block.parameters(), lr=2e-3)
     for step in range(steps):
         optimiser.zero_grad()
-        loss = (block(held, species, positions, offsets) / atoms - target).square().mean()
+        loss = (block(held, species, positions, offsets, seed=step) / atoms - target).square().mean()
         loss.backward()
         optimiser.step()
         if step % 5 == 0 or step == steps - 1:
@@ -172,4 +193,10 @@ def main(steps=20):
 
 
 if __name__ == "__main__":
-    main()
+    import argparse
+
+    parser = argparse.ArgumentParser(description="Fits a layer on ACE features to synthetic energies.")
+    parser.add_argument("--steps", type=int, default=20)
+    parser.add_argument("--hidden", type=int, default=0, help="width of the feed-forward part")
+    parser.add_argument("--dropout", type=float, default=0.0, help="share of values dropped in training")
+    main(**vars(parser.parse_args()))

@@ -57,6 +57,17 @@ __device__ inline Normal normal_of(float z) {
   return {z < 0.0f ? tail : 1.0f - tail, bell};
 }
 
+// 1 / (1 + exp(-z)) = scaled unit.  Of negative z the exponential is held times 2^24, as its instruction gives no
+// subnormal values and z times them may be a normal one.
+struct Logistic {
+  float scaled, unit;
+};
+__device__ inline Logistic logistic_of(float z) {
+  constexpr float kUnit = 5.9604644775390625e-8f;  // 2^-24
+  const float t = __builtin_amdgcn_exp2f(fmaf(-kLog2e, fabsf(z), 24.0f)), r = __builtin_amdgcn_rcpf(fmaf(t, kUnit, 1.0f));
+  return {z < 0.0f ? t * r : r, z < 0.0f ? kUnit : 1.0f};
+}
+
 // Eight values; the choice is made once for them.
 __device__ inline void activate(int act, float* v) {
   if (act == kRelu) {
@@ -64,7 +75,10 @@ __device__ inline void activate(int act, float* v) {
     for (int q = 0; q < 8; ++q) v[q] = v[q] <= 0.0f ? 0.0f : v[q];
   } else if (act == kSilu) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = v[q] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v[q]));
+    for (int q = 0; q < 8; ++q) {
+      const Logistic e = logistic_of(v[q]);
+      v[q] = v[q] * e.scaled * e.unit;
+    }
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = v[q] * normal_of(v[q]).phi;
@@ -74,8 +88,8 @@ __device__ inline void activate(int act, float* v) {
 __device__ inline float slope_of(int act, float z) {
   if (act == kRelu) return z > 0.0f ? 1.0f : 0.0f;
   if (act == kSilu) {
-    const float e = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
-    return e + z * e * (1.0f - e);
+    const Logistic e = logistic_of(z);
+    return fmaf(z * e.scaled, 1.0f - e.scaled * e.unit, e.scaled) * e.unit;
   }
   if (act == kGelu) {
     const Normal n = normal_of(z);

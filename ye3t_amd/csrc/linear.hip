@@ -166,7 +166,7 @@ int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept,
     p.out = static_cast<T*>(input_adjoint);
     if (int rc = launch_rows(p, work + dz_bytes(a), s)) return rc;
   }
-  if (weight_adjoint) {
+  if (weight_adjoint || bias_adjoint) {
     WeightProduct<T> p = weights_of<T>(a, dz);
     p.out = static_cast<T*>(weight_adjoint);
     p.sums = static_cast<T*>(bias_adjoint);
@@ -224,7 +224,7 @@ int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, c
   YE3T_REQUIRE(!any || adjoint, "the gradient needs the output's adjoint");
   YE3T_REQUIRE(!any || args->activation == linear::kNone || preactivation,
                "the gradient of an activation needs the preactivation");
-  YE3T_REQUIRE(!bias_adjoint || weight_adjoint, "the bias's gradient comes with the weight's");
+  YE3T_REQUIRE(!bias_adjoint || weight_adjoint || args->inputs == 0, "the bias's gradient comes with the weight's");
   YE3T_REQUIRE(workspace && workspace_bytes >= linear::adjoint_bytes(*args),
                "the workspace is smaller than ye3t_hip_linear_adjoint_workspace_bytes");
   char* work = static_cast<char*>(workspace);
