@@ -941,7 +941,8 @@ int ye3t_hip_atom_attention_adjoint(const ye3t_attention_args* args, const void*
 /* Atoms by species: `order` [rows] int32, the rows sorted by their species
  * (int32, species_bytes 4, or int64, 8), rows of one species as they came, and
  * `offsets` [species + 1] int64, where each species begins in it.  Rows of a
- * species outside [0, species) come last, behind offsets[species]. */
+ * species outside [0, species) come last, behind offsets[species].  The
+ * workspace is 0 bytes for few rows (-1 on invalid input). */
 int64_t ye3t_hip_species_groups_workspace_bytes(int64_t rows, int64_t species);
 int ye3t_hip_species_groups(const void* species_of_rows, int species_bytes, int64_t rows, int64_t species, void* order,
                             void* offsets, void* workspace, int64_t workspace_bytes, ye3t_stream_t stream);

@@ -22,7 +22,7 @@
 // rate.  Values of 2^-110 and below lose their last bits, 2^-133 at most.  A value
 // that is not finite, or rounds to infinity in bf16, would leave NaN where fp32
 // leaves an infinity or a number: results that are not finite are computed
-// again, value by value in fp32 (exact_dot).
+// again, value by value in fp32 (exact_dots).
 #pragma once
 
 #include <type_traits>
@@ -52,7 +52,8 @@ __device__ inline Normal normal_of(float z) {
       t * (0.248216531f +
            t * (0.248935427f +
                 t * (0.216934685f +
-                     t * (0.216993537f + t * (-0.0222940624f + t * (0.298866830f + t * (-0.279152495f + t * 0.0714997336f)))))));
+                     t * (0.216993537f +
+                          t * (-0.0222940624f + t * (0.298866830f + t * (-0.279152495f + t * 0.0714997336f)))))));
   const float bell = __builtin_amdgcn_exp2f(z * z * (-0.5f * kLog2e)), tail = 0.5f * bell * f;
   return {z < 0.0f ? tail : 1.0f - tail, bell};
 }
@@ -224,6 +225,9 @@ struct DirectLoads {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "m0");
   }
 };
+
+template <typename T, int LINES, int KT, bool ACROSS, int NT, bool DIRECT>
+using LoadsOf = std::conditional_t<DIRECT, DirectLoads<LINES, KT, ACROSS, NT>, Loads<T, LINES, KT, ACROSS, NT>>;
 
 // All but the newest N loads of this wave have arrived, its reads of LDS are done, and so are the other waves'.
 template <int N>
@@ -420,13 +424,21 @@ __device__ inline void hand_out(const f32x16 (*sum)[S::FN], int wm, int wn, int 
   });
 }
 
-// sum of a(k) b(k) over k < K in fp32, for results that are not finite
+// v[q] = sum of a(k) b(k, q) over k < K in fp32, for results that are not finite; q < most exist.
 template <typename A, typename B>
-__device__ float exact_dot(A a, B b, int64_t K) {
-  float s = 0.0f;
-#pragma unroll 4
-  for (int64_t k = 0; k < K; ++k) s = fmaf(a(k), b(k), s);
-  return s;
+__device__ void exact_dots(A a, B b, int64_t K, int most, float* v) {
+  float s[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) s[q] = 0.0f;
+#pragma unroll 2
+  for (int64_t k = 0; k < K; ++k) {
+    const float x = a(k);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < most) s[q] = fmaf(x, b(k, q), s[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = s[q];
 }
 __device__ inline bool any_not_finite(const float* v) {
   float worst = 0.0f;  // 0 v is NaN for infinities and NaN
@@ -507,6 +519,7 @@ struct WeightProduct {
   float* part;     // sums of the shares of groups with several, [2 rows / share + 1][M][N]
   float* sums_part;
   unsigned tiles_m, tiles_n;
+  bool spread;     // the slots' tiles over the XCDs
 };
 
 // Bytes of device memory that a product takes beside its operands, whatever their addresses are, and the product

@@ -26,10 +26,9 @@ __device__ inline void epilogue(const RowProduct<T>& p, const T* weight, const T
     if (kParts<T> == 3 && any_not_finite(v[e])) {
       const T* x = p.a + row[e] * p.a_row;
       const int64_t k_step = p.b_across ? p.b_row : 1, n_step = p.b_across ? 1 : p.b_row;
-      for (int q = 0; q < 8 && q < left[e]; ++q) {
-        const T* w = weight + (n[e] + q) * n_step;
-        v[e][q] = exact_dot([&](int64_t k) { return float(x[k]); }, [&](int64_t k) { return float(w[k * k_step]); }, K);
-      }
+      const T* w = weight + n[e] * n_step;
+      exact_dots([&](int64_t k) { return float(x[k]); },
+                 [&](int64_t k, int q) { return float(w[k * k_step + q * n_step]); }, K, left[e], v[e]);
     }
     if (bias) {
 #pragma unroll
@@ -98,8 +97,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
   auto tile_b = [&](int t) { return reinterpret_cast<__bf16*>(lds + t % S::BUFFERS * STEP + A::kBytes); };
   // Lines past the tile's rows or columns repeat others: their results go nowhere.  Past the contraction there are
   // zeros in both operands.
-  typedef std::conditional_t<DIRECT, DirectLoads<S::TM, S::KT, false, S::NT>, Loads<T, S::TM, S::KT, false, S::NT>> LoadsA;
-  typedef std::conditional_t<DIRECT, DirectLoads<S::TN, S::KT, ACROSS, S::NT>, Loads<T, S::TN, S::KT, ACROSS, S::NT>> LoadsB;
+  typedef LoadsOf<T, S::TM, S::KT, false, S::NT, DIRECT> LoadsA;
+  typedef LoadsOf<T, S::TN, S::KT, ACROSS, S::NT, DIRECT> LoadsB;
   LoadsA a;
   LoadsB b;
   const T *a_from[LoadsA::kEach], *b_from[LoadsB::kEach];  // of the next tile
@@ -119,7 +118,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
   if constexpr (DIRECT) {
     auto load = [&](int t, auto part, auto parts) {
       auto each = [&](auto& loads, __bf16* tile, const T** from, int64_t step, auto exists) {
-        constexpr int EACH = std::remove_reference_t<decltype(loads)>::kEach, P = decltype(part)::value, OF = decltype(parts)::value;
+        constexpr int EACH = std::remove_reference_t<decltype(loads)>::kEach;
+        constexpr int P = decltype(part)::value, OF = decltype(parts)::value;
 #pragma unroll
         for (int n = EACH * P / OF; n < EACH * (P + 1) / OF; ++n) {
           loads.load(tile, n, wave, exists(n) ? from[n] : loads.none());
@@ -132,11 +132,12 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
         each(b, tile_b(t), b_from, b_step, [](int) { return true; });
       } else {
         each(a, tile_a(t), a_from, S::KT, [&](int n) { return k0 + a.column_of(n) < K; });
-        each(b, tile_b(t), b_from, b_step, [&](int n) { return k0 + (ACROSS ? b.line_of(n) : b.column_of(n)) < K; });
+        each(b, tile_b(t), b_from, b_step,
+             [&](int n) { return k0 + (ACROSS ? b.line_of(n) : b.column_of(n)) < K; });
       }
     };
-    multiply_direct<S, A, B, LoadsA::kEach + LoadsB::kEach>(steps, tile_a, tile_b, wm, wn, wk, lane, load,
-                                                                      [](int) {}, sum);
+    multiply_direct<S, A, B, LoadsA::kEach + LoadsB::kEach>(steps, tile_a, tile_b, wm, wn, wk, lane, load, [](int) {},
+                                                            sum);
   } else {
     const bool whole = !ACROSS || n0 + S::TN <= p.N;  // no chunk of b has columns past the last
     auto load = [&](int k0) {

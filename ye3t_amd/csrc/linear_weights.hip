@@ -19,8 +19,19 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
   const int lane = int(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int wn = wave % S::WN, wm = wave / S::WN % S::WM, wk = wave / (S::WN * S::WM);
 
-  const int64_t tile = tile_of_group(), tiles = int64_t(p.tiles_m) * p.tiles_n, slot = tile / tiles;
-  const int tile_m = int(tile % tiles / p.tiles_n), tile_n = int(tile % p.tiles_n);
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+  int64_t slot, tile;
+  if (p.spread) {  // every XCD takes its part of each slot's tiles
+    const int64_t per = (tiles + 7) / 8;
+    slot = blockIdx.x / 8 / per;
+    tile = (blockIdx.x & 7) * per + blockIdx.x / 8 % per;
+    if (tile >= tiles) return;
+  } else {
+    const int64_t x = p.grouped ? int64_t(blockIdx.x) : tile_of_group();
+    slot = x / tiles;
+    tile = x % tiles;
+  }
+  const int tile_m = int(tile / p.tiles_n), tile_n = int(tile % p.tiles_n);
   const int m0 = tile_m * S::TM, n0 = tile_n * S::TN;
   int64_t group = 0, begin = 0, first = slot * p.share, length = p.rows;
   if (p.grouped) {
@@ -58,7 +69,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
       for (int q = 0; q < 8; ++q) v[q] = 0.0f;
 #pragma unroll
       for (int n = kParts<T> - 1; n >= 0; --n) {
-        const bf16x8 part = *reinterpret_cast<const bf16x8*>(from + n * A::kValues + k * S::TM + (c ^ turn<__bf16, S::TM>(k)) * 8);
+        const __bf16* at = from + n * A::kValues + k * S::TM + (c ^ turn<__bf16, S::TM>(k)) * 8;
+        const bf16x8 part = *reinterpret_cast<const bf16x8*>(at);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] += float(part[q]);
       }
@@ -135,7 +147,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
     float* held = reinterpret_cast<float*>(lds);
     static_assert(DOWN * S::TM * 4 <= LDS, "column sums fit the tiles' memory");
 #pragma unroll
-    for (int q = 0; q < 8; ++q) held[int(threadIdx.x) / ACROSS * S::TM + int(threadIdx.x) % ACROSS * 8 + q] = column[q];
+    for (int q = 0; q < 8; ++q)
+      held[int(threadIdx.x) / ACROSS * S::TM + int(threadIdx.x) % ACROSS * 8 + q] = column[q];
     __syncthreads();
     const int c = int(threadIdx.x), at = (p.sums_of_a ? m0 : n0) + c, most = p.sums_of_a ? p.M : p.N;
     if (c < S::TM && at < most) {
@@ -145,8 +158,15 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
       if (kParts<T> == 3 && 0.0f * s != 0.0f) {  // not finite: again from the values themselves
         const T* v = p.sums_of_a ? p.a : p.b;
         const int64_t step = p.sums_of_a ? p.a_row : p.b_row;
-        s = exact_dot([&](int64_t k) { const int64_t r = row_at(p.order, row0 + k, p.rows); return r < 0 ? 0.0f : float(v[r * step + at]); },
-                      [](int64_t) { return 1.0f; }, live);
+        float again[8];
+        exact_dots(
+            [](int64_t) { return 1.0f; },
+            [&](int64_t k, int) {
+              const int64_t r = row_at(p.order, row0 + k, p.rows);
+              return r < 0 ? 0.0f : float(v[r * step + at]);
+            },
+            live, 1, again);
+        s = again[0];
       }
       if (whole) p.sums[group * most + at] = T(s);
       else p.sums_part[part * most + at] = s;
@@ -164,9 +184,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
           const int64_t i = row_at(p.order, row0 + k, p.rows);
           return i < 0 ? 0.0f : float(from[i * step + at]);
         };
-        for (int q = 0; q < 8 && q < most; ++q)
-          v[e][q] = exact_dot([&](int64_t k) { return value(p.a, p.a_row, m, k); },
-                              [&](int64_t k) { return value(p.b, p.b_row, n + q, k); }, live);
+        exact_dots([&](int64_t k) { return value(p.a, p.a_row, m, k); },
+                   [&](int64_t k, int q) { return value(p.b, p.b_row, n + q, k); }, live, most, v[e]);
       }
       if (whole) {
         Chunk<T, 8> out;
@@ -286,7 +305,11 @@ int launch_shaped(WeightProduct<T> p, hipStream_t s) {
   p.tiles_m = p.M ? unsigned((p.M + S::TM - 1) / S::TM) : 1;  // no rows or columns: there may be sums
   p.tiles_n = p.N ? unsigned((p.N + S::TN - 1) / S::TN) : 1;
   const int64_t slots = p.grouped ? p.rows / p.share + p.groups : (p.rows + p.share - 1) / p.share;
-  const int64_t groups = (slots ? slots : 1) * p.tiles_m * p.tiles_n;
+  // The slots of groups are full, in part or empty, and workgroups go to the XCDs in turn: a slot's tiles are shared by all
+  // of them.  Eight species, 16 384 rows, 2 048 x 1 024, bf16: 138 us, 202 with runs of slots on one XCD.
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+  p.spread = p.grouped && tiles >= 8;
+  const int64_t groups = (slots ? slots : 1) * (p.spread ? (tiles + 7) / 8 * 8 : tiles);
   if (!fits_grid(groups, S::NT))
     return set_error(YE3T_EUNSUPPORTED, "weights of %d x %d for %lld species are too many for one launch", p.M, p.N,
                      (long long)p.groups);
@@ -299,7 +322,8 @@ int launch_shaped(WeightProduct<T> p, hipStream_t s) {
 template <typename T>
 int64_t weight_bytes(WeightProduct<T> p) {
   const int64_t groups = p.grouped ? p.groups : 1;
-  const int64_t some = share_plan(p.rows, groups, p.grouped, p.M, p.N, false).bytes, direct = share_plan(p.rows, groups, p.grouped, p.M, p.N, sizeof(T) == 2).bytes;
+  const int64_t some = share_plan(p.rows, groups, p.grouped, p.M, p.N, false).bytes;
+  const int64_t direct = share_plan(p.rows, groups, p.grouped, p.M, p.N, sizeof(T) == 2).bytes;
   return some > direct ? some : direct;
 }
 template int64_t weight_bytes(WeightProduct<float>);

@@ -56,6 +56,12 @@ int group(const SortPlan& p, const Index* tokens, int64_t rows, int64_t species,
   return check_launch("species_group_kernel");
 }
 
+// Few rows of up to 255 species are sorted in LDS alone.
+int64_t workspace_of(int64_t rows, int64_t species) {
+  const SortPlan p = sort_plan(rows, species);
+  return rows <= kSmallSort && p.passes == 1 ? 0 : p.bytes;
+}
+
 int check_species(int bytes, int64_t rows, int64_t species) {
   YE3T_REQUIRE(bytes == 4 || bytes == 8, "species must be int32 or int64");
   YE3T_REQUIRE(rows >= 0 && species >= 0, "row and species counts must not be negative");
@@ -74,7 +80,7 @@ extern "C" {
 int64_t ye3t_hip_species_groups_workspace_bytes(int64_t rows, int64_t species) {
   clear_error();
   if (check_species(4, rows, species)) return -1;
-  return sort_plan(rows, species).bytes;
+  return workspace_of(rows, species);
 }
 
 int ye3t_hip_species_groups(const void* species_of_rows, int species_bytes, int64_t rows, int64_t species, void* order,
@@ -83,7 +89,8 @@ int ye3t_hip_species_groups(const void* species_of_rows, int species_bytes, int6
   if (int rc = check_species(species_bytes, rows, species)) return rc;
   YE3T_REQUIRE(offsets && (rows == 0 || (species_of_rows && order)), "the groups need the rows' species and two outputs");
   const SortPlan p = sort_plan(rows, species);
-  YE3T_REQUIRE(rows == 0 || (workspace && workspace_bytes >= p.bytes),
+  const int64_t bytes = workspace_of(rows, species);
+  YE3T_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes),
                "the workspace is smaller than ye3t_hip_species_groups_workspace_bytes");
   const hipStream_t s = as_stream(stream);
   char* work = static_cast<char*>(workspace);

@@ -2140,9 +2140,10 @@ def species_groups(species, count):
     offsets = torch.empty(count + 1, dtype=torch.int64, device=species.device)
     with _on(species.device):
         size = lib().ye3t_hip_species_groups_workspace_bytes(N, count)
-        work = _workspace(size, "ye3t_hip_species_groups_workspace_bytes", species.device)
+        work = _workspace(size, "ye3t_hip_species_groups_workspace_bytes", species.device) if size else None
         _check(lib().ye3t_hip_species_groups(_dev(species, "species"), species.element_size(), N, count,
-                                             order.data_ptr(), offsets.data_ptr(), work.data_ptr(), size, _raw_stream()),
+                                             order.data_ptr(), offsets.data_ptr(), _opt(work, "workspace"), size,
+                                             _raw_stream()),
                "ye3t_hip_species_groups")
     return order, offsets
 
