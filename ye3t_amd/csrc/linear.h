@@ -301,23 +301,28 @@ __device__ inline void multiply_tiles(const __bf16* a, const __bf16* b, int wm, 
 // operands of the next one between its products, and the last of a tile meets the other waves first, so
 // that no product waits for a barrier.  With two buffers a tile's loads are issued in the first half
 // of the one before: in four parts, the last right before the wait, 8192^3 took 970 us, so 893.
-template <typename S, typename A, typename B, int LOADS, typename TileA, typename TileB, typename Load, typename With>
-__device__ inline void multiply_direct(int steps, TileA tile_a, TileB tile_b, int wm, int wn, int wk, int lane, Load load,
-                                       With with, f32x16 (*sum)[S::FN]) {
+// Where STARTED the first tile's loads have been issued, and `behind` (0, 16 or 32) memory operations or more after them.
+template <typename S, typename A, typename B, int LOADS, bool STARTED, typename TileA, typename TileB, typename Load,
+          typename With>
+__device__ inline void multiply_direct(int steps, int behind, TileA tile_a, TileB tile_b, int wm, int wn, int wk,
+                                       int lane, Load load, With with, f32x16 (*sum)[S::FN]) {
   typedef __bf16 T;
   constexpr int AHEAD = S::BUFFERS - 1, SUB = S::BK / 16, PARTS = AHEAD == 1 ? SUB / 2 : SUB;
   typedef std::integral_constant<int, 0> Zero;
   typedef std::integral_constant<int, 1> One;
 #pragma unroll
-  for (int t = 0; t < AHEAD; ++t)
+  for (int t = 0; t < AHEAD && !STARTED; ++t)
     if (t < steps) load(t, Zero(), One());
+  static_assert(!STARTED || AHEAD == 1, "one tile is loaded ahead");
   auto meet = [&](int t) {  // tile t is there, and tile t - 1 has been read
     if (t + AHEAD <= steps) arrive_and_meet<(AHEAD - 1) * LOADS>();
     else arrive_and_meet<0>();
   };
   Operands<T, S> o[2];
   if (steps) {
-    meet(0);
+    if (STARTED && behind >= 32) arrive_and_meet<32>();
+    else if (STARTED && behind >= 16) arrive_and_meet<16>();
+    else meet(0);
     read_operands<T, S, A, B>(tile_a(0), tile_b(0), wm, wn, wk * S::BK, lane, o[0]);
   }
   for (int t = 0; t < steps; ++t) {
@@ -399,21 +404,21 @@ __device__ inline void give_out(char* lds, const f32x16 (*sum)[S::FN], int wm, i
 }
 
 // The same without LDS: the halves of the wave exchange what makes eight columns of a lane's row whole.
-template <typename S, typename F>
+template <typename S, int BATCH, typename F>
 __device__ inline void hand_out(const f32x16 (*sum)[S::FN], int wm, int wn, int lane, F use) {
   const int half = lane / 32;
-  repeat<S::FM>([&](auto number) {
-    constexpr int i = decltype(number)::value, EACH = 2 * S::FN;
-    int r[EACH], c[EACH];
-    float v[EACH][8];
+  repeat<S::FM * 2 * S::FN / BATCH>([&](auto number) {
+    constexpr int first = decltype(number)::value * BATCH;
+    int r[BATCH], c[BATCH];
+    float v[BATCH][8];
 #pragma unroll
-    for (int n = 0; n < EACH; ++n) {
-      const int j = n / 2, b = n % 2 * 2;
+    for (int n = 0; n < BATCH; ++n) {
+      const int i = (first + n) / (2 * S::FN), j = (first + n) / 2 % S::FN, b = (first + n) % 2 * 2;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, float(sum[i][j][4 * b + q])),
-                                                           __builtin_bit_cast(unsigned, float(sum[i][j][4 * b + 4 + q])),
-                                                           false, false);
+        const unsigned x = __builtin_bit_cast(unsigned, float(sum[i][j][4 * b + q]));
+        const unsigned y = __builtin_bit_cast(unsigned, float(sum[i][j][4 * b + 4 + q]));
+        const auto both = __builtin_amdgcn_permlane32_swap(x, y, false, false);
         v[n][q] = __builtin_bit_cast(float, unsigned(both[0]));
         v[n][4 + q] = __builtin_bit_cast(float, unsigned(both[1]));
       }

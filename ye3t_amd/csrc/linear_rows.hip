@@ -136,8 +136,8 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
              [&](int n) { return k0 + (ACROSS ? b.line_of(n) : b.column_of(n)) < K; });
       }
     };
-    multiply_direct<S, A, B, LoadsA::kEach + LoadsB::kEach>(steps, tile_a, tile_b, wm, wn, wk, lane, load, [](int) {},
-                                                            sum);
+    multiply_direct<S, A, B, LoadsA::kEach + LoadsB::kEach, false>(steps, 0, tile_a, tile_b, wm, wn, wk, lane, load,
+                                                                   [](int) {}, sum);
   } else {
     const bool whole = !ACROSS || n0 + S::TN <= p.N;  // no chunk of b has columns past the last
     auto load = [&](int k0) {
@@ -193,8 +193,137 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
     }
     epilogue(p, weight, bias, seed, K, row, n, v);
   };
-  if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);
+  if constexpr (DIRECT) hand_out<S, 2 * S::FN>(sum, wm, wn, lane, finish);
   else give_out<S, sizeof(T) == 4 ? S::FN : 2 * S::FN>(lds, sum, wm, wn, wk, lane, finish);
+}
+
+// The same with tiles of direct loads that fill a compute unit: a workgroup goes through several, and the first loads
+// of the next run while the results of one are finished and written.  16 384 x 1 024 x 4 096: 132 us (1 036 TFLOP/s), 150
+// by a workgroup a tile; with gelu and the preactivation kept 186 and 207.  Bound by the matrix instructions' issue: at
+// 8 192^3 they run 57 % of the cycles, at a clock that falls with their share.
+template <typename S, bool ACROSS>
+__global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_rounds_kernel(const RowProduct<__bf16> p,
+                                                                                int64_t items) {
+  typedef __bf16 T;
+  typedef Tile<T, S::TM, S::KT, false> A;
+  typedef Tile<T, S::TN, S::KT, ACROSS> B;
+  typedef DirectLoads<S::TM, S::KT, false, S::NT> LoadsA;
+  typedef DirectLoads<S::TN, S::KT, ACROSS, S::NT> LoadsB;
+  constexpr int STEP = A::kBytes + B::kBytes;
+  static_assert(S::BUFFERS == 2 && S::WK == 1, "two buffers");
+  __shared__ __align__(256) char lds[2 * STEP];
+  const int lane = int(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int wn = wave % S::WN, wm = wave / S::WN;
+  auto tile_a = [&](int t) { return reinterpret_cast<T*>(lds + (t & 1) * STEP); };
+  auto tile_b = [&](int t) { return reinterpret_cast<T*>(lds + (t & 1) * STEP + A::kBytes); };
+
+  // This XCD's share of the tiles, and its workgroups that take them in turn
+  const int64_t all = items * p.tiles_n;
+  const unsigned x = blockIdx.x & 7, n = gridDim.x;
+  const int64_t begin = x * (all / 8) + (x < all % 8 ? x : all % 8), end = begin + all / 8 + (x < all % 8);
+  const unsigned workers = n / 8 + (x < n % 8);
+  int64_t next = begin + blockIdx.x / 8;
+
+  struct At {
+    int64_t row0, group;
+    int live, n0, K;
+  };
+  auto advance = [&](At& at) {
+    for (; next < end; next += workers) {
+      const Place place = place_of(next, items, p.tiles_n);
+      int64_t group = 0, first = place.row * S::TM, from = 0, length = p.rows;
+      int K = p.K;
+      if (p.grouped) {
+        const Item item = item_of(p.offsets, p.groups + 1, p.rows, 1, S::TM, place.row);
+        group = item.structure;
+        first = item.first;
+        from = clamped(p.offsets[group], p.rows);
+        length = (group < p.groups ? clamped(p.offsets[group + 1], p.rows) : p.rows) - from;
+        if (group == p.groups) K = 0;  // rows behind the last group
+      }
+      if (first >= length) continue;
+      const int live = length - first < S::TM ? int(length - first) : S::TM;
+      at = {from + first, group, live, place.column * S::TN, K};
+      next += workers;
+      return true;
+    }
+    return false;
+  };
+
+  const T *a_from[LoadsA::kEach], *b_from[LoadsB::kEach];
+  const int64_t b_step = ACROSS ? S::KT * p.b_row : S::KT;
+  At at;
+  auto load = [&](int t, auto part, auto parts) {
+    auto each = [&](auto loads, T* tile, const T** from, int64_t step, auto exists) {
+      constexpr int EACH = decltype(loads)::kEach, P = decltype(part)::value, OF = decltype(parts)::value;
+#pragma unroll
+      for (int k = EACH * P / OF; k < EACH * (P + 1) / OF; ++k) {
+        loads.load(tile, k, wave, exists(k) ? from[k] : loads.none());
+        from[k] += step;
+      }
+    };
+    const int k0 = t * S::KT;
+    if (k0 + S::KT <= at.K) {
+      each(LoadsA(), tile_a(t), a_from, S::KT, [](int) { return true; });
+      each(LoadsB(), tile_b(t), b_from, b_step, [](int) { return true; });
+    } else {
+      each(LoadsA(), tile_a(t), a_from, S::KT, [&](int k) { return k0 + LoadsA::column_of(k) < at.K; });
+      each(LoadsB(), tile_b(t), b_from, b_step,
+           [&](int k) { return k0 + (ACROSS ? LoadsB::line_of(k) : LoadsB::column_of(k)) < at.K; });
+    }
+  };
+  auto start = [&] {
+#pragma unroll
+    for (int k = 0; k < LoadsA::kEach; ++k) {
+      const int line = LoadsA::line_of(k);
+      const int64_t row = row_at(p.order, at.row0 + (line < at.live ? line : 0), p.rows);
+      a_from[k] = p.a + (row < 0 ? 0 : row) * p.a_row + LoadsA::column_of(k);
+    }
+    const T* weight = p.b + at.group * p.b_group;
+#pragma unroll
+    for (int k = 0; k < LoadsB::kEach; ++k) {
+      const int line = LoadsB::line_of(k), c = LoadsB::column_of(k);
+      b_from[k] = ACROSS ? weight + line * p.b_row + (at.n0 + c < p.N ? at.n0 + c : 0)
+                         : weight + (at.n0 + line < p.N ? at.n0 + line : 0) * p.b_row + c;
+    }
+    if (at.K > 0) load(0, std::integral_constant<int, 0>(), std::integral_constant<int, 1>());
+    asm volatile("" ::: "memory");  // the loads stay before what follows
+  };
+
+  const uint64_t seed = p.dropout.below ? seed_of(p.dropout) : 0;
+  if (!advance(at)) return;
+  start();
+  int behind = 0;
+  for (;;) {
+    f32x16 sum[S::FM][S::FN];
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) sum[i][j] = zeros();
+    multiply_direct<S, A, B, LoadsA::kEach + LoadsB::kEach, true>((at.K + S::KT - 1) / S::KT, behind, tile_a, tile_b, wm,
+                                                                  wn, 0, lane, load, [](int) {}, sum);
+    const At done = at;
+    // every wave has read its last operands before the next tile's loads take their place
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool more = advance(at);
+    if (more) start();
+    const T* bias = p.bias && !(p.grouped && done.group == p.groups) ? p.bias + done.group * p.N : nullptr;
+    hand_out<S, S::FN>(sum, wm, wn, lane, [&](const auto& r, const auto& c, auto& v) {
+      constexpr int EACH = sizeof(v) / sizeof(v[0]);
+      int64_t row[EACH];
+      int column[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        row[e] = r[e] < done.live ? row_at(p.order, done.row0 + r[e], p.rows) : -1;
+        column[e] = done.n0 + c[e];
+      }
+      epilogue(p, p.b, bias, seed, done.K, row, column, v);
+    });
+    if (!more) return;
+    // A whole tile's results are a store for every eight columns of 64 rows, in two outputs or one.
+    const bool whole = done.live == S::TM && done.n0 + S::TN <= p.N && !p.order;
+    behind = whole ? (p.kept ? 2 : 1) * S::FM * S::FN * 2 : 0;
+  }
 }
 
 // Adds the parts of the contraction in order and goes on as the product's own epilogue.  A lane a chunk of eight columns.
@@ -243,6 +372,18 @@ int launch_shaped(RowProduct<T> p, hipStream_t s) {
   hipLaunchKernelGGL((row_join_kernel<T>), dim3(unsigned((p.rows * chunks + kJoinThreads - 1) / kJoinThreads)),
                      dim3(kJoinThreads), 0, s, p, int(chunks));
   return check_launch("row_join_kernel");
+}
+
+constexpr int kComputeUnits = 256;
+
+template <typename S>
+int launch_rounds(RowProduct<__bf16> p, hipStream_t s) {
+  const int64_t items = p.grouped ? item_count(p.rows, p.groups + 1, S::TM) : (p.rows + S::TM - 1) / S::TM;
+  p.tiles_n = unsigned((p.N + S::TN - 1) / S::TN);
+  const int64_t all = items * p.tiles_n;
+  hipLaunchKernelGGL((p.b_across ? row_product_rounds_kernel<S, true> : row_product_rounds_kernel<S, false>),
+                     dim3(unsigned(all < kComputeUnits ? all : kComputeUnits)), dim3(S::NT), 0, s, p, items);
+  return check_launch("row_product_rounds_kernel");
 }
 
 template <typename T>
@@ -328,7 +469,7 @@ int launch_rows(RowProduct<T> p, void* work, hipStream_t s) {
   p.part_steps = c.part_steps;
   p.part = static_cast<float*>(work);
   if constexpr (sizeof(T) == 2) {
-    if (c.kind == kSquare) return launch_shaped<T, typename Shapes<T>::Square, true>(p, s);
+    if (c.kind == kSquare) return launch_rounds<typename Shapes<T>::Square>(p, s);
     if (c.kind == kDirect) return launch_shaped<T, typename Shapes<T>::Direct, true>(p, s);
   }
   if constexpr (sizeof(T) == 4) {

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
       }
       if (P + 1 == OF) look(t + 1);
     };
-    multiply_direct<S, A, B, 2 * EACH>(steps, tile_a, tile_b, wm, wn, wk, lane, load, add_columns, sum);
+    multiply_direct<S, A, B, 2 * EACH, false>(steps, 0, tile_a, tile_b, wm, wn, wk, lane, load, add_columns, sum);
   } else {
     Loads<T, S::TM, S::KT, true, S::NT> a;
     Loads<T, S::TN, S::KT, true, S::NT> b;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
       }
     }
   };
-  if constexpr (DIRECT) hand_out<S>(sum, wm, wn, lane, finish);
+  if constexpr (DIRECT) hand_out<S, 2 * S::FN>(sum, wm, wn, lane, finish);
   else give_out<S, S::FN>(lds, sum, wm, wn, wk, lane, finish);
 }
 
