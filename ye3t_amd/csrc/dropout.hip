@@ -1,7 +1,8 @@
 // y = residual + dropout(x), and its gradient, which is the same without a residual.
 //
-// A lane takes eight columns of a row, one call of the generator.  Bound by memory:
-// the generator's products take less than the rows' reads and writes.
+// A lane takes eight columns of a row, one call of the generator, and two such chunks at a time.  Bound by
+// memory: 200 000 x 513 in bf16, rows that start at any multiple of two bytes, 138 us with a residual (4.5 TB/s) and 91
+// without; the generator's twenty products a call take about a third of that.
 #include "random.h"
 #include "rows.h"
 
