@@ -220,6 +220,24 @@ def test_empty_sizes(gpu, dtype, rows, inputs, outputs, species):
     assert runtime.dropout(x.detach(), 0.5, 1).shape == x.shape
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_atoms_without_any_species(gpu, dtype):
+    """No species at all, and atoms: products and gradients of zero."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    for rows in (5, 3000):
+        x, w, b = normal((rows, 264), dtype, 1, gpu), normal((0, 264, 136), dtype, 2, gpu), normal((0, 136), dtype, 3, gpu)
+        r, g = normal((rows, 136), dtype, 4, gpu), normal((rows, 136), dtype, 5, gpu)
+        groups = runtime.species_groups(torch.zeros(rows, dtype=torch.int64, device=gpu), 0, validate=False)
+        assert groups.offsets.tolist() == [0]
+        y, z = runtime.species_linear(x, w, groups, b, activation="gelu", residual=r, return_preactivation=True)
+        assert torch.equal(y, r) and not z.any()
+        dx, dw, db = runtime.species_linear_adjoint(g, x, w, groups, preactivation=z, activation="gelu", bias=True)
+        assert dx.shape == x.shape and not dx.any() and dw.shape == w.shape and db.shape == b.shape
+
+
 # ---- autograd --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", TYPES)
