@@ -184,7 +184,14 @@ struct Loads {
 #pragma unroll
     for (int n = 0; n < kEach; ++n) held[n] = Chunk<T, 8>::load(from[n]);
   }
-  // left(n): values that exist from from[n] on
+  // left(n): values that exist from from[n] on.  Eight or none, which needs no branches (1 000 x 1 000 x 1 000 in
+  // bf16, whose last tiles are all of these: 14 us with them, 11 without), or any number.
+  template <typename L>
+  __device__ inline void load_chunks(const T* const* from, L left) {
+#pragma unroll
+    for (int n = 0; n < kEach; ++n)
+      held[n] = Chunk<T, 8>::load(left(n) > 0 ? from[n] : reinterpret_cast<const T*>(kZeros));
+  }
   template <typename L>
   __device__ inline void load(const T* const* from, L left) {
 #pragma unroll

@@ -146,15 +146,23 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
                                                                    [](int) {}, sum);
   } else {
     const bool whole = !ACROSS || n0 + S::TN <= p.N;  // no chunk of b has columns past the last
+    const bool chunks = K % 8 == 0 && (!ACROSS || p.N % 8 == 0);  // every chunk is there or not
     auto load = [&](int k0) {
       if (k0 + S::KT <= K && whole) {
         a.load(a_from);
         b.load(b_from);
       } else {
-        a.load(a_from, [&](int n) { return K - k0 - a.column_of(n); });
-        b.load(b_from, [&](int n) {
+        auto a_left = [&](int n) { return K - k0 - a.column_of(n); };
+        auto b_left = [&](int n) {
           return !ACROSS ? K - k0 - b.column_of(n) : k0 + b.line_of(n) < K ? p.N - n0 - b.column_of(n) : 0;
-        });
+        };
+        if (chunks) {
+          a.load_chunks(a_from, a_left);
+          b.load_chunks(b_from, b_left);
+        } else {
+          a.load(a_from, a_left);
+          b.load(b_from, b_left);
+        }
       }
 #pragma unroll
       for (int n = 0; n < LoadsA::kEach; ++n) a_from[n] += S::KT;
@@ -407,7 +415,7 @@ struct Shapes<float> {
   typedef Shape<2, 2, 1, 2, 2, 32, 1, 3> Large;
   typedef Shape<2, 2, 1, 2, 1, 32, 1, 3> Tall;
   typedef Shape<2, 2, 1, 1, 1, 32, 1, 3> Middle;
-  typedef Shape<1, 1, 8, 1, 1, 32, 1, 2> Few;
+  typedef Shape<1, 1, 8, 1, 1, 16, 1, 4> Few;
 };
 
 // Whether every chunk of eight values of both operands is whole and aligned
@@ -451,9 +459,12 @@ Choice choice_of(const RowProduct<T>& p, bool direct) {
   if (p.rows > 32 && tiles(64) >= 256) return {kMiddle, 1, 0};
   const int64_t groups = ((p.rows + 31) / 32 + (p.grouped ? p.groups : 0)) * ((p.N + 31) / 32);
   const int steps = (p.K + Shapes<T>::Few::KT - 1) / Shapes<T>::Few::KT;
-  if (steps < 4 || groups > 256) return {kFew, 1, 0};
-  int parts = int(512 / groups);
-  if (parts > steps / 2) parts = steps / 2;
+  const int least = 2 * Shapes<T>::Few::KT < 512 ? 512 : 2 * Shapes<T>::Few::KT;  // of the contraction, for a part
+  // as many workgroups as run at a time; 64 x 4 096 x 4 096: bf16 13 us, by twice as many 17; fp32 36 and 32
+  const int64_t most = sizeof(T) == 4 ? 512 : 256;
+  int parts = p.K / least;
+  if (parts < 2 || groups > most / 2) return {kFew, 1, 0};
+  if (parts > most / groups) parts = int(most / groups);
   const int each = (steps + parts - 1) / parts;
   return {kFew, (steps + each - 1) / each, each};
 }

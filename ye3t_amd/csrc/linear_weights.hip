@@ -129,8 +129,15 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(cons
         a.load(a_from);
         b.load(b_from);
       } else {
-        a.load(a_from, [&](int n) { return row[n] < 0 ? 0 : p.M - m0 - a.column_of(n); });
-        b.load(b_from, [&](int n) { return row[n] < 0 ? 0 : p.N - n0 - b.column_of(n); });
+        auto a_left = [&](int n) { return row[n] < 0 ? 0 : p.M - m0 - a.column_of(n); };
+        auto b_left = [&](int n) { return row[n] < 0 ? 0 : p.N - n0 - b.column_of(n); };
+        if (p.M % 8 == 0 && p.N % 8 == 0) {
+          a.load_chunks(a_from, a_left);
+          b.load_chunks(b_from, b_left);
+        } else {
+          a.load(a_from, a_left);
+          b.load(b_from, b_left);
+        }
       }
       look(t + 1);
     };

@@ -50,7 +50,7 @@ __device__ inline int turn(int line) {
 // registers than the products leave.
 __device__ inline void in_turn() { __builtin_amdgcn_sched_barrier(0); }
 
-__device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
+__device__ __align__(16) const uint32_t kZeros[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 
 __device__ inline void arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
