@@ -18,10 +18,11 @@
 // six terms hh, hm, mh, mm, hl, lh; those left out are below 2^-26 of it, less than
 // fp32's own rounding (Henry, Tang and Heinecke, "Leveraging the bfloat16
 // artificial intelligence datatype for higher-precision computations", 2019).  Six bf16
-// instructions of 32 cycles cover what eight fp32 ones of 64 would.  Values of 2^-110 and below lose their last bits, 2^-133 at most.  A value
-// that is not finite, or rounds to infinity in bf16, would leave NaN where fp32
-// leaves an infinity or a number: results that are not finite are computed
-// again, value by value in fp32 (exact_dots).
+// instructions of 32 cycles cover what eight fp32 ones of 64 would.  Values of 2^-110
+// and below lose their last bits, 2^-133 at most.  A value that is not finite, or
+// rounds to infinity in bf16, would leave NaN where fp32 leaves an infinity or a
+// number: results that are not finite are computed again, value by value in fp32
+// (exact_dots).
 #pragma once
 
 #include <type_traits>
