@@ -334,7 +334,9 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_rounds_kernel(
       epilogue(p, p.b, bias, seed, done.K, row, column, v);
     });
     if (!more) return;
-    // A whole tile's results are a store for every eight columns of 64 rows, in two outputs or one.
+    // A whole tile's results are a store for every eight columns of 64 rows, in two outputs or one: 32 or 16, the counts
+    // that multiply_direct waits by.
+    static_assert(S::FM * S::FN * 2 == 16, "multiply_direct knows the stores of a tile");
     const bool whole = done.live == S::TM && done.n0 + S::TN <= p.N && !p.order;
     behind = whole ? (p.kept ? 2 : 1) * S::FM * S::FN * 2 : 0;
   }
