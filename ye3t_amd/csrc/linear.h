@@ -5,7 +5,7 @@
 //
 // Gradient for the adjoint g of y:
 //
-//   dz = D(g) act'(z),  dx = dz W^T,  dW = x^T dz,  db = sum of dz over rows
+//   dz = D(g act'(z)),  dx = dz W^T,  dW = x^T dz,  db = sum of dz over rows
 //
 // Rows of one species are found through an order of the rows (species.hip), so
 // neither x nor y is moved.  A workgroup owns a tile of one species' rows (forward and dx,
