@@ -57,3 +57,31 @@ def test_dropped_values_through_autograd(gpu, dtype):
     assert torch.equal(torch.isfinite(y).all(1).cpu(), gone) and gone.any()
     y[gone.to(gpu)].sum().backward()
     assert torch.isfinite(x.grad[gone.to(gpu)]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dropout", [0.0, 0.25])
+def test_relu_passes_or_stops(gpu, dtype, dropout):
+    """relu's gradient is the adjoint where relu gave the preactivation, NaN among them, and zero where it gave zero, whatever
+    the adjoint holds."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"relu, dropout {dropout}, {dtype}")
+    inf, nan = float("inf"), float("nan")
+    z = torch.tensor([-inf, -1.0, -0.0, 0.0, 1e-30, 2.0, inf, nan], device=gpu).to(getattr(torch, dtype)).repeat(5, 1)
+    g = torch.tensor([1.0, inf, -inf, nan, 3.0], device=gpu).to(z.dtype)[:, None].expand(5, 8).contiguous()
+    # the gradient of the input is dz itself: a weight of one column for each
+    x, w = torch.zeros(5, 8, dtype=z.dtype, device=gpu), torch.eye(8, dtype=z.dtype, device=gpu)
+    passed = torch.where(z <= 0, torch.zeros_like(g), g)
+    for k in range(8):  # a column alone: zero times infinity in the others' products is no number
+        dx, _, db = runtime.linear_adjoint(g[:, k:k + 1].contiguous(), x, w[:, k:k + 1], preactivation=z[:, k:k + 1].contiguous(),
+                                           bias=True, activation="relu", dropout=dropout, seed=3 if dropout else None)
+        mask = plain.kept(5, 1, dropout, 3, 0).to(gpu) if dropout else torch.ones(5, 1, device=gpu)
+        one = torch.where(mask == 0, torch.zeros_like(g[:, :1]), (passed[:, k:k + 1].float() * mask).to(z.dtype))
+        assert torch.equal(torch.isnan(dx[:, k:k + 1]), torch.isnan(one))
+        there = ~torch.isnan(one)
+        assert torch.equal(dx[:, k:k + 1][there], one[there])
+        total = one.double().sum(0)
+        assert torch.isnan(db.double()).equal(torch.isnan(total)) and (torch.isnan(total).any() or torch.equal(db.double(), total))

@@ -86,17 +86,16 @@ __device__ inline void activate(int act, float* v) {
   }
 }
 
-__device__ inline float slope_of(int act, float z) {
-  if (act == kRelu) return z > 0.0f ? 1.0f : 0.0f;
+// g act'(z).  relu passes g or stops it: a unit that is dead gives zero for an infinite g too, and one of NaN, which
+// activate() passes, passes g.
+__device__ inline float through(int act, float g, float z) {
+  if (act == kRelu) return z <= 0.0f ? 0.0f : g;
   if (act == kSilu) {
     const Logistic e = logistic_of(z);
-    return fmaf(z * e.scaled, 1.0f - e.scaled * e.unit, e.scaled) * e.unit;
+    return g * (fmaf(z * e.scaled, 1.0f - e.scaled * e.unit, e.scaled) * e.unit);
   }
-  if (act == kGelu) {
-    const Normal n = normal_of(z);
-    return n.phi + z * n.bell * 0.398942280f;
-  }
-  return 1.0f;
+  const Normal n = normal_of(z);
+  return g * (n.phi + z * n.bell * 0.398942280f);
 }
 
 // f(0) .. f(N - 1) with the number as a type

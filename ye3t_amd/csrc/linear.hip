@@ -28,7 +28,7 @@ __global__ __launch_bounds__(kThreads) void epilogue_adjoint_kernel(const T* __r
     if (activation != kNone) {
       const Chunk<T, 8> z = Chunk<T, 8>::load(kept + row * N + n, left);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] *= slope_of(activation, float(z.v[q]));
+      for (int q = 0; q < 8; ++q) v[q] = through(activation, v[q], float(z.v[q]));
     }
     if (d.below) drop(d, seed, row, uint32_t(n) / 8, v);
     Chunk<T, 8> out;

@@ -246,7 +246,8 @@ def linear(input, weight, bias=None, *, activation=None, residual=None, dropout=
     ``[outputs, inputs]`` is read as it lies), ``bias [outputs]``, ``residual
     [..., outputs]``, one dtype (float32 or bfloat16).  Returns ``[..., outputs]``.
 
-    * ``activation``: None, ``"relu"``, ``"silu"`` (``z / (1 + exp(-z))``) or
+    * ``activation``: None, ``"relu"`` (zero up to zero; NaN and its gradient
+      pass), ``"silu"`` (``z / (1 + exp(-z))``) or
       ``"gelu"`` (``z`` times the normal distribution's integral up to ``z``).
     * ``dropout``, ``seed``, ``layer``: D drops values as :func:`dropout` does.
     * ``return_preactivation``: also ``input weight + bias``, rounded, which
