@@ -993,8 +993,8 @@ int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args);
  * rounded preactivation (NULL without an activation): input_adjoint [rows,
  * inputs], weight_adjoint in the weight's layout without gaps, bias_adjoint
  * [groups, outputs]; each may be NULL, the weight's only with the bias's.  The
- * residual's is the adjoint itself.  dz = D(adjoint act') is rounded to `dtype`; dropped
- * values have none, whatever they held. */
+ * residual's is the adjoint itself.  dz = D(adjoint act') is rounded to `dtype` for the two
+ * products, not for the bias's sums; dropped values have none, whatever they held. */
 int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, const void* preactivation,
                             void* input_adjoint, void* weight_adjoint, void* bias_adjoint, void* workspace,
                             int64_t workspace_bytes, ye3t_stream_t stream);

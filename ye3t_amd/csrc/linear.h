@@ -484,6 +484,11 @@ __device__ inline int64_t row_at(const int32_t* order, int64_t i, int64_t rows) 
   return r >= 0 && r < rows ? r : -1;
 }
 
+// Sums over the rows of each group in shares: where those of a group's shares begin, of which only groups of several have
+// any, and how many there are.
+__device__ inline int64_t part_of(int64_t begin, int64_t share) { return 2 * begin / share; }
+inline int64_t part_count(int64_t rows, int64_t share) { return share < rows ? 2 * rows / share + 1 : 0; }
+
 inline int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // ---- the two kinds of product ----------------------------------------------------

@@ -38,6 +38,133 @@ __global__ __launch_bounds__(kThreads) void epilogue_adjoint_kernel(const T* __r
   }
 }
 
+// The same in bf16 with the bias's gradient, summed of dz before it is rounded: it is a sum and takes no matrix instruction
+// (16 384 x 4 096, gelu: 1.7e-3 from 64 bits, the last rounding; of the rounded dz 2.4e-3).  A workgroup goes through a share of
+// one group's rows, `across` lanes of eight columns and the others down the rows, two rows of a lane in flight; shares of a group
+// that has several leave their sums in fp32, and a second kernel adds them in order.  78 us at that size, and 4 for the join.
+struct BiasSums {
+  int64_t groups;
+  bool grouped;
+  const int32_t* order;
+  const int64_t* offsets;
+  int across;           // a power of two
+  unsigned columns;     // workgroups along the columns
+  int64_t share;
+  __bf16* sums;         // [groups][N]
+  float* part;          // [part_count(rows, share)][N]
+};
+
+__global__ __launch_bounds__(kThreads) void epilogue_adjoint_sums_kernel(const __bf16* __restrict__ adjoint,
+                                                                         const __bf16* __restrict__ kept, int64_t rows,
+                                                                         int N, int activation, Dropout d, BiasSums b,
+                                                                         __bf16* __restrict__ dz) {
+  constexpr int STEPS = 2;
+  __shared__ float held[kThreads * 8];
+  const int64_t slot = blockIdx.x / b.columns;
+  const int column = int(threadIdx.x) & (b.across - 1), line = int(threadIdx.x) / b.across, down = kThreads / b.across;
+  const int n0 = int(blockIdx.x % b.columns) * b.across * 8, n = n0 + column * 8, left = N - n;
+  int64_t group = 0, begin = 0, first = slot * b.share, length = rows;
+  if (b.grouped) {
+    auto bound = [&](int64_t g) { return clamped(b.offsets[g], rows) / b.share + g; };
+    group = find_owner(b.groups, slot, bound);
+    first = (slot - bound(group)) * b.share;
+    begin = clamped(b.offsets[group], rows);
+    length = clamped(b.offsets[group + 1], rows) - begin;
+  }
+  if (first && first >= length) return;  // the first share of a group without rows writes its zeros
+  const int64_t row0 = begin + first, rest = length - first;
+  const int live = int(rest < 0 ? 0 : rest < b.share ? rest : b.share);
+  const uint64_t seed = d.below ? seed_of(d) : 0;
+  float sum[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sum[q] = 0.0f;
+  for (int k0 = line; left > 0 && k0 < live; k0 += STEPS * down) {
+    Chunk<__bf16, 8> g[STEPS], z[STEPS];
+    int64_t row[STEPS];
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e) {
+      const int k = k0 + e * down;
+      row[e] = k < live ? row_at(b.order, row0 + k, rows) : -1;
+      if (row[e] < 0) continue;
+      g[e] = Chunk<__bf16, 8>::load(adjoint + row[e] * N + n, left);
+      if (activation != kNone) z[e] = Chunk<__bf16, 8>::load(kept + row[e] * N + n, left);
+    }
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e) {
+      if (row[e] < 0) continue;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = float(g[e].v[q]);
+      if (activation != kNone) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = through(activation, v[q], float(z[e].v[q]));
+      }
+      if (d.below) drop(d, seed, row[e], uint32_t(n) / 8, v);
+      Chunk<__bf16, 8> out;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        sum[q] += v[q];
+        out.v[q] = __bf16(v[q]);
+      }
+      out.store(dz + row[e] * N + n, left);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) held[int(threadIdx.x) * 8 + q] = sum[q];
+  __syncthreads();
+  const int c = int(threadIdx.x);
+  if (c >= b.across * 8 || n0 + c >= N) return;
+  float s = 0.0f;
+#pragma unroll 16
+  for (int k = 0; k < down; ++k) s += held[k * b.across * 8 + c];
+  if (length <= b.share) b.sums[group * N + n0 + c] = __bf16(s);
+  else b.part[(part_of(begin, b.share) + first / b.share) * N + n0 + c] = s;
+}
+
+// A lane a column of a group that has several shares, sixteen lanes its shares
+__global__ __launch_bounds__(kThreads) void bias_join_kernel(BiasSums b, int64_t rows, int N) {
+  constexpr int COLUMNS = 16, DOWN = kThreads / COLUMNS;
+  __shared__ float held[DOWN][COLUMNS];
+  const int column = int(threadIdx.x) % COLUMNS, line = int(threadIdx.x) / COLUMNS, n = int(blockIdx.x) * COLUMNS + column;
+  for (int64_t g = blockIdx.y; g < (b.grouped ? b.groups : 1); g += gridDim.y) {
+    const int64_t begin = b.grouped ? clamped(b.offsets[g], rows) : 0;
+    const int64_t length = (b.grouped ? clamped(b.offsets[g + 1], rows) : rows) - begin;
+    if (length <= b.share) continue;  // the same for all lanes
+    const float* from = b.part + part_of(begin, b.share) * N + n;
+    const int shares = int((length + b.share - 1) / b.share);
+    float s = 0.0f;
+    if (n < N) {
+#pragma unroll 8
+      for (int k = line; k < shares; k += DOWN) s += from[int64_t(k) * N];
+    }
+    held[line][column] = s;
+    __syncthreads();
+    if (line == 0 && n < N) {
+#pragma unroll
+      for (int k = 1; k < DOWN; ++k) s += held[k][column];
+      b.sums[g * N + n] = __bf16(s);
+    }
+    __syncthreads();
+  }
+}
+
+// Shares that make about 4 096 workgroups, 512 at most of one group for the join, of a lane's two rows at least.  Sixteen
+// lanes across and these shares: 16 384 x 4 096 78 us, by eight and half as many workgroups 94; 2 000 x 512 7 and 14.
+BiasSums bias_sums(const ye3t_linear_args& a) {
+  BiasSums b{};
+  b.grouped = a.groups_given != 0;
+  b.groups = a.groups;
+  b.order = b.grouped ? a.order : nullptr;
+  b.offsets = b.grouped ? a.offsets : nullptr;
+  for (b.across = 1; b.across < 16 && b.across * 8 < a.outputs; b.across *= 2) {}
+  b.columns = unsigned((a.outputs + b.across * 8 - 1) / (b.across * 8));
+  const int64_t all = (a.rows * b.columns + 4095) / 4096, most = (a.rows + 511) / 512, least = 2 * kThreads / b.across;
+  b.share = all > most ? all : most;
+  if (b.share < least) b.share = least;
+  if (b.share > (1 << 30)) b.share = 1 << 30;
+  return b;
+}
+
 int check_linear(const ye3t_linear_args& a) {
   constexpr int64_t most = (int64_t(1) << 31) - 256;
   YE3T_REQUIRE(a.rows >= 0 && a.inputs >= 0 && a.outputs >= 0 && a.groups >= 0, "sizes must not be negative");
@@ -136,9 +263,14 @@ WeightProduct<T> weights_of(const ye3t_linear_args& a, const T* dz) {
   return p;
 }
 
-// dz in the workspace and the sums of the shares behind it; the same whatever the adjoint's address is.
+// dz in the workspace, the bias's sums of its shares of rows behind it, and the sums of the products' shares behind those; the
+// same whatever the adjoint's address is.
 int64_t dz_bytes(const ye3t_linear_args& a) {
   return shaped(a) ? up(a.rows * a.outputs * (a.dtype == YE3T_F32 ? 4 : 2)) : 0;
+}
+int64_t bias_bytes(const ye3t_linear_args& a) {
+  if (!shaped(a) || a.dtype == YE3T_F32 || a.rows == 0 || a.outputs == 0) return 0;
+  return up(part_count(a.rows, bias_sums(a).share) * a.outputs * 4);
 }
 // dx and dW are made one after the other: what one takes for its parts the other takes after it.
 int64_t adjoint_bytes(const ye3t_linear_args& a) {
@@ -146,34 +278,70 @@ int64_t adjoint_bytes(const ye3t_linear_args& a) {
                                             : row_bytes(backward_of<__bf16>(a, nullptr));
   const int64_t shares = a.dtype == YE3T_F32 ? weight_bytes(weights_of<float>(a, nullptr))
                                              : weight_bytes(weights_of<__bf16>(a, nullptr));
-  return dz_bytes(a) + (shares > parts ? shares : parts) + 256;
+  return dz_bytes(a) + bias_bytes(a) + (shares > parts ? shares : parts) + 256;
+}
+
+template <typename T>
+int launch_epilogue(const ye3t_linear_args& a, const T* adjoint, const T* kept, T* dz, hipStream_t s) {
+  const int64_t chunks = (a.outputs + 7) / 8;
+  int64_t groups = (a.rows * chunks + kThreads - 1) / kThreads;
+  if (groups > (1 << 20)) groups = 1 << 20;
+  hipLaunchKernelGGL((epilogue_adjoint_kernel<T>), dim3(unsigned(groups)), dim3(kThreads), 0, s, adjoint, kept, a.rows,
+                     int(a.outputs), int(chunks), a.activation, dropout_of(a.drop_below, a.layer, a.seed, a.device_seed), dz);
+  return check_launch("epilogue_adjoint_kernel");
+}
+
+int launch_epilogue_sums(const ye3t_linear_args& a, const __bf16* adjoint, const __bf16* kept, __bf16* dz, __bf16* sums,
+                         void* part, hipStream_t s) {
+  BiasSums b = bias_sums(a);
+  b.sums = sums;
+  b.part = static_cast<float*>(part);
+  const int64_t slots = b.grouped ? a.rows / b.share + b.groups : (a.rows + b.share - 1) / b.share;
+  if (!fits_grid(slots * b.columns, kThreads))
+    return set_error(YE3T_EUNSUPPORTED, "biases of %lld for %lld species are too many for one launch", (long long)a.outputs,
+                     (long long)a.groups);
+  hipLaunchKernelGGL(epilogue_adjoint_sums_kernel, dim3(unsigned(slots * b.columns)), dim3(kThreads), 0, s, adjoint, kept,
+                     a.rows, int(a.outputs), a.activation, dropout_of(a.drop_below, a.layer, a.seed, a.device_seed), b, dz);
+  if (int rc = check_launch("epilogue_adjoint_sums_kernel")) return rc;
+  if (a.rows <= b.share) return YE3T_OK;
+  const int64_t groups = b.grouped ? b.groups : 1;
+  hipLaunchKernelGGL(bias_join_kernel, dim3(unsigned((a.outputs + 15) / 16), unsigned(groups < 65535 ? groups : 65535)),
+                     dim3(kThreads), 0, s, b, a.rows, int(a.outputs));
+  return check_launch("bias_join_kernel");
 }
 
 template <typename T>
 int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept, void* input_adjoint,
                void* weight_adjoint, void* bias_adjoint, char* work, hipStream_t s) {
   const T* dz = static_cast<const T*>(adjoint);
+  char* behind = work + dz_bytes(a) + bias_bytes(a);
   if (shaped(a) && a.rows > 0 && a.outputs > 0) {
     T* to = reinterpret_cast<T*>(work);
-    const int64_t chunks = (a.outputs + 7) / 8;
-    int64_t groups = (a.rows * chunks + kThreads - 1) / kThreads;
-    if (groups > (1 << 20)) groups = 1 << 20;
-    hipLaunchKernelGGL((epilogue_adjoint_kernel<T>), dim3(unsigned(groups)), dim3(kThreads), 0, s, dz,
-                       static_cast<const T*>(kept), a.rows, int(a.outputs), int(chunks), a.activation,
-                       dropout_of(a.drop_below, a.layer, a.seed, a.device_seed), to);
-    if (int rc = check_launch("epilogue_adjoint_kernel")) return rc;
+    bool summed = false;
+    if constexpr (sizeof(T) == 2) {
+      summed = bias_adjoint && (!a.groups_given || a.groups > 0);
+      if (summed) {
+        if (int rc = launch_epilogue_sums(a, dz, static_cast<const T*>(kept), to, static_cast<T*>(bias_adjoint),
+                                          work + dz_bytes(a), s))
+          return rc;
+        bias_adjoint = nullptr;  // made
+      }
+    }
+    if (!summed) {
+      if (int rc = launch_epilogue(a, dz, static_cast<const T*>(kept), to, s)) return rc;
+    }
     dz = to;
   }
   if (input_adjoint) {
     RowProduct<T> p = backward_of(a, dz);
     p.out = static_cast<T*>(input_adjoint);
-    if (int rc = launch_rows(p, work + dz_bytes(a), s)) return rc;
+    if (int rc = launch_rows(p, behind, s)) return rc;
   }
   if (weight_adjoint || bias_adjoint) {
     WeightProduct<T> p = weights_of<T>(a, dz);
     p.out = static_cast<T*>(weight_adjoint);
     p.sums = static_cast<T*>(bias_adjoint);
-    if (int rc = launch_weights(p, work + dz_bytes(a), s)) return rc;
+    if (int rc = launch_weights(p, behind, s)) return rc;
   }
   return YE3T_OK;
 }

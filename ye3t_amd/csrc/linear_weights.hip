@@ -11,9 +11,6 @@ namespace ye3t {
 namespace linear {
 namespace {
 
-// Where the sums of a group's shares begin; only groups of several shares have any there.
-__device__ inline int64_t part_of(int64_t begin, int64_t share) { return 2 * begin / share; }
-
 template <typename T, typename S, bool DIRECT>
 __global__ __launch_bounds__(S::NT, S::kPerSimd) void weight_product_kernel(const WeightProduct<T> p) {
   typedef Tile<T, S::TM, S::KT, true> A;
@@ -302,7 +299,7 @@ SharePlan share_plan(int64_t rows, int64_t groups, bool grouped, int64_t M, int6
   f.share = (rows + parts - 1) / parts;
   if (f.share < kLeastShare) f.share = kLeastShare;
   if (f.share > (1 << 30)) f.share = 1 << 30;
-  f.slots = f.share < rows ? 2 * rows / f.share + 1 : 0;
+  f.slots = part_count(rows, f.share);
   f.part_bytes = up(f.slots * M * N * 4);
   f.sums_bytes = up(f.slots * (M > N ? M : N) * 4);
   f.bytes = f.part_bytes + f.sums_bytes;

@@ -7,7 +7,7 @@ by species once for all layers.  Storage is float32 or bfloat16; sums are held
 in 32 bits and every output is rounded once.  float32 products are taken from
 three bfloat16 parts of each value and are as good as float32's own rounding.
 The gradient of what is behind the product is rounded to the storage type
-before it is multiplied.  Dropped values follow from a seed and their place:
+before it is multiplied, but not where it is summed for the bias.  Dropped values follow from a seed and their place:
 no mask is stored.  The forward operators are differentiable once; each has its
 adjoint as a function of its own.  No reference counterparts.
 """
