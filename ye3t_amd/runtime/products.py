@@ -178,13 +178,13 @@ def _rows(t):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, input, weight, bias, residual, order, offsets, shape):
+    def forward(ctx, input, weight, bias, residual, order, offsets, shape, wanted):
         activation, below, layer, seed = shape
         problem = native.Linear(input, weight, bias, residual, order, offsets, *shape)
-        out, kept = problem.forward(activation != 0)
+        out, kept = problem.forward(wanted or activation != 0)
         held = isinstance(seed, torch.Tensor)
         # a seed that has changed by then is an error
-        ctx.save_for_backward(input, weight, kept, order, offsets, seed if held else None)
+        ctx.save_for_backward(input, weight, kept if activation else None, order, offsets, seed if held else None)
         ctx.shape = (activation, below, layer, None if held else seed)
         ctx.set_materialize_grads(False)
         if kept is not None:
@@ -195,7 +195,7 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
-            return (None,) * 7
+            return (None,) * 8
         input, weight, kept, order, offsets, seed = ctx.saved_tensors
         activation, below, layer, number = ctx.shape
         problem = native.Linear(input, weight, None, None, order, offsets, activation, below, layer,
@@ -204,7 +204,7 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         if any(need[:3]):
             dx, dw, db = problem.adjoint(grad.contiguous(), kept, *need[:3])
-        return dx, dw, db, grad if need[3] else None, None, None, None
+        return dx, dw, db, grad if need[3] else None, None, None, None, None
 
 
 def _product(name, input, weight, groups, bias, activation, residual, probability, seed, layer, return_preactivation):
@@ -215,10 +215,7 @@ def _product(name, input, weight, groups, bias, activation, residual, probabilit
     args = (_unit_rows(_rows(input)), _laid_out(weight), None if bias is None else bias.contiguous(),
             None if residual is None else _rows(residual).contiguous())
     if _tracked(*args):
-        out, kept = _Linear.apply(*args, order, offsets, shape)
-        if return_preactivation and kept is None:  # without an activation
-            with torch.no_grad():
-                kept = native.Linear(args[0], args[1], args[2], None, order, offsets, 0, 0, 0, 0).forward(False)[0]
+        out, kept = _Linear.apply(*args, order, offsets, shape, return_preactivation)
     else:
         out, kept = native.Linear(*args, order, offsets, *shape).forward(return_preactivation)
     if len(lead) != 1:
