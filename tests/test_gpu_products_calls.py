@@ -51,3 +51,52 @@ def test_the_preactivation_under_autograd_is_of_the_same_product(gpu, calls, dty
     other = w.clone().requires_grad_()
     (want,) = torch.autograd.grad(forward(x, other, *groups, b, **kw), other, g)
     assert torch.equal(grad, want)
+
+
+def memory(call):
+    """The result and the bytes that the call took at most beside what was held before it."""
+    import torch
+
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    result = call()
+    torch.cuda.synchronize()
+    return result, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,inputs,outputs", [(700, 24, 40), (0, 8, 6), (9000, 40, 130), (300, 2048, 1024), (70001, 33, 9)])
+@pytest.mark.parametrize("by_species", [False, True])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("activation", [None, "silu"])
+def test_a_bias_without_its_weight(gpu, dtype, rows, inputs, outputs, by_species, turned, activation):
+    """Frozen weights: the biases' gradients alone and with the input's are what they are beside the weight's, to the order of
+    their sums, and no gradient of the weight is made."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"biases of {rows} x {inputs} x {outputs}, by species {by_species}, turned {turned}, {activation}, {dtype}")
+    lead = (3,) if by_species else ()
+    x = normal((rows, inputs), dtype, 1, gpu)
+    w = normal((*lead, outputs, inputs), dtype, 2, gpu, inputs ** -0.5).transpose(-1, -2) if turned else \
+        normal((*lead, inputs, outputs), dtype, 2, gpu, inputs ** -0.5)
+    b, g = normal((*lead, outputs), dtype, 3, gpu), normal((rows, outputs), dtype, 5, gpu)
+    s = species_of(rows, 3, "rare", gpu) if by_species else None
+    groups = (runtime.species_groups(s, 3),) if by_species else ()
+    forward = runtime.species_linear if by_species else runtime.linear
+    kw = dict(activation=activation, dropout=0.2, seed=3) if activation else {}
+    z = forward(x, w, *groups, b, return_preactivation=True, **kw)[1]
+    want = plain.backward(g, x, w, z, s, activation, plain.kept(rows, outputs, 0.2, 3, 0) if activation else None)
+    for with_input in (False, True):
+        leaf, rows_of = b.clone().requires_grad_(), x.clone().requires_grad_(with_input)
+        y = forward(rows_of, w, *groups, leaf, **kw)
+        grads, taken = memory(lambda: torch.autograd.grad(y, [leaf, rows_of] if with_input else [leaf], g))
+        plain.check("bias", grads[0], want["bias"], dtype)
+        if with_input:
+            plain.check("input", grads[1], want["input"], dtype)
+        if inputs >= 2048 and not with_input:
+            assert taken < w.numel() * w.element_size()
+        again = torch.autograd.grad(forward(rows_of, w, *groups, leaf, **kw), leaf, g)[0]
+        assert torch.equal(again, grads[0])

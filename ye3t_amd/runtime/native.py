@@ -2190,21 +2190,29 @@ class Linear:
         x, w = self.input, self.weight
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_input else None
         dw = db = None
-        if need_weight or need_bias:
+        if need_weight:
             shape = (*w.shape[:-2], w.shape[-1], w.shape[-2]) if self.turned else w.shape
             dw = torch.empty(shape, dtype=w.dtype, device=w.device)
         if need_bias:
             db = torch.empty((*w.shape[:-2], w.shape[-1]), dtype=w.dtype, device=w.device)
-        with _on(x.device):
-            size = lib().ye3t_hip_linear_adjoint_workspace_bytes(self.args)
-            work = _workspace(size, "ye3t_hip_linear_adjoint_workspace_bytes", x.device)
-            _check(lib().ye3t_hip_linear_adjoint(self.args, _dev(adjoint, "adjoint"),
-                                                 _opt(kept, "preactivation"), _opt(dx, "input_adjoint"),
-                                                 _opt(dw, "weight_adjoint"), _opt(db, "bias_adjoint"), work.data_ptr(),
-                                                 size, _raw_stream()), "ye3t_hip_linear_adjoint")
-        if not need_weight:
-            dw = None
+        if need_bias and not need_weight:  # the bias's comes with the weight's, or with that of a weight of no inputs
+            fields = list(_LINEAR_ARGS.unpack(self.args))
+            fields[_LINEAR_FIELDS.index("inputs")] = 0
+            self._adjoint(_LINEAR_ARGS.pack(*fields), adjoint, kept, None, None, db)
+            if need_input:
+                self._adjoint(self.args, adjoint, kept, dx, None, None)
+        else:
+            self._adjoint(self.args, adjoint, kept, dx, dw, db)
         return dx, dw.transpose(-1, -2) if dw is not None and self.turned else dw, db
+
+    def _adjoint(self, args, adjoint, kept, dx, dw, db):
+        with _on(self.input.device):
+            size = lib().ye3t_hip_linear_adjoint_workspace_bytes(args)
+            work = _workspace(size, "ye3t_hip_linear_adjoint_workspace_bytes", self.input.device)
+            _check(lib().ye3t_hip_linear_adjoint(args, _dev(adjoint, "adjoint"), _opt(kept, "preactivation"),
+                                                 _opt(dx, "input_adjoint"), _opt(dw, "weight_adjoint"),
+                                                 _opt(db, "bias_adjoint"), work.data_ptr(), size, _raw_stream()),
+                   "ye3t_hip_linear_adjoint")
 
 
 def dropout(input, residual, below, layer, seed):
