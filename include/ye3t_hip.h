@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define YE3T_HIP_ABI_VERSION 64 /* reference native ABI floor is 42 (execution_plan.py:35) */
+#define YE3T_HIP_ABI_VERSION 65 /* reference native ABI floor is 42 (execution_plan.py:35) */
 
 typedef struct ihipStream_t* ye3t_stream_t; /* == hipStream_t */
 
@@ -986,8 +986,10 @@ int64_t ye3t_hip_linear_workspace_bytes(const ye3t_linear_args* args);
 int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out, void* workspace,
                     int64_t workspace_bytes, ye3t_stream_t stream);
 
-/* Device workspace bytes of ye3t_hip_linear_adjoint (-1 on invalid input). */
+/* Device workspace bytes of ye3t_hip_linear_adjoint (-1 on invalid input): for all three gradients, or for those that are
+ * asked for.  The shares of a weight's gradient take the most. */
 int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args);
+int64_t ye3t_hip_linear_adjoint_workspace_bytes_of(const ye3t_linear_args* args, int input, int weight, int bias);
 
 /* Gradients of ye3t_hip_linear for the output's adjoint [rows, outputs], at the
  * rounded preactivation (NULL without an activation): input_adjoint [rows,

@@ -100,3 +100,21 @@ def test_a_bias_without_its_weight(gpu, dtype, rows, inputs, outputs, by_species
             assert taken < w.numel() * w.element_size()
         again = torch.autograd.grad(forward(rows_of, w, *groups, leaf, **kw), leaf, g)[0]
         assert torch.equal(again, grads[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_rows_gradient_takes_no_shares_of_the_weights(gpu, dtype):
+    """Frozen weights: beside the result only the memory of the allocator's rounding."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    rows, inputs, outputs = 16384, 2048, 1024
+    flush(f"memory of the gradient of {rows} x {inputs} x {outputs} by 8 species, {dtype}")
+    x, w = normal((rows, inputs), dtype, 1, gpu), normal((8, inputs, outputs), dtype, 2, gpu, inputs ** -0.5)
+    g, s = normal((rows, outputs), dtype, 3, gpu), species_of(rows, 8, "any", gpu)
+    leaf = x.clone().requires_grad_()
+    y = runtime.species_linear(leaf, w, runtime.species_groups(s, 8))
+    (dx,), taken = memory(lambda: torch.autograd.grad(y, leaf, g))
+    assert taken < dx.numel() * dx.element_size() + (4 << 20)
+    plain.check("input", dx, plain.backward(g, x, w, None, s)["input"], dtype)

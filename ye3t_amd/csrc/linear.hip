@@ -273,12 +273,13 @@ int64_t bias_bytes(const ye3t_linear_args& a) {
   return up(part_count(a.rows, bias_sums(a).share) * a.outputs * 4);
 }
 // dx and dW are made one after the other: what one takes for its parts the other takes after it.
-int64_t adjoint_bytes(const ye3t_linear_args& a) {
-  const int64_t parts = a.dtype == YE3T_F32 ? row_bytes(backward_of<float>(a, nullptr))
-                                            : row_bytes(backward_of<__bf16>(a, nullptr));
-  const int64_t shares = a.dtype == YE3T_F32 ? weight_bytes(weights_of<float>(a, nullptr))
-                                             : weight_bytes(weights_of<__bf16>(a, nullptr));
-  return dz_bytes(a) + bias_bytes(a) + (shares > parts ? shares : parts) + 256;
+int64_t adjoint_bytes(const ye3t_linear_args& a, bool input, bool weight, bool bias) {
+  int64_t parts = 0, shares = 0;
+  if (input)
+    parts = a.dtype == YE3T_F32 ? row_bytes(backward_of<float>(a, nullptr)) : row_bytes(backward_of<__bf16>(a, nullptr));
+  if (weight || bias)
+    shares = a.dtype == YE3T_F32 ? weight_bytes(weights_of<float>(a, nullptr)) : weight_bytes(weights_of<__bf16>(a, nullptr));
+  return dz_bytes(a) + (bias ? bias_bytes(a) : 0) + (shares > parts ? shares : parts) + 256;
 }
 
 template <typename T>
@@ -314,7 +315,7 @@ template <typename T>
 int adjoint_as(const ye3t_linear_args& a, const void* adjoint, const void* kept, void* input_adjoint,
                void* weight_adjoint, void* bias_adjoint, char* work, hipStream_t s) {
   const T* dz = static_cast<const T*>(adjoint);
-  char* behind = work + dz_bytes(a) + bias_bytes(a);
+  char* behind = work + dz_bytes(a) + (bias_adjoint ? bias_bytes(a) : 0);
   if (shaped(a) && a.rows > 0 && a.outputs > 0) {
     T* to = reinterpret_cast<T*>(work);
     bool summed = false;
@@ -377,11 +378,15 @@ int ye3t_hip_linear(const ye3t_linear_args* args, void* preactivation, void* out
              : linear::forward_as<__bf16>(*args, preactivation, out, workspace, as_stream(stream));
 }
 
-int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args) {
+int64_t ye3t_hip_linear_adjoint_workspace_bytes_of(const ye3t_linear_args* args, int input, int weight, int bias) {
   clear_error();
   if (!args) return set_error(YE3T_EINVAL, "the product needs its arguments");
   if (linear::check_linear(*args)) return -1;
-  return linear::adjoint_bytes(*args);
+  return linear::adjoint_bytes(*args, input, weight, bias);
+}
+
+int64_t ye3t_hip_linear_adjoint_workspace_bytes(const ye3t_linear_args* args) {
+  return ye3t_hip_linear_adjoint_workspace_bytes_of(args, 1, 1, 1);
 }
 
 int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, const void* preactivation,
@@ -396,7 +401,7 @@ int ye3t_hip_linear_adjoint(const ye3t_linear_args* args, const void* adjoint, c
   YE3T_REQUIRE(!any || args->activation == linear::kNone || preactivation,
                "the gradient of an activation needs the preactivation");
   YE3T_REQUIRE(!bias_adjoint || weight_adjoint || args->inputs == 0, "the bias's gradient comes with the weight's");
-  YE3T_REQUIRE(workspace && workspace_bytes >= linear::adjoint_bytes(*args),
+  YE3T_REQUIRE(workspace && workspace_bytes >= linear::adjoint_bytes(*args, input_adjoint, weight_adjoint, bias_adjoint),
                "the workspace is smaller than ye3t_hip_linear_adjoint_workspace_bytes");
   char* work = static_cast<char*>(workspace);
   return args->dtype == YE3T_F32

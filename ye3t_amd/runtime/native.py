@@ -13,7 +13,7 @@ import numpy as np
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "libye3t_hip.so")
-ABI_VERSION = 64
+ABI_VERSION = 65
 _LIB = None
 
 F32, F64, BF16 = 0, 1, 4
@@ -249,6 +249,8 @@ def lib():
     L.ye3t_hip_linear.argtypes = [_vp, _vp, _vp, _vp, _i64, _vp]
     L.ye3t_hip_linear_adjoint_workspace_bytes.argtypes = [_vp]
     L.ye3t_hip_linear_adjoint_workspace_bytes.restype = _i64
+    L.ye3t_hip_linear_adjoint_workspace_bytes_of.argtypes = [_vp] + [ctypes.c_int] * 3
+    L.ye3t_hip_linear_adjoint_workspace_bytes_of.restype = _i64
     L.ye3t_hip_linear_adjoint.argtypes = [_vp] + [_vp] * 6 + [_i64, _vp]
     L.ye3t_hip_dropout.argtypes = [ctypes.c_int, _vp, _vp, _i64, _i64, _i64, ctypes.c_uint32, ctypes.c_uint64, _vp, _vp,
                                    _vp]
@@ -294,7 +296,8 @@ EXPORTED_SYMBOLS = (
     "ye3t_hip_atom_attention_adjoint_workspace_bytes", "ye3t_hip_atom_attention_adjoint",
     "ye3t_hip_species_groups_workspace_bytes", "ye3t_hip_species_groups",
     "ye3t_hip_linear_workspace_bytes", "ye3t_hip_linear",
-    "ye3t_hip_linear_adjoint_workspace_bytes", "ye3t_hip_linear_adjoint", "ye3t_hip_dropout",
+    "ye3t_hip_linear_adjoint_workspace_bytes", "ye3t_hip_linear_adjoint_workspace_bytes_of",
+    "ye3t_hip_linear_adjoint", "ye3t_hip_dropout",
 )
 
 
@@ -2207,8 +2210,8 @@ class Linear:
 
     def _adjoint(self, args, adjoint, kept, dx, dw, db):
         with _on(self.input.device):
-            size = lib().ye3t_hip_linear_adjoint_workspace_bytes(args)
-            work = _workspace(size, "ye3t_hip_linear_adjoint_workspace_bytes", self.input.device)
+            size = lib().ye3t_hip_linear_adjoint_workspace_bytes_of(args, dx is not None, dw is not None, db is not None)
+            work = _workspace(size, "ye3t_hip_linear_adjoint_workspace_bytes_of", self.input.device)
             _check(lib().ye3t_hip_linear_adjoint(args, _dev(adjoint, "adjoint"), _opt(kept, "preactivation"),
                                                  _opt(dx, "input_adjoint"), _opt(dw, "weight_adjoint"),
                                                  _opt(db, "bias_adjoint"), work.data_ptr(), size, _raw_stream()),
