@@ -11,7 +11,7 @@ In training values of the features and of what is added to x may be dropped (D; 
 :class:`AceFeatures` makes the features of positions, differentiable through
 the fused density and the product's reverse mode; :class:`AtomBlock` is the layer.
 ``python -m ye3t_amd.ace.atom_block`` fits one to synthetic energies and prints
-energies and forces.  The products with the weights of the first two lines are Torch's.
+energies and forces.  The products with M, O and r and those for the attention's queries, keys and values are Torch's.
 """
 
 import dataclasses
@@ -89,12 +89,15 @@ class AceFeatures:
 class AtomBlock(torch.nn.Module):
     """Energies of packed structures from their atoms' features and species.  ``hidden``: the width of a feed-forward
     part behind the attention, whose second matrix is the species' own (0: none); ``dropout``: the share of values that
-    are dropped in training, of the features and of the feed-forward part."""
+    are dropped in training, of the features and of the feed-forward part; ``layer``: the number of the first of its two
+    masks.  Blocks that run with one seed take numbers of their own (0, 2, 4, ...), or they drop the same places."""
 
-    def __init__(self, feature_width, species_count, width=128, heads=8, cap=0.0, hidden=0, dropout=0.0):
+    def __init__(self, feature_width, species_count, width=128, heads=8, cap=0.0, hidden=0, dropout=0.0, layer=0):
         super().__init__()
         if width % heads:
             raise ValueError("width must be a multiple of heads")
+        if not 0 <= layer < 2 ** 32 - 1:
+            raise ValueError("layer must be 0 .. 2^32 - 2")
         self.width, self.heads, self.cap = int(width), int(heads), float(cap)
         matrix = lambda a, b: torch.nn.Parameter(torch.randn(a, b) / math.sqrt(a))  # noqa: E731
         ones = lambda n: torch.nn.Parameter(torch.ones(n))  # noqa: E731
@@ -104,7 +107,8 @@ class AtomBlock(torch.nn.Module):
         # distances in Angstrom: from local heads to heads that see the whole structure
         self.slope_logs = torch.nn.Parameter(torch.linspace(0.0, -3.0, heads))
         self.out_norm, self.readout = ones(width), torch.nn.Parameter(torch.randn(width) / width)
-        self.species_count, self.hidden, self.dropout = int(species_count), int(hidden), float(dropout)
+        self.species_count, self.hidden = int(species_count), int(hidden)
+        self.dropout, self.layer = float(dropout), int(layer)
         if hidden:
             zeros = lambda *n: torch.nn.Parameter(torch.zeros(*n))  # noqa: E731
             self.hidden_norm, self.widen, self.widen_bias = ones(width), matrix(width, hidden), zeros(hidden)
@@ -114,14 +118,15 @@ class AtomBlock(torch.nn.Module):
     def forward(self, features, species, positions, offsets, key_mask=None, seed=None):
         """``[structures]`` energies of ``features [N, F]``, ``species [N]``, ``positions [N, 3]``
         (float32) and row offsets ``[structures + 1]``; ``key_mask [N]`` hides ghost atoms: what their
-        features and positions hold reaches nothing.  With a ``seed`` (another one each step) values are dropped."""
+        features and positions hold reaches nothing.  With a ``seed`` (another one each step, and for each rank of a
+        data-parallel run) values are dropped."""
         atoms = int(features.shape[0])
         if key_mask is not None:
             # their rows are computed with the others', and zero times what is not a number is none either
             features, positions = (t.masked_fill(~key_mask[:, None], 0.0) for t in (features, positions))
         dropped = self.dropout if seed is not None else 0.0
         if dropped:
-            features = runtime.dropout(features, dropped, seed, layer=0)
+            features = runtime.dropout(features, dropped, seed, layer=self.layer)
         mixed = runtime.rms_norm(features, self.feature_norm) @ self.mix
         vectors = runtime.embedding(species, self.species, scale=math.sqrt(self.width))
         y, x = runtime.rms_norm(mixed, self.attend_norm, residual=vectors)
@@ -134,7 +139,8 @@ class AtomBlock(torch.nn.Module):
             wide = runtime.linear(y, self.widen, self.widen_bias, activation="silu")
             groups = runtime.species_groups(species, self.species_count, validate=False)  # the embedding has checked them
             y = runtime.rms_norm(runtime.species_linear(wide, self.narrow, groups, self.narrow_bias, residual=x,
-                                                        dropout=dropped, seed=seed, layer=1), self.out_norm)
+                                                        dropout=dropped, seed=seed, layer=self.layer + 1),
+                                 self.out_norm)
         else:
             y, x = runtime.rms_norm(joined, self.out_norm, residual=x)
         each = (y @ self.readout).float()
