@@ -6,8 +6,9 @@ or a call fails, a ``RuntimeError`` carrying the library's message is raised.
 """
 
 import ctypes
-import struct
+import inspect
 import os
+import struct
 
 import numpy as np
 
@@ -92,14 +93,18 @@ class AttentionArgs(ctypes.Structure):
 # ye3t_linear_args, packed as bytes: a Structure of as many fields takes three times as long to fill, which shows in the
 # smallest calls
 _LINEAR_ARGS = struct.Struct("@iqqqiqPPPqPqqiPPiqIQP")
-_LINEAR_FIELDS = ("dtype", "rows", "inputs", "outputs", "groups_given", "groups", "order", "offsets", "input",
-                  "input_row_stride", "weight", "weight_group_stride", "weight_row_stride", "turned", "bias", "residual",
-                  "activation", "drop_below", "layer", "seed", "device_seed")
 
 
-def linear_args(**fields):
-    """``ye3t_linear_args`` by the fields' names, those that are not given zero."""
-    return _LINEAR_ARGS.pack(*(fields.get(n, 0) for n in _LINEAR_FIELDS))
+def linear_args(dtype=0, rows=0, inputs=0, outputs=0, groups_given=0, groups=0, order=0, offsets=0, input=0,
+                input_row_stride=0, weight=0, weight_group_stride=0, weight_row_stride=0, turned=0, bias=0, residual=0,
+                activation=0, drop_below=0, layer=0, seed=0, device_seed=0):
+    """``ye3t_linear_args``: the struct's fields in its order, those that are not given zero."""
+    return _LINEAR_ARGS.pack(dtype, rows, inputs, outputs, groups_given, groups, order, offsets, input, input_row_stride,
+                             weight, weight_group_stride, weight_row_stride, turned, bias, residual, activation, drop_below,
+                             layer, seed, device_seed)
+
+
+_LINEAR_FIELDS = tuple(inspect.signature(linear_args).parameters)
 
 
 class Caps(ctypes.Structure):
@@ -2132,7 +2137,7 @@ class Attention:
         return dq, dk, dv, ds, dp, dkp
 
 
-# ---- products with learned weights and dropout (ye3t_amd.runtime.linear checks the arguments) ----
+# ---- products with learned weights and dropout (ye3t_amd.runtime.products checks the arguments) ----
 
 def species_groups(species, count):
     """``ye3t_hip_species_groups`` of contiguous ``species [rows]``: ``(order, offsets)``."""
@@ -2165,7 +2170,7 @@ class Linear:
         turned = self.turned = strides[-1] != 1 and outputs > 1
         number = isinstance(seed, int)
         grouped = order is not None
-        self.args = _LINEAR_ARGS.pack(
+        self.args = linear_args(
             _storage_code(input.dtype), rows, inputs, outputs, grouped, weight.shape[0] if grouped else 0,
             order.data_ptr() if grouped else 0, offsets.data_ptr() if grouped else 0, input.data_ptr(), input.stride(0),
             weight.data_ptr(), strides[0] if grouped else 0, strides[-1 if turned else -2], turned,
