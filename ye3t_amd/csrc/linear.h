@@ -436,29 +436,23 @@ __device__ inline void hand_out(const f32x16 (*sum)[S::FN], int wm, int wn, int 
 }
 
 // v[q] = sum of a(k) b(k, q) over k < K in fp32, for results that are not finite; q < most exist.  Sums that have all become
-// NaN stay so, and the rest is left out.
+// NaN stay so, and the rest is left out.  One step at a time: two took registers that the kernels' own loops need.
 template <typename A, typename B>
-__device__ void exact_dots(A a, B b, int64_t K, int most, float* v) {
-  constexpr int STEPS = 16;
-  float s[8];
+__device__ void exact_dots(A a, B b, int K, int most, float* v) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) s[q] = 0.0f;
-  for (int64_t k0 = 0; k0 < K; k0 += STEPS) {
-    const int64_t end = k0 + STEPS < K ? k0 + STEPS : K;
-#pragma unroll 2
-    for (int64_t k = k0; k < end; ++k) {
-      const float x = a(k);
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-        if (q < most) s[q] = fmaf(x, b(k, q), s[q]);
-    }
+  for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+#pragma unroll 1
+  for (int k = 0; k < K; ++k) {
+    const float x = a(k);
     bool open = false;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) open |= q < most && s[q] == s[q];
+    for (int q = 0; q < 8; ++q)
+      if (q < most) {
+        v[q] = fmaf(x, b(k, q), v[q]);
+        open |= v[q] == v[q];
+      }
     if (!open) break;
   }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = s[q];
 }
 __device__ inline bool any_not_finite(const float* v) {
   float worst = 0.0f;  // 0 v is NaN for infinities and NaN
