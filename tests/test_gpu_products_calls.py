@@ -118,3 +118,72 @@ def test_the_rows_gradient_takes_no_shares_of_the_weights(gpu, dtype):
     (dx,), taken = memory(lambda: torch.autograd.grad(y, leaf, g))
     assert taken < dx.numel() * dx.element_size() + (4 << 20)
     plain.check("input", dx, plain.backward(g, x, w, None, s)["input"], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("frozen", [False, True])
+def test_a_captured_training_step(gpu, dtype, frozen):
+    """Forward and autograd's gradients in one graph, biases with and without their weights' gradients, replayed with other
+    inputs and seeds beside a second graph of the same pool, with eager work between."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"captured training step, frozen weights {frozen}, {dtype}")
+    rows, a, b = 3000, 136, 264
+    seed = torch.tensor([1], device=gpu)
+    s = species_of(rows, 4, "rare", gpu)
+    x, g = normal((rows, a), dtype, 1, gpu), normal((rows, b), dtype, 4, gpu)
+    w, bias = normal((4, a, b), dtype, 2, gpu, 0.1), normal((4, b), dtype, 3, gpu)
+
+    def step(leaves):
+        groups = runtime.species_groups(s, 4, validate=False)
+        y = runtime.species_linear(x, leaves[0], groups, leaves[1], activation="gelu", dropout=0.2, seed=seed, layer=1)
+        return [y.detach(), *torch.autograd.grad(y, leaves[1:] if frozen else leaves, g)]
+
+    fresh = lambda: [w.clone().requires_grad_(not frozen), bias.clone().requires_grad_()]  # noqa: E731
+    step(fresh())
+    torch.cuda.synchronize()
+    leaves, others = fresh(), fresh()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(leaves)
+    with torch.cuda.graph(other, pool=graph.pool()):
+        step(others)
+    for k in range(4):
+        seed.fill_(10 + k)
+        x.copy_(normal((rows, a), dtype, 30 + k, gpu))
+        s.copy_(species_of(rows, 4, "any" if k % 2 else "rare", gpu))
+        if k % 2:
+            other.replay()
+        graph.replay()
+        got = [t.clone() for t in held]
+        torch.cuda.synchronize()
+        for n, c in zip(got, step(fresh())):
+            assert torch.equal(n, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_streams_of_gradients(gpu, dtype):
+    """Gradients on two streams at once, each with workspaces of its own."""
+    import torch
+
+    from ye3t_amd import runtime
+
+    flush(f"gradients on two streams, {dtype}")
+    data = []
+    for k in range(2):
+        x, w = normal((9000, 72), dtype, k, gpu), normal((72, 136), dtype, k + 2, gpu, 0.1)
+        data.append((normal((9000, 136), dtype, k + 5, gpu), x, w, normal((9000, 136), dtype, k + 7, gpu)))
+    call = lambda d: runtime.linear_adjoint(*d[:3], preactivation=d[3], bias=True, activation="silu", dropout=0.1, seed=3)  # noqa: E731,E501
+    want = [call(d) for d in data]
+    streams = [torch.cuda.Stream() for _ in data]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for d, stream in zip(data, streams):
+            with torch.cuda.stream(stream):
+                got.append(call(d))
+        torch.cuda.synchronize()
+        for one, other in zip(got, want):
+            assert all(torch.equal(t, c) for t, c in zip(one, other))
