@@ -212,9 +212,10 @@ __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_kernel(const R
 }
 
 // The same with tiles of direct loads that fill a compute unit: a workgroup goes through several, and the first loads
-// of the next run while the results of one are finished and written.  16 384 x 1 024 x 4 096: 132 us (1 036 TFLOP/s), 150
-// by a workgroup a tile; with gelu and the preactivation kept 186 and 207.  Bound by the matrix instructions: at
-// 8 192^3 they run 66 % of the cycles, at a clock that falls with their share.
+// of the next run while the results of one are finished and written.  16 384 x 1 024 x 4 096: 132 to 145 us (1 036 to
+// 948 TFLOP/s from card to card), by a workgroup a tile 14 % more; with a bias and gelu 186, the preactivation kept too
+// 205, among a training step's other kernels 211 to 219.  Bound by the matrix instructions: at 8 192^3 they run 66 % of the
+// cycles, at a clock that falls with their share.
 template <typename S, bool ACROSS>
 __global__ __launch_bounds__(S::NT, S::kPerSimd) void row_product_rounds_kernel(const RowProduct<__bf16> p,
                                                                                 int64_t items) {
@@ -462,7 +463,8 @@ Choice choice_of(const RowProduct<T>& p, bool direct) {
   const int64_t groups = ((p.rows + 31) / 32 + (p.grouped ? p.groups : 0)) * ((p.N + 31) / 32);
   const int steps = (p.K + Shapes<T>::Few::KT - 1) / Shapes<T>::Few::KT;
   const int least = 2 * Shapes<T>::Few::KT < 512 ? 512 : 2 * Shapes<T>::Few::KT;  // of the contraction, for a part
-  // as many workgroups as run at a time; 64 x 4 096 x 4 096: bf16 13 us, by twice as many 17; fp32 36 and 32
+  // as many workgroups as run at a time; 64 x 4 096 x 4 096 with the join: bf16 14 us (one part), by twice as many 18; fp32
+  // 34 (two parts), by half as many 37, by twice as many 36
   const int64_t most = sizeof(T) == 4 ? 512 : 256;
   int parts = p.K / least;
   if (parts < 2 || groups > most / 2) return {kFew, 1, 0};

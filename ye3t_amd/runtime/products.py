@@ -5,7 +5,8 @@ each species, and dropout.
 residual in the product's own kernel; ``species_groups`` orders a batch's atoms
 by species once for all layers.  Storage is float32 or bfloat16; sums are held
 in 32 bits and every output is rounded once.  float32 products are taken from
-three bfloat16 parts of each value and are as good as float32's own rounding.
+three bfloat16 parts of each value; what that leaves out is below 2^-26 of each
+term, and the sums' own roundings are the larger part of their errors.
 The gradient of what is behind the product is rounded to the storage type
 before it is multiplied, but not where it is summed for the bias.  Dropped values follow from a seed and their place:
 no mask is stored.  The forward operators are differentiable once; each has its
